@@ -48,6 +48,8 @@ extern "C" {
 #define TM_GEMM_TILE_M 64      /* rows of one expert processed per GEMM tile */
 #define TM_OP4_MAX_PARTS 64    /* row ranges per node in the argmax workspace  */
 #define TM_OP4_NOALLOC_MAX_NODES 2048  /* N limit of tm_op4_argmax_walk_noalloc */
+#define TM_MAX_NORM_HIDDEN 65536  /* columns of tm_rms_norm */
+#define TM_MAX_SAMPLE_VOCAB 262144  /* columns of tm_sample_tokens */
 
 /* ABI version (major*10000 + minor*100 + patch): 5.0.0.  Version 2 added
  * num_edges to tm_op4_argmax_walk / tm_op4_sample_walk and softmax_argmax to
@@ -426,6 +428,99 @@ int tm_tree_attention_plan(int64_t N, int64_t Hq, int64_t kvh, int64_t hd,
  */
 int tm_tree_mask_pack(const uint8_t* mask, int64_t N, int64_t row_stride,
                       uint64_t* bits, void* stream);
+
+/*
+ * Root-mean-square norm of T rows of H elements, with the residual's addition:
+ *   s = x (+ residual),  out = s / sqrt(mean(s^2) + eps) * weight,  res_out = s,
+ * computed in fp32 and rounded once per output.  Replaces `rms_norm` and the
+ * residual additions around it in the reference's decoder layer
+ * (treemoe/model/mixtral.py:268-340).  x, out: dtype.  residual may be NULL; it
+ * and res_out (which may be the same memory) have res_dtype, weight has
+ * weight_dtype, each `dtype` or fp32.  Strides in elements, rows contiguous,
+ * H <= TM_MAX_NORM_HIDDEN.  16-byte aligned rows with H % 8 == 0 take vector
+ * loads; any other alignment and width is served too.
+ */
+int tm_rms_norm(const void* x, int64_t x_stride, const void* residual,
+                int64_t res_stride, int res_dtype, const void* weight,
+                int weight_dtype, int64_t T, int64_t H, float eps, int dtype,
+                void* out, int64_t out_stride, void* res_out,
+                int64_t res_out_stride, void* stream);
+
+/*
+ * The same norm with an output of OCP e4m3 bytes and fp32 scales: for every row
+ * (group = 0) or every `group` columns of a row (32, 64, 128, 256 or 512, a
+ * divisor of H), scale = max|y| / 448 (1 where that is 0) and
+ * out = e4m3(y / scale).  scales: [T, H / group] or [T], row stride scale_stride.
+ * A row or group with a NaN has scale NaN, one with an infinity scale infinity.
+ */
+int tm_rms_norm_fp8(const void* x, int64_t x_stride, const void* residual,
+                    int64_t res_stride, int res_dtype, const void* weight,
+                    int weight_dtype, int64_t T, int64_t H, float eps, int dtype,
+                    void* out, int64_t out_stride, float* scales,
+                    int64_t scale_stride, int64_t group, void* res_out,
+                    int64_t res_out_stride, void* stream);
+
+/*
+ * Rotary positions on queries [T, q_heads, hd] and keys [T, kv_heads, hd] (either
+ * count may be 0); replaces the rotation in `MixtralForward._attention`
+ * (treemoe/model/mixtral.py:172-206).  Pair i < part / 2 of a head turns by
+ * positions[t] * turns[i] 2^-64 turns and is scaled by `magnitude`; it is the
+ * elements (i, i + part / 2), or (2 i, 2 i + 1) when interleaved.  Elements from
+ * `part` on are copied.  positions: [T] int32, or int64 with long_positions.
+ * Heads contiguous, token strides in elements; hd and part multiples of 16,
+ * 16-byte aligned tokens.  The outputs may be the inputs' memory.
+ */
+int tm_rotary(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+              void* q_out, int64_t q_out_stride, void* k_out,
+              int64_t k_out_stride, const void* positions, int long_positions,
+              const uint64_t* turns, float magnitude, int64_t T, int64_t q_heads,
+              int64_t kv_heads, int64_t hd, int64_t part, int interleaved,
+              int dtype, void* stream);
+
+/*
+ * The same for the tokens at positions start_pos .. start_pos + T - 1 of one
+ * sequence, storing the rotated keys and the values [T, kv_heads, hd] in the
+ * layer's cache pages (position p: page block_table[p / page_size], slot
+ * p % page_size); replaces the rotation followed by `PagedKVCache.append`
+ * (treemoe/model/kv_cache.py:62-78).  A page id outside [0, cache_pages) stores
+ * nothing.  Cache strides in elements, heads of a slot contiguous.
+ */
+int tm_rotary_append(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                     const void* v, int64_t v_stride, void* q_out,
+                     int64_t q_out_stride, void* k_cache, void* v_cache,
+                     int64_t stride_page, int64_t stride_slot, int64_t page_size,
+                     int64_t cache_pages, const int32_t* block_table,
+                     int64_t num_table_pages, int64_t start_pos,
+                     const uint64_t* turns, float magnitude, int64_t T,
+                     int64_t q_heads, int64_t kv_heads, int64_t hd, int64_t part,
+                     int interleaved, int dtype, void* stream);
+
+/*
+ * One token of every row of logits [N, V] (dtype; row stride in elements) from a
+ * uniform number of [0, 1), and, with probs, the distribution that it was drawn
+ * from (fp32 [N, V]): the draft side of the sampling mode, whose verification takes
+ * those rows as draft_probs (treemoe/kernels/op4_commit.py:187-196,
+ * treemoe/ref/verify_ref.py:60-89).
+ *
+ * w_i = exp((l_i - max) / temperature); in the order "larger logit first, lower
+ * index first among equals" top_k keeps the first k (0, or >= V: all), top_p the
+ * shortest prefix of those that weighs top_p of them (1: all; at least one), min_p
+ * what weighs at least min_p times the largest.  The token is the first index at
+ * which the running sum of the kept weights, in index order, exceeds u times
+ * their sum.  A temperature of 0 takes the largest logit, the lowest index
+ * among equals.  NaN logits count as -infinity; a row without any logit above
+ * -infinity gives token -1 and zero probabilities.  Weights below 2^-45 are 0.
+ *
+ * temperatures, top_ks, top_ps, min_ps: one value a row, or NULL for the scalar
+ * beside it.  A row value out of its range acts as the nearest one in it.
+ * V <= TM_MAX_SAMPLE_VOCAB.
+ */
+int tm_sample_tokens(const void* logits, int dtype, int64_t N, int64_t V,
+                     int64_t row_stride, const float* uniforms,
+                     const float* temperatures, double temperature,
+                     const int32_t* top_ks, int64_t top_k, const float* top_ps,
+                     double top_p, const float* min_ps, double min_p, int64_t* tokens,
+                     float* probs, int64_t probs_stride, void* stream);
 
 #ifdef __cplusplus
 }

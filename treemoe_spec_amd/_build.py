@@ -23,7 +23,7 @@ ORACLE_C = ROOT / "oracle" / "c"
 ORACLE_LIB = ROOT / "oracle" / "liboracle_c.so"
 
 HIP_SOURCES = ["capi.hip", "op1_route.hip", "op1_gemm.hip", "op1_prefill.hip", "op4_verify.hip",
-               "tree_attn.hip"]
+               "tree_attn.hip", "rms_norm.hip", "rotary.hip", "sample.hip"]
 ARCH = os.environ.get("TREEMOE_AMD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [
@@ -81,17 +81,17 @@ def build_oracle() -> Path:
     return ORACLE_LIB
 
 
-def build_fast_binding() -> Path:
-    """_tmfast: CPython-API calls of the per-step op4 entry points, linked
-    against libtreemoe_amd.so in the same directory."""
+def build_fast_binding(module: str = "_tmfast", source: str = "pyfast.cpp") -> Path:
+    """CPython-API calls of libtreemoe_amd.so in the same directory, linked against
+    it: _tmfast (op4 and tree attention) and _tmlayer (the prompt side and sampling)."""
     import sysconfig
 
     suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
-    out = PKG / ("_tmfast" + suffix)
+    out = PKG / (module + suffix)
     tmp = out.with_suffix(".tmp")
     cxx = os.environ.get("CXX", "g++")
     _run([cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
-          f"-I{sysconfig.get_paths()['include']}", "-o", str(tmp), str(CSRC / "pyfast.cpp"),
+          f"-I{sysconfig.get_paths()['include']}", "-o", str(tmp), str(CSRC / source),
           f"-L{PKG}", "-ltreemoe_amd", "-Wl,-rpath,$ORIGIN"])
     os.replace(tmp, out)
     return out
@@ -101,6 +101,7 @@ def build_all() -> None:
     build_oracle()
     build_library()
     build_fast_binding()
+    build_fast_binding("_tmlayer", "pylayer.cpp")
 
 
 if __name__ == "__main__":

@@ -7,6 +7,7 @@ product path has no CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from pathlib import Path
 
@@ -17,6 +18,7 @@ P = ctypes.c_void_p
 I64 = ctypes.c_int64
 I32 = ctypes.c_int
 F32 = ctypes.c_float
+F64 = ctypes.c_double
 
 # name -> argtypes; every entry point returns int (0 = ok)
 SIGNATURES: dict[str, list] = {
@@ -45,6 +47,13 @@ SIGNATURES: dict[str, list] = {
                           I64, I64, I64, I64, F32, P, I64, I64, P, I64, P],
     "tm_tree_attention_plan": [I64, I64, I64, I64, I64, I64, I64, P, P],
     "tm_tree_mask_pack": [P, I64, I64, P, P],
+    "tm_rms_norm": [P, I64, P, I64, I32, P, I32, I64, I64, F32, I32, P, I64, P, I64, P],
+    "tm_rms_norm_fp8": [P, I64, P, I64, I32, P, I32, I64, I64, F32, I32, P, I64, P, I64, I64, P,
+                        I64, P],
+    "tm_rotary": [P, I64] * 4 + [P, I32, P, F32] + [I64] * 5 + [I32, I32, P],
+    "tm_rotary_append": [P, I64] * 4 + [P, P, I64, I64, I64, I64, P, I64, I64, P, F32]
+                        + [I64] * 5 + [I32, I32, P],
+    "tm_sample_tokens": [P, I32, I64, I64, I64, P, P, F64, P, I64, P, F64, P, F64, P, P, I64, P],
 }
 
 TM_OBJECTIVE = {"mass": 0, "critical_path": 1}
@@ -54,6 +63,8 @@ TM_DTYPE_F16 = 2
 TM_GEMM_TILE_M = 64
 TM_OP4_MAX_PARTS = 64
 TM_OP4_NOALLOC_MAX_NODES = 2048
+TM_MAX_NORM_HIDDEN = 65536
+TM_MAX_SAMPLE_VOCAB = 262144
 
 _lib = None
 
@@ -88,6 +99,69 @@ def fast_binding():
     except ImportError:
         return None
     return _tmfast
+
+
+@functools.cache
+def entry(name: str):
+    """An entry point as a callable that returns its status: the CPython binding
+    _tmlayer where it is built for the library in use, else ctypes."""
+    lib()
+    if _LIB_PATH.resolve() == Path(__file__).resolve().parent / "libtreemoe_amd.so":
+        try:
+            from treemoe_spec_amd import _tmlayer
+
+            return getattr(_tmlayer, name)
+        except ImportError:
+            pass
+    return getattr(lib(), name)
+
+
+def launch(name: str, device, *args) -> None:
+    """An entry point on torch's current stream of ``device`` (a torch.device with
+    an index), with that device current during the call."""
+    import torch
+
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = entry(name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = entry(name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, name)
+
+
+def dtype_code(dtype) -> int | None:
+    """TM_DTYPE_* of a torch dtype, None for one that the kernels do not take."""
+    global _dtype_codes
+    if _dtype_codes is None:
+        import torch
+
+        _dtype_codes = {torch.float32: TM_DTYPE_F32, torch.bfloat16: TM_DTYPE_BF16,
+                        torch.float16: TM_DTYPE_F16}
+    return _dtype_codes.get(dtype)
+
+
+_dtype_codes: dict | None = None
+
+
+def require(what: str, device, **tensors) -> None:
+    """All given tensors on ``device``, a ROCm device, and none that a gradient is
+    asked of: these operators have no backward pass."""
+    import torch
+
+    if device.type != "cuda":
+        raise RuntimeError(f"treemoe_spec_amd {what} runs on ROCm devices only; "
+                           f"got a tensor on {device}")
+    grad = torch.is_grad_enabled()
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device}")
+        if grad and t.requires_grad:
+            raise RuntimeError(f"{what} has no backward pass, but {name} requires a gradient; "
+                               "call it under torch.no_grad()")
 
 
 def check(rc: int, what: str) -> None:
