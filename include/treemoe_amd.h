@@ -49,6 +49,7 @@ extern "C" {
 #define TM_OP4_MAX_PARTS 64    /* row ranges per node in the argmax workspace  */
 #define TM_OP4_NOALLOC_MAX_NODES 2048  /* N limit of tm_op4_argmax_walk_noalloc */
 #define TM_MAX_NORM_HIDDEN 65536  /* columns of tm_rms_norm */
+#define TM_MAX_PROMPT_KEYS (1 << 24)  /* keys of one sequence of prompt attention */
 #define TM_MAX_SAMPLE_VOCAB 262144  /* columns of tm_sample_tokens */
 
 /* ABI version (major*10000 + minor*100 + patch): 5.0.0.  Version 2 added
@@ -521,6 +522,61 @@ int tm_sample_tokens(const void* logits, int dtype, int64_t N, int64_t V,
                      const int32_t* top_ks, int64_t top_k, const float* top_ps,
                      double top_p, const float* min_ps, double min_p, int64_t* tokens,
                      float* probs, int64_t probs_stride, void* stream);
+
+/*
+ * Work list of tm_prompt_attention for B packed sequences, made once per batch on
+ * the host and used by every layer: sequence b has q_lens[b] queries, the last of
+ * its k_lens[b] >= q_lens[b] keys, all sequences one after the other in q and in
+ * k and v.  Writes num_items x 8 int32 to `items` and num_joins x 8 to `joins`
+ * (host memory, to be copied to the device), and
+ *   sizes[0..5] = num_items, num_joins, num_slots, tile_rows, sum of q_lens, sum of
+ *                 k_lens.
+ * With items and joins NULL it only writes sizes.  A length of 0 is allowed.
+ */
+int tm_prompt_plan(const int64_t* q_lens, const int64_t* k_lens, int64_t B,
+                   int64_t Hq, int64_t kvh, int32_t* items, int64_t max_items,
+                   int32_t* joins, int64_t max_joins, int64_t* sizes);
+
+/*
+ * Causal attention over packed sequences: the prompt branch of
+ * `MixtralForward._attention` (treemoe/model/mixtral.py:208-250) for many prompts at
+ * once.  Query i of a sequence, head h, attends to the sequence's keys
+ * 0 .. k_len - q_len + i of KV head h / (Hq / kvh).  q, out [Tq, Hq, hd] and k, v
+ * [Sk, kvh, hd], bf16 or fp16, heads contiguous, token strides in elements, 16-byte
+ * aligned; hd 64 or 128.  items, joins (device memory, 32-byte aligned) and the four
+ * numbers come from tm_prompt_plan for sequences that fit Tq and Sk.  Rows of
+ * out behind the last sequence are not written.  workspace: num_slots * kvh *
+ * tile_rows * (hd + 2) * 4 bytes.
+ */
+int tm_prompt_attention(const void* q, int64_t q_stride, const void* k,
+                        int64_t k_stride, const void* v, int64_t v_stride,
+                        const int32_t* items, int64_t num_items,
+                        const int32_t* joins, int64_t num_joins, int64_t num_slots,
+                        int64_t tile_rows, int64_t Hq, int64_t kvh, int64_t hd,
+                        float scale, int dtype, void* out, int64_t out_stride,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of tm_prompt_attention_cached for these sizes. */
+int tm_prompt_cached_workspace(int64_t T, int64_t seq_len, int64_t Hq, int64_t kvh,
+                               int64_t hd, int64_t* bytes);
+
+/*
+ * The same for the last T of one sequence's seq_len cached positions, a prompt, a
+ * later chunk of one or a decoded token: replaces `PagedKVCache.gather`
+ * (treemoe/model/kv_cache.py:110-123) and the causal
+ * `F.scaled_dot_product_attention` behind it.  Keys are read in place through the
+ * block table (position p: page block_table[p / page_size], slot p % page_size;
+ * page_size a power of two).  Page ids are clamped to [0, cache_pages).
+ */
+int tm_prompt_attention_cached(const void* q, int64_t q_stride, int64_t T,
+                               const void* k_cache, const void* v_cache,
+                               int64_t stride_page, int64_t stride_slot,
+                               int64_t page_size, int64_t cache_pages,
+                               const int32_t* block_table, int64_t num_table_pages,
+                               int64_t seq_len, int64_t Hq, int64_t kvh, int64_t hd,
+                               float scale, int dtype, void* out, int64_t out_stride,
+                               void* workspace, int64_t workspace_bytes,
+                               void* stream);
 
 #ifdef __cplusplus
 }

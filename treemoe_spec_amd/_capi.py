@@ -54,6 +54,11 @@ SIGNATURES: dict[str, list] = {
     "tm_rotary_append": [P, I64] * 4 + [P, P, I64, I64, I64, I64, P, I64, I64, P, F32]
                         + [I64] * 5 + [I32, I32, P],
     "tm_sample_tokens": [P, I32, I64, I64, I64, P, P, F64, P, I64, P, F64, P, F64, P, P, I64, P],
+    "tm_prompt_plan": [P, P, I64, I64, I64, P, I64, P, I64, P],
+    "tm_prompt_attention": [P, I64] * 3 + [P, I64, P] + [I64] * 6 + [F32, I32, P, I64, P, I64, P],
+    "tm_prompt_cached_workspace": [I64] * 5 + [P],
+    "tm_prompt_attention_cached": [P, I64, I64, P, P, I64, I64, I64, I64, P, I64, I64, I64, I64,
+                                   I64, F32, I32, P, I64, P, I64, P],
 }
 
 TM_OBJECTIVE = {"mass": 0, "critical_path": 1}
@@ -65,6 +70,7 @@ TM_OP4_MAX_PARTS = 64
 TM_OP4_NOALLOC_MAX_NODES = 2048
 TM_MAX_NORM_HIDDEN = 65536
 TM_MAX_SAMPLE_VOCAB = 262144
+TM_MAX_PROMPT_KEYS = 1 << 24
 
 _lib = None
 

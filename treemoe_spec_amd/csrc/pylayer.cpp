@@ -63,6 +63,9 @@ PyMethodDef kMethods[] = {
     TM_ENTRY(tm_rotary),
     TM_ENTRY(tm_rotary_append),
     TM_ENTRY(tm_sample_tokens),
+    TM_ENTRY(tm_prompt_attention),
+    TM_ENTRY(tm_prompt_cached_workspace),
+    TM_ENTRY(tm_prompt_attention_cached),
     {nullptr, nullptr, 0, nullptr},
 };
 

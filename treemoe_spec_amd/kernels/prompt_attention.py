@@ -1,0 +1,169 @@
+"""Causal attention of prompts, packed or over the paged cache, down to one token.
+
+The reference's prompt branch (treemoe/model/mixtral.py:208-250) appends the prompt's
+keys to the cache, gathers the whole sequence and calls
+``F.scaled_dot_product_attention`` with a causal mask, one sequence at a time.
+``prompt_attention`` takes many sequences packed one after the other,
+``prompt_attention_cached`` reads one sequence's pages in place: a prompt, a later
+chunk of one, or a decoded token.  The context comes back as [T, Hq * hd], the layout
+``o_proj`` takes.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import operator
+
+import torch
+
+from treemoe_spec_amd import _capi
+from treemoe_spec_amd.kv_cache import device_tables_of
+
+
+class PromptPlan:
+    """The work list of ``prompt_attention`` for one batch, made once and used by
+    every layer.  ``q_lens``: each sequence's queries; ``k_lens`` (default: the same):
+    its keys, of which the queries are the last."""
+
+    def __init__(self, q_lens, k_lens=None, *, num_heads: int, num_kv_heads: int,
+                 device="cuda"):
+        q_lens = [operator.index(n) for n in q_lens]
+        k_lens = q_lens if k_lens is None else [operator.index(n) for n in k_lens]
+        if len(k_lens) != len(q_lens):
+            raise ValueError("q_lens and k_lens must have the same length")
+        for nq, nk in zip(q_lens, k_lens):
+            if not 0 <= nq <= nk <= _capi.TM_MAX_PROMPT_KEYS:
+                raise ValueError("every sequence needs 0 <= queries <= keys <= "
+                                 f"{_capi.TM_MAX_PROMPT_KEYS}, got {nq} and {nk}")
+        if num_kv_heads < 1 or num_heads < num_kv_heads or num_heads % num_kv_heads:
+            raise ValueError("num_heads must be a multiple of num_kv_heads")
+        n = len(q_lens)
+        ql, kl = (ctypes.c_int64 * n)(*q_lens), (ctypes.c_int64 * n)(*k_lens)
+        sizes = (ctypes.c_int64 * 6)()
+        _capi.call("tm_prompt_plan", ql, kl, n, num_heads, num_kv_heads, None, 0, None, 0, sizes)
+        items = torch.zeros(max(1, sizes[0]), 8, dtype=torch.int32)
+        joins = torch.zeros(max(1, sizes[1]), 8, dtype=torch.int32)
+        _capi.call("tm_prompt_plan", ql, kl, n, num_heads, num_kv_heads, items.data_ptr(),
+                   sizes[0], joins.data_ptr(), sizes[1], sizes)
+        self.num_items, self.num_joins, self.num_slots, self.tile_rows, self.q_rows, \
+            self.k_rows = list(sizes)
+        self.num_heads, self.num_kv_heads = num_heads, num_kv_heads
+        self.items, self.joins = items.to(device), joins.to(device)
+        self.device = self.items.device
+
+
+def _check_q(q: torch.Tensor, out: torch.Tensor | None) -> tuple[int, int, int, int]:
+    """(dtype code, T, Hq, hd) of q; checks ``out``."""
+    dt = _capi.dtype_code(q.dtype)
+    if dt is None or dt == _capi.TM_DTYPE_F32:
+        raise ValueError(f"q must be bfloat16 or float16, got {q.dtype}")
+    if q.dim() != 3:
+        raise ValueError("q must be [T, heads, head_dim]")
+    t, hq, hd = q.shape
+    st = q.stride()
+    if hd not in (64, 128):
+        raise ValueError(f"head_dim must be 64 or 128, got {hd}")
+    if st[2] != 1 or (st[1] != hd and hq > 1):
+        raise ValueError("q must have contiguous heads")
+    if out is not None and (out.shape != (t, hq * hd) or out.dtype != q.dtype
+                            or out.stride(1) != 1):
+        raise ValueError("out must be [T, Hq * hd] of q's dtype")
+    return dt, t, hq, hd
+
+
+def _check_scale(scale: float | None, hd: int) -> float:
+    if scale is None:
+        return hd ** -0.5
+    scale = float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError("scale must be positive")
+    return scale
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PromptPlan, *,
+                     scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """q [T, Hq, hd], k and v [S, kvh, hd] (bfloat16 or float16, head_dim 64 or 128,
+    heads contiguous): ``plan``'s sequences one after the other.  A query attends to
+    its sequence's keys up to its own position.  Returns [T, Hq * hd]; T and S may
+    exceed the plan's rows (a padded batch): in a new result the rows behind the last
+    sequence are 0, in ``out`` they stay as they were."""
+    dt, t, hq, hd = _check_q(q, out)
+    dev = q.device
+    _capi.require("prompt_attention", dev, q=q, k=k, v=v, plan=plan.items, out=out)
+    for name, x in (("k", k), ("v", v)):
+        if x.dim() != 3 or x.shape[2] != hd or x.dtype != q.dtype or x.shape != k.shape:
+            raise ValueError("k and v must be [S, kv_heads, head_dim] of q's dtype")
+        if x.stride(2) != 1 or (x.stride(1) != hd and x.shape[1] > 1):
+            raise ValueError(f"{name} must have contiguous heads")
+    if hq != plan.num_heads or k.shape[1] != plan.num_kv_heads:
+        raise ValueError(f"the plan is for {plan.num_heads} heads over {plan.num_kv_heads}, "
+                         f"got {hq} over {k.shape[1]}")
+    if t < plan.q_rows or k.shape[0] < plan.k_rows:
+        raise ValueError(f"the plan's sequences need {plan.q_rows} queries and {plan.k_rows} "
+                         f"keys, got {t} and {k.shape[0]}")
+    scale = _check_scale(scale, hd)
+    if out is None:
+        out = torch.empty((t, hq * hd), dtype=q.dtype, device=dev)
+        if t > plan.q_rows:
+            out[plan.q_rows:].zero_()
+    nbytes = plan.num_slots * plan.num_kv_heads * plan.tile_rows * (hd + 2) * 4
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _capi.launch("tm_prompt_attention", dev, q.data_ptr(), _stride(q, hq * hd), k.data_ptr(),
+                 _stride(k, k.shape[1] * hd), v.data_ptr(), _stride(v, k.shape[1] * hd),
+                 plan.items.data_ptr(), plan.num_items, plan.joins.data_ptr(), plan.num_joins,
+                 plan.num_slots, plan.tile_rows, hq, k.shape[1], hd, scale, dt, out.data_ptr(),
+                 _stride(out, hq * hd), _capi.ptr(ws), nbytes)
+    return out
+
+
+def _stride(x: torch.Tensor, width: int) -> int:
+    """Token stride; one token, whose stride says nothing, counts as contiguous."""
+    return x.stride(0) if x.shape[0] > 1 else width
+
+
+def prompt_attention_cached(q: torch.Tensor, kv, layer: int, *, scale: float | None = None,
+                            out: torch.Tensor | None = None) -> torch.Tensor:
+    """q [T, Hq, hd]: the last T of ``kv``'s ``seq_len`` positions, whose keys and values
+    the cache holds already (``rotary_append``, ``append``).  Query t attends to
+    positions 0 .. seq_len - T + t of ``layer``, read in place through the block table.
+    The cache is [L, pages, page, kv_heads, head_dim] of q's dtype, page size a power of
+    two.  Returns [T, Hq * hd]."""
+    dt, t, hq, hd = _check_q(q, out)
+    dev = q.device
+    kc, vc = kv.k, kv.v
+    _capi.require("prompt_attention_cached", dev, q=q, k_cache=kc, v_cache=vc, out=out)
+    cshape, cst = kc.shape, kc.stride()
+    if kc.dtype != q.dtype or vc.dtype != q.dtype or vc.shape != cshape or vc.stride() != cst \
+            or len(cshape) != 5 or cshape[4] != hd or cst[4] != 1 \
+            or (cst[3] != hd and cshape[3] > 1) or cshape[2] != kv.block_size:
+        raise ValueError("cache layout must be [L, pages, page, kv_heads, head_dim] of q's dtype")
+    kvh, page = cshape[3], cshape[2]
+    if hq % kvh:
+        raise ValueError("num_heads must be a multiple of num_kv_heads")
+    if page & (page - 1):
+        raise ValueError(f"page size must be a power of two, got {page}")
+    layer = operator.index(layer)
+    layers = cshape[0]
+    if not -layers <= layer < layers:
+        raise IndexError(f"layer {layer} is out of range for a cache of {layers} layers")
+    seq_len = kv.seq_len
+    if t > seq_len:
+        raise ValueError(f"{t} queries over a cache of {seq_len} positions")
+    scale = _check_scale(scale, hd)
+    if out is None:
+        out = torch.empty((t, hq * hd), dtype=q.dtype, device=dev)
+    if t == 0:
+        return out
+    table, _ = device_tables_of(kv, dev)
+    size = ctypes.c_int64()
+    rc = _capi.entry("tm_prompt_cached_workspace")(t, seq_len, hq, kvh, hd,
+                                                   ctypes.addressof(size))
+    _capi.check(rc, "tm_prompt_cached_workspace")
+    nbytes = size.value
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    off = kc.element_size() * cst[0] * (layer % layers)
+    _capi.launch("tm_prompt_attention_cached", dev, q.data_ptr(), q.stride(0), t,
+                 kc.data_ptr() + off, vc.data_ptr() + off, cst[1], cst[2], page, cshape[1],
+                 table.data_ptr(), len(kv.block_table), seq_len, hq, kvh, hd, scale, dt,
+                 out.data_ptr(), out.stride(0), _capi.ptr(ws), nbytes)
+    return out
