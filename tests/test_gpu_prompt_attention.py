@@ -109,7 +109,9 @@ def test_large_tiles(dtype):
     lens = [1900, 2300, 777]
     assert PromptPlan(lens, num_heads=64, num_kv_heads=16).tile_rows in (128, 256)
     _packed(lens, lens, 64, 16, 64, dtype, 5)
-    _packed([4500], [4500], 32, 8, 128, dtype, 6)
+    lens = [900, 2, 4000, 0, 3400]
+    assert PromptPlan(lens, num_heads=32, num_kv_heads=8).tile_rows == 256
+    _packed(lens, lens, 32, 8, 128, dtype, 6)
 
 
 def _cache(s, kvh, hd, dtype, page, seed, layers=2):

@@ -117,7 +117,6 @@ struct Shape {
   static constexpr int kRow = HD * 2;              // bytes of a key's row
   static constexpr int kChunks = kRow / 16;        // 16-byte chunks of a row
   static constexpr int kTile = kKeys * kRow;       // bytes of a stage's K, or V
-  static constexpr int kLoads = kTile / 4096;      // loads of a wave per stage and operand
   static constexpr int kKeysPerLoad = 1024 / kRow;
   // Chunk c of key j lies at c ^ swizzle(j).  K is read 16 bytes a lane, 8 or more
   // keys at one logical chunk: the keys' low bits spread them over the banks.  V
@@ -132,52 +131,59 @@ struct Shape {
   }
 };
 
-// Keys kb .. kb + 63 of K and V into LDS.  Keys at or past the last are that of the
-// last one: their scores are masked.
-template <int HD, bool PAGED>
+// Keys kb .. kb + 63 of K or V into LDS, by NW waves.  Keys past the sequence's last
+// are that one again: their scores are masked.
+template <int HD, bool PAGED, int NW>
 struct Loader {
   typedef Shape<HD> S;
-  const uint16_t* k;
-  const uint16_t* v;
-  int last;          // the sequence's last key
-  int page_of[S::kLoads];  // pages of the next stage's keys (paged)
+  static constexpr int kLoads = S::kTile / (1024 * NW);  // loads of a wave per tile
+  const uint16_t* base;
+  int64_t stride;    // of a key, or of a page's slot
+  int last;
 
   __device__ __forceinline__ int key_in(int i) const {  // within the stage
-    return ((int)(threadIdx.x >> 6) * S::kLoads + i) * S::kKeysPerLoad +
+    return ((int)(threadIdx.x >> 6) * kLoads + i) * S::kKeysPerLoad +
            (int)(threadIdx.x & 63) / S::kChunks;
   }
-  __device__ __forceinline__ void look_up(const PromptParams& p, int kb) {
+  // Pages of the keys kb .. (paged): looked up a stage before they are loaded.
+  __device__ __forceinline__ void look_up(const PromptParams& p, int kb, int (&pages)[kLoads]) const {
     if constexpr (PAGED) {
 #pragma unroll
-      for (int i = 0; i < S::kLoads; ++i)
-        page_of[i] = p.table[min(kb + key_in(i), last) >> p.page_shift];
+      for (int i = 0; i < kLoads; ++i)
+        pages[i] = p.table[min(kb + key_in(i), last) >> p.page_shift];
     }
   }
-  __device__ __forceinline__ void load(const PromptParams& p, int kb, uint8_t* kt, uint8_t* vt) {
+  template <bool V>
+  __device__ __forceinline__ void load(const PromptParams& p, int kb, const int (&pages)[kLoads],
+                                       uint8_t* tile) const {
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int chunk = (int)threadIdx.x & (S::kChunks - 1);
 #pragma unroll
-    for (int i = 0; i < S::kLoads; ++i) {
+    for (int i = 0; i < kLoads; ++i) {
       const int j = key_in(i);
-      const int key = min(kb + j, last);
-      int64_t ko, vo;
+      const int c = (chunk ^ (V ? S::swz_v(j) : S::swz_k(j))) * 8;
+      const uint16_t* from;
       if constexpr (PAGED) {
-        const int page = min(max(page_of[i], 0), p.cache_pages - 1);
-        ko = (int64_t)page * p.stride_page +
-             (int64_t)(key & ((1 << p.page_shift) - 1)) * p.k_stride;
-        vo = ko;
+        const int key = min(kb + j, last);
+        from = base + ((int64_t)min(max(pages[i], 0), p.cache_pages - 1) * p.stride_page +
+                       (int64_t)(key & ((1 << p.page_shift) - 1)) * stride + c);
       } else {
-        ko = (int64_t)key * p.k_stride;
-        vo = (int64_t)key * p.v_stride;
+        // the stage's first row is wave-uniform, a lane's offset from it fits 32 bits
+        const uint16_t* const row0 = base + (int64_t)kb * stride;
+        from = row0 + (uint32_t)(min(j, last - kb) * (int)stride + c);
       }
-      const int at = (wave * S::kLoads + i) * 1024;
-      __builtin_amdgcn_global_load_lds((glb_void*)(k + ko + (chunk ^ S::swz_k(j)) * 8),
-                                       (lds_void*)(kt + at), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((glb_void*)(v + vo + (chunk ^ S::swz_v(j)) * 8),
-                                       (lds_void*)(vt + at), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((glb_void*)from,
+                                       (lds_void*)(tile + (wave * kLoads + i) * 1024), 16, 0, 0);
     }
   }
 };
+
+// A value that the compiler takes as new, so that addresses made from it are not kept
+// in registers from one stage to the next.
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 
 __device__ __forceinline__ u32x2_t read_tr(const uint8_t* p) {
   return __builtin_bit_cast(
@@ -185,240 +191,323 @@ __device__ __forceinline__ u32x2_t read_tr(const uint8_t* p) {
                    (__attribute__((address_space(3))) s16x4_t*)(lds_void*)const_cast<uint8_t*>(p)));
 }
 
-// V^T fragment of head-dim tile ht for the 16 keys from `key` on.
+// Byte offsets of a lane's part of V^T fragments: keys 0-3 (lo) or 8-11 (hi) of a k-step,
+// head-dim tile 0; tile ht is at ^ 64 ht.
 template <int HD>
-__device__ __forceinline__ u32x4_t v_frag(const uint8_t* vt, int ht, int key, int lane) {
+__device__ __forceinline__ void v_offsets(int& lo, int& hi) {
   typedef Shape<HD> S;
-  const int i = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int k0 = 4 * (g >> 1) + (i >> 2);
-  const int chunk = 4 * ht + 2 * (g & 1) + ((i & 3) >> 1);
-  const uint8_t* const lo =
-      vt + (key + k0) * S::kRow + ((chunk ^ S::swz_v(k0)) * 16) + (i & 1) * 8;
-  const uint8_t* const hi =
-      vt + (key + k0 + 8) * S::kRow + ((chunk ^ S::swz_v(k0 + 8)) * 16) + (i & 1) * 8;
-  const u32x2_t a = read_tr(lo), b = read_tr(hi);
-  return u32x4_t{a.x, a.y, b.x, b.y};
+  const int chunk = 2 * (g & 1) + ((i & 3) >> 1);
+  lo = k0 * S::kRow + (chunk ^ S::swz_v(k0)) * 16 + (i & 1) * 8;
+  hi = (k0 + 8) * S::kRow + (chunk ^ S::swz_v(k0 + 8)) * 16 + (i & 1) * 8;
 }
 
-// Softmax state and output of one tile of 32 rows (a lane's column is one row).
+// The wave's 32 rows (a lane's column is one row; its lane ^ 32 holds the same).
 template <int HD>
-struct RowTile {
-  u32x4_t q[HD / 16];
-  f32x16_t o[HD / 32];
-  float m, l;     // reference maximum (base 2), and this lane's part of the sum
-  int seen;       // the row's last visible key
+struct Rows {
+  u32x4_t q[HD / 16];    // Q^T fragments
+  f32x16_t o[HD / 32];   // O^T
+  f32x16_t sc[2];        // S^T of a stage
+  u32x4_t pw[4];         // its weights: k-step (kt, m) at 2 kt + m
+  float m, l;            // reference maximum (base 2), and this lane's part of the sum
+  int seen;              // the row's last visible key
 };
 
-// Keys kb .. of the stage at kt / vt against QT row tiles.
-template <int DT, int HD, int QT, bool MASK>
-__device__ __forceinline__ void attend(const PromptParams& p, const uint8_t* kt_, const uint8_t* vt,
-                                       int kb, RowTile<HD> (&rt)[QT]) {
+// S^T = K Q^T of the stage at kt_.
+template <int DT, int HD>
+__device__ __forceinline__ void scores(const uint8_t* kt_, Rows<HD>& r) {
   typedef Shape<HD> S;
   const int lane = threadIdx.x & 63, half = lane >> 5, c32 = lane & 31;
-  f32x16_t sc[QT][2];
 #pragma unroll
-  for (int t = 0; t < QT; ++t)
+  for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int x = 0; x < 16; ++x) r.sc[kt][x] = 0.0f;
+  // chunk 2 ks + half of row c32 (+ 32 kt)
+  const int at = fresh(c32 * S::kRow + (half ^ S::swz_k(c32)) * 16);
 #pragma unroll
-      for (int x = 0; x < 16; ++x) sc[t][kt][x] = 0.0f;
-  const uint8_t* const krow = kt_ + c32 * S::kRow;
-#pragma unroll
-  for (int ks = 0; ks < HD / 16; ++ks) {
+  for (int ks = 0; ks < HD / 16; ++ks)
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
-      const u32x4_t a = *reinterpret_cast<const u32x4_t*>(
-          krow + 32 * kt * S::kRow + (((2 * ks + half) ^ S::swz_k(c32)) * 16));
-#pragma unroll
-      for (int t = 0; t < QT; ++t) sc[t][kt] = mfma32<DT>(a, rt[t].q[ks], sc[t][kt]);
+      const u32x4_t a =
+          *reinterpret_cast<const u32x4_t*>(kt_ + 32 * kt * S::kRow + (at ^ (32 * ks)));
+      r.sc[kt] = mfma32<DT>(a, r.q[ks], r.sc[kt]);
     }
-  }
-  u32x4_t pw[QT][4];  // weights of k-step (kt, m) at 2 kt + m
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    if constexpr (MASK) {
-      const int left = rt[t].seen - kb - 4 * half;  // keys up to this one are visible
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int x = 0; x < 16; ++x)
-          sc[t][kt][x] =
-              32 * kt + 8 * (x >> 2) + (x & 3) <= left ? sc[t][kt][x] : -INFINITY;
-    }
-    float mx = fmaxf(sc[t][0][0], sc[t][1][0]);
-#pragma unroll
-    for (int x = 1; x < 16; ++x) mx = fmaxf(fmaxf(mx, sc[t][0][x]), sc[t][1][x]);
-    const float cand = max_halves(mx) * p.scale_log2;
-    const bool bump = cand > rt[t].m + 8.0f;
-    if (__any(bump)) {
-      const float m = bump ? cand : rt[t].m;
-      const float a = bump ? __builtin_amdgcn_exp2f(rt[t].m - m) : 1.0f;
-#pragma unroll
-      for (int ht = 0; ht < HD / 32; ++ht)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) rt[t].o[ht][x] *= a;
-      rt[t].l *= a;
-      rt[t].m = m;
-    }
-    const float base = rt[t].m == -INFINITY ? 0.0f : -rt[t].m;
+}
+
+// The weights of the stage's keys kb .. against the running maximum.  mask: some key
+// lies past the last one that some row sees.
+template <int DT, int HD>
+__device__ __forceinline__ void weigh(float scale_log2, int kb, bool mask, Rows<HD>& r) {
+  if (mask) {
+    const int left = r.seen - kb - 4 * ((int)(threadIdx.x & 63) >> 5);
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float e0 = __builtin_amdgcn_exp2f(
-              fmaf(sc[t][kt][8 * m + 2 * j], p.scale_log2, base));
-          const float e1 = __builtin_amdgcn_exp2f(
-              fmaf(sc[t][kt][8 * m + 2 * j + 1], p.scale_log2, base));
-          const uint32_t w = tm_pack2<DT>(e0, e1);
-          rt[t].l = add_pair<DT>(w, rt[t].l);
-          pw[t][2 * kt + m][j] = w;
-        }
+      for (int x = 0; x < 16; ++x)
+        r.sc[kt][x] = 32 * kt + 8 * (x >> 2) + (x & 3) <= left ? r.sc[kt][x] : -INFINITY;
   }
+  float mx = fmaxf(r.sc[0][0], r.sc[1][0]);
 #pragma unroll
-  for (int s = 0; s < 4; ++s) {
+  for (int x = 1; x < 16; ++x) mx = fmaxf(fmaxf(mx, r.sc[0][x]), r.sc[1][x]);
+  const float cand = max_halves(mx) * scale_log2;
+  const bool bump = cand > r.m + 8.0f;
+  if (__any(bump)) {
+    const float m = bump ? cand : r.m;
+    const float a = bump ? __builtin_amdgcn_exp2f(r.m - m) : 1.0f;
 #pragma unroll
-    for (int ht = 0; ht < HD / 32; ++ht) {
-      const u32x4_t a = v_frag<HD>(vt, ht, 16 * s, lane);
+    for (int ht = 0; ht < HD / 32; ++ht)
 #pragma unroll
-      for (int t = 0; t < QT; ++t) rt[t].o[ht] = mfma32<DT>(a, pw[t][s], rt[t].o[ht]);
+      for (int x = 0; x < 16; ++x) r.o[ht][x] *= a;
+    r.l *= a;
+    r.m = m;
+  }
+  const float base = r.m == -INFINITY ? 0.0f : -r.m;
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int x = 8 * (s & 1) + 2 * j;
+      const float e0 = __builtin_amdgcn_exp2f(fmaf(r.sc[s >> 1][x], scale_log2, base));
+      const float e1 = __builtin_amdgcn_exp2f(fmaf(r.sc[s >> 1][x + 1], scale_log2, base));
+      const uint32_t w = tm_pack2<DT>(e0, e1);
+      r.l = add_pair<DT>(w, r.l);
+      r.pw[s][j] = w;
     }
-  }
 }
 
-template <int DT, int HD, int QT, bool PAGED>
-__global__ void __launch_bounds__(kThreads, QT == 1 ? 2 : 1) tm_prompt_attn_kernel(PromptParams p) {
+// O^T += V^T P^T of the stage at vt.
+template <int DT, int HD>
+__device__ __forceinline__ void gather(const uint8_t* vt, Rows<HD>& r) {
+  int lo, hi;
+  v_offsets<HD>(lo, hi);
+  lo = fresh(lo);
+  hi = fresh(hi);
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int ht = 0; ht < HD / 32; ++ht) {
+      const u32x2_t a = read_tr(vt + 16 * s * Shape<HD>::kRow + (lo ^ (64 * ht)));
+      const u32x2_t b = read_tr(vt + 16 * s * Shape<HD>::kRow + (hi ^ (64 * ht)));
+      r.o[ht] = mfma32<DT>(u32x4_t{a.x, a.y, b.x, b.y}, r.pw[s], r.o[ht]);
+    }
+}
+
+// What a workgroup works on.
+__device__ __forceinline__ Item item_of(const PromptParams& p, int at, int rows) {
+  if (p.items != nullptr) return p.items[at];
+  Item it;
+  it.q0 = it.k0 = 0;
+  it.q_len = p.q_len;
+  it.k_len = p.k_len;
+  it.tile = p.tiles - 1 - at / p.chunks;
+  const int chunk = at % p.chunks;
+  const int last_token = min(it.q_len - 1, (it.tile * rows + rows - 1) / p.group);
+  it.begin = chunk * p.chunk_len;
+  it.end = min(it.begin + p.chunk_len, it.k_len - it.q_len + last_token + 1);
+  it.slot = p.chunks > 1 ? it.tile * p.chunks + chunk : -1;
+  return it;
+}
+
+// NW waves of 32 rows.  NW = 8: the two waves of a SIMD take turns, one in the matrix
+// products of its stage while the other weighs, a barrier between the turns.
+// NW = 4: two workgroups a CU, which drift apart by themselves.
+template <int DT, int HD, int NW, bool PAGED>
+__global__ void __launch_bounds__(64 * NW, 2) tm_prompt_attn_kernel(PromptParams p) {
   typedef Shape<HD> S;
-  constexpr int kRows = 128 * QT;
+  typedef Loader<HD, PAGED, NW> L;
+  constexpr int kRows = 32 * NW;
+  constexpr int kRing = NW == 8 ? 3 : 2;
   __shared__ __attribute__((aligned(1024))) uint8_t s_k0[S::kTile];
   __shared__ __attribute__((aligned(1024))) uint8_t s_v0[S::kTile];
   __shared__ __attribute__((aligned(1024))) uint8_t s_k1[S::kTile];
   __shared__ __attribute__((aligned(1024))) uint8_t s_v1[S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_k2[kRing == 3 ? S::kTile : 16];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_v2[kRing == 3 ? S::kTile : 16];
 
   // KV heads innermost: with 8 of them a head's workgroups, which share its keys, run
   // on one XCD; the tiles with the most keys first
   const int kvhead = (int)blockIdx.x % p.kvh;
-  const int at = (int)blockIdx.x / p.kvh;
-  Item it;
-  if (p.items != nullptr) {
-    it = p.items[at];
-  } else {
-    it.q0 = it.k0 = 0;
-    it.q_len = p.q_len;
-    it.k_len = p.k_len;
-    it.tile = p.tiles - 1 - at / p.chunks;
-    const int chunk = at % p.chunks;
-    const int last_token = min(it.q_len - 1, (it.tile * kRows + kRows - 1) / p.group);
-    const int keys = it.k_len - it.q_len + last_token + 1;
-    it.begin = chunk * p.chunk_len;
-    it.end = min(it.begin + p.chunk_len, keys);
-    it.slot = p.chunks > 1 ? it.tile * p.chunks + chunk : -1;
-  }
+  const Item it = item_of(p, (int)blockIdx.x / p.kvh, kRows);
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, c32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int past = it.k_len - it.q_len;
   const int all_rows = it.q_len * p.group;
 
-  // this lane's rows: column c32 of each of the wave's tiles
-  RowTile<HD> rt[QT];
-  int64_t qat[QT];   // element offset of the row's head in q, or -1
-  int wave_seen = -1;  // the last key that any row of this wave sees
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int first = it.tile * kRows + (wave * QT + t) * 32;
-    const int row = first + c32;
-    const bool ok = row < all_rows;
-    const int token = ok ? row / p.group : 0;
-    const int head = kvhead * p.group + (ok ? row - token * p.group : 0);
+  // this lane's row
+  const int first = it.tile * kRows + wave * 32;
+  const bool ok = first + c32 < all_rows;
+  const int token = ok ? (first + c32) / p.group : 0;
+  const int head = kvhead * p.group + (ok ? first + c32 - token * p.group : 0);
+  Rows<HD> r;
+  {
     const uint16_t* const qr =
         p.q + (int64_t)(it.q0 + token) * p.q_stride + (int64_t)head * HD + 8 * half;
 #pragma unroll
     for (int ks = 0; ks < HD / 16; ++ks) {
       const u32x4_t x = *reinterpret_cast<const u32x4_t*>(qr + 16 * ks);
       const u32x4_t zero = {0u, 0u, 0u, 0u};
-      rt[t].q[ks] = ok ? x : zero;
+      r.q[ks] = ok ? x : zero;
     }
+  }
+#pragma unroll
+  for (int ht = 0; ht < HD / 32; ++ht)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) r.o[ht][x] = 0.0f;
+  r.m = -INFINITY;
+  r.l = 0.0f;
+  // a range's end hides what lies past it
+  r.seen = min(ok ? past + token : -1, it.end - 1);
+  // keys up to this one are seen by every row of the wave
+  const int full = min(first + 32 <= all_rows ? past + first / p.group : -1, it.end - 1);
+
+  L lk, lv;
+  lk.base = p.k + (int64_t)kvhead * HD + (PAGED ? 0 : (int64_t)it.k0 * p.k_stride);
+  lv.base = p.v + (int64_t)kvhead * HD + (PAGED ? 0 : (int64_t)it.k0 * p.v_stride);
+  lk.stride = p.k_stride;
+  lv.stride = p.v_stride;
+  lk.last = lv.last = it.k_len - 1;
+  const int n = it.end > it.begin ? (it.end - it.begin + kKeys - 1) / kKeys : 0;
+  const float scale_log2 = p.scale_log2;
+
+  if constexpr (NW == 4) {
+    int pages[L::kLoads] = {};
+    auto step = [&](int s, const uint8_t* kc, const uint8_t* vc, uint8_t* kn, uint8_t* vn) {
+      wait_vm<0>();      // this wave's loads of stage s
+      tm_lds_barrier();  // everyone's; and the reads of stage s - 1 are over
+      const int kb = it.begin + s * kKeys;
+      if (s + 1 < n) {
+        lk.template load<false>(p, kb + kKeys, pages, kn);
+        lv.template load<true>(p, kb + kKeys, pages, vn);
+        lk.look_up(p, kb + 2 * kKeys, pages);
+      }
+      scores<DT, HD>(kc, r);
+      weigh<DT, HD>(scale_log2, kb, kb + kKeys - 1 > full, r);
+      gather<DT, HD>(vc, r);
+    };
+    if (n > 0) {
+      lk.look_up(p, it.begin, pages);
+      lk.template load<false>(p, it.begin, pages, s_k0);
+      lv.template load<true>(p, it.begin, pages, s_v0);
+      lk.look_up(p, it.begin + kKeys, pages);
+    }
+    for (int s = 0; s < n; s += 2) {
+      step(s, s_k0, s_v0, s_k1, s_v1);
+      if (s + 1 < n) step(s + 1, s_k1, s_v1, s_k0, s_v0);
+    }
+  } else if (n > 0) {
+    // Load group g(s), in ring slot s % 3: K of stage s and V of stage s - 1, what
+    // turn M(s) = {O += V P of s - 1, S = K Q of s} reads.  W(s) weighs stage s.
+    // Waves 0-3 take M(s) in turn 2 s and W(s) in turn 2 s + 1, waves 4-7 one turn
+    // later.  In turn 2 s + 1 every wave requests g(s + 2), whose slot the last
+    // wave left in turn 2 s - 1, and at its end waits for its part of g(s + 1).
+    constexpr int kGroup = (PAGED ? 3 : 2) * L::kLoads;  // a request's loads, look-ups included
+    int pages[L::kLoads] = {};   // of K's stage; those of V's are the ones before
+    int vpages[L::kLoads] = {};
+    auto request = [&](int s, uint8_t* kn, uint8_t* vn) {
+      if (s > n) return;
+      const int kb = it.begin + s * kKeys;
+      if (s < n) lk.template load<false>(p, kb, pages, kn);
+      if (s > 0) lv.template load<true>(p, kb - kKeys, vpages, vn);
+      if constexpr (PAGED) {
+#pragma unroll
+        for (int i = 0; i < L::kLoads; ++i) vpages[i] = pages[i];
+        lk.look_up(p, kb + kKeys, pages);
+      }
+    };
+    lk.look_up(p, it.begin, pages);
+    request(0, s_k0, s_v0);
+    request(1, s_k1, s_v1);
+    wait_vm<0>();
+    tm_lds_barrier();
+    auto turn_end = [&]() {
+      __builtin_amdgcn_sched_barrier(0);
+      tm_lds_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    // this wave's part of g(s) is there; g(s + 1) may be under way
+    auto await = [&](int s) {
+      if (s + 1 < n)
+        wait_vm<kGroup>();
+      else
+        wait_vm<0>();
+    };
+    // W(s) and M(s + 1), which reads g(s + 1) at kc, vc; g(s + 2 + LATE) goes to kn, vn.
+    // False after the last.
+    auto early = [&](int s, uint8_t* kc, uint8_t* vc, uint8_t* kn, uint8_t* vn) {
+      const int kb = it.begin + s * kKeys;
+      request(s + 2, kn, vn);
+      weigh<DT, HD>(scale_log2, kb, kb + kKeys - 1 > full, r);
+      await(s + 1);
+      turn_end();
+      gather<DT, HD>(vc, r);
+      if (s + 1 == n) return false;
+      scores<DT, HD>(kc, r);
+      turn_end();
+      return true;
+    };
+    auto late = [&](int s, uint8_t* kc, uint8_t* vc, uint8_t* kn, uint8_t* vn) {
+      const int kb = it.begin + s * kKeys;
+      weigh<DT, HD>(scale_log2, kb, kb + kKeys - 1 > full, r);
+      turn_end();
+      request(s + 3, kn, vn);
+      gather<DT, HD>(vc, r);
+      if (s + 1 == n) return false;
+      scores<DT, HD>(kc, r);
+      await(s + 2);
+      turn_end();
+      return true;
+    };
+    if (wave < 4) {
+      scores<DT, HD>(s_k0, r);
+      turn_end();
+      for (int s = 0;; s += 3) {
+        if (!early(s, s_k1, s_v1, s_k2, s_v2)) break;
+        if (!early(s + 1, s_k2, s_v2, s_k0, s_v0)) break;
+        if (!early(s + 2, s_k0, s_v0, s_k1, s_v1)) break;
+      }
+      turn_end();
+    } else {
+      turn_end();
+      request(2, s_k2, s_v2);
+      scores<DT, HD>(s_k0, r);
+      await(1);
+      turn_end();
+      for (int s = 0;; s += 3) {
+        if (!late(s, s_k1, s_v1, s_k0, s_v0)) break;
+        if (!late(s + 1, s_k2, s_v2, s_k1, s_v1)) break;
+        if (!late(s + 2, s_k0, s_v0, s_k2, s_v2)) break;
+      }
+    }
+  }
+
+  const float l = r.l + __shfl_xor(r.l, 32);
+  if (!ok) return;
+  if (it.slot < 0) {
+    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // NaN stays
+    uint16_t* const o = p.out + (int64_t)(it.q0 + token) * p.out_stride + (int64_t)head * HD +
+                        4 * half;
 #pragma unroll
     for (int ht = 0; ht < HD / 32; ++ht)
 #pragma unroll
-      for (int x = 0; x < 16; ++x) rt[t].o[ht][x] = 0.0f;
-    rt[t].m = -INFINITY;
-    rt[t].l = 0.0f;
-    rt[t].seen = ok ? past + token : -1;
-    qat[t] = ok ? (int64_t)token * p.group + (head - kvhead * p.group) : -1;
-    if (first < all_rows) wave_seen = past + min(it.q_len - 1, (first + 31) / p.group);
-  }
-  // keys that every row of the wave sees: its first row's
-  const int first_row = it.tile * kRows + wave * QT * 32;
-  const int wave_full = first_row + QT * 32 <= all_rows ? past + first_row / p.group : -1;
-
-  Loader<HD, PAGED> ld;
-  ld.k = p.k + (int64_t)kvhead * HD + (PAGED ? 0 : (int64_t)it.k0 * p.k_stride);
-  ld.v = p.v + (int64_t)kvhead * HD + (PAGED ? 0 : (int64_t)it.k0 * p.v_stride);
-  ld.last = it.k_len - 1;
-  const int stages = it.end > it.begin ? (it.end - it.begin + kKeys - 1) / kKeys : 0;
-  if (stages > 0) {
-    ld.look_up(p, it.begin);
-    ld.load(p, it.begin, s_k0, s_v0);
-    ld.look_up(p, it.begin + kKeys);
-  }
-  // stage s in one pair of buffers while stage s + 1 loads into the other
-  auto step = [&](int s, uint8_t* kc, uint8_t* vc, uint8_t* kn, uint8_t* vn) {
-    wait_vm<0>();      // this wave's loads of stage s
-    tm_lds_barrier();  // everyone's; and the reads of stage s - 1 are over
-    const int kb = it.begin + s * kKeys;
-    if (s + 1 < stages) {
-      ld.load(p, kb + kKeys, kn, vn);
-      ld.look_up(p, kb + 2 * kKeys);
-    }
-    if (kb > wave_seen) return;  // nothing of the stage is visible to this wave
-    if (kb + kKeys - 1 <= wave_full && kb + kKeys <= it.end)
-      attend<DT, HD, QT, false>(p, kc, vc, kb, rt);
-    else
-      attend<DT, HD, QT, true>(p, kc, vc, kb, rt);
-  };
-  // a chunk's border hides what lies past it
-#pragma unroll
-  for (int t = 0; t < QT; ++t) rt[t].seen = min(rt[t].seen, it.end - 1);
-  for (int s = 0; s < stages; s += 2) {
-    step(s, s_k0, s_v0, s_k1, s_v1);
-    if (s + 1 < stages) step(s + 1, s_k1, s_v1, s_k0, s_v0);
-  }
-
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const float l = rt[t].l + __shfl_xor(rt[t].l, 32);
-    if (qat[t] < 0) continue;
-    if (it.slot < 0) {
-      const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // NaN stays
-      const int token = (int)(qat[t] / p.group), g = (int)(qat[t] - (int64_t)token * p.group);
-      uint16_t* const o = p.out + (int64_t)(it.q0 + token) * p.out_stride +
-                          (int64_t)(kvhead * p.group + g) * HD + 4 * half;
-#pragma unroll
-      for (int ht = 0; ht < HD / 32; ++ht)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          u32x2_t w;
-          w.x = tm_pack2<DT>(rt[t].o[ht][4 * x] * inv, rt[t].o[ht][4 * x + 1] * inv);
-          w.y = tm_pack2<DT>(rt[t].o[ht][4 * x + 2] * inv, rt[t].o[ht][4 * x + 3] * inv);
-          *reinterpret_cast<u32x2_t*>(o + 32 * ht + 8 * x) = w;
-        }
-    } else {
-      const int r = (wave * QT + t) * 32 + c32;
-      const int64_t slot = ((int64_t)it.slot * p.kvh + kvhead) * kRows + r;
-      float* const o = p.part + slot * HD + 4 * half;
-#pragma unroll
-      for (int ht = 0; ht < HD / 32; ++ht)
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-          *reinterpret_cast<f32x4_t*>(o + 32 * ht + 8 * x) =
-              f32x4_t{rt[t].o[ht][4 * x], rt[t].o[ht][4 * x + 1], rt[t].o[ht][4 * x + 2],
-                      rt[t].o[ht][4 * x + 3]};
-      if (half == 0) {
-        p.stats[slot * 2] = rt[t].m;
-        p.stats[slot * 2 + 1] = l;
+      for (int x = 0; x < 4; ++x) {
+        u32x2_t w;
+        w.x = tm_pack2<DT>(r.o[ht][4 * x] * inv, r.o[ht][4 * x + 1] * inv);
+        w.y = tm_pack2<DT>(r.o[ht][4 * x + 2] * inv, r.o[ht][4 * x + 3] * inv);
+        *reinterpret_cast<u32x2_t*>(o + 32 * ht + 8 * x) = w;
       }
+  } else {
+    const int64_t slot = ((int64_t)it.slot * p.kvh + kvhead) * kRows + wave * 32 + c32;
+    float* const o = p.part + slot * HD + 4 * half;
+#pragma unroll
+    for (int ht = 0; ht < HD / 32; ++ht)
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        *reinterpret_cast<f32x4_t*>(o + 32 * ht + 8 * x) =
+            f32x4_t{r.o[ht][4 * x], r.o[ht][4 * x + 1], r.o[ht][4 * x + 2], r.o[ht][4 * x + 3]};
+    if (half == 0) {
+      p.stats[slot * 2] = r.m;
+      p.stats[slot * 2 + 1] = l;
     }
   }
 }
@@ -517,9 +606,9 @@ void launch_rows(const PromptParams& p, int64_t rows, int64_t blocks, int64_t jo
                  hipStream_t st) {
   const dim3 grid((unsigned)blocks), block(kThreads);
   if (rows == 256)
-    hipLaunchKernelGGL((tm_prompt_attn_kernel<DT, HD, 2, PAGED>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((tm_prompt_attn_kernel<DT, HD, 8, PAGED>), grid, dim3(512), 0, st, p);
   else
-    hipLaunchKernelGGL((tm_prompt_attn_kernel<DT, HD, 1, PAGED>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((tm_prompt_attn_kernel<DT, HD, 4, PAGED>), grid, block, 0, st, p);
   if (joins > 0)
     hipLaunchKernelGGL((tm_prompt_join_kernel<DT, HD>),
                        dim3((unsigned)(joins * p.kvh * rows / 4)), block, 0, st, p, (int)rows);
