@@ -214,25 +214,91 @@ struct Rows {
   int seen;              // the row's last visible key
 };
 
-// S^T = K Q^T of the stage at kt_.
-template <int DT, int HD>
-__device__ __forceinline__ void scores(const uint8_t* kt_, Rows<HD>& r) {
-  typedef Shape<HD> S;
-  const int lane = threadIdx.x & 63, half = lane >> 5, c32 = lane & 31;
+// Fragments of k-steps 2 i and 2 i + 1 of the K stage at kt_.
+template <int HD>
+__device__ __forceinline__ void read_k(const uint8_t* kt_, int at, int i, u32x4_t (&f)[4]) {
 #pragma unroll
-  for (int kt = 0; kt < 2; ++kt)
+  for (int j = 0; j < 4; ++j)
+    f[j] = *reinterpret_cast<const u32x4_t*>(kt_ + 32 * (j & 1) * Shape<HD>::kRow +
+                                             (at ^ (32 * (2 * i + (j >> 1)))));
+}
+// Byte offset of chunk `half` of row l % 32 of K; k-step ks is at ^ 32 ks.
+template <int HD>
+__device__ __forceinline__ int k_offset() {
+  const int lane = threadIdx.x & 63, c32 = lane & 31;
+  return fresh(c32 * Shape<HD>::kRow + ((lane >> 5) ^ Shape<HD>::swz_k(c32)) * 16);
+}
+// Fragments of the 16 keys from 16 s on of the V stage at vt.
+template <int HD>
+__device__ __forceinline__ void read_v(const uint8_t* vt, int lo, int hi, int s,
+                                       u32x4_t (&f)[HD / 32]) {
 #pragma unroll
-    for (int x = 0; x < 16; ++x) r.sc[kt][x] = 0.0f;
-  // chunk 2 ks + half of row c32 (+ 32 kt)
-  const int at = fresh(c32 * S::kRow + (half ^ S::swz_k(c32)) * 16);
+  for (int ht = 0; ht < HD / 32; ++ht) {
+    const u32x2_t a = read_tr(vt + 16 * s * Shape<HD>::kRow + (lo ^ (64 * ht)));
+    const u32x2_t b = read_tr(vt + 16 * s * Shape<HD>::kRow + (hi ^ (64 * ht)));
+    f[ht] = u32x4_t{a.x, a.y, b.x, b.y};
+  }
+}
+
+// One product, then `reads` LDS reads, `n` times: each product covers the reads of
+// the step behind it.
+template <int N, int READS>
+__device__ __forceinline__ void interleave() {
 #pragma unroll
-  for (int ks = 0; ks < HD / 16; ++ks)
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+  }
+}
+
+// O^T += V^T P^T of the stage at vt (G), then S^T = K Q^T of the stage at kt_ (S).  A
+// step's fragments are read between the products of the step before it.
+template <int DT, int HD, bool G, bool S>
+__device__ __forceinline__ void products(const uint8_t* vt, const uint8_t* kt_, Rows<HD>& r) {
+  constexpr int HT = HD / 32, KP = HD / 32;  // output tiles; pairs of k-steps
+  u32x4_t kf[2][4];
+  int at = 0;
+  if constexpr (S) at = k_offset<HD>();
+  __builtin_amdgcn_sched_barrier(0);
+  if constexpr (G) {
+    u32x4_t vf[2][HT];
+    int lo, hi;
+    v_offsets<HD>(lo, hi);
+    lo = fresh(lo);
+    hi = fresh(hi);
+    read_v<HD>(vt, lo, hi, 0, vf[0]);
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      const u32x4_t a =
-          *reinterpret_cast<const u32x4_t*>(kt_ + 32 * kt * S::kRow + (at ^ (32 * ks)));
-      r.sc[kt] = mfma32<DT>(a, r.q[ks], r.sc[kt]);
+    for (int s = 0; s < 4; ++s) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (s < 3)
+        read_v<HD>(vt, lo, hi, s + 1, vf[(s + 1) & 1]);
+      else if (S)
+        read_k<HD>(kt_, at, 0, kf[0]);
+#pragma unroll
+      for (int ht = 0; ht < HT; ++ht) r.o[ht] = mfma32<DT>(vf[s & 1][ht], r.pw[s], r.o[ht]);
+      if (s < 3)
+        interleave<HT, 2>();
+      else if (S)
+        interleave<HT, 4 / HT>();
     }
+  } else {
+    read_k<HD>(kt_, at, 0, kf[0]);
+  }
+  if constexpr (S) {
+#pragma unroll
+    for (int i = 0; i < KP; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (i + 1 < KP) read_k<HD>(kt_, at, i + 1, kf[(i + 1) & 1]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x16_t zero = {};
+        r.sc[j & 1] = mfma32<DT>(kf[i & 1][j], r.q[2 * i + (j >> 1)],
+                                 i == 0 && j < 2 ? zero : r.sc[j & 1]);
+      }
+      if (i + 1 < KP) interleave<4, 1>();
+    }
+  }
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // The weights of the stage's keys kb .. against the running maximum.  mask: some key
@@ -270,26 +336,10 @@ __device__ __forceinline__ void weigh(float scale_log2, int kb, bool mask, Rows<
       const int x = 8 * (s & 1) + 2 * j;
       const float e0 = __builtin_amdgcn_exp2f(fmaf(r.sc[s >> 1][x], scale_log2, base));
       const float e1 = __builtin_amdgcn_exp2f(fmaf(r.sc[s >> 1][x + 1], scale_log2, base));
-      const uint32_t w = tm_pack2<DT>(e0, e1);
+      // made here, not moved into the products
+      const uint32_t w = (uint32_t)fresh((int)tm_pack2<DT>(e0, e1));
       r.l = add_pair<DT>(w, r.l);
       r.pw[s][j] = w;
-    }
-}
-
-// O^T += V^T P^T of the stage at vt.
-template <int DT, int HD>
-__device__ __forceinline__ void gather(const uint8_t* vt, Rows<HD>& r) {
-  int lo, hi;
-  v_offsets<HD>(lo, hi);
-  lo = fresh(lo);
-  hi = fresh(hi);
-#pragma unroll
-  for (int s = 0; s < 4; ++s)
-#pragma unroll
-    for (int ht = 0; ht < HD / 32; ++ht) {
-      const u32x2_t a = read_tr(vt + 16 * s * Shape<HD>::kRow + (lo ^ (64 * ht)));
-      const u32x2_t b = read_tr(vt + 16 * s * Shape<HD>::kRow + (hi ^ (64 * ht)));
-      r.o[ht] = mfma32<DT>(u32x4_t{a.x, a.y, b.x, b.y}, r.pw[s], r.o[ht]);
     }
 }
 
@@ -381,9 +431,9 @@ __global__ void __launch_bounds__(64 * NW, 2) tm_prompt_attn_kernel(PromptParams
         lv.template load<true>(p, kb + kKeys, pages, vn);
         lk.look_up(p, kb + 2 * kKeys, pages);
       }
-      scores<DT, HD>(kc, r);
+      products<DT, HD, false, true>(vc, kc, r);
       weigh<DT, HD>(scale_log2, kb, kb + kKeys - 1 > full, r);
-      gather<DT, HD>(vc, r);
+      products<DT, HD, true, false>(vc, kc, r);
     };
     if (n > 0) {
       lk.look_up(p, it.begin, pages);
@@ -433,51 +483,50 @@ __global__ void __launch_bounds__(64 * NW, 2) tm_prompt_attn_kernel(PromptParams
         wait_vm<0>();
     };
     // W(s) and M(s + 1), which reads g(s + 1) at kc, vc; g(s + 2 + LATE) goes to kn, vn.
-    // False after the last.
+    // (the last one's scores, of a stage that is not there, are not used)
     auto early = [&](int s, uint8_t* kc, uint8_t* vc, uint8_t* kn, uint8_t* vn) {
       const int kb = it.begin + s * kKeys;
       request(s + 2, kn, vn);
       weigh<DT, HD>(scale_log2, kb, kb + kKeys - 1 > full, r);
       await(s + 1);
       turn_end();
-      gather<DT, HD>(vc, r);
-      if (s + 1 == n) return false;
-      scores<DT, HD>(kc, r);
+      products<DT, HD, true, true>(vc, kc, r);
       turn_end();
-      return true;
     };
     auto late = [&](int s, uint8_t* kc, uint8_t* vc, uint8_t* kn, uint8_t* vn) {
       const int kb = it.begin + s * kKeys;
       weigh<DT, HD>(scale_log2, kb, kb + kKeys - 1 > full, r);
       turn_end();
       request(s + 3, kn, vn);
-      gather<DT, HD>(vc, r);
-      if (s + 1 == n) return false;
-      scores<DT, HD>(kc, r);
+      products<DT, HD, true, true>(vc, kc, r);
       await(s + 2);
       turn_end();
-      return true;
     };
+    int s = 0;
     if (wave < 4) {
-      scores<DT, HD>(s_k0, r);
+      products<DT, HD, false, true>(s_v0, s_k0, r);
       turn_end();
-      for (int s = 0;; s += 3) {
-        if (!early(s, s_k1, s_v1, s_k2, s_v2)) break;
-        if (!early(s + 1, s_k2, s_v2, s_k0, s_v0)) break;
-        if (!early(s + 2, s_k0, s_v0, s_k1, s_v1)) break;
+      for (; s + 3 <= n; s += 3) {
+        early(s, s_k1, s_v1, s_k2, s_v2);
+        early(s + 1, s_k2, s_v2, s_k0, s_v0);
+        early(s + 2, s_k0, s_v0, s_k1, s_v1);
       }
+      if (s < n) early(s, s_k1, s_v1, s_k2, s_v2);
+      if (s + 1 < n) early(s + 1, s_k2, s_v2, s_k0, s_v0);
       turn_end();
     } else {
       turn_end();
       request(2, s_k2, s_v2);
-      scores<DT, HD>(s_k0, r);
+      products<DT, HD, false, true>(s_v0, s_k0, r);
       await(1);
       turn_end();
-      for (int s = 0;; s += 3) {
-        if (!late(s, s_k1, s_v1, s_k0, s_v0)) break;
-        if (!late(s + 1, s_k2, s_v2, s_k1, s_v1)) break;
-        if (!late(s + 2, s_k0, s_v0, s_k2, s_v2)) break;
+      for (; s + 3 <= n; s += 3) {
+        late(s, s_k1, s_v1, s_k0, s_v0);
+        late(s + 1, s_k2, s_v2, s_k1, s_v1);
+        late(s + 2, s_k0, s_v0, s_k2, s_v2);
       }
+      if (s < n) late(s, s_k1, s_v1, s_k0, s_v0);
+      if (s + 1 < n) late(s + 1, s_k2, s_v2, s_k1, s_v1);
     }
   }
 
