@@ -131,49 +131,71 @@ struct Shape {
   }
 };
 
-// Keys kb .. kb + 63 of K or V into LDS, by NW waves.  Keys past the sequence's last
-// are that one again: their scores are masked.
-template <int HD, bool PAGED, int NW>
+// Stages of 64 keys of K or V into LDS, by NW waves, one after the other.  Keys past
+// the sequence's last are that one again: their scores are masked.
+template <int HD, bool PAGED, int NW, bool V>
 struct Loader {
   typedef Shape<HD> S;
-  static constexpr int kLoads = S::kTile / (1024 * NW);  // loads of a wave per tile
-  const uint16_t* base;
-  int64_t stride;    // of a key, or of a page's slot
-  int last;
+  static constexpr int kLoads = S::kTile / (1024 * NW);  // loads of a wave per stage
+  const uint16_t* at;   // the next stage's first row (paged: the cache)
+  int64_t stage_stride;
+  int left;             // the sequence's last key from the next stage's first on
+  int stride;           // of a key, or of a page's slot
+  int lane_off[kLoads]; // of this lane's piece from the stage's first row
+  int pages[kLoads];    // the next stage's pages, looked up a stage ahead
+  int first;            // the next stage's first key (paged)
 
   __device__ __forceinline__ int key_in(int i) const {  // within the stage
     return ((int)(threadIdx.x >> 6) * kLoads + i) * S::kKeysPerLoad +
            (int)(threadIdx.x & 63) / S::kChunks;
   }
-  // Pages of the keys kb .. (paged): looked up a stage before they are loaded.
-  __device__ __forceinline__ void look_up(const PromptParams& p, int kb, int (&pages)[kLoads]) const {
+  __device__ __forceinline__ int chunk_off(int i) const {
+    const int j = key_in(i);
+    return (((int)threadIdx.x & (S::kChunks - 1)) ^ (V ? S::swz_v(j) : S::swz_k(j))) * 8;
+  }
+  __device__ __forceinline__ void look_up(const PromptParams& p) {
     if constexpr (PAGED) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i)
-        pages[i] = p.table[min(kb + key_in(i), last) >> p.page_shift];
+        pages[i] = p.table[(first + min(key_in(i), left)) >> p.page_shift];
     }
   }
-  template <bool V>
-  __device__ __forceinline__ void load(const PromptParams& p, int kb, const int (&pages)[kLoads],
-                                       uint8_t* tile) const {
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int chunk = (int)threadIdx.x & (S::kChunks - 1);
+  // From key `begin` on of the sequence whose first row is `row0` and last key `last`.
+  __device__ __forceinline__ void start(const PromptParams& p, const uint16_t* row0,
+                                        int64_t row_stride, int begin, int last) {
+    at = PAGED ? row0 : row0 + (int64_t)begin * row_stride;
+    stage_stride = kKeys * row_stride;
+    stride = (int)row_stride;
+    left = last - begin;
+    first = begin;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int j = key_in(i);
-      const int c = (chunk ^ (V ? S::swz_v(j) : S::swz_k(j))) * 8;
-      const uint16_t* from;
-      if constexpr (PAGED) {
-        const int key = min(kb + j, last);
-        from = base + ((int64_t)min(max(pages[i], 0), p.cache_pages - 1) * p.stride_page +
-                       (int64_t)(key & ((1 << p.page_shift) - 1)) * stride + c);
-      } else {
-        // the stage's first row is wave-uniform, a lane's offset from it fits 32 bits
-        const uint16_t* const row0 = base + (int64_t)kb * stride;
-        from = row0 + (uint32_t)(min(j, last - kb) * (int)stride + c);
+    for (int i = 0; i < kLoads; ++i) lane_off[i] = key_in(i) * stride + chunk_off(i);
+    look_up(p);
+  }
+  __device__ __forceinline__ void load(const PromptParams& p, uint8_t* tile) {
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    if constexpr (PAGED) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int slot = (first + min(key_in(i), left)) & ((1 << p.page_shift) - 1);
+        const int64_t o = (int64_t)min(max(pages[i], 0), p.cache_pages - 1) * p.stride_page +
+                          (int64_t)slot * stride + chunk_off(i);
+        __builtin_amdgcn_global_load_lds((glb_void*)(at + o),
+                                         (lds_void*)(tile + (wave * kLoads + i) * 1024), 16, 0, 0);
       }
-      __builtin_amdgcn_global_load_lds((glb_void*)from,
-                                       (lds_void*)(tile + (wave * kLoads + i) * 1024), 16, 0, 0);
+      first += kKeys;
+      left -= kKeys;
+      look_up(p);
+    } else {
+      const bool whole = left >= kKeys - 1;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int o = whole ? lane_off[i] : min(key_in(i), left) * stride + chunk_off(i);
+        __builtin_amdgcn_global_load_lds((glb_void*)(at + (uint32_t)o),
+                                         (lds_void*)(tile + (wave * kLoads + i) * 1024), 16, 0, 0);
+      }
+      at += stage_stride;
+      left -= kKeys;
     }
   }
 };
@@ -313,10 +335,10 @@ __device__ __forceinline__ void weigh(float scale_log2, int kb, bool mask, Rows<
       for (int x = 0; x < 16; ++x)
         r.sc[kt][x] = 32 * kt + 8 * (x >> 2) + (x & 3) <= left ? r.sc[kt][x] : -INFINITY;
   }
-  float mx = fmaxf(r.sc[0][0], r.sc[1][0]);
+  float mx[2] = {fmaxf(r.sc[0][0], r.sc[1][0]), fmaxf(r.sc[0][1], r.sc[1][1])};
 #pragma unroll
-  for (int x = 1; x < 16; ++x) mx = fmaxf(fmaxf(mx, r.sc[0][x]), r.sc[1][x]);
-  const float cand = max_halves(mx) * scale_log2;
+  for (int x = 2; x < 16; ++x) mx[x & 1] = fmaxf(fmaxf(mx[x & 1], r.sc[0][x]), r.sc[1][x]);
+  const float cand = max_halves(fmaxf(mx[0], mx[1])) * scale_log2;
   const bool bump = cand > r.m + 8.0f;
   if (__any(bump)) {
     const float m = bump ? cand : r.m;
@@ -329,6 +351,7 @@ __device__ __forceinline__ void weigh(float scale_log2, int kb, bool mask, Rows<
     r.m = m;
   }
   const float base = r.m == -INFINITY ? 0.0f : -r.m;
+  float sum[2] = {0.0f, 0.0f};
 #pragma unroll
   for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -338,9 +361,10 @@ __device__ __forceinline__ void weigh(float scale_log2, int kb, bool mask, Rows<
       const float e1 = __builtin_amdgcn_exp2f(fmaf(r.sc[s >> 1][x + 1], scale_log2, base));
       // made here, not moved into the products
       const uint32_t w = (uint32_t)fresh((int)tm_pack2<DT>(e0, e1));
-      r.l = add_pair<DT>(w, r.l);
+      sum[j & 1] = add_pair<DT>(w, sum[j & 1]);
       r.pw[s][j] = w;
     }
+  r.l += sum[0] + sum[1];
 }
 
 // What a workgroup works on.
@@ -365,7 +389,6 @@ __device__ __forceinline__ Item item_of(const PromptParams& p, int at, int rows)
 template <int DT, int HD, int NW, bool PAGED>
 __global__ void __launch_bounds__(64 * NW, 2) tm_prompt_attn_kernel(PromptParams p) {
   typedef Shape<HD> S;
-  typedef Loader<HD, PAGED, NW> L;
   constexpr int kRows = 32 * NW;
   constexpr int kRing = NW == 8 ? 3 : 2;
   __shared__ __attribute__((aligned(1024))) uint8_t s_k0[S::kTile];
@@ -411,35 +434,33 @@ __global__ void __launch_bounds__(64 * NW, 2) tm_prompt_attn_kernel(PromptParams
   // keys up to this one are seen by every row of the wave
   const int full = min(first + 32 <= all_rows ? past + first / p.group : -1, it.end - 1);
 
-  L lk, lv;
-  lk.base = p.k + (int64_t)kvhead * HD + (PAGED ? 0 : (int64_t)it.k0 * p.k_stride);
-  lv.base = p.v + (int64_t)kvhead * HD + (PAGED ? 0 : (int64_t)it.k0 * p.v_stride);
-  lk.stride = p.k_stride;
-  lv.stride = p.v_stride;
-  lk.last = lv.last = it.k_len - 1;
+  Loader<HD, PAGED, NW, false> lk;
+  Loader<HD, PAGED, NW, true> lv;
   const int n = it.end > it.begin ? (it.end - it.begin + kKeys - 1) / kKeys : 0;
   const float scale_log2 = p.scale_log2;
+  if (n > 0) {
+    const int64_t k0 = (int64_t)kvhead * HD + (PAGED ? 0 : (int64_t)it.k0 * p.k_stride);
+    const int64_t v0 = (int64_t)kvhead * HD + (PAGED ? 0 : (int64_t)it.k0 * p.v_stride);
+    lk.start(p, p.k + k0, p.k_stride, it.begin, it.k_len - 1);
+    lv.start(p, p.v + v0, p.v_stride, it.begin, it.k_len - 1);
+  }
 
   if constexpr (NW == 4) {
-    int pages[L::kLoads] = {};
     auto step = [&](int s, const uint8_t* kc, const uint8_t* vc, uint8_t* kn, uint8_t* vn) {
       wait_vm<0>();      // this wave's loads of stage s
       tm_lds_barrier();  // everyone's; and the reads of stage s - 1 are over
       const int kb = it.begin + s * kKeys;
       if (s + 1 < n) {
-        lk.template load<false>(p, kb + kKeys, pages, kn);
-        lv.template load<true>(p, kb + kKeys, pages, vn);
-        lk.look_up(p, kb + 2 * kKeys, pages);
+        lk.load(p, kn);
+        lv.load(p, vn);
       }
       products<DT, HD, false, true>(vc, kc, r);
       weigh<DT, HD>(scale_log2, kb, kb + kKeys - 1 > full, r);
       products<DT, HD, true, false>(vc, kc, r);
     };
     if (n > 0) {
-      lk.look_up(p, it.begin, pages);
-      lk.template load<false>(p, it.begin, pages, s_k0);
-      lv.template load<true>(p, it.begin, pages, s_v0);
-      lk.look_up(p, it.begin + kKeys, pages);
+      lk.load(p, s_k0);
+      lv.load(p, s_v0);
     }
     for (int s = 0; s < n; s += 2) {
       step(s, s_k0, s_v0, s_k1, s_v1);
@@ -451,21 +472,13 @@ __global__ void __launch_bounds__(64 * NW, 2) tm_prompt_attn_kernel(PromptParams
     // Waves 0-3 take M(s) in turn 2 s and W(s) in turn 2 s + 1, waves 4-7 one turn
     // later.  In turn 2 s + 1 every wave requests g(s + 2), whose slot the last
     // wave left in turn 2 s - 1, and at its end waits for its part of g(s + 1).
-    constexpr int kGroup = (PAGED ? 3 : 2) * L::kLoads;  // a request's loads, look-ups included
-    int pages[L::kLoads] = {};   // of K's stage; those of V's are the ones before
-    int vpages[L::kLoads] = {};
+    // a request's loads, look-ups of pages included
+    constexpr int kGroup = (PAGED ? 4 : 2) * decltype(lk)::kLoads;
     auto request = [&](int s, uint8_t* kn, uint8_t* vn) {
       if (s > n) return;
-      const int kb = it.begin + s * kKeys;
-      if (s < n) lk.template load<false>(p, kb, pages, kn);
-      if (s > 0) lv.template load<true>(p, kb - kKeys, vpages, vn);
-      if constexpr (PAGED) {
-#pragma unroll
-        for (int i = 0; i < L::kLoads; ++i) vpages[i] = pages[i];
-        lk.look_up(p, kb + kKeys, pages);
-      }
+      if (s < n) lk.load(p, kn);
+      if (s > 0) lv.load(p, vn);
     };
-    lk.look_up(p, it.begin, pages);
     request(0, s_k0, s_v0);
     request(1, s_k1, s_v1);
     wait_vm<0>();
@@ -606,6 +619,7 @@ __global__ void __launch_bounds__(kThreads) tm_prompt_join_kernel(PromptParams p
 
 // ------------------------------------------------------------------- host --
 
+constexpr int64_t kMaxStride = 1 << 24;  // of a key's row: 64 of them from 32-bit offsets
 constexpr int64_t kSlotsPerCU = 2;   // workgroups of 128 rows a CU holds
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -777,7 +791,8 @@ extern "C" int tm_prompt_attention(const void* q, int64_t q_stride, const void* 
       num_items * kvh > INT32_MAX || num_joins * kvh * tile_rows / 4 > INT32_MAX ||
       num_slots > INT32_MAX)
     return TM_ERR_SHAPE;
-  if (q_stride < Hq * hd || out_stride < Hq * hd || k_stride < kvh * hd || v_stride < kvh * hd)
+  if (q_stride < Hq * hd || out_stride < Hq * hd || k_stride < kvh * hd || v_stride < kvh * hd ||
+      k_stride > kMaxStride || v_stride > kMaxStride)
     return TM_ERR_SHAPE;
   if (num_slots * kvh * tile_rows * (hd + 2) * 4 > workspace_bytes) return TM_ERR_SHAPE;
   if (num_items == 0) return TM_OK;
@@ -840,7 +855,7 @@ extern "C" int tm_prompt_attention_cached(const void* q, int64_t q_stride, int64
   if (T == 0) return TM_OK;
   if (cache_pages < 1 || ceil_div(seq_len, page_size) > num_table_pages) return TM_ERR_SHAPE;
   if ((T > 1 && (q_stride < Hq * hd || out_stride < Hq * hd)) || stride_slot < kvh * hd ||
-      stride_page < page_size * stride_slot)
+      stride_slot > kMaxStride || stride_page < page_size * stride_slot)
     return TM_ERR_SHAPE;
   if (o.bytes > workspace_bytes || o.tiles * o.chunks * kvh > INT32_MAX ||
       o.tiles * kvh * o.rows / 4 > INT32_MAX)
