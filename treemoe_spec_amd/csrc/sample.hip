@@ -21,8 +21,13 @@
 // step, then within the step over the 64-bit keys (ordered bits of l, inverted
 // index), all distinct, in 2048 steps of the remaining range at a time.
 //
-// One workgroup of 16 waves takes a row.  Up to 32768 logits it holds them in
-// registers between its passes, above that it reads them again through L2.
+// One workgroup of 16 waves takes a row, up to 32768 logits in registers, more read
+// again through L2.  A row is passed over two or three times: for its largest logit,
+// for the first histogram, and to collect what lies above the cut's step (or min-p's
+// bound) into a list in LDS, in index order.  What follows runs on the list: a few
+// logits a thread where top-k or top-p leave few, the row itself where they leave
+// more than the list holds.  The 64-bit exponential of a whole row, which top-p
+// without top-k and plain sampling need once, is what costs most.
 #include <cmath>
 
 #include "tm_vec.h"
@@ -34,6 +39,7 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kRound = kThreads * 4;            // logits of one round: 4 consecutive a thread
 constexpr int kRegRounds = 8;                   // rounds held in registers
 constexpr int kBins = 2048;
+constexpr int kList = 8192;                     // logits that the list holds
 constexpr int kMaxRounds = TM_MAX_SAMPLE_VOCAB / kRound;
 constexpr float kSpan = 31.25f;                 // (l_max - l) / temperature of the last bin's end
 constexpr double kUnit = 17592186044416.0;      // 2^44
@@ -57,7 +63,7 @@ struct Row {
   float top;       // largest logit
   float inv_t;     // 1 / temperature
   double inv_y;    // 32 log2(e) / temperature
-  const double* powers;  // 2^(j / 32), j < 32
+  const double* powers;  // 2^(44 + j / 32), j < 32
 };
 
 // Ordered bits: larger floats have larger keys.
@@ -69,31 +75,43 @@ __device__ __forceinline__ uint64_t key_of(float l, int index) {
   return ((uint64_t)order_bits(l) << 32) | (uint32_t)~index;
 }
 
-// (l_max - l) / temperature in fp32, monotone in l; a logit is a candidate where
-// it is below kSpan.
-__device__ __forceinline__ float depth_of(const Row& r, float l) {
-  return l == r.top ? 0.0f : (r.top - l) * r.inv_t;
+__device__ __forceinline__ float logit_of(uint64_t key) {
+  const uint32_t o = (uint32_t)(key >> 32);
+  return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
+}
+__device__ __forceinline__ int index_of(uint64_t key) { return (int)~(uint32_t)key; }
+
+// The step of a logit, from (l_max - l) / temperature in fp32, monotone in l; -1 for
+// one too far below to weigh anything.
+__device__ __forceinline__ int step_of(const Row& r, float l) {
+  const float d = l == r.top ? 0.0f : (r.top - l) * r.inv_t;
+  return d < kSpan ? min(kBins - 1, (int)(d * ((float)kBins / kSpan))) : -1;
 }
 
-// The weight of a candidate in 64 bits: e^z = 2^(k / 32) e^r with k the nearest integer
-// to 32 z log2(e), 2^(k % 32 / 32) from a table and e^r, |r| <= ln 2 / 64, from its
-// Taylor polynomial of degree 5 (truncation below 3e-15).  A logit equal to the
-// largest weighs 1 (also infinities).
+// 2^44 times the weight of a logit with a step, in 64 bits: e^z = 2^(k / 32) e^x with k
+// the nearest integer to 32 z log2(e), 2^(44 + k % 32 / 32) from a table and e^x,
+// |x| <= ln 2 / 64, from its Taylor polynomial of degree 5 (truncation below 3e-15).
+// A logit equal to the largest weighs 1 (also infinities).
 __device__ __forceinline__ double weight_of(const Row& r, float l) {
+  constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to integers
   const double y = ((double)l - (double)r.top) * r.inv_y;  // 32 z log2(e), > -1443
-  const double kd = rint(y);
-  const double x = (y - kd) * 0.021660849392498290;  // ln 2 / 32
+  const double t = y + kMagic;
+  const double x = (y - (t - kMagic)) * 0.021660849392498290;  // ln 2 / 32
   double q = fma(x, 8.3333333333333333e-3, 4.1666666666666667e-2);
   q = fma(q, x, 1.6666666666666667e-1);
   q = fma(q, x, 0.5);
   q = fma(q, x, 1.0);
   q = fma(q, x, 1.0);
-  const int k = (int)kd;
-  const double w = q * r.powers[k & 31];
-  const uint64_t bits = (uint64_t)__double_as_longlong(w) + ((uint64_t)(int64_t)(k >> 5) << 52);
-  return l == r.top ? 1.0 : __longlong_as_double((long long)bits);
+  const int k = (int)(uint32_t)(uint64_t)__double_as_longlong(t);
+  const uint64_t w = (uint64_t)__double_as_longlong(q * r.powers[k & 31]);
+  const uint32_t hi = (uint32_t)(w >> 32) + ((uint32_t)(k >> 5) << 20);
+  const double v = __longlong_as_double((long long)(((uint64_t)hi << 32) | (uint32_t)w));
+  return l == r.top ? kUnit : v;
 }
-__device__ __forceinline__ uint64_t fixed_of(double w) { return (uint64_t)(w * kUnit + 0.5); }
+// The weight as an integer, to the nearest: the low bits of 2^52 + w.
+__device__ __forceinline__ uint64_t fixed_of(double w) {
+  return (uint64_t)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
+}
 
 __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int m) {
   const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)v, m);
@@ -123,6 +141,7 @@ __device__ __forceinline__ uint64_t sum_wave(uint64_t v) {
 struct Shared {
   uint64_t weight[kBins];
   uint32_t count[kBins];
+  uint64_t list[kList];
   uint64_t seg[kMaxRounds * kWaves];
   uint64_t wave[kWaves];
   double powers[32];
@@ -131,6 +150,25 @@ struct Shared {
   int found;
 };
 
+// Exclusive sum of v over the workgroup's threads in order, and the total.
+__device__ __forceinline__ uint64_t scan_block(Shared& s, uint64_t v, uint64_t* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint64_t incl = scan_wave(v, lane);
+  __syncthreads();  // s.wave is free
+  if (lane == 63) s.wave[wave] = incl;
+  __syncthreads();
+  uint64_t at = incl - v, sum = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const uint64_t x = s.wave[w];
+    if (w < wave) at += x;
+    sum += x;
+  }
+  *total = sum;
+  return at;
+}
+
+// A row of logits.
 template <int DT, bool REG>
 struct Logits {
   float v[REG ? kRegRounds : 1][4];
@@ -158,23 +196,71 @@ struct Logits {
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] = i + e < vocab ? tm_load1<DT>(row, i + e) : -INFINITY;
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = x[e] == x[e] ? x[e] + 0.0f : -INFINITY;
   }
-  // f(round, first index, 4 logits) over the thread's logits
-  template <class F>
-  __device__ __forceinline__ void each(F&& f) const {
+  static __device__ __forceinline__ float clean(float x) { return x == x ? x + 0.0f : -INFINITY; }
+  __device__ __forceinline__ void hold() {
     if constexpr (REG) {
 #pragma unroll
       for (int r = 0; r < kRegRounds; ++r)
-        if (r < rounds) f(r, r * kRound + (int)threadIdx.x * 4, v[r]);
-    } else {
-      for (int r = 0; r < rounds; ++r) {
+        if (r < rounds) fetch(r, v[r]);
+#pragma unroll
+      for (int r = 0; r < kRegRounds; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[r][e] = r < rounds ? clean(v[r][e]) : -INFINITY;
+    }
+  }
+  // f(round, first index, 4 logits) over the thread's logits
+  template <class F>
+  __device__ __forceinline__ void rounds_of(F&& f) const {
+    if constexpr (REG) {
+#pragma unroll
+      for (int r = 0; r < kRegRounds; ++r) {
+        // taken as new values, and one round at a time, so that what one pass makes of
+        // them does not stay in registers for the next
         float x[4];
-        fetch(r, x);
-        f(r, r * kRound + (int)threadIdx.x * 4, x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = v[r][e];
+          asm volatile("" : "+v"(x[e]));
+        }
+        if (r < rounds) f(r, r * kRound + (int)threadIdx.x * 4, x);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+      constexpr int A = 4;  // rounds read ahead
+      for (int r0 = 0; r0 < rounds; r0 += A) {
+        float x[A][4];
+#pragma unroll
+        for (int a = 0; a < A; ++a)
+          if (r0 + a < rounds) fetch(r0 + a, x[a]);
+#pragma unroll
+        for (int a = 0; a < A; ++a)
+          if (r0 + a < rounds) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[a][e] = clean(x[a][e]);
+            f(r0 + a, (r0 + a) * kRound + (int)threadIdx.x * 4, x[a]);
+          }
       }
     }
+  }
+  // f(logit, key) over the thread's logits
+  template <class F>
+  __device__ __forceinline__ void each(F&& f) const {
+    rounds_of([&](int, int i, const float (&x)[4]) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f(x[e], key_of(x[e], i + e));
+    });
+  }
+};
+
+// The list in LDS: n keys in index order, `per` consecutive ones a thread.
+struct List {
+  const uint64_t* keys;
+  int n, per;
+  template <class F>
+  __device__ __forceinline__ void each(F&& f) const {
+    const int end = min(n, ((int)threadIdx.x + 1) * per);
+    for (int i = (int)threadIdx.x * per; i < end; ++i) f(logit_of(keys[i]), keys[i]);
   }
 };
 
@@ -192,20 +278,31 @@ __device__ __forceinline__ void clear_bins(Shared& s) {
   __syncthreads();
 }
 
-// The bin at which the running measure over bins 0, 1, ... reaches `target` (>= 1):
-// s.found (-1 where it does not), s.before the measure in front of it, s.in_bin its
-// elements.
 template <bool WEIGHT>
-__device__ __forceinline__ void find_bin(Shared& s, uint64_t target) {
+__device__ __forceinline__ void add_to_bin(Shared& s, const Row& row, int bin, float l) {
+  atomicAdd(&s.count[bin], 1u);
+  if constexpr (WEIGHT)
+    atomicAdd((unsigned long long*)&s.weight[bin],
+              (unsigned long long)fixed_of(weight_of(row, l)));
+}
+
+// The bin at which the running measure over bins 0, 1, ... reaches a target (a number
+// of elements, or the share `top_p` of the weight of all, at least 1): s.found (-1 where it
+// does not), s.before the measure in front of it, s.in_bin its elements.  Returns the
+// target.
+template <bool WEIGHT>
+__device__ __forceinline__ uint64_t find_bin(Shared& s, uint64_t target, double top_p) {
   __syncthreads();  // the bins are filled
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int t = threadIdx.x;
   const uint64_t a = WEIGHT ? s.weight[2 * t] : (uint64_t)s.count[2 * t];
   const uint64_t b = WEIGHT ? s.weight[2 * t + 1] : (uint64_t)s.count[2 * t + 1];
-  const uint64_t incl = scan_wave(a + b, lane);
-  if (lane == 63) s.wave[wave] = incl;
-  __syncthreads();
-  uint64_t at = incl - (a + b);
-  for (int w = 0; w < wave; ++w) at += s.wave[w];
+  uint64_t total;
+  const uint64_t at = scan_block(s, a + b, &total);
+  if (target == 0) {
+    const double want = ceil(top_p * (double)total);
+    target = want > 1.0 ? (uint64_t)want : 1;
+    target = target < total ? target : total;
+  }
   if (at < target && at + a + b >= target) {  // one thread at most
     const bool second = at + a < target;
     s.found = 2 * t + (second ? 1 : 0);
@@ -213,42 +310,20 @@ __device__ __forceinline__ void find_bin(Shared& s, uint64_t target) {
     s.in_bin = s.count[2 * t + (second ? 1 : 0)];
   }
   __syncthreads();
+  return target;
 }
 
-// The key of the element at which the running measure of the candidates with
-// key >= cut reaches `target`; 0 where it does not (everything stays).
+// The key of the element of step `step` at which the running measure over the step's
+// elements with key >= cut reaches `target`.
 template <bool WEIGHT, class L>
-__device__ uint64_t cut_at(Shared& s, const L& lg, const Row& row, uint64_t cut,
-                           uint64_t target) {
-  constexpr float kScale = (float)kBins / kSpan;
+__device__ uint64_t cut_in_step(Shared& s, const L& src, const Row& row, uint64_t cut, int step,
+                                uint64_t target) {
   clear_bins(s);
-  lg.each([&](int, int i, const float (&x)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float d = depth_of(row, x[e]);
-      if (!(d < kSpan) || key_of(x[e], i + e) < cut) continue;
-      const int bin = min(kBins - 1, (int)(d * kScale));
-      atomicAdd(&s.count[bin], 1u);
-      if constexpr (WEIGHT)
-        atomicAdd((unsigned long long*)&s.weight[bin],
-                  (unsigned long long)fixed_of(weight_of(row, x[e])));
-    }
-  });
-  find_bin<WEIGHT>(s, target);
-  const int step = s.found;
-  if (step < 0) return 0;
-  target -= s.before;
-  // the keys of the step's elements
   uint64_t lo = ~0ull, hi = 0;
-  lg.each([&](int, int i, const float (&x)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float d = depth_of(row, x[e]);
-      const uint64_t key = key_of(x[e], i + e);
-      if (!(d < kSpan) || key < cut || min(kBins - 1, (int)(d * kScale)) != step) continue;
-      lo = key < lo ? key : lo;
-      hi = key > hi ? key : hi;
-    }
+  src.each([&](float l, uint64_t key) {
+    if (key < cut || step_of(row, l) != step) return;
+    lo = key < lo ? key : lo;
+    hi = key > hi ? key : hi;
   });
   if (lo <= hi) {
     atomicMin((unsigned long long*)&s.lo, (unsigned long long)lo);
@@ -257,25 +332,17 @@ __device__ uint64_t cut_at(Shared& s, const L& lg, const Row& row, uint64_t cut,
   __syncthreads();
   lo = s.lo;
   hi = s.hi;
-  // every round leaves at most 1 / 1024 of the range; one key ends it
+  // every pass leaves at most 1 / 1024 of the range; one key ends it
   while (lo < hi) {
     const int shift = max(0, 53 - (int)__clzll((long long)(hi - lo)));  // range >> shift < 2048
     clear_bins(s);
-    lg.each([&](int, int i, const float (&x)[4]) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint64_t key = key_of(x[e], i + e);
-        if (key < lo || key > hi || !(depth_of(row, x[e]) < kSpan)) continue;
-        const int bin = (int)((hi - key) >> shift);
-        atomicAdd(&s.count[bin], 1u);
-        if constexpr (WEIGHT)
-          atomicAdd((unsigned long long*)&s.weight[bin],
-                    (unsigned long long)fixed_of(weight_of(row, x[e])));
-      }
+    src.each([&](float l, uint64_t key) {
+      if (key < lo || key > hi) return;
+      add_to_bin<WEIGHT>(s, row, (int)((hi - key) >> shift), l);
     });
-    find_bin<WEIGHT>(s, target);
+    find_bin<WEIGHT>(s, target, 1.0);
     const int bin = s.found;
-    if (bin < 0) return lo;  // not reached by rounding of the target: all of the step stays
+    if (bin < 0) return lo;  // cannot be: the step holds the target
     target -= s.before;
     const uint32_t n = s.in_bin;
     const uint64_t top = hi - ((uint64_t)bin << shift);
@@ -286,6 +353,58 @@ __device__ uint64_t cut_at(Shared& s, const L& lg, const Row& row, uint64_t cut,
     hi = top;
   }
   return lo;
+}
+
+// First histogram over the elements with key >= cut.
+template <bool WEIGHT, class L>
+__device__ __forceinline__ uint64_t first_bins(Shared& s, const L& src, const Row& row,
+                                               uint64_t cut, uint64_t target, double top_p) {
+  clear_bins(s);
+  src.each([&](float l, uint64_t key) {
+    const int step = step_of(row, l);
+    if (step >= 0 && key >= cut) add_to_bin<WEIGHT>(s, row, step, l);
+  });
+  return find_bin<WEIGHT>(s, target, top_p);
+}
+
+struct Cuts {
+  int k_step, p_step;                // steps of the cuts of top-k and top-p, or kBins
+  uint64_t k_target, p_target;       // within them
+  bool later_p;                      // top-p is taken over what top-k keeps
+  double top_p, min_w;               // min_w: 2^44 min_p
+};
+
+// The token of one source (the list, or the row): cuts, weights, and the element at
+// which their running sum exceeds u times their sum.
+template <class L>
+__device__ __forceinline__ uint64_t cut_of(Shared& s, const L& src, const Row& row, Cuts c) {
+  uint64_t cut = 0;
+  if (c.k_step < kBins) cut = cut_in_step<false>(s, src, row, 0, c.k_step, c.k_target);
+  if (c.later_p) {
+    const uint64_t target = first_bins<true>(s, src, row, cut, 0, c.top_p);
+    c.p_step = s.found;
+    c.p_target = target - s.before;
+  }
+  if (c.p_step < kBins) {
+    const uint64_t k = cut_in_step<true>(s, src, row, cut, c.p_step, c.p_target);
+    cut = k > cut ? k : cut;
+  }
+  return cut;
+}
+
+// A kept logit's weight, or 0.
+__device__ __forceinline__ double kept(const Row& row, float l, uint64_t key, uint64_t cut,
+                                       double min_w) {
+  if (step_of(row, l) < 0 || key < cut) return 0.0;
+  const double w = weight_of(row, l);
+  return w >= min_w ? w : 0.0;
+}
+
+// What the running sum has to exceed.
+__device__ __forceinline__ uint64_t goal_of(float u, uint64_t total) {
+  const double x = floor((u > 0.0f ? (double)u : 0.0) * (double)total);
+  const uint64_t goal = (uint64_t)x;
+  return x < (double)total && goal < total ? goal : total - 1;
 }
 
 template <int DT, bool REG>
@@ -299,26 +418,18 @@ __global__ void __launch_bounds__(kThreads) tm_sample_kernel(SampleParams p) {
   lg.vocab = p.vocab;
   lg.rounds = (p.vocab + kRound - 1) / kRound;
   lg.aligned = p.aligned != 0;
-  if constexpr (REG) {
-#pragma unroll
-    for (int r = 0; r < kRegRounds; ++r) {
-      if (r < lg.rounds) {
-        lg.fetch(r, lg.v[r]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) lg.v[r][e] = -INFINITY;
-      }
-    }
-  }
+  lg.hold();
+  const double temp = p.temperatures ? (double)p.temperatures[n] : p.temperature;
+  const float u = p.uniforms[n];
+  const int top_k = p.top_ks ? p.top_ks[n] : p.top_k;
+  const double top_p = p.top_ps ? (double)p.top_ps[n] : p.top_p;
+  const double min_p = p.min_ps ? (double)p.min_ps[n] : p.min_p;
+  float* const probs = p.probs ? p.probs + n * p.probs_stride : nullptr;
+  if (t < 32) s.powers[t] = exp2((double)t / 32.0) * kUnit;
+
   // the first element of the order
   uint64_t best = 0;
-  lg.each([&](int, int i, const float (&x)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint64_t key = key_of(x[e], i + e);
-      best = key > best ? key : best;
-    }
-  });
+  lg.each([&](float, uint64_t key) { best = key > best ? key : best; });
 #pragma unroll
   for (int m = 32; m > 0; m >>= 1) {
     const uint64_t o = shfl_xor64(best, m);
@@ -330,19 +441,10 @@ __global__ void __launch_bounds__(kThreads) tm_sample_kernel(SampleParams p) {
   for (int w = 0; w < kWaves; ++w) best = s.wave[w] > best ? s.wave[w] : best;
 
   Row row;
-  const uint32_t ob = (uint32_t)(best >> 32);
-  row.top = __uint_as_float(ob ^ ((ob >> 31) ? 0x80000000u : 0xffffffffu));
-  const double temp = p.temperatures ? (double)p.temperatures[n] : p.temperature;
-  const float u = p.uniforms[n];
-  const int top_k = p.top_ks ? p.top_ks[n] : p.top_k;
-  const double top_p = p.top_ps ? (double)p.top_ps[n] : p.top_p;
-  const double min_p = p.min_ps ? (double)p.min_ps[n] : p.min_p;
-  float* const probs = p.probs ? p.probs + n * p.probs_stride : nullptr;
-
-  const int first = (int)~(uint32_t)best;
+  row.top = logit_of(best);
   if (row.top == -INFINITY || !(temp > 0.0)) {
     // nothing to choose from, or the largest logit itself
-    const int token = row.top == -INFINITY ? -1 : first;
+    const int token = row.top == -INFINITY ? -1 : index_of(best);
     if (t == 0) p.tokens[n] = token;
     if (probs)
       for (int i = t; i < p.vocab; i += kThreads) probs[i] = i == token ? 1.0f : 0.0f;
@@ -351,62 +453,128 @@ __global__ void __launch_bounds__(kThreads) tm_sample_kernel(SampleParams p) {
   row.inv_t = (float)(1.0 / temp);
   row.inv_y = 46.166241308446828384 / temp;
   row.powers = s.powers;
-  if (t < 32) s.powers[t] = exp2((double)t / 32.0);
-  __syncthreads();
 
-  uint64_t cut = 0;
-  if (top_k > 0 && top_k < p.vocab) cut = cut_at<false>(s, lg, row, cut, (uint64_t)top_k);
-  if (top_p < 1.0) {
-    uint64_t sum = 0;
-    lg.each([&](int, int i, const float (&x)[4]) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (depth_of(row, x[e]) < kSpan && key_of(x[e], i + e) >= cut)
-          sum += fixed_of(weight_of(row, x[e]));
-    });
-    sum = sum_wave(sum);
-    __syncthreads();
-    if (lane == 0) s.wave[wave] = sum;
-    __syncthreads();
-    sum = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) sum += s.wave[w];
-    const double want = ceil(top_p * (double)sum);
-    const uint64_t target = want > 1.0 ? (uint64_t)want : 1;
-    const uint64_t c = cut_at<true>(s, lg, row, cut, target < sum ? target : sum);
-    cut = c > cut ? c : cut;
+  const bool by_k = top_k > 0 && top_k < p.vocab, by_p = top_p < 1.0, by_m = min_p > 0.0;
+  Cuts c;
+  c.k_step = c.p_step = kBins;
+  c.k_target = c.p_target = 0;
+  c.top_p = top_p;
+  c.min_w = by_m ? (min_p < 1.0 ? min_p : 1.0) * kUnit : 0.0;
+  if (by_k) {
+    first_bins<false>(s, lg, row, 0, (uint64_t)top_k, 1.0);
+    if (s.found >= 0) {  // (fewer than k weigh anything otherwise)
+      c.k_step = s.found;
+      c.k_target = (uint64_t)top_k - s.before;
+    }
+  } else if (by_p) {
+    const uint64_t target = first_bins<true>(s, lg, row, 0, 0, top_p);
+    c.p_step = s.found;
+    c.p_target = target - s.before;
+  }
+  c.later_p = by_k && by_p;
+  // the last step that can be kept: that of a cut, or the one behind min-p's (whose
+  // own bound is exact); top-p after top-k has to see all that top-k keeps
+  int last = min(c.k_step, c.p_step);
+  if (by_m && !c.later_p) {
+    const float d = -logf((float)(c.min_w / kUnit));
+    const int m = d < kSpan ? (int)(d * ((float)kBins / kSpan)) + 1 : kBins;
+    if (m < last) {
+      last = m;
+      c.k_step = c.p_step = kBins;  // the cuts lie behind it
+    }
   }
 
+  // everything up to that step, in index order
+  List list;
+  list.keys = s.list;
+  list.n = 0;
+  bool listed = last < kBins;
+  if (listed) {
+    __syncthreads();
+    lg.rounds_of([&](int r, int i, const float (&x)[4]) {
+      int m = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int step = step_of(row, x[e]);
+        m += step >= 0 && step <= last ? 1 : 0;
+      }
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) m += __shfl_xor(m, d);
+      if (lane == 0) s.seg[r * kWaves + wave] = (uint64_t)m;
+    });
+    __syncthreads();
+    uint64_t total;
+    const uint64_t mine = t < lg.rounds * kWaves ? s.seg[t] : 0;
+    const uint64_t at = scan_block(s, mine, &total);
+    listed = total <= (uint64_t)kList;
+    if (listed) {
+      __syncthreads();
+      s.seg[t] = at;
+      __syncthreads();
+      lg.rounds_of([&](int r, int i, const float (&x)[4]) {
+        const uint64_t low = ((uint64_t)1 << lane) - 1;  // lanes below this one
+        int pos = (int)s.seg[r * kWaves + wave];
+        bool keep[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int step = step_of(row, x[e]);
+          keep[e] = step >= 0 && step <= last;
+          pos += __popcll(__ballot(keep[e]) & low);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (keep[e]) s.list[pos++] = key_of(x[e], i + e);
+      });
+      list.n = (int)total;
+      list.per = (list.n + kThreads - 1) / kThreads;
+      if (probs) {
+        if (((uintptr_t)probs & 15) == 0 && (p.vocab & 3) == 0) {
+          const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+          for (int i = 4 * t; i < p.vocab; i += 4 * kThreads)
+            *reinterpret_cast<f32x4_t*>(probs + i) = zero;
+        } else {
+          for (int i = t; i < p.vocab; i += kThreads) probs[i] = 0.0f;
+        }
+      }
+      __syncthreads();
+    }
+  }
+
+  if (listed) {
+    const uint64_t cut = cut_of(s, list, row, c);
+    uint64_t sum = 0, total;
+    list.each([&](float l, uint64_t key) { sum += fixed_of(kept(row, l, key, cut, c.min_w)); });
+    uint64_t run = scan_block(s, sum, &total);
+    const uint64_t goal = goal_of(u, total);
+    const double inv = 1.0 / (double)total;
+    const bool here = run <= goal && goal < run + sum;  // one thread's
+    if (here || probs)
+      list.each([&](float l, uint64_t key) {
+        const double w = kept(row, l, key, cut, c.min_w);
+        if (probs && w > 0.0) probs[index_of(key)] = (float)(w * inv);
+        const uint64_t f = fixed_of(w);
+        if (here && run <= goal && goal < run + f) p.tokens[n] = index_of(key);
+        run += f;
+      });
+    return;
+  }
+
+  const uint64_t cut = cut_of(s, lg, row, c);
   // sums of 256 consecutive indices: a wave's part of a round
-  const double floor_w = min_p > 0.0 ? (min_p < 1.0 ? min_p : 1.0) : 0.0;
-  auto kept = [&](float x, int i) -> double {
-    if (!(depth_of(row, x) < kSpan) || key_of(x, i) < cut) return 0.0;
-    const double w = weight_of(row, x);
-    return w >= floor_w ? w : 0.0;
-  };
   __syncthreads();
-  lg.each([&](int r, int i, const float (&x)[4]) {
+  lg.rounds_of([&](int r, int i, const float (&x)[4]) {
     uint64_t sum = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sum += fixed_of(kept(x[e], i + e));
+    for (int e = 0; e < 4; ++e)
+      sum += fixed_of(kept(row, x[e], key_of(x[e], i + e), cut, c.min_w));
     sum = sum_wave(sum);
     if (lane == 0) s.seg[r * kWaves + wave] = sum;
   });
   __syncthreads();
-  const int segs = lg.rounds * kWaves;  // at most kThreads
-  const uint64_t mine = t < segs ? s.seg[t] : 0;
-  const uint64_t incl = scan_wave(mine, lane);
-  if (lane == 63) s.wave[wave] = incl;
-  __syncthreads();
-  uint64_t at = incl - mine, total = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) at += s.wave[w];
-    total += s.wave[w];
-  }
-  double x = floor((u > 0.0f ? (double)u : 0.0) * (double)total);
-  uint64_t goal = (uint64_t)x;  // the running sum has to exceed it
-  if (!(x < (double)total) || goal >= total) goal = total - 1;
+  const uint64_t mine = t < lg.rounds * kWaves ? s.seg[t] : 0;
+  uint64_t total;
+  const uint64_t at = scan_block(s, mine, &total);
+  const uint64_t goal = goal_of(u, total);
   if (at <= goal && goal < at + mine) {
     s.found = t;
     s.before = at;
@@ -421,7 +589,8 @@ __global__ void __launch_bounds__(kThreads) tm_sample_kernel(SampleParams p) {
     uint64_t w[4], four = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      w[e] = fixed_of(kept(l[e], i + e));
+      l[e] = lg.clean(l[e]);
+      w[e] = fixed_of(kept(row, l[e], key_of(l[e], i + e), cut, c.min_w));
       four += w[e];
     }
     uint64_t run = s.before + scan_wave(four, lane) - four;
@@ -436,11 +605,12 @@ __global__ void __launch_bounds__(kThreads) tm_sample_kernel(SampleParams p) {
     }
   }
   if (probs) {
-    const double inv = kUnit / (double)total;
-    lg.each([&](int, int i, const float (&l)[4]) {
+    const double inv = 1.0 / (double)total;
+    lg.rounds_of([&](int, int i, const float (&l)[4]) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (i + e < p.vocab) probs[i + e] = (float)(kept(l[e], i + e) * inv);
+        if (i + e < p.vocab)
+          probs[i + e] = (float)(kept(row, l[e], key_of(l[e], i + e), cut, c.min_w) * inv);
     });
   }
 }
