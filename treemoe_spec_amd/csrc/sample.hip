@@ -22,12 +22,13 @@
 // index), all distinct, in 2048 steps of the remaining range at a time.
 //
 // One workgroup of 16 waves takes a row, up to 32768 logits in registers, more read
-// again through L2.  A row is passed over two or three times: for its largest logit,
-// for the first histogram, and to collect what lies above the cut's step (or min-p's
-// bound) into a list in LDS, in index order.  What follows runs on the list: a few
-// logits a thread where top-k or top-p leave few, the row itself where they leave
-// more than the list holds.  The 64-bit exponential of a whole row, which top-p
-// without top-k and plain sampling need once, is what costs most.
+// again through L2; a wave owns consecutive indices.  All that can be kept lies above a
+// value that is found cheaply: min-p's own bound, or one that some k of the 1024
+// threads' largest logits reach, since then k logits do.  What lies above goes into a
+// list in LDS, in index order, and the rest runs on the list: up to 256 elements are
+// ranked by counting, more are cut by histograms.  top-p without top-k needs the weight
+// of the whole row, one pass of 64-bit exponentials; where the list turns out to hold
+// too little of it, or overflows, the row itself is cut by histograms.
 #include <cmath>
 
 #include "tm_vec.h"
@@ -39,10 +40,12 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kRound = kThreads * 4;            // logits of one round: 4 consecutive a thread
 constexpr int kRegRounds = 8;                   // rounds held in registers
 constexpr int kBins = 2048;
-constexpr int kList = 8192;                     // logits that the list holds
-constexpr int kMaxRounds = TM_MAX_SAMPLE_VOCAB / kRound;
+constexpr int kList = 1024;                     // logits of a wave that the list holds
+constexpr int kRank = 256;                      // up to so many in all are ranked by counting
+constexpr int kRankStep = 8;                    // so many at a time
 constexpr float kSpan = 31.25f;                 // (l_max - l) / temperature of the last bin's end
 constexpr double kUnit = 17592186044416.0;      // 2^44
+constexpr double kTwo52 = 4503599627370496.0;   // where doubles are integers
 
 struct SampleParams {
   const void* logits;
@@ -63,6 +66,7 @@ struct Row {
   float top;       // largest logit
   float inv_t;     // 1 / temperature
   double inv_y;    // 32 log2(e) / temperature
+  double deepest;  // l_max - l at which the weight is 0 for long
   const double* powers;  // 2^(44 + j / 32), j < 32
 };
 
@@ -88,61 +92,58 @@ __device__ __forceinline__ int step_of(const Row& r, float l) {
   return d < kSpan ? min(kBins - 1, (int)(d * ((float)kBins / kSpan))) : -1;
 }
 
-// 2^44 times the weight of a logit with a step, in 64 bits: e^z = 2^(k / 32) e^x with k
-// the nearest integer to 32 z log2(e), 2^(44 + k % 32 / 32) from a table and e^x,
-// |x| <= ln 2 / 64, from its Taylor polynomial of degree 5 (truncation below 3e-15).
-// A logit equal to the largest weighs 1 (also infinities).
+// 2^44 times the weight of a logit, in 64 bits: with d = l_max - l and t = 32 d log2(e) /
+// temperature, e^(-d / temperature) = 2^(-k / 32) e^x for k the integer nearest to t
+// and x = (k - t) ln 2 / 32, |x| <= ln 2 / 64: 2^(44 + j / 32) from a table, e^x from its
+// Taylor polynomial of degree 5 (truncation below 3e-15).  d is clamped to where the
+// weight is far below 1/2; a difference of infinities counts as 0.
 __device__ __forceinline__ double weight_of(const Row& r, float l) {
   constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to integers
-  const double y = ((double)l - (double)r.top) * r.inv_y;  // 32 z log2(e), > -1443
-  const double t = y + kMagic;
-  const double x = (y - (t - kMagic)) * 0.021660849392498290;  // ln 2 / 32
-  double q = fma(x, 8.3333333333333333e-3, 4.1666666666666667e-2);
-  q = fma(q, x, 1.6666666666666667e-1);
-  q = fma(q, x, 0.5);
-  q = fma(q, x, 1.0);
+  constexpr double c = 0.021660849392498290;     // ln 2 / 32
+  const double d = fmin(fmax((double)r.top - (double)l, 0.0), r.deepest);
+  const double t = fma(d, -r.inv_y, kMagic);
+  const double x = fma(d, -r.inv_y, kMagic - t);
+  double q = fma(x, c * c * c * c * c / 120.0, c * c * c * c / 24.0);
+  q = fma(q, x, c * c * c / 6.0);
+  q = fma(q, x, c * c / 2.0);
+  q = fma(q, x, c);
   q = fma(q, x, 1.0);
   const int k = (int)(uint32_t)(uint64_t)__double_as_longlong(t);
-  const uint64_t w = (uint64_t)__double_as_longlong(q * r.powers[k & 31]);
-  const uint32_t hi = (uint32_t)(w >> 32) + ((uint32_t)(k >> 5) << 20);
-  const double v = __longlong_as_double((long long)(((uint64_t)hi << 32) | (uint32_t)w));
-  return l == r.top ? kUnit : v;
+  return ldexp(q * r.powers[k & 31], k >> 5);
 }
 // The weight as an integer, to the nearest: the low bits of 2^52 + w.
 __device__ __forceinline__ uint64_t fixed_of(double w) {
-  return (uint64_t)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
+  return (uint64_t)__double_as_longlong(w + kTwo52) & 0xfffffffffffffull;
 }
 
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int m) {
-  const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)v, m);
-  const uint32_t hi = (uint32_t)__shfl_xor((int)(uint32_t)(v >> 32), m);
-  return ((uint64_t)hi << 32) | lo;
+// The value DPP moves into a lane: v of another lane of the wave, 0 where none is.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
 }
-__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
-  const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)v, d);
-  const uint32_t hi = (uint32_t)__shfl_up((int)(uint32_t)(v >> 32), d);
-  return ((uint64_t)hi << 32) | lo;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t plus_moved(uint64_t v) {
+  return v + (((uint64_t)moved<CTRL, ROWS>((uint32_t)(v >> 32)) << 32) |
+              moved<CTRL, ROWS>((uint32_t)v));
 }
-// Inclusive sum over the lanes of a wave.
-__device__ __forceinline__ uint64_t scan_wave(uint64_t v, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint64_t o = shfl_up64(v, d);
-    if (lane >= d) v += o;
-  }
-  return v;
+// Inclusive sum over the lanes of a wave: within rows of 16 lanes, then row to row.
+__device__ __forceinline__ uint64_t scan_wave(uint64_t v) {
+  v = plus_moved<0x111, 0xf>(v);  // 1, 2, 4 and 8 lanes up
+  v = plus_moved<0x112, 0xf>(v);
+  v = plus_moved<0x114, 0xf>(v);
+  v = plus_moved<0x118, 0xf>(v);
+  v = plus_moved<0x142, 0xa>(v);  // lane 15 of a row to the next row
+  return plus_moved<0x143, 0xc>(v);  // lane 31 to the upper half
 }
-__device__ __forceinline__ uint64_t sum_wave(uint64_t v) {
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) v += shfl_xor64(v, m);
-  return v;
+__device__ __forceinline__ uint64_t last_lane(uint64_t v) {
+  return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), 63) << 32) |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63);
 }
 
 struct Shared {
+  uint64_t list[kWaves][kList];  // each wave's elements
   uint64_t weight[kBins];
   uint32_t count[kBins];
-  uint64_t list[kList];
-  uint64_t seg[kMaxRounds * kWaves];
   uint64_t wave[kWaves];
   double powers[32];
   uint64_t lo, hi, before;
@@ -153,7 +154,7 @@ struct Shared {
 // Exclusive sum of v over the workgroup's threads in order, and the total.
 __device__ __forceinline__ uint64_t scan_block(Shared& s, uint64_t v, uint64_t* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint64_t incl = scan_wave(v, lane);
+  const uint64_t incl = scan_wave(v);
   __syncthreads();  // s.wave is free
   if (lane == 63) s.wave[wave] = incl;
   __syncthreads();
@@ -176,10 +177,13 @@ struct Logits {
   int vocab, rounds;
   bool aligned;
 
-  // The thread's 4 logits of round r; NaN and what lies past the end as -inf,
-  // -0 as +0.
+  // Round r of wave w: indices 256 (w rounds + r) .., 4 consecutive a lane.
+  __device__ __forceinline__ int index_at(int r) const {
+    return ((int)(threadIdx.x >> 6) * rounds + r) * 256 + (int)(threadIdx.x & 63) * 4;
+  }
+  // The thread's 4 logits of round r; what lies past the end as -inf.
   __device__ __forceinline__ void fetch(int r, float (&x)[4]) const {
-    const int i = r * kRound + (int)threadIdx.x * 4;
+    const int i = index_at(r);
     if (aligned && i + 4 <= vocab) {
       if constexpr (DT == TM_DTYPE_F32) {
         const f32x4_t a =
@@ -197,6 +201,7 @@ struct Logits {
       for (int e = 0; e < 4; ++e) x[e] = i + e < vocab ? tm_load1<DT>(row, i + e) : -INFINITY;
     }
   }
+  // NaN as -inf, -0 as +0.
   static __device__ __forceinline__ float clean(float x) { return x == x ? x + 0.0f : -INFINITY; }
   __device__ __forceinline__ void hold() {
     if constexpr (REG) {
@@ -223,7 +228,7 @@ struct Logits {
           x[e] = v[r][e];
           asm volatile("" : "+v"(x[e]));
         }
-        if (r < rounds) f(r, r * kRound + (int)threadIdx.x * 4, x);
+        if (r < rounds) f(r, index_at(r), x);
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
@@ -238,7 +243,7 @@ struct Logits {
           if (r0 + a < rounds) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[a][e] = clean(x[a][e]);
-            f(r0 + a, (r0 + a) * kRound + (int)threadIdx.x * 4, x[a]);
+            f(r0 + a, index_at(r0 + a), x[a]);
           }
       }
     }
@@ -253,21 +258,23 @@ struct Logits {
   }
 };
 
-// The list in LDS: n keys in index order, `per` consecutive ones a thread.
+// The list in LDS: each wave's keys in index order, consecutive ones a lane.
 struct List {
-  const uint64_t* keys;
-  int n, per;
+  const uint64_t* keys;  // this wave's
+  int n;
   template <class F>
   __device__ __forceinline__ void each(F&& f) const {
-    const int end = min(n, ((int)threadIdx.x + 1) * per);
-    for (int i = (int)threadIdx.x * per; i < end; ++i) f(logit_of(keys[i]), keys[i]);
+    const int per = (n + 63) / 64, lane = (int)threadIdx.x & 63;
+    const int end = min(n, (lane + 1) * per);
+    for (int i = lane * per; i < end; ++i) f(logit_of(keys[i]), keys[i]);
   }
 };
 
+template <bool WEIGHT>
 __device__ __forceinline__ void clear_bins(Shared& s) {
   __syncthreads();  // the last reads are over
   for (int i = threadIdx.x; i < kBins; i += kThreads) {
-    s.weight[i] = 0;
+    if (WEIGHT) s.weight[i] = 0;
     s.count[i] = 0;
   }
   if (threadIdx.x == 0) {
@@ -318,7 +325,7 @@ __device__ __forceinline__ uint64_t find_bin(Shared& s, uint64_t target, double 
 template <bool WEIGHT, class L>
 __device__ uint64_t cut_in_step(Shared& s, const L& src, const Row& row, uint64_t cut, int step,
                                 uint64_t target) {
-  clear_bins(s);
+  clear_bins<false>(s);
   uint64_t lo = ~0ull, hi = 0;
   src.each([&](float l, uint64_t key) {
     if (key < cut || step_of(row, l) != step) return;
@@ -335,7 +342,7 @@ __device__ uint64_t cut_in_step(Shared& s, const L& src, const Row& row, uint64_
   // every pass leaves at most 1 / 1024 of the range; one key ends it
   while (lo < hi) {
     const int shift = max(0, 53 - (int)__clzll((long long)(hi - lo)));  // range >> shift < 2048
-    clear_bins(s);
+    clear_bins<WEIGHT>(s);
     src.each([&](float l, uint64_t key) {
       if (key < lo || key > hi) return;
       add_to_bin<WEIGHT>(s, row, (int)((hi - key) >> shift), l);
@@ -359,7 +366,7 @@ __device__ uint64_t cut_in_step(Shared& s, const L& src, const Row& row, uint64_
 template <bool WEIGHT, class L>
 __device__ __forceinline__ uint64_t first_bins(Shared& s, const L& src, const Row& row,
                                                uint64_t cut, uint64_t target, double top_p) {
-  clear_bins(s);
+  clear_bins<WEIGHT>(s);
   src.each([&](float l, uint64_t key) {
     const int step = step_of(row, l);
     if (step >= 0 && key >= cut) add_to_bin<WEIGHT>(s, row, step, l);
@@ -367,27 +374,31 @@ __device__ __forceinline__ uint64_t first_bins(Shared& s, const L& src, const Ro
   return find_bin<WEIGHT>(s, target, top_p);
 }
 
-struct Cuts {
-  int k_step, p_step;                // steps of the cuts of top-k and top-p, or kBins
-  uint64_t k_target, p_target;       // within them
-  bool later_p;                      // top-p is taken over what top-k keeps
-  double top_p, min_w;               // min_w: 2^44 min_p
+struct Filter {
+  bool by_k, by_p;
+  uint64_t k;
+  double top_p, min_w;   // min_w: 2^44 min_p
+  uint64_t p_target;     // top-p's target where it is known (without top-k), or 0
 };
 
-// The token of one source (the list, or the row): cuts, weights, and the element at
-// which their running sum exceeds u times their sum.
+// The smallest key that top-k and top-p keep of the elements of `src` (0: all).
 template <class L>
-__device__ __forceinline__ uint64_t cut_of(Shared& s, const L& src, const Row& row, Cuts c) {
+__device__ __forceinline__ uint64_t cut_of(Shared& s, const L& src, const Row& row,
+                                           const Filter& f) {
   uint64_t cut = 0;
-  if (c.k_step < kBins) cut = cut_in_step<false>(s, src, row, 0, c.k_step, c.k_target);
-  if (c.later_p) {
-    const uint64_t target = first_bins<true>(s, src, row, cut, 0, c.top_p);
-    c.p_step = s.found;
-    c.p_target = target - s.before;
+  if (f.by_k) {
+    first_bins<false>(s, src, row, 0, f.k, 1.0);
+    const int step = s.found;
+    // (fewer than k weigh anything otherwise)
+    if (step >= 0) cut = cut_in_step<false>(s, src, row, 0, step, f.k - s.before);
   }
-  if (c.p_step < kBins) {
-    const uint64_t k = cut_in_step<true>(s, src, row, cut, c.p_step, c.p_target);
-    cut = k > cut ? k : cut;
+  if (f.by_p) {
+    const uint64_t target = first_bins<true>(s, src, row, cut, f.p_target, f.top_p);
+    const int step = s.found;
+    if (step >= 0) {
+      const uint64_t c = cut_in_step<true>(s, src, row, cut, step, target - s.before);
+      cut = c > cut ? c : cut;
+    }
   }
   return cut;
 }
@@ -407,6 +418,45 @@ __device__ __forceinline__ uint64_t goal_of(float u, uint64_t total) {
   return x < (double)total && goal < total ? goal : total - 1;
 }
 
+// The largest of v over the workgroup.
+__device__ __forceinline__ float max_block(Shared& s, float v) {
+#define TM_MAX(ctrl, rows)                                                                \
+  v = fmaxf(v, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(                     \
+                   (int)__float_as_uint(v), (int)__float_as_uint(v), ctrl, rows, 0xf, false)))
+  TM_MAX(0x111, 0xf);
+  TM_MAX(0x112, 0xf);
+  TM_MAX(0x114, 0xf);
+  TM_MAX(0x118, 0xf);
+  TM_MAX(0x142, 0xa);
+  TM_MAX(0x143, 0xc);
+#undef TM_MAX
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) s.wave[threadIdx.x >> 6] = __float_as_uint(v);
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) v = fmaxf(v, __uint_as_float((uint32_t)s.wave[w]));
+  return v;
+}
+
+// The logit `depth` temperatures below the largest, or a little less: 2^-19 of the terms
+// covers the roundings here and in step_of, a few 2^-24 of them.
+__device__ __forceinline__ float below(const Row& row, float depth) {
+  if (row.top == INFINITY) return INFINITY;
+  const float d = depth / row.inv_t;
+  return row.top - d - 1.9e-6f * (d + fabsf(row.top));
+}
+
+// A value that at least `k` (<= 1024) of the threads' `most` reach, -infinity where
+// fewer of them weigh anything.
+__device__ __forceinline__ float reached_by(Shared& s, const Row& row, float most, int k) {
+  clear_bins<false>(s);
+  const int step = step_of(row, most);
+  if (step >= 0) atomicAdd(&s.count[step], 1u);
+  find_bin<false>(s, (uint64_t)k, 1.0);
+  if (s.found < 0) return -INFINITY;
+  return below(row, (float)(s.found + 1) * (kSpan / (float)kBins));
+}
+
 template <int DT, bool REG>
 __global__ void __launch_bounds__(kThreads) tm_sample_kernel(SampleParams p) {
   __shared__ Shared s;
@@ -419,7 +469,7 @@ __global__ void __launch_bounds__(kThreads) tm_sample_kernel(SampleParams p) {
   lg.rounds = (p.vocab + kRound - 1) / kRound;
   lg.aligned = p.aligned != 0;
   lg.hold();
-  const double temp = p.temperatures ? (double)p.temperatures[n] : p.temperature;
+  double temp = p.temperatures ? (double)p.temperatures[n] : p.temperature;
   const float u = p.uniforms[n];
   const int top_k = p.top_ks ? p.top_ks[n] : p.top_k;
   const double top_p = p.top_ps ? (double)p.top_ps[n] : p.top_p;
@@ -427,181 +477,229 @@ __global__ void __launch_bounds__(kThreads) tm_sample_kernel(SampleParams p) {
   float* const probs = p.probs ? p.probs + n * p.probs_stride : nullptr;
   if (t < 32) s.powers[t] = exp2((double)t / 32.0) * kUnit;
 
-  // the first element of the order
-  uint64_t best = 0;
-  lg.each([&](float, uint64_t key) { best = key > best ? key : best; });
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) {
-    const uint64_t o = shfl_xor64(best, m);
-    best = o > best ? o : best;
-  }
-  if (lane == 0) s.wave[wave] = best;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) best = s.wave[w] > best ? s.wave[w] : best;
-
+  float most = -INFINITY;  // of this thread's logits
+  lg.rounds_of([&](int, int, const float (&x)[4]) {
+    most = fmaxf(fmaxf(fmaxf(most, x[0]), fmaxf(x[1], x[2])), x[3]);
+  });
   Row row;
-  row.top = logit_of(best);
+  row.top = max_block(s, most);
   if (row.top == -INFINITY || !(temp > 0.0)) {
-    // nothing to choose from, or the largest logit itself
-    const int token = row.top == -INFINITY ? -1 : index_of(best);
+    // nothing to choose from, or the first of the largest logits
+    if (t == 0) s.lo = ~0ull;
+    __syncthreads();
+    if (most == row.top && row.top != -INFINITY) {
+      int at = INT32_MAX;
+      lg.rounds_of([&](int, int i, const float (&x)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (x[e] == row.top && i + e < at) at = i + e;
+      });
+      atomicMin((unsigned long long*)&s.lo, (unsigned long long)at);
+    }
+    __syncthreads();
+    const int token = s.lo == ~0ull ? -1 : (int)s.lo;
     if (t == 0) p.tokens[n] = token;
     if (probs)
       for (int i = t; i < p.vocab; i += kThreads) probs[i] = i == token ? 1.0f : 0.0f;
     return;
   }
+  temp = fmax(temp, 1e-300);  // its inverse finite
   row.inv_t = (float)(1.0 / temp);
   row.inv_y = 46.166241308446828384 / temp;
+  row.deepest = 32.5 * temp;  // 2^44 e^-32.5 < 0.14
   row.powers = s.powers;
 
-  const bool by_k = top_k > 0 && top_k < p.vocab, by_p = top_p < 1.0, by_m = min_p > 0.0;
-  Cuts c;
-  c.k_step = c.p_step = kBins;
-  c.k_target = c.p_target = 0;
-  c.top_p = top_p;
-  c.min_w = by_m ? (min_p < 1.0 ? min_p : 1.0) * kUnit : 0.0;
-  if (by_k) {
-    first_bins<false>(s, lg, row, 0, (uint64_t)top_k, 1.0);
-    if (s.found >= 0) {  // (fewer than k weigh anything otherwise)
-      c.k_step = s.found;
-      c.k_target = (uint64_t)top_k - s.before;
-    }
-  } else if (by_p) {
-    const uint64_t target = first_bins<true>(s, lg, row, 0, 0, top_p);
-    c.p_step = s.found;
-    c.p_target = target - s.before;
-  }
-  c.later_p = by_k && by_p;
-  // the last step that can be kept: that of a cut, or the one behind min-p's (whose
-  // own bound is exact); top-p after top-k has to see all that top-k keeps
-  int last = min(c.k_step, c.p_step);
-  if (by_m && !c.later_p) {
-    const float d = -logf((float)(c.min_w / kUnit));
-    const int m = d < kSpan ? (int)(d * ((float)kBins / kSpan)) + 1 : kBins;
-    if (m < last) {
-      last = m;
-      c.k_step = c.p_step = kBins;  // the cuts lie behind it
-    }
-  }
+  Filter f;
+  f.by_k = top_k > 0 && top_k < p.vocab;
+  f.by_p = top_p < 1.0;
+  f.k = (uint64_t)(f.by_k ? top_k : 0);
+  f.top_p = top_p;
+  f.p_target = 0;
+  const bool by_m = min_p > 0.0;
+  f.min_w = by_m ? (min_p < 1.0 ? min_p : 1.0) * kUnit : 0.0;
 
-  // everything up to that step, in index order
+  // a value above which all lies that can be kept, where one is known beforehand
+  bool listed = true;
+  float above = -INFINITY;
+  if (f.by_k && top_k <= kThreads) {
+    above = reached_by(s, row, most, top_k);
+  } else if (f.by_k) {
+    listed = false;
+  } else if (by_m) {
+    above = below(row, 1e-6f - logf((float)(f.min_w / kUnit)));
+  } else if (f.by_p) {
+    // most of the row's weight in all likelihood: all but two threads hold a logit
+    // as large, so some 6000 are
+    above = reached_by(s, row, most, kThreads - 2);
+  } else {
+    listed = false;
+  }
+  // the list, and for top-p without top-k the whole row's weight
   List list;
-  list.keys = s.list;
+  list.keys = s.list[wave];
   list.n = 0;
-  bool listed = last < kBins;
-  if (listed) {
-    __syncthreads();
-    lg.rounds_of([&](int r, int i, const float (&x)[4]) {
-      int m = 0;
+  const bool whole = f.by_p && !f.by_k;
+  if (listed || whole) {
+    int count = 0;           // of this wave
+    double sum = kTwo52;     // of this thread: whole numbers, each weight rounded to one
+    lg.rounds_of([&](int, int i, const float (&x)[4]) {
+      if (whole) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += weight_of(row, x[e]);
+      }
+      if (!listed) return;
+      uint64_t m[4];
+      int more = 0, before = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int step = step_of(row, x[e]);
-        m += step >= 0 && step <= last ? 1 : 0;
+        m[e] = __ballot(x[e] >= above && x[e] != -INFINITY);
+        more += __popcll(m[e]);
       }
+      if (more == 0) return;
 #pragma unroll
-      for (int d = 32; d > 0; d >>= 1) m += __shfl_xor(m, d);
-      if (lane == 0) s.seg[r * kWaves + wave] = (uint64_t)m;
-    });
-    __syncthreads();
-    uint64_t total;
-    const uint64_t mine = t < lg.rounds * kWaves ? s.seg[t] : 0;
-    const uint64_t at = scan_block(s, mine, &total);
-    listed = total <= (uint64_t)kList;
-    if (listed) {
-      __syncthreads();
-      s.seg[t] = at;
-      __syncthreads();
-      lg.rounds_of([&](int r, int i, const float (&x)[4]) {
-        const uint64_t low = ((uint64_t)1 << lane) - 1;  // lanes below this one
-        int pos = (int)s.seg[r * kWaves + wave];
-        bool keep[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int step = step_of(row, x[e]);
-          keep[e] = step >= 0 && step <= last;
-          pos += __popcll(__ballot(keep[e]) & low);
-        }
+      for (int e = 0; e < 4; ++e)
+        before += (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m[e] >> 32),
+                                                 __builtin_amdgcn_mbcnt_lo((uint32_t)m[e], 0u));
+      if (count + more <= kList) {
+        int at = count + before;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (keep[e]) s.list[pos++] = key_of(x[e], i + e);
-      });
-      list.n = (int)total;
-      list.per = (list.n + kThreads - 1) / kThreads;
-      if (probs) {
-        if (((uintptr_t)probs & 15) == 0 && (p.vocab & 3) == 0) {
-          const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
-          for (int i = 4 * t; i < p.vocab; i += 4 * kThreads)
-            *reinterpret_cast<f32x4_t*>(probs + i) = zero;
-        } else {
-          for (int i = t; i < p.vocab; i += kThreads) probs[i] = 0.0f;
-        }
+          if ((m[e] >> lane) & 1) s.list[wave][at++] = key_of(x[e], i + e);
       }
-      __syncthreads();
+      count += more;
+    });
+    if (listed) {
+      list.n = min(count, kList);
+      listed = __syncthreads_count(count > kList) == 0;
+    }
+    if (whole) {
+      uint64_t total;
+      scan_block(s, (uint64_t)(sum - kTwo52), &total);
+      const double want = ceil(top_p * (double)total);
+      f.p_target = want > 1.0 ? (uint64_t)want : 1;
+      f.p_target = f.p_target < total ? f.p_target : total;
+    }
+  }
+  if (listed && whole) {
+    // whether the cut of top-p lies in the list
+    uint64_t sum = 0, total;
+    list.each([&](float l, uint64_t key) { sum += fixed_of(kept(row, l, key, 0, f.min_w)); });
+    scan_block(s, sum, &total);
+    if (total < f.p_target) {
+      if (by_m)
+        f.by_p = false;  // it lies behind min-p's
+      else
+        listed = false;
     }
   }
 
   if (listed) {
-    const uint64_t cut = cut_of(s, list, row, c);
+    if (probs) {
+      if (((uintptr_t)probs & 15) == 0) {
+        const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        const int even = p.vocab & ~3;
+        for (int i = 4 * t; i < even; i += 4 * kThreads)
+          *reinterpret_cast<f32x4_t*>(probs + i) = zero;
+        if (even + t < p.vocab) probs[even + t] = 0.0f;
+      } else {
+        for (int i = t; i < p.vocab; i += kThreads) probs[i] = 0.0f;
+      }
+    }
+    uint64_t all;
+    const uint64_t first = scan_block(s, lane == 63 ? (uint64_t)list.n : 0, &all);
+    const int n_all = (int)all;
+    if (n_all <= kRank) {
+      // the waves' elements one after the other, in s.weight; then a thread each
+      for (int i = lane; i < list.n; i += 64) s.weight[(int)first + i] = list.keys[i];
+      if (t < kRankStep) s.weight[n_all + t] = 0;
+      __syncthreads();  // (also: the zeros before the kept probabilities)
+      uint64_t key = 0, w = 0;
+      double wd = 0.0;
+      int rank = 0;
+      if (t < n_all) {
+        key = s.weight[t];
+        for (int j = 0; j < n_all; j += kRankStep)
+#pragma unroll
+          for (int e = 0; e < kRankStep; ++e) rank += s.weight[j + e] > key ? 1 : 0;
+        wd = kept(row, logit_of(key), key, 0, 0.0);
+        w = fixed_of(wd);
+        s.list[0][rank] = w;  // the order's weights
+      }
+      const int keep_k = f.by_k && f.k < (uint64_t)n_all ? (int)f.k : n_all;
+      int keep = keep_k;
+      if (f.by_p) {
+        __syncthreads();
+        uint64_t total;
+        const uint64_t before = scan_block(s, t < keep_k ? s.list[0][t] : 0, &total);
+        if (f.p_target == 0) {
+          const double want = ceil(top_p * (double)total);
+          f.p_target = want > 1.0 ? (uint64_t)want : 1;
+        }
+        keep = __syncthreads_count(t < keep_k && before < f.p_target);
+      }
+      if (rank >= keep || wd < f.min_w) {
+        wd = 0.0;
+        w = 0;
+      }
+      uint64_t total;
+      const uint64_t run = scan_block(s, w, &total);
+      const uint64_t goal = goal_of(u, total);
+      if (run <= goal && goal < run + w) p.tokens[n] = index_of(key);
+      if (probs && w > 0) probs[index_of(key)] = (float)(wd / (double)total);
+      return;
+    }
+    __syncthreads();  // the zeros before the kept probabilities
+    const uint64_t cut = cut_of(s, list, row, f);
     uint64_t sum = 0, total;
-    list.each([&](float l, uint64_t key) { sum += fixed_of(kept(row, l, key, cut, c.min_w)); });
+    list.each([&](float l, uint64_t key) { sum += fixed_of(kept(row, l, key, cut, f.min_w)); });
     uint64_t run = scan_block(s, sum, &total);
     const uint64_t goal = goal_of(u, total);
     const double inv = 1.0 / (double)total;
     const bool here = run <= goal && goal < run + sum;  // one thread's
     if (here || probs)
       list.each([&](float l, uint64_t key) {
-        const double w = kept(row, l, key, cut, c.min_w);
+        const double w = kept(row, l, key, cut, f.min_w);
         if (probs && w > 0.0) probs[index_of(key)] = (float)(w * inv);
-        const uint64_t f = fixed_of(w);
-        if (here && run <= goal && goal < run + f) p.tokens[n] = index_of(key);
-        run += f;
+        const uint64_t x = fixed_of(w);
+        if (here && run <= goal && goal < run + x) p.tokens[n] = index_of(key);
+        run += x;
       });
     return;
   }
 
-  const uint64_t cut = cut_of(s, lg, row, c);
-  // sums of 256 consecutive indices: a wave's part of a round
-  __syncthreads();
-  lg.rounds_of([&](int r, int i, const float (&x)[4]) {
-    uint64_t sum = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      sum += fixed_of(kept(row, x[e], key_of(x[e], i + e), cut, c.min_w));
-    sum = sum_wave(sum);
-    if (lane == 0) s.seg[r * kWaves + wave] = sum;
-  });
-  __syncthreads();
-  const uint64_t mine = t < lg.rounds * kWaves ? s.seg[t] : 0;
-  uint64_t total;
-  const uint64_t at = scan_block(s, mine, &total);
+  const uint64_t cut = cut_of(s, lg, row, f);
+  uint64_t sum = 0, total;
+  lg.each([&](float l, uint64_t key) { sum += fixed_of(kept(row, l, key, cut, f.min_w)); });
+  // a wave's indices are consecutive: its sum, then the round, then the lane
+  const uint64_t mine = last_lane(scan_wave(sum));
+  // (counted at the wave's last lane, so every lane has the waves before it)
+  uint64_t from = scan_block(s, lane == 63 ? mine : 0, &total);
   const uint64_t goal = goal_of(u, total);
-  if (at <= goal && goal < at + mine) {
-    s.found = t;
-    s.before = at;
-  }
-  __syncthreads();
-  const int seg = s.found;
-  if (seg % kWaves == wave) {
-    float l[4];
-    const int r = seg / kWaves;
-    lg.fetch(r, l);
-    const int i = r * kRound + t * 4;
-    uint64_t w[4], four = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      l[e] = lg.clean(l[e]);
-      w[e] = fixed_of(kept(row, l[e], key_of(l[e], i + e), cut, c.min_w));
-      four += w[e];
-    }
-    uint64_t run = s.before + scan_wave(four, lane) - four;
-    if (run <= goal && goal < run + four) {
-      int token = i;
+  if (from <= goal && goal < from + mine) {
+    for (int r = 0; r < lg.rounds; ++r) {
+      float l[4];
+      lg.fetch(r, l);
+      const int i = lg.index_at(r);
+      uint64_t w[4], four = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (run <= goal && goal < run + w[e]) token = i + e;
-        run += w[e];
+        l[e] = lg.clean(l[e]);
+        w[e] = fixed_of(kept(row, l[e], key_of(l[e], i + e), cut, f.min_w));
+        four += w[e];
       }
-      p.tokens[n] = token;
+      const uint64_t upto = scan_wave(four);
+      uint64_t x = from + upto - four;
+      if (x <= goal && goal < x + four) {
+        int token = i;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (x <= goal && goal < x + w[e]) token = i + e;
+          x += w[e];
+        }
+        p.tokens[n] = token;
+      }
+      from += last_lane(upto);
+      if (from > goal) break;
     }
   }
   if (probs) {
@@ -610,7 +708,7 @@ __global__ void __launch_bounds__(kThreads) tm_sample_kernel(SampleParams p) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (i + e < p.vocab)
-          probs[i + e] = (float)(kept(row, l[e], key_of(l[e], i + e), cut, c.min_w) * inv);
+          probs[i + e] = (float)(kept(row, l[e], key_of(l[e], i + e), cut, f.min_w) * inv);
     });
   }
 }
