@@ -47,6 +47,17 @@ constexpr float kSpan = 31.25f;                 // (l_max - l) / temperature of 
 constexpr double kUnit = 17592186044416.0;      // 2^44
 constexpr double kTwo52 = 4503599627370496.0;   // where doubles are integers
 
+// 2^(44 + j / 32)
+__constant__ const double kPowers[32] = {
+    0x1.0000000000000p+44, 0x1.059b0d3158574p+44, 0x1.0b5586cf9890fp+44, 0x1.11301d0125b51p+44,
+    0x1.172b83c7d517bp+44, 0x1.1d4873168b9aap+44, 0x1.2387a6e756238p+44, 0x1.29e9df51fdee1p+44,
+    0x1.306fe0a31b715p+44, 0x1.371a7373aa9cbp+44, 0x1.3dea64c123422p+44, 0x1.44e086061892dp+44,
+    0x1.4bfdad5362a27p+44, 0x1.5342b569d4f82p+44, 0x1.5ab07dd485429p+44, 0x1.6247eb03a5585p+44,
+    0x1.6a09e667f3bcdp+44, 0x1.71f75e8ec5f74p+44, 0x1.7a11473eb0187p+44, 0x1.82589994cce13p+44,
+    0x1.8ace5422aa0dbp+44, 0x1.93737b0cdc5e5p+44, 0x1.9c49182a3f090p+44, 0x1.a5503b23e255dp+44,
+    0x1.ae89f995ad3adp+44, 0x1.b7f76f2fb5e47p+44, 0x1.c199bdd85529cp+44, 0x1.cb720dcef9069p+44,
+    0x1.d5818dcfba487p+44, 0x1.dfc97337b9b5fp+44, 0x1.ea4afa2a490dap+44, 0x1.f50765b6e4540p+44};
+
 struct SampleParams {
   const void* logits;
   int64_t row_stride;
@@ -72,7 +83,7 @@ struct Row {
 
 // Ordered bits: larger floats have larger keys.
 __device__ __forceinline__ uint32_t order_bits(float f) {
-  const uint32_t u = __float_as_uint(f);
+  const uint32_t u = __float_as_uint(f + 0.0f);  // -0 as +0
   return u ^ (uint32_t)(((int32_t)u >> 31) | 0x80000000);
 }
 __device__ __forceinline__ uint64_t key_of(float l, int index) {
@@ -96,11 +107,11 @@ __device__ __forceinline__ int step_of(const Row& r, float l) {
 // temperature, e^(-d / temperature) = 2^(-k / 32) e^x for k the integer nearest to t
 // and x = (k - t) ln 2 / 32, |x| <= ln 2 / 64: 2^(44 + j / 32) from a table, e^x from its
 // Taylor polynomial of degree 5 (truncation below 3e-15).  d is clamped to where the
-// weight is far below 1/2; a difference of infinities counts as 0.
+// weight is far below 1/2.
 __device__ __forceinline__ double weight_of(const Row& r, float l) {
   constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to integers
   constexpr double c = 0.021660849392498290;     // ln 2 / 32
-  const double d = fmin(fmax((double)r.top - (double)l, 0.0), r.deepest);
+  const double d = fmin((double)r.top - (double)l, r.deepest);
   const double t = fma(d, -r.inv_y, kMagic);
   const double x = fma(d, -r.inv_y, kMagic - t);
   double q = fma(x, c * c * c * c * c / 120.0, c * c * c * c / 24.0);
@@ -176,33 +187,52 @@ struct Logits {
   const void* row;
   int vocab, rounds;
   bool aligned;
+  bool infinite = false;
 
   // Round r of wave w: indices 256 (w rounds + r) .., 4 consecutive a lane.
+  __device__ __forceinline__ int base_at(int r) const {
+    return (__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) * rounds + r) * 256;
+  }
   __device__ __forceinline__ int index_at(int r) const {
-    return ((int)(threadIdx.x >> 6) * rounds + r) * 256 + (int)(threadIdx.x & 63) * 4;
+    return base_at(r) + (int)(threadIdx.x & 63) * 4;
   }
   // The thread's 4 logits of round r; what lies past the end as -inf.
   __device__ __forceinline__ void fetch(int r, float (&x)[4]) const {
-    const int i = index_at(r);
-    if (aligned && i + 4 <= vocab) {
+    const int base = base_at(r), lane4 = (int)(threadIdx.x & 63) * 4;
+    if (aligned && base + 256 <= vocab) {
       if constexpr (DT == TM_DTYPE_F32) {
-        const f32x4_t a =
-            *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(row) + i);
+        const f32x4_t a = *reinterpret_cast<const f32x4_t*>(
+            reinterpret_cast<const float*>(row) + base + lane4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = a[e];
       } else {
-        const u16x4_t a =
-            *reinterpret_cast<const u16x4_t*>(reinterpret_cast<const uint16_t*>(row) + i);
+        const u16x4_t a = *reinterpret_cast<const u16x4_t*>(
+            reinterpret_cast<const uint16_t*>(row) + base + lane4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = Half16<DT>::to_f32(a[e]);
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = i + e < vocab ? tm_load1<DT>(row, i + e) : -INFINITY;
+      for (int e = 0; e < 4; ++e) {
+        const int i = base + lane4 + e;
+        x[e] = i < vocab ? tm_load1<DT>(row, i) : -INFINITY;
+      }
     }
   }
-  // NaN as -inf, -0 as +0.
-  static __device__ __forceinline__ float clean(float x) { return x == x ? x + 0.0f : -INFINITY; }
+  // NaN as -inf; where +inf is the largest logit, those as 0 and all others as -inf.
+  __device__ __forceinline__ float clean(float x) const {
+    x = fmaxf(x, -INFINITY);
+    return !infinite ? x : x == INFINITY ? 0.0f : -INFINITY;
+  }
+  __device__ __forceinline__ void make_infinite() {
+    infinite = true;
+    if constexpr (REG) {
+#pragma unroll
+      for (int r = 0; r < kRegRounds; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[r][e] = clean(v[r][e]);
+    }
+  }
   __device__ __forceinline__ void hold() {
     if constexpr (REG) {
 #pragma unroll
@@ -439,21 +469,20 @@ __device__ __forceinline__ float max_block(Shared& s, float v) {
 }
 
 // The logit `depth` temperatures below the largest, or a little less: 2^-19 of the terms
-// covers the roundings here and in step_of, a few 2^-24 of them.
+// covers the roundings here and in step_of, a few 2^-24 of them.  Above -infinity.
 __device__ __forceinline__ float below(const Row& row, float depth) {
-  if (row.top == INFINITY) return INFINITY;
   const float d = depth / row.inv_t;
-  return row.top - d - 1.9e-6f * (d + fabsf(row.top));
+  return fmaxf(row.top - d - 1.9e-6f * (d + fabsf(row.top)), -3.402823466e38f);
 }
 
-// A value that at least `k` (<= 1024) of the threads' `most` reach, -infinity where
+// A value that at least `k` (<= 1024) of the threads' `most` reach, the lowest one where
 // fewer of them weigh anything.
 __device__ __forceinline__ float reached_by(Shared& s, const Row& row, float most, int k) {
   clear_bins<false>(s);
   const int step = step_of(row, most);
   if (step >= 0) atomicAdd(&s.count[step], 1u);
   find_bin<false>(s, (uint64_t)k, 1.0);
-  if (s.found < 0) return -INFINITY;
+  if (s.found < 0) return -3.402823466e38f;
   return below(row, (float)(s.found + 1) * (kSpan / (float)kBins));
 }
 
@@ -468,6 +497,7 @@ __global__ void __launch_bounds__(kThreads) tm_sample_kernel(SampleParams p) {
   lg.vocab = p.vocab;
   lg.rounds = (p.vocab + kRound - 1) / kRound;
   lg.aligned = p.aligned != 0;
+  const double power = kPowers[t & 31];
   lg.hold();
   double temp = p.temperatures ? (double)p.temperatures[n] : p.temperature;
   const float u = p.uniforms[n];
@@ -475,7 +505,7 @@ __global__ void __launch_bounds__(kThreads) tm_sample_kernel(SampleParams p) {
   const double top_p = p.top_ps ? (double)p.top_ps[n] : p.top_p;
   const double min_p = p.min_ps ? (double)p.min_ps[n] : p.min_p;
   float* const probs = p.probs ? p.probs + n * p.probs_stride : nullptr;
-  if (t < 32) s.powers[t] = exp2((double)t / 32.0) * kUnit;
+  if (t < 32) s.powers[t] = power;
 
   float most = -INFINITY;  // of this thread's logits
   lg.rounds_of([&](int, int, const float (&x)[4]) {
@@ -505,6 +535,11 @@ __global__ void __launch_bounds__(kThreads) tm_sample_kernel(SampleParams p) {
   }
   temp = fmax(temp, 1e-300);  // its inverse finite
   row.inv_t = (float)(1.0 / temp);
+  if (row.top == INFINITY) {
+    lg.make_infinite();
+    most = most == INFINITY ? 0.0f : -INFINITY;
+    row.top = 0.0f;
+  }
   row.inv_y = 46.166241308446828384 / temp;
   row.deepest = 32.5 * temp;  // 2^44 e^-32.5 < 0.14
   row.powers = s.powers;
@@ -520,7 +555,7 @@ __global__ void __launch_bounds__(kThreads) tm_sample_kernel(SampleParams p) {
 
   // a value above which all lies that can be kept, where one is known beforehand
   bool listed = true;
-  float above = -INFINITY;
+  float above = 0.0f;
   if (f.by_k && top_k <= kThreads) {
     above = reached_by(s, row, most, top_k);
   } else if (f.by_k) {
@@ -548,23 +583,21 @@ __global__ void __launch_bounds__(kThreads) tm_sample_kernel(SampleParams p) {
         for (int e = 0; e < 4; ++e) sum += weight_of(row, x[e]);
       }
       if (!listed) return;
+      if (!__any(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= above)) return;
       uint64_t m[4];
       int more = 0, before = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        m[e] = __ballot(x[e] >= above && x[e] != -INFINITY);
+        m[e] = __ballot(x[e] >= above);
         more += __popcll(m[e]);
-      }
-      if (more == 0) return;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
         before += (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m[e] >> 32),
                                                  __builtin_amdgcn_mbcnt_lo((uint32_t)m[e], 0u));
+      }
       if (count + more <= kList) {
         int at = count + before;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if ((m[e] >> lane) & 1) s.list[wave][at++] = key_of(x[e], i + e);
+          if (x[e] >= above) s.list[wave][at++] = key_of(x[e], i + e);
       }
       count += more;
     });
@@ -613,6 +646,40 @@ __global__ void __launch_bounds__(kThreads) tm_sample_kernel(SampleParams p) {
       for (int i = lane; i < list.n; i += 64) s.weight[(int)first + i] = list.keys[i];
       if (t < kRankStep) s.weight[n_all + t] = 0;
       __syncthreads();  // (also: the zeros before the kept probabilities)
+      if (n_all <= 64) {
+        // one wave, without further barriers
+        if (wave > 0) return;
+        const uint64_t key = t < n_all ? s.weight[t] : 0;
+        int rank = 0;
+        for (int j = 0; j < n_all; j += kRankStep)
+#pragma unroll
+          for (int e = 0; e < kRankStep; ++e) rank += s.weight[j + e] > key ? 1 : 0;
+        double wd = t < n_all ? kept(row, logit_of(key), key, 0, 0.0) : 0.0;
+        uint64_t w = fixed_of(wd);
+        int keep = f.by_k && f.k < (uint64_t)n_all ? (int)f.k : n_all;
+        if (f.by_p) {
+          // the order's weights, exchanged through LDS within the wave
+          if (t < n_all) s.list[0][rank] = w;
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          const uint64_t o = t < keep ? s.list[0][t] : 0;
+          const uint64_t upto = scan_wave(o);
+          if (f.p_target == 0) {
+            const double want = ceil(top_p * (double)last_lane(upto));
+            f.p_target = want > 1.0 ? (uint64_t)want : 1;
+          }
+          keep = __popcll(__ballot(t < keep && upto - o < f.p_target));
+        }
+        if (rank >= keep || wd < f.min_w) {
+          wd = 0.0;
+          w = 0;
+        }
+        const uint64_t upto = scan_wave(w);
+        const uint64_t total = last_lane(upto), run = upto - w;
+        const uint64_t goal = goal_of(u, total);
+        if (run <= goal && goal < upto) p.tokens[n] = index_of(key);
+        if (probs && w > 0) probs[index_of(key)] = (float)(wd / (double)total);
+        return;
+      }
       uint64_t key = 0, w = 0;
       double wd = 0.0;
       int rank = 0;
