@@ -108,26 +108,30 @@ def fast_binding():
 
 
 @functools.cache
+def layer_binding():
+    """The CPython binding _tmlayer, or None where it is not built or
+    TREEMOE_AMD_LIB names a library other than the one it is linked to."""
+    if _LIB_PATH.resolve() != Path(__file__).resolve().parent / "libtreemoe_amd.so":
+        return None
+    try:
+        from treemoe_spec_amd import _tmlayer
+    except ImportError:
+        return None
+    return _tmlayer
+
+
+@functools.cache
 def entry(name: str):
-    """An entry point as a callable that returns its status: the CPython binding
-    _tmlayer where it is built for the library in use, else ctypes."""
-    lib()
-    if _LIB_PATH.resolve() == Path(__file__).resolve().parent / "libtreemoe_amd.so":
-        try:
-            from treemoe_spec_amd import _tmlayer
-
-            return getattr(_tmlayer, name)
-        except ImportError:
-            pass
-    return getattr(lib(), name)
+    """An entry point as a callable that returns its status: that of the CPython
+    binding where there is one, else ctypes."""
+    return getattr(layer_binding() or lib(), name)
 
 
-def launch(name: str, device, *args) -> None:
-    """An entry point on torch's current stream of ``device`` (a torch.device with
-    an index), with that device current during the call."""
+def launch(name: str, index: int, *args) -> None:
+    """An entry point on torch's current stream of device ``index``, with that device
+    current during the call."""
     import torch
 
-    index = device.index
     if index == torch._C._cuda_getDevice():
         rc = entry(name)(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
@@ -137,23 +141,20 @@ def launch(name: str, device, *args) -> None:
         check(rc, name)
 
 
+@functools.cache
 def dtype_code(dtype) -> int | None:
     """TM_DTYPE_* of a torch dtype, None for one that the kernels do not take."""
-    global _dtype_codes
-    if _dtype_codes is None:
-        import torch
+    import torch
 
-        _dtype_codes = {torch.float32: TM_DTYPE_F32, torch.bfloat16: TM_DTYPE_BF16,
-                        torch.float16: TM_DTYPE_F16}
-    return _dtype_codes.get(dtype)
-
-
-_dtype_codes: dict | None = None
+    return {torch.float32: TM_DTYPE_F32, torch.bfloat16: TM_DTYPE_BF16,
+            torch.float16: TM_DTYPE_F16}.get(dtype)
 
 
 def require(what: str, device, **tensors) -> None:
     """All given tensors on ``device``, a ROCm device, and none that a gradient is
-    asked of: these operators have no backward pass."""
+    asked of: these operators have no backward pass.  (Callers look for the common
+    case themselves and come here for the error: host time is what bounds their
+    smallest calls.)"""
     import torch
 
     if device.type != "cuda":

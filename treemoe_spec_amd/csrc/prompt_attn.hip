@@ -144,10 +144,14 @@ struct Loader {
   int lane_off[kLoads]; // of this lane's piece from the stage's first row
   int pages[kLoads];    // the next stage's pages, looked up a stage ahead
   int first;            // the next stage's first key (paged)
+  int step;             // keys from one stage to the next
 
+  // of the waves that load a stage together
+  static __device__ __forceinline__ int wave() {
+    return NW == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  }
   __device__ __forceinline__ int key_in(int i) const {  // within the stage
-    return ((int)(threadIdx.x >> 6) * kLoads + i) * S::kKeysPerLoad +
-           (int)(threadIdx.x & 63) / S::kChunks;
+    return (wave() * kLoads + i) * S::kKeysPerLoad + (int)(threadIdx.x & 63) / S::kChunks;
   }
   __device__ __forceinline__ int chunk_off(int i) const {
     const int j = key_in(i);
@@ -157,14 +161,17 @@ struct Loader {
     if constexpr (PAGED) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i)
+        // (a stage behind the last one looks up the last key again)
         pages[i] = p.table[(first + min(key_in(i), left)) >> p.page_shift];
     }
   }
   // From key `begin` on of the sequence whose first row is `row0` and last key `last`.
   __device__ __forceinline__ void start(const PromptParams& p, const uint16_t* row0,
-                                        int64_t row_stride, int begin, int last) {
+                                        int64_t row_stride, int begin, int last,
+                                        int step_ = kKeys) {
     at = PAGED ? row0 : row0 + (int64_t)begin * row_stride;
-    stage_stride = kKeys * row_stride;
+    step = step_;
+    stage_stride = step * row_stride;
     stride = (int)row_stride;
     left = last - begin;
     first = begin;
@@ -173,7 +180,6 @@ struct Loader {
     look_up(p);
   }
   __device__ __forceinline__ void load(const PromptParams& p, uint8_t* tile) {
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     if constexpr (PAGED) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
@@ -181,10 +187,10 @@ struct Loader {
         const int64_t o = (int64_t)min(max(pages[i], 0), p.cache_pages - 1) * p.stride_page +
                           (int64_t)slot * stride + chunk_off(i);
         __builtin_amdgcn_global_load_lds((glb_void*)(at + o),
-                                         (lds_void*)(tile + (wave * kLoads + i) * 1024), 16, 0, 0);
+                                         (lds_void*)(tile + (wave() * kLoads + i) * 1024), 16, 0, 0);
       }
-      first += kKeys;
-      left -= kKeys;
+      first += step;
+      left -= step;
       look_up(p);
     } else {
       const bool whole = left >= kKeys - 1;
@@ -192,10 +198,10 @@ struct Loader {
       for (int i = 0; i < kLoads; ++i) {
         const int o = whole ? lane_off[i] : min(key_in(i), left) * stride + chunk_off(i);
         __builtin_amdgcn_global_load_lds((glb_void*)(at + (uint32_t)o),
-                                         (lds_void*)(tile + (wave * kLoads + i) * 1024), 16, 0, 0);
+                                         (lds_void*)(tile + (wave() * kLoads + i) * 1024), 16, 0, 0);
       }
       at += stage_stride;
-      left -= kKeys;
+      left -= step;
     }
   }
 };
@@ -383,6 +389,21 @@ __device__ __forceinline__ Item item_of(const PromptParams& p, int at, int rows)
   return it;
 }
 
+// Elements e .. e + 3 of row `row` of a sequence whose first query is q0, divided by the
+// row's sum (0 where nothing was seen; NaN stays).
+template <int DT>
+__device__ __forceinline__ void store_row(const PromptParams& p, int q0, int row, int kvhead,
+                                          int hd, int e, f32x4_t o, float sum) {
+  const float inv = sum > 0.0f ? 1.0f / sum : sum;
+  const int token = row / p.group;
+  const int head = kvhead * p.group + row - token * p.group;
+  u32x2_t w;
+  w.x = tm_pack2<DT>(o[0] * inv, o[1] * inv);
+  w.y = tm_pack2<DT>(o[2] * inv, o[3] * inv);
+  *reinterpret_cast<u32x2_t*>(p.out + (int64_t)(q0 + token) * p.out_stride + (int64_t)head * hd +
+                              e) = w;
+}
+
 // NW waves of 32 rows.  NW = 8: the two waves of a SIMD take turns, one in the matrix
 // products of its stage while the other weighs, a barrier between the turns.
 // NW = 4: two workgroups a CU, which drift apart by themselves.
@@ -546,7 +567,7 @@ __global__ void __launch_bounds__(64 * NW, 2) tm_prompt_attn_kernel(PromptParams
   const float l = r.l + __shfl_xor(r.l, 32);
   if (!ok) return;
   if (it.slot < 0) {
-    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // NaN stays
+    const float inv = l > 0.0f ? 1.0f / l : l;  // (as store_row)
     uint16_t* const o = p.out + (int64_t)(it.q0 + token) * p.out_stride + (int64_t)head * HD +
                         4 * half;
 #pragma unroll
@@ -574,13 +595,141 @@ __global__ void __launch_bounds__(64 * NW, 2) tm_prompt_attn_kernel(PromptParams
   }
 }
 
-// Joins the partials of one row in key order: a wave takes a row of one tile and KV
-// head, two elements of the head dimension a lane (hd 128) or one (hd 64).
+// Few rows (a decoded token's heads): a tile of 32, and the four waves take the stages
+// of the range in turn, each with its own part of LDS and no barrier between them, so
+// that a CU has 128 KB of keys under way.  A wave asks for its next K when it has the
+// scores, for its next V when it has the products.  At the end the waves' outputs are
+// joined through LDS.
+template <int DT, int HD, bool PAGED>
+__global__ void __launch_bounds__(kThreads, 1) tm_prompt_few_kernel(PromptParams p) {
+  typedef Shape<HD> S;
+  constexpr int kLoads = Loader<HD, PAGED, 1, false>::kLoads;
+  __shared__ __attribute__((aligned(1024))) uint8_t s_k[4][S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_v[4][S::kTile];
+  __shared__ float s_stat[4][32][2];
+
+  const int kvhead = (int)blockIdx.x % p.kvh;
+  const Item it = item_of(p, (int)blockIdx.x / p.kvh, 32);
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, c32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int past = it.k_len - it.q_len;
+  const int all_rows = it.q_len * p.group;
+
+  // row c32 of the tile, in every wave
+  const int first = it.tile * 32;
+  const bool ok = first + c32 < all_rows;
+  const int token = ok ? (first + c32) / p.group : 0;
+  const int head = kvhead * p.group + (ok ? first + c32 - token * p.group : 0);
+  Rows<HD> r;
+  const int n = it.end > it.begin ? (it.end - it.begin + kKeys - 1) / kKeys : 0;
+  Loader<HD, PAGED, 1, false> lk;
+  Loader<HD, PAGED, 1, true> lv;
+  uint8_t* const kt = s_k[wave];
+  uint8_t* const vt = s_v[wave];
+  if (wave < n) {
+    const int64_t k0 = (int64_t)kvhead * HD + (PAGED ? 0 : (int64_t)it.k0 * p.k_stride);
+    const int64_t v0 = (int64_t)kvhead * HD + (PAGED ? 0 : (int64_t)it.k0 * p.v_stride);
+    const int begin = it.begin + wave * kKeys;
+    lk.start(p, p.k + k0, p.k_stride, begin, it.k_len - 1, 4 * kKeys);
+    lk.load(p, kt);
+    lv.start(p, p.v + v0, p.v_stride, begin, it.k_len - 1, 4 * kKeys);
+    lv.load(p, vt);
+  }
+  {
+    const uint16_t* const qr =
+        p.q + (int64_t)(it.q0 + token) * p.q_stride + (int64_t)head * HD + 8 * half;
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) {
+      const u32x4_t x = *reinterpret_cast<const u32x4_t*>(qr + 16 * ks);
+      const u32x4_t zero = {0u, 0u, 0u, 0u};
+      r.q[ks] = ok ? x : zero;
+    }
+  }
+#pragma unroll
+  for (int ht = 0; ht < HD / 32; ++ht)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) r.o[ht][x] = 0.0f;
+  r.m = -INFINITY;
+  r.l = 0.0f;
+  r.seen = min(ok ? past + token : -1, it.end - 1);
+  const int full = min(first + 32 <= all_rows ? past + first / p.group : -1, it.end - 1);
+
+  for (int s = wave; s < n; s += 4) {
+    const int kb = it.begin + s * kKeys;
+    const bool more = s + 4 < n;
+    if (s == wave)
+      wait_vm<0>();  // K and V, the query rows and the pages
+    else
+      wait_vm<kLoads>();  // K: V is behind it
+    products<DT, HD, false, true>(vt, kt, r);
+    __builtin_amdgcn_sched_barrier(0);
+    if (more) lk.load(p, kt);
+    weigh<DT, HD>(p.scale_log2, kb, kb + kKeys - 1 > full, r);
+    if (more)
+      wait_vm<kLoads>();
+    else
+      wait_vm<0>();
+    products<DT, HD, true, false>(vt, kt, r);
+    __builtin_amdgcn_sched_barrier(0);
+    if (more) lv.load(p, vt);
+  }
+  const float l = r.l + __shfl_xor(r.l, 32);
+
+  // each wave's O [32][HD] where its K was
+  float* const mine = reinterpret_cast<float*>(kt) + c32 * HD + 4 * half;
+#pragma unroll
+  for (int ht = 0; ht < HD / 32; ++ht)
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      *reinterpret_cast<f32x4_t*>(mine + 32 * ht + 8 * x) =
+          f32x4_t{r.o[ht][4 * x], r.o[ht][4 * x + 1], r.o[ht][4 * x + 2], r.o[ht][4 * x + 3]};
+  if (half == 0) {
+    s_stat[wave][c32][0] = r.m;
+    s_stat[wave][c32][1] = l;
+  }
+  __syncthreads();
+  constexpr int kLanes = HD / 4;  // of a row, four elements each
+  for (int row = tid / kLanes; row < 32; row += kThreads / kLanes) {
+    if (first + row >= all_rows) break;
+    float m = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) m = fmaxf(m, s_stat[w][row][0]);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float a = __builtin_amdgcn_exp2f(s_stat[w][row][0] - ref);
+      sum += s_stat[w][row][1] * a;
+      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(
+          reinterpret_cast<const float*>(s_k[w]) + row * HD + 4 * (tid % kLanes));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += x[e] * a;
+    }
+    if (it.slot < 0) {
+      store_row<DT>(p, it.q0, first + row, kvhead, HD, 4 * (tid % kLanes), o, sum);
+    } else {
+      const int64_t slot = ((int64_t)it.slot * p.kvh + kvhead) * 32 + row;
+      *reinterpret_cast<f32x4_t*>(p.part + slot * HD + 4 * (tid % kLanes)) = o;
+      if (tid % kLanes == 0) {
+        p.stats[slot * 2] = m;
+        p.stats[slot * 2 + 1] = sum;
+      }
+    }
+  }
+}
+
+constexpr int kMaxChunks = 512;  // of one tile's keys
+
+// Joins the partials of one row, a wave each: the maximum and the sum over the chunks
+// first, a lane per chunk, then the weighted outputs in chunk order, four elements a
+// lane and the lanes' groups a chunk each.
 template <int DT, int HD>
-__global__ void __launch_bounds__(kThreads) tm_prompt_join_kernel(PromptParams p, int rows) {
-  const int lane = threadIdx.x & 63;
-  const int unit = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6);
-  const int r = unit % rows;
+__global__ void __launch_bounds__(kThreads) tm_prompt_join_kernel(PromptParams p, int tile_rows,
+                                                                  int rows) {
+  __shared__ float s_a[4][kMaxChunks];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int unit = (int)blockIdx.x * 4 + wave;
+  const int r = unit % rows;          // of the tile's `rows` that may hold some
   const int kv = unit / rows;
   const int kvhead = kv % p.kvh, at = kv / p.kvh;
   Join j;
@@ -594,27 +743,39 @@ __global__ void __launch_bounds__(kThreads) tm_prompt_join_kernel(PromptParams p
     j.slot0 = at * p.chunks;
     j.count = p.chunks;
   }
-  const int64_t row = (int64_t)j.tile * rows + r;
-  if (row >= (int64_t)j.q_len * p.group) return;
-  constexpr int E = HD / 64;
-  float m = -INFINITY, l = 0.0f, o[E] = {};
-  for (int c = 0; c < j.count; ++c) {
-    const int64_t slot = ((int64_t)(j.slot0 + c) * p.kvh + kvhead) * rows + r;
-    const float m1 = p.stats[slot * 2], l1 = p.stats[slot * 2 + 1];
-    const float mn = fmaxf(m, m1);
-    const float ref = mn == -INFINITY ? 0.0f : mn;
-    const float a = exp2f(m - ref), b = exp2f(m1 - ref);
-    l = l * a + l1 * b;
+  const int row = j.tile * tile_rows + r;
+  if (row >= j.q_len * p.group) return;
+  const int64_t slot0 = ((int64_t)j.slot0 * p.kvh + kvhead) * tile_rows + r;
+  const int64_t step = (int64_t)p.kvh * tile_rows;  // from chunk to chunk
+  float m = -INFINITY;
+  for (int c = lane; c < j.count; c += 64) m = fmaxf(m, p.stats[(slot0 + c * step) * 2]);
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * a + p.part[slot * HD + lane * E + e] * b;
-    m = mn;
+  for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float sum = 0.0f;
+  for (int c = lane; c < j.count; c += 64) {
+    const float a = __builtin_amdgcn_exp2f(p.stats[(slot0 + c * step) * 2] - ref);
+    sum += p.stats[(slot0 + c * step) * 2 + 1] * a;
+    s_a[wave][c] = a;
   }
-  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-  const int token = (int)(row / p.group), g = (int)(row - (int64_t)token * p.group);
-  uint16_t* const out = p.out + (int64_t)(j.q0 + token) * p.out_stride +
-                        (int64_t)(kvhead * p.group + g) * HD + lane * E;
 #pragma unroll
-  for (int e = 0; e < E; ++e) out[e] = Half16<DT>::round(o[e] * inv);
+  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  constexpr int kLanes = HD / 4, kGroups = 64 / kLanes;
+  const float* const from = p.part + slot0 * HD + 4 * (lane % kLanes);
+  f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+  for (int c = lane / kLanes; c < j.count; c += kGroups) {
+    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(from + c * step * HD);
+    const float a = s_a[wave][c];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], a, o[e]);
+  }
+#pragma unroll
+  for (int d = 32; d >= kLanes; d >>= 1)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], d);
+  if (lane < kLanes) store_row<DT>(p, j.q0, row, kvhead, HD, 4 * lane, o, sum);
 }
 
 // ------------------------------------------------------------------- host --
@@ -630,14 +791,22 @@ int64_t tile_keys(int64_t q_len, int64_t k_len, int64_t tile, int64_t rows, int6
   return k_len - q_len + last + 1;
 }
 
-// Rows of a tile: 128 rows a workgroup of which a CU holds two, or 256 where these
-// fill the chip twice over.
-int64_t rows_of(int64_t units128) { return units128 >= 4 * kCUs * kSlotsPerCU ? 256 : 128; }
+// Rows of a tile, by the rows of the longest sequence and the tiles of 128 of all:
+//   32   where no sequence has more: a decoded token's heads;
+//   256  where tiles of 128 would fill the chip's slots four times over;
+//   128  otherwise.
+int64_t rows_of(int64_t longest, int64_t units128) {
+  return longest <= 32 ? 32 : units128 >= 4 * kCUs * kSlotsPerCU ? 256 : 128;
+}
 
-// Key ranges of one sequence's tiles: as many as fill the chip's workgroup slots, at
-// least 4 stages each.
-int64_t chunks_of(int64_t units, int64_t keys) {
-  const int64_t want = kCUs * kSlotsPerCU / std::max<int64_t>(units, 1);
+// Keys of a workgroup's step: a stage, or one of each of the four waves.
+int64_t step_of(int64_t rows) { return rows == 32 ? 4 * kKeys : kKeys; }
+
+// Key ranges of one sequence's tiles: as many as fill the chip's workgroup slots (one a
+// CU for tiles of 32 rows), at least one step or four stages each.
+int64_t chunks_of(int64_t rows, int64_t units, int64_t keys) {
+  const int64_t slots = rows == 32 ? kCUs : kCUs * kSlotsPerCU;
+  const int64_t want = std::min<int64_t>(slots / std::max<int64_t>(units, 1), kMaxChunks);
   return std::max<int64_t>(1, std::min(want, ceil_div(keys, 4 * kKeys)));
 }
 
@@ -655,10 +824,11 @@ int plan_one(int64_t T, int64_t S, int64_t Hq, int64_t kvh, int64_t hd, OnePlan*
   const int64_t group = Hq / kvh;
   if (T < 0 || S < T || S > TM_MAX_PROMPT_KEYS || T * group > INT32_MAX - 1024)
     return TM_ERR_SHAPE;
-  o->rows = rows_of(ceil_div(T * group, 128) * kvh);
+  o->rows = rows_of(T * group, ceil_div(T * group, 128) * kvh);
   o->tiles = ceil_div(T * group, o->rows);
-  o->chunks = chunks_of(o->tiles * kvh, S);
-  o->chunk_len = std::max<int64_t>(kKeys, ceil_div(ceil_div(S, o->chunks), kKeys) * kKeys);
+  o->chunks = chunks_of(o->rows, o->tiles * kvh, S);
+  const int64_t step = step_of(o->rows);
+  o->chunk_len = std::max(step, ceil_div(ceil_div(S, o->chunks), step) * step);
   o->chunks = std::max<int64_t>(1, ceil_div(S, o->chunk_len));
   o->bytes = o->chunks > 1 ? o->tiles * o->chunks * kvh * o->rows * (hd + 2) * 4 : 0;
   return TM_OK;
@@ -666,30 +836,33 @@ int plan_one(int64_t T, int64_t S, int64_t Hq, int64_t kvh, int64_t hd, OnePlan*
 
 template <int DT, int HD, bool PAGED>
 void launch_rows(const PromptParams& p, int64_t rows, int64_t blocks, int64_t joins,
-                 hipStream_t st) {
+                 int64_t join_rows, hipStream_t st) {
   const dim3 grid((unsigned)blocks), block(kThreads);
-  if (rows == 256)
+  if (rows == 32)
+    hipLaunchKernelGGL((tm_prompt_few_kernel<DT, HD, PAGED>), grid, block, 0, st, p);
+  else if (rows == 256)
     hipLaunchKernelGGL((tm_prompt_attn_kernel<DT, HD, 8, PAGED>), grid, dim3(512), 0, st, p);
   else
     hipLaunchKernelGGL((tm_prompt_attn_kernel<DT, HD, 4, PAGED>), grid, block, 0, st, p);
   if (joins > 0)
     hipLaunchKernelGGL((tm_prompt_join_kernel<DT, HD>),
-                       dim3((unsigned)(joins * p.kvh * rows / 4)), block, 0, st, p, (int)rows);
+                       dim3((unsigned)ceil_div(joins * p.kvh * join_rows, 4)), block, 0, st, p,
+                       (int)rows, (int)join_rows);
 }
 
 template <bool PAGED>
 void launch(const PromptParams& p, int dtype, int64_t hd, int64_t rows, int64_t blocks,
-            int64_t joins, hipStream_t st) {
+            int64_t joins, int64_t join_rows, hipStream_t st) {
   if (dtype == TM_DTYPE_F16) {
     if (hd == 128)
-      launch_rows<TM_DTYPE_F16, 128, PAGED>(p, rows, blocks, joins, st);
+      launch_rows<TM_DTYPE_F16, 128, PAGED>(p, rows, blocks, joins, join_rows, st);
     else
-      launch_rows<TM_DTYPE_F16, 64, PAGED>(p, rows, blocks, joins, st);
+      launch_rows<TM_DTYPE_F16, 64, PAGED>(p, rows, blocks, joins, join_rows, st);
   } else {
     if (hd == 128)
-      launch_rows<TM_DTYPE_BF16, 128, PAGED>(p, rows, blocks, joins, st);
+      launch_rows<TM_DTYPE_BF16, 128, PAGED>(p, rows, blocks, joins, join_rows, st);
     else
-      launch_rows<TM_DTYPE_BF16, 64, PAGED>(p, rows, blocks, joins, st);
+      launch_rows<TM_DTYPE_BF16, 64, PAGED>(p, rows, blocks, joins, join_rows, st);
   }
 }
 
@@ -707,7 +880,7 @@ extern "C" int tm_prompt_plan(const int64_t* q_lens, const int64_t* k_lens, int6
   if (sizes == nullptr || B < 0 || (B > 0 && (q_lens == nullptr || k_lens == nullptr)))
     return TM_ERR_ARG;
   const int64_t group = Hq / kvh;
-  int64_t units = 0, q_rows = 0, k_rows = 0;
+  int64_t units = 0, q_rows = 0, k_rows = 0, longest = 0;
   for (int64_t b = 0; b < B; ++b) {
     if (q_lens[b] < 0 || k_lens[b] < q_lens[b] || k_lens[b] > TM_MAX_PROMPT_KEYS)
       return TM_ERR_SHAPE;
@@ -715,15 +888,17 @@ extern "C" int tm_prompt_plan(const int64_t* q_lens, const int64_t* k_lens, int6
     k_rows += k_lens[b];
     if (q_rows * group > INT32_MAX - 1024 || k_rows > INT32_MAX) return TM_ERR_SHAPE;
     units += ceil_div(q_lens[b] * group, 128) * kvh;
+    longest = std::max(longest, q_lens[b] * group);
   }
-  const int64_t rows = rows_of(units);
+  const int64_t rows = rows_of(longest, units);
+  const int64_t step = step_of(rows);
   // stages of all workgroups, and how many one of them may have before its keys are
   // split: twice an even share of the chip's slots
   int64_t stages = 0;
   for (int64_t b = 0; b < B; ++b)
     for (int64_t t = 0; t * rows < q_lens[b] * group; ++t)
       stages += ceil_div(tile_keys(q_lens[b], k_lens[b], t, rows, group), kKeys) * kvh;
-  const int64_t share = std::max<int64_t>(4, ceil_div(stages, kCUs * kSlotsPerCU));
+  const int64_t share = std::max<int64_t>(4, ceil_div(stages, kCUs * (rows == 32 ? 1 : kSlotsPerCU)));
   std::vector<std::pair<int64_t, Item>> list;  // (keys, item)
   std::vector<Join> jlist;
   int64_t q0 = 0, k0 = 0, slots = 0;
@@ -732,7 +907,7 @@ extern "C" int tm_prompt_plan(const int64_t* q_lens, const int64_t* k_lens, int6
       const int64_t keys = tile_keys(q_lens[b], k_lens[b], t, rows, group);
       const int64_t n = ceil_div(keys, kKeys);
       const int64_t chunks = n > 2 * share ? ceil_div(n, share) : 1;
-      const int64_t len = ceil_div(n, chunks) * kKeys;
+      const int64_t len = ceil_div(ceil_div(n, chunks) * kKeys, step) * step;
       const int64_t parts = ceil_div(keys, len);
       for (int64_t c = 0; c < parts; ++c) {
         Item it;
@@ -787,7 +962,7 @@ extern "C" int tm_prompt_attention(const void* q, int64_t q_stride, const void* 
   if (rc) return rc;
   if ((dtype != TM_DTYPE_BF16 && dtype != TM_DTYPE_F16) || !(scale > 0.0f) || scale == INFINITY)
     return TM_ERR_ARG;
-  if ((tile_rows != 128 && tile_rows != 256) || num_items < 0 || num_joins < 0 || num_slots < 0 ||
+  if ((tile_rows != 32 && tile_rows != 128 && tile_rows != 256) || num_items < 0 || num_joins < 0 || num_slots < 0 ||
       num_items * kvh > INT32_MAX || num_joins * kvh * tile_rows / 4 > INT32_MAX ||
       num_slots > INT32_MAX)
     return TM_ERR_SHAPE;
@@ -816,7 +991,8 @@ extern "C" int tm_prompt_attention(const void* q, int64_t q_stride, const void* 
   p.kvh = (int)kvh;
   p.group = (int)(Hq / kvh);
   p.scale_log2 = scale * 1.4426950408889634f;
-  launch<false>(p, dtype, hd, tile_rows, num_items * kvh, num_joins, (hipStream_t)stream);
+  launch<false>(p, dtype, hd, tile_rows, num_items * kvh, num_joins, tile_rows,
+                (hipStream_t)stream);
   TM_HIP_CHECK_LAUNCH();
   return TM_OK;
 }
@@ -889,7 +1065,7 @@ extern "C" int tm_prompt_attention_cached(const void* q, int64_t q_stride, int64
   p.cache_pages = (int)cache_pages;
   p.scale_log2 = scale * 1.4426950408889634f;
   launch<true>(p, dtype, hd, o.rows, o.tiles * o.chunks * kvh, o.chunks > 1 ? o.tiles : 0,
-               (hipStream_t)stream);
+               std::min(o.rows, T * p.group), (hipStream_t)stream);
   TM_HIP_CHECK_LAUNCH();
   return TM_OK;
 }

@@ -54,6 +54,19 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return invoke<F>(F, args, n, indexes(F));
 }
 
+// prompt_cached_workspace(T, seq_len, Hq, kvh, hd) -> (status, bytes)
+PyObject* cached_workspace(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 5) {
+    PyErr_SetString(PyExc_TypeError, "expected 5 arguments");
+    return nullptr;
+  }
+  int64_t a[5], bytes = 0;
+  for (int i = 0; i < 5; ++i) a[i] = convert<int64_t>(args[i]);
+  if (PyErr_Occurred()) return nullptr;
+  const int rc = tm_prompt_cached_workspace(a[0], a[1], a[2], a[3], a[4], &bytes);
+  return Py_BuildValue("iL", rc, (long long)bytes);
+}
+
 #define TM_ENTRY(name) \
   {#name, (PyCFunction)(void (*)(void))entry<name>, METH_FASTCALL, nullptr}
 
@@ -64,7 +77,8 @@ PyMethodDef kMethods[] = {
     TM_ENTRY(tm_rotary_append),
     TM_ENTRY(tm_sample_tokens),
     TM_ENTRY(tm_prompt_attention),
-    TM_ENTRY(tm_prompt_cached_workspace),
+    {"prompt_cached_workspace", (PyCFunction)(void (*)(void))cached_workspace, METH_FASTCALL,
+     nullptr},
     TM_ENTRY(tm_prompt_attention_cached),
     {nullptr, nullptr, 0, nullptr},
 };

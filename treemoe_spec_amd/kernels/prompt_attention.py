@@ -17,6 +17,7 @@ import operator
 import torch
 
 from treemoe_spec_amd import _capi
+from treemoe_spec_amd._capi import dtype_code, ptr
 from treemoe_spec_amd.kv_cache import device_tables_of
 
 
@@ -52,23 +53,28 @@ class PromptPlan:
         self.device = self.items.device
 
 
-def _check_q(q: torch.Tensor, out: torch.Tensor | None) -> tuple[int, int, int, int]:
-    """(dtype code, T, Hq, hd) of q; checks ``out``."""
-    dt = _capi.dtype_code(q.dtype)
+def _check_q(q: torch.Tensor, out: torch.Tensor | None):
+    """(dtype code, T, Hq, hd, token stride of q, of out) of q; checks ``out``."""
+    dt = dtype_code(q.dtype)
     if dt is None or dt == _capi.TM_DTYPE_F32:
         raise ValueError(f"q must be bfloat16 or float16, got {q.dtype}")
-    if q.dim() != 3:
+    shape = q.shape
+    if len(shape) != 3:
         raise ValueError("q must be [T, heads, head_dim]")
-    t, hq, hd = q.shape
+    t, hq, hd = shape
     st = q.stride()
-    if hd not in (64, 128):
+    if hd != 128 and hd != 64:
         raise ValueError(f"head_dim must be 64 or 128, got {hd}")
     if st[2] != 1 or (st[1] != hd and hq > 1):
         raise ValueError("q must have contiguous heads")
-    if out is not None and (out.shape != (t, hq * hd) or out.dtype != q.dtype
-                            or out.stride(1) != 1):
-        raise ValueError("out must be [T, Hq * hd] of q's dtype")
-    return dt, t, hq, hd
+    width = hq * hd
+    os = width
+    if out is not None:
+        if out.shape != (t, width) or out.dtype != q.dtype or out.stride(1) != 1:
+            raise ValueError("out must be [T, Hq * hd] of q's dtype")
+        os = out.stride(0) if t > 1 else width
+    # (the stride of one token says nothing)
+    return dt, t, hq, hd, st[0] if t > 1 else width, os
 
 
 def _check_scale(scale: float | None, hd: int) -> float:
@@ -87,38 +93,50 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pr
     its sequence's keys up to its own position.  Returns [T, Hq * hd]; T and S may
     exceed the plan's rows (a padded batch): in a new result the rows behind the last
     sequence are 0, in ``out`` they stay as they were."""
-    dt, t, hq, hd = _check_q(q, out)
-    dev = q.device
-    _capi.require("prompt_attention", dev, q=q, k=k, v=v, plan=plan.items, out=out)
+    dt, t, hq, hd, qs, os = _check_q(q, out)
+    index = q.get_device()
+    if index < 0 or k.get_device() != index or v.get_device() != index \
+            or plan.items.get_device() != index or out is not None or q.requires_grad \
+            or k.requires_grad or v.requires_grad:
+        _capi.require("prompt_attention", q.device, q=q, k=k, v=v, plan=plan.items, out=out)
     for name, x in (("k", k), ("v", v)):
         if x.dim() != 3 or x.shape[2] != hd or x.dtype != q.dtype or x.shape != k.shape:
             raise ValueError("k and v must be [S, kv_heads, head_dim] of q's dtype")
         if x.stride(2) != 1 or (x.stride(1) != hd and x.shape[1] > 1):
             raise ValueError(f"{name} must have contiguous heads")
-    if hq != plan.num_heads or k.shape[1] != plan.num_kv_heads:
+    s, kvh, _ = k.shape
+    if hq != plan.num_heads or kvh != plan.num_kv_heads:
         raise ValueError(f"the plan is for {plan.num_heads} heads over {plan.num_kv_heads}, "
-                         f"got {hq} over {k.shape[1]}")
-    if t < plan.q_rows or k.shape[0] < plan.k_rows:
+                         f"got {hq} over {kvh}")
+    if t < plan.q_rows or s < plan.k_rows:
         raise ValueError(f"the plan's sequences need {plan.q_rows} queries and {plan.k_rows} "
-                         f"keys, got {t} and {k.shape[0]}")
+                         f"keys, got {t} and {s}")
     scale = _check_scale(scale, hd)
     if out is None:
-        out = torch.empty((t, hq * hd), dtype=q.dtype, device=dev)
+        out = torch.empty((t, hq * hd), dtype=q.dtype, device=q.device)
         if t > plan.q_rows:
             out[plan.q_rows:].zero_()
-    nbytes = plan.num_slots * plan.num_kv_heads * plan.tile_rows * (hd + 2) * 4
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _capi.launch("tm_prompt_attention", dev, q.data_ptr(), _stride(q, hq * hd), k.data_ptr(),
-                 _stride(k, k.shape[1] * hd), v.data_ptr(), _stride(v, k.shape[1] * hd),
-                 plan.items.data_ptr(), plan.num_items, plan.joins.data_ptr(), plan.num_joins,
-                 plan.num_slots, plan.tile_rows, hq, k.shape[1], hd, scale, dt, out.data_ptr(),
-                 _stride(out, hq * hd), _capi.ptr(ws), nbytes)
+    nbytes = plan.num_slots * kvh * plan.tile_rows * (hd + 2) * 4
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _capi.launch("tm_prompt_attention", index, q.data_ptr(), qs, k.data_ptr(),
+                 k.stride(0) if s > 1 else kvh * hd, v.data_ptr(),
+                 v.stride(0) if s > 1 else kvh * hd, plan.items.data_ptr(), plan.num_items,
+                 plan.joins.data_ptr(), plan.num_joins, plan.num_slots, plan.tile_rows, hq, kvh,
+                 hd, scale, dt, out.data_ptr(), os, ptr(ws), nbytes)
     return out
 
 
-def _stride(x: torch.Tensor, width: int) -> int:
-    """Token stride; one token, whose stride says nothing, counts as contiguous."""
-    return x.stride(0) if x.shape[0] > 1 else width
+def _workspace_bytes(*sizes) -> int:
+    """tm_prompt_cached_workspace(T, seq_len, Hq, kvh, hd)."""
+    fast = _capi.layer_binding()
+    if fast is not None:
+        rc, nbytes = fast.prompt_cached_workspace(*sizes)
+        if rc:
+            _capi.check(rc, "tm_prompt_cached_workspace")
+        return nbytes
+    size = ctypes.c_int64()
+    _capi.call("tm_prompt_cached_workspace", *sizes, ctypes.byref(size))
+    return size.value
 
 
 def prompt_attention_cached(q: torch.Tensor, kv, layer: int, *, scale: float | None = None,
@@ -128,42 +146,40 @@ def prompt_attention_cached(q: torch.Tensor, kv, layer: int, *, scale: float | N
     positions 0 .. seq_len - T + t of ``layer``, read in place through the block table.
     The cache is [L, pages, page, kv_heads, head_dim] of q's dtype, page size a power of
     two.  Returns [T, Hq * hd]."""
-    dt, t, hq, hd = _check_q(q, out)
-    dev = q.device
+    dt, t, hq, hd, qs, os = _check_q(q, out)
     kc, vc = kv.k, kv.v
-    _capi.require("prompt_attention_cached", dev, q=q, k_cache=kc, v_cache=vc, out=out)
+    index = q.get_device()
+    if index < 0 or kc.get_device() != index or vc.get_device() != index or out is not None \
+            or q.requires_grad or kc.requires_grad or vc.requires_grad:
+        _capi.require("prompt_attention_cached", q.device, q=q, k_cache=kc, v_cache=vc, out=out)
     cshape, cst = kc.shape, kc.stride()
     if kc.dtype != q.dtype or vc.dtype != q.dtype or vc.shape != cshape or vc.stride() != cst \
             or len(cshape) != 5 or cshape[4] != hd or cst[4] != 1 \
             or (cst[3] != hd and cshape[3] > 1) or cshape[2] != kv.block_size:
         raise ValueError("cache layout must be [L, pages, page, kv_heads, head_dim] of q's dtype")
-    kvh, page = cshape[3], cshape[2]
+    layers, pages, page, kvh, _ = cshape
     if hq % kvh:
         raise ValueError("num_heads must be a multiple of num_kv_heads")
     if page & (page - 1):
         raise ValueError(f"page size must be a power of two, got {page}")
     layer = operator.index(layer)
-    layers = cshape[0]
     if not -layers <= layer < layers:
         raise IndexError(f"layer {layer} is out of range for a cache of {layers} layers")
     seq_len = kv.seq_len
     if t > seq_len:
         raise ValueError(f"{t} queries over a cache of {seq_len} positions")
     scale = _check_scale(scale, hd)
+    dev = q.device
     if out is None:
         out = torch.empty((t, hq * hd), dtype=q.dtype, device=dev)
     if t == 0:
         return out
     table, _ = device_tables_of(kv, dev)
-    size = ctypes.c_int64()
-    rc = _capi.entry("tm_prompt_cached_workspace")(t, seq_len, hq, kvh, hd,
-                                                   ctypes.addressof(size))
-    _capi.check(rc, "tm_prompt_cached_workspace")
-    nbytes = size.value
+    nbytes = _workspace_bytes(t, seq_len, hq, kvh, hd)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     off = kc.element_size() * cst[0] * (layer % layers)
-    _capi.launch("tm_prompt_attention_cached", dev, q.data_ptr(), q.stride(0), t,
-                 kc.data_ptr() + off, vc.data_ptr() + off, cst[1], cst[2], page, cshape[1],
-                 table.data_ptr(), len(kv.block_table), seq_len, hq, kvh, hd, scale, dt,
-                 out.data_ptr(), out.stride(0), _capi.ptr(ws), nbytes)
+    _capi.launch("tm_prompt_attention_cached", index, q.data_ptr(), qs, t, kc.data_ptr() + off,
+                 vc.data_ptr() + off, cst[1], cst[2], page, pages, table.data_ptr(),
+                 len(kv.block_table), seq_len, hq, kvh, hd, scale, dt, out.data_ptr(), os,
+                 ptr(ws), nbytes)
     return out

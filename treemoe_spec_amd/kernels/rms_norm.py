@@ -12,41 +12,51 @@ from __future__ import annotations
 import torch
 
 from treemoe_spec_amd import _capi
+from treemoe_spec_amd._capi import dtype_code
 
 _SCALE_GROUPS = (32, 64, 128, 256, 512)
+_ROWS = torch.contiguous_format
 
 
 def _checked(what, x, weight, eps, residual, residual_out):
-    if x.dim() != 2 or weight.dim() != 1 or weight.shape[0] != x.shape[1]:
+    """(device index, T, H, x's row stride, dtype codes of x, weight and residual)."""
+    shape, wshape = x.shape, weight.shape
+    if len(shape) != 2 or len(wshape) != 1 or wshape[0] != shape[1]:
         raise ValueError("x must be [T, H] and weight [H]")
-    dt, wdt = _capi.dtype_code(x.dtype), _capi.dtype_code(weight.dtype)
+    t, h = shape
+    dt, wdt = dtype_code(x.dtype), dtype_code(weight.dtype)
     if dt is None:
         raise ValueError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
     if wdt != dt and wdt != _capi.TM_DTYPE_F32:
         raise ValueError("weight must have x's dtype or float32")
-    if x.shape[1] < 1 or x.shape[1] > _capi.TM_MAX_NORM_HIDDEN:
-        raise ValueError(f"H must be 1..{_capi.TM_MAX_NORM_HIDDEN}, got {x.shape[1]}")
+    if h < 1 or h > _capi.TM_MAX_NORM_HIDDEN:
+        raise ValueError(f"H must be 1..{_capi.TM_MAX_NORM_HIDDEN}, got {h}")
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
-    _capi.require(what, x.device, x=x, weight=weight, residual=residual,
-                  residual_out=residual_out)
-    if x.stride(1) != 1 or weight.stride(0) != 1:
+    index = x.get_device()
+    if index < 0 or weight.get_device() != index or residual_out is not None \
+            or (residual is not None and (residual.get_device() != index
+                                          or residual.requires_grad)) \
+            or x.requires_grad or weight.requires_grad:
+        _capi.require(what, x.device, x=x, weight=weight, residual=residual,
+                      residual_out=residual_out)
+    xs, step = x.stride()
+    if step != 1 or weight.stride(0) != 1:
         raise ValueError("x and weight must have unit stride along H")
-    if residual is None:
-        if residual_out is not None:
-            raise ValueError("residual_out without a residual")
-        return dt, wdt, 0, None
-    rdt = _capi.dtype_code(residual.dtype)
-    if residual.shape != x.shape or residual.stride(1) != 1:
-        raise ValueError("residual must be [T, H] like x, with unit stride along H")
-    if rdt != dt and rdt != _capi.TM_DTYPE_F32:
-        raise ValueError("residual must have x's dtype or float32")
-    if residual_out is None:
-        residual_out = torch.empty_like(residual, memory_format=torch.contiguous_format)
-    elif residual_out.shape != x.shape or residual_out.dtype != residual.dtype \
-            or residual_out.stride(1) != 1:
-        raise ValueError("residual_out must be [T, H] of the residual's dtype")
-    return dt, wdt, rdt, residual_out
+    rdt = 0
+    if residual is not None:
+        rdt = dtype_code(residual.dtype)
+        if residual.shape != shape or residual.stride(1) != 1:
+            raise ValueError("residual must be [T, H] like x, with unit stride along H")
+        if rdt != dt and rdt != _capi.TM_DTYPE_F32:
+            raise ValueError("residual must have x's dtype or float32")
+        if residual_out is not None and (residual_out.shape != shape
+                                         or residual_out.dtype != residual.dtype
+                                         or residual_out.stride(1) != 1):
+            raise ValueError("residual_out must be [T, H] of the residual's dtype")
+    elif residual_out is not None:
+        raise ValueError("residual_out without a residual")
+    return index, t, h, xs, dt, wdt, rdt
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *,
@@ -57,21 +67,27 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *,
     dtype.  x [T, H] float32, bfloat16 or float16, rows at any stride; weight [H] and
     residual [T, H] in x's dtype or float32.  The norm takes ``s`` before it is
     rounded.  ``out`` may be ``x`` and ``residual_out`` may be ``residual``."""
-    dt, wdt, rdt, residual_out = _checked("rms_norm", x, weight, eps, residual, residual_out)
+    index, t, h, xs, dt, wdt, rdt = _checked("rms_norm", x, weight, eps, residual, residual_out)
     if out is None:
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.stride(1) != 1 \
-            or out.device != x.device:
-        raise ValueError("out must be [T, H] of x's dtype, on x's device")
+        out = torch.empty_like(x, memory_format=_ROWS)
+        os = h
+    else:
+        if out.shape != x.shape or out.dtype != x.dtype or out.stride(1) != 1 \
+                or out.get_device() != index:
+            raise ValueError("out must be [T, H] of x's dtype, on x's device")
+        os = out.stride(0)
     if residual is None:
-        _capi.launch("tm_rms_norm", x.device, x.data_ptr(), x.stride(0), 0, 0, dt,
-                     weight.data_ptr(), wdt, x.shape[0], x.shape[1], eps, dt, out.data_ptr(),
-                     out.stride(0), 0, 0)
+        _capi.launch("tm_rms_norm", index, x.data_ptr(), xs, 0, 0, dt, weight.data_ptr(), wdt,
+                     t, h, eps, dt, out.data_ptr(), os, 0, 0)
         return out
-    _capi.launch("tm_rms_norm", x.device, x.data_ptr(), x.stride(0), residual.data_ptr(),
-                 residual.stride(0), rdt, weight.data_ptr(), wdt, x.shape[0], x.shape[1], eps,
-                 dt, out.data_ptr(), out.stride(0), residual_out.data_ptr(),
-                 residual_out.stride(0))
+    if residual_out is None:
+        residual_out = torch.empty_like(residual, memory_format=_ROWS)
+        ros = h
+    else:
+        ros = residual_out.stride(0)
+    _capi.launch("tm_rms_norm", index, x.data_ptr(), xs, residual.data_ptr(), residual.stride(0),
+                 rdt, weight.data_ptr(), wdt, t, h, eps, dt, out.data_ptr(), os,
+                 residual_out.data_ptr(), ros)
     return out, residual_out
 
 
@@ -86,18 +102,22 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *,
     if scale_group is not None and (scale_group not in _SCALE_GROUPS
                                     or x.shape[-1] % scale_group != 0):
         raise ValueError(f"scale_group must be one of {_SCALE_GROUPS} and divide H")
-    dt, wdt, rdt, residual_out = _checked("rms_norm_fp8", x, weight, eps, residual, residual_out)
-    t, h = x.shape
+    index, t, h, xs, dt, wdt, rdt = _checked("rms_norm_fp8", x, weight, eps, residual,
+                                             residual_out)
     dev = x.device
     out = torch.empty((t, h), dtype=torch.float8_e4m3fn, device=dev)
     groups = 1 if scale_group is None else h // scale_group
     scales = torch.empty((t,) if scale_group is None else (t, groups), dtype=torch.float32,
                          device=dev)
-    none = residual is None
-    _capi.launch("tm_rms_norm_fp8", dev, x.data_ptr(), x.stride(0),
-                 0 if none else residual.data_ptr(), 0 if none else residual.stride(0),
-                 dt if none else rdt, weight.data_ptr(), wdt, t, h, eps, dt, out.data_ptr(), h,
-                 scales.data_ptr(), groups, 0 if scale_group is None else scale_group,
-                 0 if none else residual_out.data_ptr(),
-                 0 if none else residual_out.stride(0))
-    return (out, scales) if none else (out, scales, residual_out)
+    if residual is None:
+        _capi.launch("tm_rms_norm_fp8", index, x.data_ptr(), xs, 0, 0, dt, weight.data_ptr(),
+                     wdt, t, h, eps, dt, out.data_ptr(), h, scales.data_ptr(), groups,
+                     scale_group or 0, 0, 0)
+        return out, scales
+    if residual_out is None:
+        residual_out = torch.empty_like(residual, memory_format=_ROWS)
+    _capi.launch("tm_rms_norm_fp8", index, x.data_ptr(), xs, residual.data_ptr(),
+                 residual.stride(0), rdt, weight.data_ptr(), wdt, t, h, eps, dt, out.data_ptr(),
+                 h, scales.data_ptr(), groups, scale_group or 0, residual_out.data_ptr(),
+                 residual_out.stride(0))
+    return out, scales, residual_out

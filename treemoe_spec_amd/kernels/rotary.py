@@ -18,6 +18,7 @@ from fractions import Fraction
 import torch
 
 from treemoe_spec_amd import _capi
+from treemoe_spec_amd._capi import dtype_code
 from treemoe_spec_amd.kv_cache import device_tables_of
 
 # 2 pi to 36 digits, as a fraction: more than the 64 bits of a turn
@@ -99,7 +100,7 @@ class RotaryPlan:
             freq, self.magnitude = [float(f) for f in inv_freq], 1.0
             if len(freq) != rotary_dim // 2 or not all(math.isfinite(f) for f in freq):
                 raise ValueError("inv_freq must hold rotary_dim / 2 finite values")
-        self.head_dim, self.rotary_dim, self.interleaved = head_dim, rotary_dim, bool(interleaved)
+        self.head_dim, self.rotary_dim, self.interleaved = head_dim, rotary_dim, int(interleaved)
         self.inv_freq = freq
         turns = []
         for f in freq:
@@ -109,14 +110,28 @@ class RotaryPlan:
         self.device = self.turns.device
 
 
-def _heads_of(name: str, t: torch.Tensor, hd: int, dtype, tokens: int) -> None:
-    if t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != hd:
+def _heads_of(name: str, t: torch.Tensor, hd: int, dtype, tokens: int) -> tuple[int, int]:
+    """(heads, token stride) of a [T, heads, hd] tensor."""
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != hd:
         raise ValueError(f"{name} must be [T, heads, {hd}] with {tokens} tokens")
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}")
     st = t.stride()
-    if st[2] != 1 or (st[1] != hd and t.shape[1] > 1):
+    if st[2] != 1 or (st[1] != hd and shape[1] > 1):
         raise ValueError(f"{name} must have contiguous heads")
+    return shape[1], st[0]
+
+
+def _output(name: str, out: torch.Tensor | None, x: torch.Tensor, heads: int, hd: int,
+            index: int) -> tuple[torch.Tensor, int]:
+    """(output like ``x``, its token stride)."""
+    if out is None:
+        return torch.empty_like(x, memory_format=torch.contiguous_format), heads * hd
+    n, stride = _heads_of(name, out, hd, x.dtype, x.shape[0])
+    if n != heads or out.get_device() != index:
+        raise ValueError(f"{name} must have the shape of its input, on the same device")
+    return out, stride
 
 
 def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
@@ -126,40 +141,33 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     or int64); returns (q', k').  float32, bfloat16 or float16, heads contiguous,
     tokens at any 16-byte aligned stride.  ``q_out`` may be ``q``, ``k_out`` may be
     ``k``."""
-    dt, dev, hd = _capi.dtype_code(q.dtype), q.device, plan.head_dim
+    dtype, hd = q.dtype, plan.head_dim
+    dt = dtype_code(dtype)
     if dt is None:
-        raise ValueError(f"q must be float32, bfloat16 or float16, got {q.dtype}")
-    _capi.require("rotary_embed", dev, q=q, k=k, positions=positions, plan=plan.turns,
-                  q_out=q_out, k_out=k_out)
+        raise ValueError(f"q must be float32, bfloat16 or float16, got {dtype}")
+    index = q.get_device()
+    turns = plan.turns
+    if index < 0 or positions.get_device() != index or turns.get_device() != index \
+            or q.requires_grad or (k is not None and (k.get_device() != index
+                                                      or k.requires_grad)):
+        _capi.require("rotary_embed", q.device, q=q, k=k, positions=positions, plan=turns)
     t = q.shape[0]
-    _heads_of("q", q, hd, q.dtype, t)
-    if positions.dim() != 1 or positions.shape[0] != t or positions.dtype not in (
-            torch.int32, torch.int64) or (t > 1 and positions.stride(0) != 1):
+    heads, qs = _heads_of("q", q, hd, dtype, t)
+    wide = positions.dtype == torch.int64
+    if positions.shape != (t,) or not (wide or positions.dtype == torch.int32) \
+            or (t > 1 and positions.stride(0) != 1):
         raise ValueError("positions must be a contiguous int32 or int64 tensor of T entries")
-    if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    else:
-        _heads_of("q_out", q_out, hd, q.dtype, t)
-        if q_out.shape != q.shape:
-            raise ValueError("q_out must have q's shape")
+    q_out, qos = _output("q_out", q_out, q, heads, hd, index)
     kp = ks = kop = kos = kvh = 0
     if k is not None:
-        _heads_of("k", k, hd, q.dtype, t)
-        if k_out is None:
-            k_out = torch.empty(k.shape, dtype=k.dtype, device=dev)
-        else:
-            _heads_of("k_out", k_out, hd, q.dtype, t)
-            if k_out.shape != k.shape:
-                raise ValueError("k_out must have k's shape")
-        kp, ks, kop, kos, kvh = k.data_ptr(), k.stride(0), k_out.data_ptr(), k_out.stride(0), \
-            k.shape[1]
+        kvh, ks = _heads_of("k", k, hd, dtype, t)
+        k_out, kos = _output("k_out", k_out, k, kvh, hd, index)
+        kp, kop = k.data_ptr(), k_out.data_ptr()
     elif k_out is not None:
         raise ValueError("k_out without k")
-    _capi.launch("tm_rotary", dev, q.data_ptr(), q.stride(0), kp, ks, q_out.data_ptr(),
-                 q_out.stride(0), kop, kos, positions.data_ptr(),
-                 1 if positions.dtype == torch.int64 else 0, plan.turns.data_ptr(),
-                 plan.magnitude, t, q.shape[1], kvh, hd, plan.rotary_dim,
-                 1 if plan.interleaved else 0, dt)
+    _capi.launch("tm_rotary", index, q.data_ptr(), qs, kp, ks, q_out.data_ptr(), qos, kop, kos,
+                 positions.data_ptr(), 1 if wide else 0, turns.data_ptr(), plan.magnitude, t,
+                 heads, kvh, hd, plan.rotary_dim, plan.interleaved, dt)
     return q_out, k_out
 
 
@@ -169,20 +177,26 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Rotar
     rotated, and stores the rotated k and v [T, kvh, hd] at those positions of the
     paged cache ``kv``, mapping pages as ``append`` does (treemoe/model/kv_cache.py:
     62-78); ``kv.seq_len`` grows to cover them."""
-    dt, dev, hd = _capi.dtype_code(q.dtype), q.device, plan.head_dim
+    dtype, hd = q.dtype, plan.head_dim
+    dt = dtype_code(dtype)
     if dt is None:
-        raise ValueError(f"q must be float32, bfloat16 or float16, got {q.dtype}")
-    kc, vc = kv.k, kv.v
-    _capi.require("rotary_append", dev, q=q, k=k, v=v, plan=plan.turns, q_out=q_out,
-                  k_cache=kc, v_cache=vc)
+        raise ValueError(f"q must be float32, bfloat16 or float16, got {dtype}")
+    kc, vc, turns = kv.k, kv.v, plan.turns
+    index = q.get_device()
+    if index < 0 or k.get_device() != index or v.get_device() != index \
+            or turns.get_device() != index or kc.get_device() != index \
+            or vc.get_device() != index or q.requires_grad or k.requires_grad \
+            or v.requires_grad or kc.requires_grad or vc.requires_grad:
+        _capi.require("rotary_append", q.device, q=q, k=k, v=v, plan=turns, k_cache=kc,
+                      v_cache=vc)
     t = q.shape[0]
-    for name, x in (("q", q), ("k", k), ("v", v)):
-        _heads_of(name, x, hd, q.dtype, t)
-    kvh = k.shape[1]
-    if v.shape != k.shape:
+    heads, qs = _heads_of("q", q, hd, dtype, t)
+    kvh, ks = _heads_of("k", k, hd, dtype, t)
+    vh, vs = _heads_of("v", v, hd, dtype, t)
+    if vh != kvh:
         raise ValueError("k and v must have the same shape")
     cshape, cst = kc.shape, kc.stride()
-    if kc.dtype != q.dtype or vc.dtype != q.dtype or vc.shape != cshape or vc.stride() != cst \
+    if kc.dtype != dtype or vc.dtype != dtype or vc.shape != cshape or vc.stride() != cst \
             or len(cshape) != 5 or cshape[3] != kvh or cshape[4] != hd or cst[4] != 1 \
             or (cst[3] != hd and kvh > 1) or cshape[2] != kv.block_size:
         raise ValueError("cache layout must be [L, pages, page, kv_heads, head_dim] of q's dtype")
@@ -192,23 +206,17 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Rotar
         raise IndexError(f"layer {layer} is out of range for a cache of {layers} layers")
     if start_pos < 0:
         raise ValueError("start_pos must not be negative")
-    if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    else:
-        _heads_of("q_out", q_out, hd, q.dtype, t)
-        if q_out.shape != q.shape:
-            raise ValueError("q_out must have q's shape")
+    q_out, qos = _output("q_out", q_out, q, heads, hd, index)
     if t == 0:
         return q_out
     end = start_pos + t
     kv._ensure_capacity(end)
-    table, _ = device_tables_of(kv, dev)
+    table, _ = device_tables_of(kv, q.device)
     off = kc.element_size() * cst[0] * (layer % layers)
-    _capi.launch("tm_rotary_append", dev, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0),
-                 v.data_ptr(), v.stride(0), q_out.data_ptr(), q_out.stride(0),
-                 kc.data_ptr() + off, vc.data_ptr() + off, cst[1], cst[2], kv.block_size,
-                 cshape[1], table.data_ptr(), len(kv.block_table), start_pos,
-                 plan.turns.data_ptr(), plan.magnitude, t, q.shape[1], kvh, hd,
-                 plan.rotary_dim, 1 if plan.interleaved else 0, dt)
+    _capi.launch("tm_rotary_append", index, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+                 q_out.data_ptr(), qos, kc.data_ptr() + off, vc.data_ptr() + off, cst[1], cst[2],
+                 cshape[2], cshape[1], table.data_ptr(), len(kv.block_table), start_pos,
+                 turns.data_ptr(), plan.magnitude, t, heads, kvh, hd, plan.rotary_dim,
+                 plan.interleaved, dt)
     kv.seq_len = max(kv.seq_len, end)
     return q_out

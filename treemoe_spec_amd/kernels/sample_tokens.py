@@ -16,6 +16,7 @@ import sys
 import torch
 
 from treemoe_spec_amd import _capi
+from treemoe_spec_amd._capi import dtype_code, ptr
 
 
 def _per_row(name, value, n, dtype, lo, hi):
@@ -25,7 +26,7 @@ def _per_row(name, value, n, dtype, lo, hi):
                 or (n > 1 and value.stride(0) != 1):
             raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor of N entries")
         return value, lo
-    value = operator.index(value) if dtype == torch.int32 else float(value)
+    value = operator.index(value) if dtype is torch.int32 else float(value)
     if not lo <= value <= hi:
         raise ValueError(f"{name} must be {lo}..{hi}, got {value}")
     return None, value
@@ -51,39 +52,44 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *,
     ``return_probs`` returns (tokens, probs): the distribution of every row, float32
     [N, V], in ``probs_out`` where given: the rows that ``fused_verify_commit`` takes
     as ``draft_probs``."""
-    if logits.dim() != 2:
+    shape = logits.shape
+    if len(shape) != 2:
         raise ValueError("logits must be [N, V]")
-    dev = logits.device
-    dt = _capi.dtype_code(logits.dtype)
+    n, v = shape
+    dt = dtype_code(logits.dtype)
     if dt is None:
         raise ValueError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
-    n, v = logits.shape
     if not 1 <= v <= _capi.TM_MAX_SAMPLE_VOCAB:
         raise ValueError(f"V must be 1..{_capi.TM_MAX_SAMPLE_VOCAB}, got {v}")
-    if uniforms.dim() != 1 or uniforms.shape[0] != n or uniforms.dtype != torch.float32 \
+    if uniforms.shape != (n,) or uniforms.dtype != torch.float32 \
             or (n > 1 and uniforms.stride(0) != 1):
         raise ValueError("uniforms must be a contiguous float32 tensor of N entries")
-    if v > 1 and logits.stride(1) != 1:
+    ls = logits.stride()
+    if v > 1 and ls[1] != 1:
         raise ValueError("logits must have unit stride along V")
     temps, temp = _per_row("temperature", temperature, n, torch.float32, 0.0, sys.float_info.max)
     ks, k = _per_row("top_k", top_k, n, torch.int32, 0, math.inf)
     ps, p = _per_row("top_p", top_p, n, torch.float32, 0.0, 1.0)
     ms, m = _per_row("min_p", min_p, n, torch.float32, 0.0, 1.0)
-    _capi.require("sample_tokens", dev, logits=logits, uniforms=uniforms, temperature=temps,
-                  top_k=ks, top_p=ps, min_p=ms, probs_out=probs_out)
-    probs = None
+    index = logits.get_device()
+    if index < 0 or uniforms.get_device() != index or logits.requires_grad \
+            or uniforms.requires_grad or probs_out is not None \
+            or not (temps is ks is ps is ms is None):
+        _capi.require("sample_tokens", logits.device, logits=logits, uniforms=uniforms,
+                      temperature=temps, top_k=ks, top_p=ps, min_p=ms, probs_out=probs_out)
+    probs, pp, pst = None, 0, 0
     if return_probs:
         probs = probs_out
         if probs is None:
-            probs = torch.empty((n, v), dtype=torch.float32, device=dev)
-        elif probs.shape != (n, v) or probs.dtype != torch.float32 \
+            probs = torch.empty((n, v), dtype=torch.float32, device=logits.device)
+        elif probs.shape != shape or probs.dtype != torch.float32 \
                 or (v > 1 and probs.stride(1) != 1):
             raise ValueError("probs_out must be float32 [N, V] with unit stride along V")
+        pp, pst = probs.data_ptr(), probs.stride(0)
     elif probs_out is not None:
         raise ValueError("probs_out without return_probs")
-    tokens = torch.empty(n, dtype=torch.int64, device=dev)
-    _capi.launch("tm_sample_tokens", dev, logits.data_ptr(), dt, n, v, logits.stride(0),
-                 uniforms.data_ptr(), _capi.ptr(temps), temp, _capi.ptr(ks), min(k, v),
-                 _capi.ptr(ps), p, _capi.ptr(ms), m, tokens.data_ptr(), _capi.ptr(probs),
-                 0 if probs is None else probs.stride(0))
+    tokens = torch.empty(n, dtype=torch.int64, device=logits.device)
+    _capi.launch("tm_sample_tokens", index, logits.data_ptr(), dt, n, v, ls[0],
+                 uniforms.data_ptr(), ptr(temps), temp, ptr(ks), min(k, v), ptr(ps), p, ptr(ms),
+                 m, tokens.data_ptr(), pp, pst)
     return (tokens, probs) if return_probs else tokens
