@@ -529,8 +529,8 @@ int tm_sample_tokens(const void* logits, int dtype, int64_t N, int64_t V,
  * its k_lens[b] >= q_lens[b] keys, all sequences one after the other in q and in
  * k and v.  Writes num_items x 8 int32 to `items` and num_joins x 8 to `joins`
  * (host memory, to be copied to the device), and
- *   sizes[0..5] = num_items, num_joins, num_slots, tile_rows, sum of q_lens, sum of
- *                 k_lens.
+ *   sizes[0..6] = num_items, num_joins, num_slots, tiling, sum of q_lens, sum of
+ *                 k_lens, tile_rows.
  * With items and joins NULL it only writes sizes.  A length of 0 is allowed.
  */
 int tm_prompt_plan(const int64_t* q_lens, const int64_t* k_lens, int64_t B,
@@ -552,7 +552,7 @@ int tm_prompt_attention(const void* q, int64_t q_stride, const void* k,
                         int64_t k_stride, const void* v, int64_t v_stride,
                         const int32_t* items, int64_t num_items,
                         const int32_t* joins, int64_t num_joins, int64_t num_slots,
-                        int64_t tile_rows, int64_t Hq, int64_t kvh, int64_t hd,
+                        int64_t tiling, int64_t Hq, int64_t kvh, int64_t hd,
                         float scale, int dtype, void* out, int64_t out_stride,
                         void* workspace, int64_t workspace_bytes, void* stream);
 

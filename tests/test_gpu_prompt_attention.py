@@ -107,7 +107,7 @@ def test_large_tiles(dtype):
 
     _say(f"large tiles {dtype}")
     lens = [1900, 2300, 777]
-    assert PromptPlan(lens, num_heads=64, num_kv_heads=16).tile_rows in (128, 256)
+    assert PromptPlan(lens, num_heads=64, num_kv_heads=16).tile_rows == 256
     _packed(lens, lens, 64, 16, 64, dtype, 5)
     lens = [900, 2, 4000, 0, 3400]
     assert PromptPlan(lens, num_heads=32, num_kv_heads=8).tile_rows == 256
@@ -215,3 +215,57 @@ def test_same_on_every_run_and_another_stream():
             a, b = prompt_attention(q, k, v, plan), prompt_attention_cached(q, kv, 0)
         st.synchronize()
         assert torch.equal(a, want) and torch.equal(b, wantc)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("t,past,hd", [(70, 0, 128), (3, 900, 128), (300, 200, 64)])
+def test_what_a_row_does_not_see_does_not_reach_it(bad, t, past, hd):
+    """NaN and infinities in the keys and values of later tokens, and of the next
+    sequence: the rows before them are what they are without, rows that see one
+    are what the formula gives."""
+    from treemoe_spec_amd.kernels.prompt_attention import (PromptPlan, prompt_attention,
+                                                           prompt_attention_cached)
+
+    _say(f"prompt non-finite {bad} t={t} past={past}")
+    s, n = t + past, 40
+    q, k, v = _qkv(t + n, s + n, 4, 2, hd, torch.bfloat16, t)
+    plan = PromptPlan([t, n], [s, n], num_heads=4, num_kv_heads=2)
+    clean = prompt_attention(q.cuda(), k.cuda(), v.cuda(), plan)
+    hit = s - max(1, t // 3)            # a key that the last third sees
+    first = hit - past                  # and its query
+    for where in (k, v):
+        kk, vv = k.clone(), v.clone()
+        (kk if where is k else vv)[hit, :, 5] = bad
+        (kk if where is k else vv)[s + 7] = bad
+        out = prompt_attention(q.cuda(), kk.cuda(), vv.cuda(), plan)
+        kv = _cache(s, 2, hd, torch.bfloat16, 16, s)
+        kv.append(0, kk[:s].cuda(), vv[:s].cuda(), 0)
+        outc = prompt_attention_cached(q[:t].cuda(), kv, 0)
+        torch.cuda.synchronize()
+        for got in (out[:t], outc):
+            _check(got[:first], q[:first], k, v, past)
+            if where is v:
+                # column 5 of every head is the bad value, the others as without it
+                g = got[first:].view(-1, 4, hd).cpu().float()
+                c = clean[first:t].view(-1, 4, hd).cpu().float()
+                assert bool((g[..., 5] == bad).all()) if bad == bad else bool(g[..., 5].isnan().all())
+                rest = torch.arange(hd) != 5
+                assert float((g - c)[..., rest].norm()) <= 8e-3 * float(c[..., rest].norm())
+        _check(out[t:t + 7], q[t:t + 7], k[s:s + 7], v[s:s + 7], 0)
+
+
+def test_overflowing_scores_and_rows_of_nan():
+    """A query of NaN spoils its own row; others of its tile stay."""
+    from treemoe_spec_amd.kernels.prompt_attention import PromptPlan, prompt_attention
+
+    _say("prompt NaN query")
+    q, k, v = _qkv(90, 90, 4, 2, 128, torch.float16, 4)
+    q[33] = float("nan")
+    plan = PromptPlan([90], num_heads=4, num_kv_heads=2)
+    out = prompt_attention(q.cuda(), k.cuda(), v.cuda(), plan)
+    assert bool(out[33].isnan().all())
+    q[33] = 0
+    keep = [i for i in range(90) if i != 33]
+    want, mag = _want(q, k, v, 0, 128 ** -0.5)
+    assert not bool(out[keep].isnan().any())
+    assert float((out[keep].double().cpu() - want[keep]).norm()) <= 2e-3 * float(want[keep].norm())

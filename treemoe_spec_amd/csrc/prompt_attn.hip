@@ -42,6 +42,9 @@ typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(1))) void glb_void;
 
+// A lambda kept as a call would keep what it captures, a wave's rows, in memory.
+#define TM_INLINE __attribute__((always_inline))
+
 constexpr int kThreads = 256;
 constexpr int kKeys = 64;   // keys of a stage
 constexpr int kCUs = 256;   // MI355X compute units
@@ -73,6 +76,7 @@ struct PromptParams {
   int64_t stride_page;
   int kvh, group, q_len, k_len, tiles, chunks, chunk_len;  // one sequence's
   int page_shift, table_pages, cache_pages;
+  int wide;                    // the keys that a wave loads of a stage lie in one page
   float scale_log2;
 };
 
@@ -131,78 +135,119 @@ struct Shape {
   }
 };
 
-// Stages of 64 keys of K or V into LDS, by NW waves, one after the other.  Keys past
-// the sequence's last are that one again: their scores are masked.
-template <int HD, bool PAGED, int NW, bool V>
-struct Loader {
+// Stages of 64 keys into LDS by NW waves, one after the other, V of a stage at any time
+// between its K and the next one's.  Keys past the sequence's last are that one again:
+// their scores are masked.
+template <int HD, bool PAGED, int NW>
+struct Feed {
   typedef Shape<HD> S;
-  static constexpr int kLoads = S::kTile / (1024 * NW);  // loads of a wave per stage
-  const uint16_t* at;   // the next stage's first row (paged: the cache)
-  int64_t stage_stride;
-  int left;             // the sequence's last key from the next stage's first on
-  int stride;           // of a key, or of a page's slot
-  int lane_off[kLoads]; // of this lane's piece from the stage's first row
-  int pages[kLoads];    // the next stage's pages, looked up a stage ahead
-  int first;            // the next stage's first key (paged)
-  int step;             // keys from one stage to the next
+  static constexpr int kLoads = S::kTile / (1024 * NW);  // loads of a wave per tile
+  // of K and V of a stage, and of the look-up behind them
+  static constexpr int kGroup = 2 * kLoads + (PAGED ? 1 : 0);
+  const uint16_t *k, *v;   // the next stage's first row (paged: the cache)
+  int64_t k_step, v_step;  // from stage to stage
+  int k_stride, v_stride;  // of a key, or of a page's slot
+  int k_lane[kLoads], v_lane[kLoads];  // this lane's piece from the stage's first row
+                                       // (paged: from the wave's)
+  int first, left, step;   // the next stage's first key, the last key from there on, and
+                           // the keys to the stage behind
+  int v_first, v_left;     // of the stage whose K came last
+  int64_t off;             // its wave's first row in the cache
+  int page;                // the next stage's page of the wave, asked for a stage ahead
 
-  // of the waves that load a stage together
+  // of the NW waves that load a stage together
   static __device__ __forceinline__ int wave() {
-    return NW == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) & (NW - 1);
   }
-  __device__ __forceinline__ int key_in(int i) const {  // within the stage
-    return (wave() * kLoads + i) * S::kKeysPerLoad + (int)(threadIdx.x & 63) / S::kChunks;
+  static __device__ __forceinline__ int wave_key() { return wave() * kLoads * S::kKeysPerLoad; }
+  static __device__ __forceinline__ int key_in(int i) {  // within the stage
+    return wave_key() + i * S::kKeysPerLoad + (int)(threadIdx.x & 63) / S::kChunks;
   }
-  __device__ __forceinline__ int chunk_off(int i) const {
+  template <bool V>
+  static __device__ __forceinline__ int chunk_off(int i) {
     const int j = key_in(i);
     return (((int)threadIdx.x & (S::kChunks - 1)) ^ (V ? S::swz_v(j) : S::swz_k(j))) * 8;
   }
-  __device__ __forceinline__ void look_up(const PromptParams& p) {
-    if constexpr (PAGED) {
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        // (a stage behind the last one looks up the last key again)
-        pages[i] = p.table[(first + min(key_in(i), left)) >> p.page_shift];
-    }
+  static __device__ __forceinline__ void to_lds(const uint16_t* from, uint8_t* tile, int i) {
+    __builtin_amdgcn_global_load_lds((glb_void*)from,
+                                     (lds_void*)(tile + (wave() * kLoads + i) * 1024), 16, 0, 0);
   }
-  // From key `begin` on of the sequence whose first row is `row0` and last key `last`.
-  __device__ __forceinline__ void start(const PromptParams& p, const uint16_t* row0,
-                                        int64_t row_stride, int begin, int last,
-                                        int step_ = kKeys) {
-    at = PAGED ? row0 : row0 + (int64_t)begin * row_stride;
+  __device__ __forceinline__ void look_up(const PromptParams& p) {
+    if constexpr (PAGED) page = p.table[(first + min(wave_key(), left)) >> p.page_shift];
+  }
+  // From key `begin` on of the item's sequence, `step` keys from stage to stage.
+  __device__ __forceinline__ void start(const PromptParams& p, const Item& it, int kvhead,
+                                        int begin, int step_) {
+    k = p.k + (int64_t)kvhead * HD + (PAGED ? 0 : (int64_t)(it.k0 + begin) * p.k_stride);
+    v = p.v + (int64_t)kvhead * HD + (PAGED ? 0 : (int64_t)(it.k0 + begin) * p.v_stride);
     step = step_;
-    stage_stride = step * row_stride;
-    stride = (int)row_stride;
-    left = last - begin;
+    k_step = step * p.k_stride;
+    v_step = step * p.v_stride;
+    k_stride = (int)p.k_stride;
+    v_stride = (int)p.v_stride;
     first = begin;
+    left = it.k_len - 1 - begin;
+    v_first = v_left = 0;
+    off = 0;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) lane_off[i] = key_in(i) * stride + chunk_off(i);
+    for (int i = 0; i < kLoads; ++i) {
+      const int key = key_in(i) - (PAGED ? wave_key() : 0);
+      k_lane[i] = key * k_stride + chunk_off<false>(i);
+      v_lane[i] = key * v_stride + chunk_off<true>(i);
+    }
     look_up(p);
   }
-  __device__ __forceinline__ void load(const PromptParams& p, uint8_t* tile) {
-    if constexpr (PAGED) {
+  // K or V of a stage row by row: near the sequence's end (`left_` is negative for a
+  // stage behind it), or where a wave's keys lie in several pages.
+  template <bool V>
+  __device__ __forceinline__ void load_rows(const PromptParams& p, int first_, int left_,
+                                            uint8_t* tile) const {
+    const uint16_t* const base = V ? v : k;
+    const int stride = V ? v_stride : k_stride;
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int slot = (first + min(key_in(i), left)) & ((1 << p.page_shift) - 1);
-        const int64_t o = (int64_t)min(max(pages[i], 0), p.cache_pages - 1) * p.stride_page +
-                          (int64_t)slot * stride + chunk_off(i);
-        __builtin_amdgcn_global_load_lds((glb_void*)(at + o),
-                                         (lds_void*)(tile + (wave() * kLoads + i) * 1024), 16, 0, 0);
+    for (int i = 0; i < kLoads; ++i) {
+      const int j = min(key_in(i), left_);
+      int64_t o;
+      if constexpr (PAGED) {
+        const int key = first_ + j;
+        const int pg = min(max(p.table[key >> p.page_shift], 0), p.cache_pages - 1);
+        o = (int64_t)pg * p.stride_page +
+            (int64_t)(key & ((1 << p.page_shift) - 1)) * stride + chunk_off<V>(i);
+      } else {
+        o = (int64_t)j * stride + chunk_off<V>(i);
       }
-      first += step;
-      left -= step;
-      look_up(p);
-    } else {
-      const bool whole = left >= kKeys - 1;
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int o = whole ? lane_off[i] : min(key_in(i), left) * stride + chunk_off(i);
-        __builtin_amdgcn_global_load_lds((glb_void*)(at + (uint32_t)o),
-                                         (lds_void*)(tile + (wave() * kLoads + i) * 1024), 16, 0, 0);
-      }
-      at += stage_stride;
-      left -= step;
+      to_lds(base + o, tile, i);
     }
+  }
+  __device__ __forceinline__ bool whole(const PromptParams& p, int left_) const {
+    return left_ >= kKeys - 1 && (!PAGED || p.wide);
+  }
+  __device__ __forceinline__ void load_k(const PromptParams& p, uint8_t* tile) {
+    if (whole(p, left)) {
+      if constexpr (PAGED)
+        off = (int64_t)min(max(__builtin_amdgcn_readfirstlane(page), 0), p.cache_pages - 1) *
+                  p.stride_page +
+              (int64_t)((first + wave_key()) & ((1 << p.page_shift) - 1)) * k_stride;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) to_lds(k + off + (uint32_t)k_lane[i], tile, i);
+    } else {
+      load_rows<false>(p, first, left, tile);
+    }
+    v_first = first;
+    v_left = left;
+    first += step;
+    left -= step;
+    if constexpr (!PAGED) k += k_step;
+    look_up(p);
+  }
+  __device__ __forceinline__ void load_v(const PromptParams& p, uint8_t* tile) {
+    if (whole(p, v_left)) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) to_lds(v + off + (uint32_t)v_lane[i], tile, i);
+    } else {
+      load_rows<true>(p, v_first, v_left, tile);
+    }
+    if constexpr (!PAGED) v += v_step;
   }
 };
 
@@ -404,45 +449,31 @@ __device__ __forceinline__ void store_row(const PromptParams& p, int q0, int row
                               e) = w;
 }
 
-// NW waves of 32 rows.  NW = 8: the two waves of a SIMD take turns, one in the matrix
-// products of its stage while the other weighs, a barrier between the turns.
-// NW = 4: two workgroups a CU, which drift apart by themselves.
-template <int DT, int HD, int NW, bool PAGED>
-__global__ void __launch_bounds__(64 * NW, 2) tm_prompt_attn_kernel(PromptParams p) {
-  typedef Shape<HD> S;
-  constexpr int kRows = 32 * NW;
-  constexpr int kRing = NW == 8 ? 3 : 2;
-  __shared__ __attribute__((aligned(1024))) uint8_t s_k0[S::kTile];
-  __shared__ __attribute__((aligned(1024))) uint8_t s_v0[S::kTile];
-  __shared__ __attribute__((aligned(1024))) uint8_t s_k1[S::kTile];
-  __shared__ __attribute__((aligned(1024))) uint8_t s_v1[S::kTile];
-  __shared__ __attribute__((aligned(1024))) uint8_t s_k2[kRing == 3 ? S::kTile : 16];
-  __shared__ __attribute__((aligned(1024))) uint8_t s_v2[kRing == 3 ? S::kTile : 16];
+// Where a wave's rows lie.
+struct Place {
+  bool ok;          // this lane's column is a row
+  int row;          // of the sequence
+  int full;         // the last key that every row of the wave sees, within the range
+};
 
-  // KV heads innermost: with 8 of them a head's workgroups, which share its keys, run
-  // on one XCD; the tiles with the most keys first
-  const int kvhead = (int)blockIdx.x % p.kvh;
-  const Item it = item_of(p, (int)blockIdx.x / p.kvh, kRows);
-  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, c32 = lane & 31;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int past = it.k_len - it.q_len;
-  const int all_rows = it.q_len * p.group;
-
-  // this lane's row
-  const int first = it.tile * kRows + wave * 32;
-  const bool ok = first + c32 < all_rows;
-  const int token = ok ? (first + c32) / p.group : 0;
-  const int head = kvhead * p.group + (ok ? first + c32 - token * p.group : 0);
-  Rows<HD> r;
-  {
-    const uint16_t* const qr =
-        p.q + (int64_t)(it.q0 + token) * p.q_stride + (int64_t)head * HD + 8 * half;
+// Rows first .. first + 31 of the sequence: their Q^T fragments, nothing seen yet.
+template <int HD>
+__device__ __forceinline__ Place begin_rows(const PromptParams& p, const Item& it, int kvhead,
+                                            int first, Rows<HD>& r) {
+  const int lane = threadIdx.x & 63, half = lane >> 5, c32 = lane & 31;
+  const int past = it.k_len - it.q_len, all_rows = it.q_len * p.group;
+  Place at;
+  at.row = first + c32;
+  at.ok = at.row < all_rows;
+  const int token = at.ok ? at.row / p.group : 0;
+  const int head = kvhead * p.group + (at.ok ? at.row - token * p.group : 0);
+  const uint16_t* const qr =
+      p.q + (int64_t)(it.q0 + token) * p.q_stride + (int64_t)head * HD + 8 * half;
 #pragma unroll
-    for (int ks = 0; ks < HD / 16; ++ks) {
-      const u32x4_t x = *reinterpret_cast<const u32x4_t*>(qr + 16 * ks);
-      const u32x4_t zero = {0u, 0u, 0u, 0u};
-      r.q[ks] = ok ? x : zero;
-    }
+  for (int ks = 0; ks < HD / 16; ++ks) {
+    const u32x4_t x = *reinterpret_cast<const u32x4_t*>(qr + 16 * ks);
+    const u32x4_t zero = {0u, 0u, 0u, 0u};
+    r.q[ks] = at.ok ? x : zero;
   }
 #pragma unroll
   for (int ht = 0; ht < HD / 32; ++ht)
@@ -451,125 +482,90 @@ __global__ void __launch_bounds__(64 * NW, 2) tm_prompt_attn_kernel(PromptParams
   r.m = -INFINITY;
   r.l = 0.0f;
   // a range's end hides what lies past it
-  r.seen = min(ok ? past + token : -1, it.end - 1);
-  // keys up to this one are seen by every row of the wave
-  const int full = min(first + 32 <= all_rows ? past + first / p.group : -1, it.end - 1);
+  r.seen = min(at.ok ? past + token : -1, it.end - 1);
+  at.full = min(first + 32 <= all_rows ? past + first / p.group : -1, it.end - 1);
+  return at;
+}
 
-  Loader<HD, PAGED, NW, false> lk;
-  Loader<HD, PAGED, NW, true> lv;
-  const int n = it.end > it.begin ? (it.end - it.begin + kKeys - 1) / kKeys : 0;
-  const float scale_log2 = p.scale_log2;
-  if (n > 0) {
-    const int64_t k0 = (int64_t)kvhead * HD + (PAGED ? 0 : (int64_t)it.k0 * p.k_stride);
-    const int64_t v0 = (int64_t)kvhead * HD + (PAGED ? 0 : (int64_t)it.k0 * p.v_stride);
-    lk.start(p, p.k + k0, p.k_stride, it.begin, it.k_len - 1);
-    lv.start(p, p.v + v0, p.v_stride, it.begin, it.k_len - 1);
-  }
-
-  if constexpr (NW == 4) {
-    auto step = [&](int s, const uint8_t* kc, const uint8_t* vc, uint8_t* kn, uint8_t* vn) {
-      wait_vm<0>();      // this wave's loads of stage s
-      tm_lds_barrier();  // everyone's; and the reads of stage s - 1 are over
-      const int kb = it.begin + s * kKeys;
-      if (s + 1 < n) {
-        lk.load(p, kn);
-        lv.load(p, vn);
+// The weight 0 of a key that a row does not see still makes NaN of an infinity or NaN in
+// its value, by the products.  Rows whose output is not finite are therefore taken again,
+// key by key over what each sees: stages s0, s0 + step, ... of the range.  Slow, and
+// only reached where an input is not finite or a product overflows.
+template <int DT, int HD, bool PAGED>
+__device__ __forceinline__ void retake(const PromptParams& p, const Item& it, int kvhead, int s0,
+                                       int step, int n, Rows<HD>& r) {
+  float bad = 0.0f;
+#pragma unroll
+  for (int ht = 0; ht < HD / 32; ++ht)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) bad += r.o[ht][x] * 0.0f;
+  bad += r.l * 0.0f;
+  if (!__any(bad != 0.0f)) return;  // 0 times what is not finite is NaN
+  const int half = (int)(threadIdx.x & 63) >> 5;
+  float m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int ht = 0; ht < HD / 32; ++ht)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) r.o[ht][x] = 0.0f;
+  for (int s = s0; s < n; s += step) {
+    const int first = it.begin + s * kKeys, end = min(first + kKeys, it.end);
+#pragma unroll 1
+    for (int key = first; key < end; ++key) {
+      int64_t ka, va;
+      if constexpr (PAGED) {
+        const int page = min(max(p.table[key >> p.page_shift], 0), p.cache_pages - 1);
+        ka = (int64_t)page * p.stride_page +
+             (int64_t)(key & ((1 << p.page_shift) - 1)) * p.k_stride;
+        va = ka;
+      } else {
+        ka = (int64_t)(it.k0 + key) * p.k_stride;
+        va = (int64_t)(it.k0 + key) * p.v_stride;
       }
-      products<DT, HD, false, true>(vc, kc, r);
-      weigh<DT, HD>(scale_log2, kb, kb + kKeys - 1 > full, r);
-      products<DT, HD, true, false>(vc, kc, r);
-    };
-    if (n > 0) {
-      lk.load(p, s_k0);
-      lv.load(p, s_v0);
-    }
-    for (int s = 0; s < n; s += 2) {
-      step(s, s_k0, s_v0, s_k1, s_v1);
-      if (s + 1 < n) step(s + 1, s_k1, s_v1, s_k0, s_v0);
-    }
-  } else if (n > 0) {
-    // Load group g(s), in ring slot s % 3: K of stage s and V of stage s - 1, what
-    // turn M(s) = {O += V P of s - 1, S = K Q of s} reads.  W(s) weighs stage s.
-    // Waves 0-3 take M(s) in turn 2 s and W(s) in turn 2 s + 1, waves 4-7 one turn
-    // later.  In turn 2 s + 1 every wave requests g(s + 2), whose slot the last
-    // wave left in turn 2 s - 1, and at its end waits for its part of g(s + 1).
-    // a request's loads, look-ups of pages included
-    constexpr int kGroup = (PAGED ? 4 : 2) * decltype(lk)::kLoads;
-    auto request = [&](int s, uint8_t* kn, uint8_t* vn) {
-      if (s > n) return;
-      if (s < n) lk.load(p, kn);
-      if (s > 0) lv.load(p, vn);
-    };
-    request(0, s_k0, s_v0);
-    request(1, s_k1, s_v1);
-    wait_vm<0>();
-    tm_lds_barrier();
-    auto turn_end = [&]() {
-      __builtin_amdgcn_sched_barrier(0);
-      tm_lds_barrier();
-      __builtin_amdgcn_sched_barrier(0);
-    };
-    // this wave's part of g(s) is there; g(s + 1) may be under way
-    auto await = [&](int s) {
-      if (s + 1 < n)
-        wait_vm<kGroup>();
-      else
-        wait_vm<0>();
-    };
-    // W(s) and M(s + 1), which reads g(s + 1) at kc, vc; g(s + 2 + LATE) goes to kn, vn.
-    // (the last one's scores, of a stage that is not there, are not used)
-    auto early = [&](int s, uint8_t* kc, uint8_t* vc, uint8_t* kn, uint8_t* vn) {
-      const int kb = it.begin + s * kKeys;
-      request(s + 2, kn, vn);
-      weigh<DT, HD>(scale_log2, kb, kb + kKeys - 1 > full, r);
-      await(s + 1);
-      turn_end();
-      products<DT, HD, true, true>(vc, kc, r);
-      turn_end();
-    };
-    auto late = [&](int s, uint8_t* kc, uint8_t* vc, uint8_t* kn, uint8_t* vn) {
-      const int kb = it.begin + s * kKeys;
-      weigh<DT, HD>(scale_log2, kb, kb + kKeys - 1 > full, r);
-      turn_end();
-      request(s + 3, kn, vn);
-      products<DT, HD, true, true>(vc, kc, r);
-      await(s + 2);
-      turn_end();
-    };
-    int s = 0;
-    if (wave < 4) {
-      products<DT, HD, false, true>(s_v0, s_k0, r);
-      turn_end();
-      for (; s + 3 <= n; s += 3) {
-        early(s, s_k1, s_v1, s_k2, s_v2);
-        early(s + 1, s_k2, s_v2, s_k0, s_v0);
-        early(s + 2, s_k0, s_v0, s_k1, s_v1);
+      const uint16_t* const kr = p.k + ka + kvhead * HD + 8 * half;
+      const uint16_t* const vr = p.v + va + kvhead * HD + 4 * half;
+      float dot = 0.0f;
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks) {
+        float a[8], b[8];
+        tm_load8<DT>(kr, 16 * ks, a);
+        tm_load8<DT>(&r.q[ks], 0, b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dot = fmaf(a[e], b[e], dot);
       }
-      if (s < n) early(s, s_k1, s_v1, s_k2, s_v2);
-      if (s + 1 < n) early(s + 1, s_k2, s_v2, s_k0, s_v0);
-      turn_end();
-    } else {
-      turn_end();
-      request(2, s_k2, s_v2);
-      products<DT, HD, false, true>(s_v0, s_k0, r);
-      await(1);
-      turn_end();
-      for (; s + 3 <= n; s += 3) {
-        late(s, s_k1, s_v1, s_k0, s_v0);
-        late(s + 1, s_k2, s_v2, s_k1, s_v1);
-        late(s + 2, s_k0, s_v0, s_k2, s_v2);
-      }
-      if (s < n) late(s, s_k1, s_v1, s_k0, s_v0);
-      if (s + 1 < n) late(s + 1, s_k2, s_v2, s_k1, s_v1);
+      dot += __shfl_xor(dot, 32);
+      if (key > r.seen) continue;
+      const float x = dot * p.scale_log2;
+      const float mn = fmaxf(m, x);
+      const float a = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+      const float w = x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - mn);
+      l = l * a + w;
+      m = mn;
+#pragma unroll
+      for (int ht = 0; ht < HD / 32; ++ht)
+#pragma unroll
+        for (int x4 = 0; x4 < 4; ++x4)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            r.o[ht][4 * x4 + e] =
+                r.o[ht][4 * x4 + e] * a + w * tm_load1<DT>(vr, 32 * ht + 8 * x4 + e);
     }
   }
+  r.m = m;
+  r.l = half == 0 ? l : 0.0f;
+}
 
+// The wave's rows as the output, or as a partial of a tile of `tile_rows`.
+template <int DT, int HD>
+__device__ __forceinline__ void end_rows(const PromptParams& p, const Item& it, int kvhead,
+                                         int tile_rows, const Place& at, const Rows<HD>& r) {
+  const int half = (int)(threadIdx.x & 63) >> 5;
   const float l = r.l + __shfl_xor(r.l, 32);
-  if (!ok) return;
+  if (!at.ok) return;
   if (it.slot < 0) {
-    const float inv = l > 0.0f ? 1.0f / l : l;  // (as store_row)
-    uint16_t* const o = p.out + (int64_t)(it.q0 + token) * p.out_stride + (int64_t)head * HD +
-                        4 * half;
+    const float inv = l > 0.0f ? 1.0f / l : l;  // 0 where nothing was seen; NaN stays
+    const int token = at.row / p.group;
+    uint16_t* const o = p.out + (int64_t)(it.q0 + token) * p.out_stride +
+                        (int64_t)(kvhead * p.group + at.row - token * p.group) * HD + 4 * half;
 #pragma unroll
     for (int ht = 0; ht < HD / 32; ++ht)
 #pragma unroll
@@ -580,7 +576,8 @@ __global__ void __launch_bounds__(64 * NW, 2) tm_prompt_attn_kernel(PromptParams
         *reinterpret_cast<u32x2_t*>(o + 32 * ht + 8 * x) = w;
       }
   } else {
-    const int64_t slot = ((int64_t)it.slot * p.kvh + kvhead) * kRows + wave * 32 + c32;
+    const int64_t slot =
+        ((int64_t)it.slot * p.kvh + kvhead) * tile_rows + (at.row - it.tile * tile_rows);
     float* const o = p.part + slot * HD + 4 * half;
 #pragma unroll
     for (int ht = 0; ht < HD / 32; ++ht)
@@ -595,6 +592,267 @@ __global__ void __launch_bounds__(64 * NW, 2) tm_prompt_attn_kernel(PromptParams
   }
 }
 
+// The end of a turn: no wave of the workgroup goes on before all have come here.  What
+// a turn read from LDS its products have used, so no reads are waited for.
+__device__ __forceinline__ void turn_end() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_barrier" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// Eight waves, two a SIMD, that take turns: one is in the matrix products of its stage
+// while the other weighs, a barrier between the turns.  Tiles of 256 rows: every wave has
+// 32 rows of its own, and all read the same stages.
+template <int DT, int HD, bool PAGED>
+__global__ void __launch_bounds__(512, 2) tm_prompt_tall_kernel(PromptParams p) {
+  typedef Shape<HD> S;
+  __shared__ __attribute__((aligned(1024))) uint8_t s_k0[S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_v0[S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_k1[S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_v1[S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_k2[S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_v2[S::kTile];
+
+  // KV heads innermost: with 8 of them a head's workgroups, which share its keys, run
+  // on one XCD; the tiles with the most keys first
+  const int kvhead = (int)blockIdx.x % p.kvh;
+  const Item it = item_of(p, (int)blockIdx.x / p.kvh, 256);
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  Rows<HD> r;
+  const Place at = begin_rows<HD>(p, it, kvhead, it.tile * 256 + wave * 32, r);
+  const int full = at.full;
+  const int n = it.end > it.begin ? (it.end - it.begin + kKeys - 1) / kKeys : 0;
+  const float scale_log2 = p.scale_log2;
+  if (n > 0) {
+    Feed<HD, PAGED, 8> feed;
+    feed.start(p, it, kvhead, it.begin, kKeys);
+    // Load group g(s), in ring slot s % 3: K of stage s and V of stage s - 1, what the
+    // products M(s) = {O += V P of s - 1, S = K Q of s} read.  W(s) weighs stage s.
+    // Waves 0-3 take M(s) in turn 2 s and W(s) in turn 2 s + 1, waves 4-7, which share
+    // their SIMDs, one turn later.  A wave requests g(s + 2) behind its products M(s), the
+    // late waves having left its slot in turn 2 s - 1; in turn 2 s + 1 all wait for their
+    // part of g(s + 1).
+    auto request = [&](int s, uint8_t* kn, uint8_t* vn) TM_INLINE {
+      if (s > n) return;
+      if (s > 0) feed.load_v(p, vn);
+      if (s < n) feed.load_k(p, kn);
+    };
+    // this wave's part of g(s) is there; g(s + 1) may be under way
+    auto await = [&](int s) TM_INLINE {
+      if (s + 1 < n)
+        wait_vm<Feed<HD, PAGED, 8>::kGroup>();
+      else
+        wait_vm<0>();
+    };
+    // W(s) and M(s + 1), which reads g(s + 1) at kc, vc; g(s + 3) goes to kn, vn.  (The last
+    // one's scores, of a stage that is not there, are not used.)
+    auto early = [&](int s, uint8_t* kc, uint8_t* vc, uint8_t* kn, uint8_t* vn) TM_INLINE {
+      const int kb = it.begin + s * kKeys;
+      weigh<DT, HD>(scale_log2, kb, kb + kKeys - 1 > full, r);
+      await(s + 1);
+      turn_end();
+      products<DT, HD, true, true>(vc, kc, r);
+      request(s + 3, kn, vn);
+      turn_end();
+    };
+    auto late = [&](int s, uint8_t* kc, uint8_t* vc, uint8_t* kn, uint8_t* vn) TM_INLINE {
+      const int kb = it.begin + s * kKeys;
+      weigh<DT, HD>(scale_log2, kb, kb + kKeys - 1 > full, r);
+      turn_end();
+      products<DT, HD, true, true>(vc, kc, r);
+      request(s + 3, kn, vn);
+      await(s + 2);
+      turn_end();
+    };
+    request(0, s_k0, s_v0);
+    request(1, s_k1, s_v1);
+    wait_vm<0>();
+    turn_end();
+    int s = 0;
+    if (wave < 4) {
+      products<DT, HD, false, true>(s_v0, s_k0, r);
+      request(2, s_k2, s_v2);
+      turn_end();
+      for (; s + 3 <= n; s += 3) {
+        early(s, s_k1, s_v1, s_k0, s_v0);
+        early(s + 1, s_k2, s_v2, s_k1, s_v1);
+        early(s + 2, s_k0, s_v0, s_k2, s_v2);
+      }
+      if (s < n) early(s, s_k1, s_v1, s_k0, s_v0);
+      if (s + 1 < n) early(s + 1, s_k2, s_v2, s_k1, s_v1);
+      turn_end();
+    } else {
+      turn_end();
+      products<DT, HD, false, true>(s_v0, s_k0, r);
+      request(2, s_k2, s_v2);
+      await(1);
+      turn_end();
+      for (; s + 3 <= n; s += 3) {
+        late(s, s_k1, s_v1, s_k0, s_v0);
+        late(s + 1, s_k2, s_v2, s_k1, s_v1);
+        late(s + 2, s_k0, s_v0, s_k2, s_v2);
+      }
+      if (s < n) late(s, s_k1, s_v1, s_k0, s_v0);
+      if (s + 1 < n) late(s + 1, s_k2, s_v2, s_k1, s_v1);
+    }
+  }
+  retake<DT, HD, PAGED>(p, it, kvhead, 0, 1, n, r);
+  end_rows<DT, HD>(p, it, kvhead, 256, at, r);
+}
+
+// The same turns on tiles of 128 rows: waves w and w + 4 have the same 32 rows, waves 0-3
+// take the even stages and waves 4-7 the odd ones, each four with buffers of their own.
+// At the end the two outputs of a row are joined through LDS.
+template <int DT, int HD, bool PAGED>
+__global__ void __launch_bounds__(512, 2) tm_prompt_pair_kernel(PromptParams p) {
+  typedef Shape<HD> S;
+  __shared__ __attribute__((aligned(1024))) uint8_t s_ka0[S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_va0[S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_ka1[S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_va1[S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_kb0[S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_vb0[S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_kb1[S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_vb1[S::kTile];
+  __shared__ float s_stat[4][64][2];
+
+  const int kvhead = (int)blockIdx.x % p.kvh;
+  const Item it = item_of(p, (int)blockIdx.x / p.kvh, 128);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int second = wave >> 2;
+  Rows<HD> r;
+  const Place at = begin_rows<HD>(p, it, kvhead, it.tile * 128 + (wave & 3) * 32, r);
+  const int full = at.full;
+  const int n = it.end > it.begin ? (it.end - it.begin + kKeys - 1) / kKeys : 0;
+  // stages of the first four waves; the last of the second four may lie past the range,
+  // all of it masked
+  const int rounds = (n + 1) / 2;
+  const float scale_log2 = p.scale_log2;
+  if (n > 0) {
+    Feed<HD, PAGED, 4> feed;
+    const int begin = it.begin + second * kKeys;
+    feed.start(p, it, kvhead, begin, 2 * kKeys);
+    // Load group g(s), in slot s % 2: K of round s and V of round s - 1, what the products
+    // M(s) = {O += V P of s - 1, S = K Q of s} read.  Round s: W(s) weighs its scores, then
+    // M(s + 1), and behind it g(s + 2) is requested, whose slot all four waves left with
+    // M(s) two turns before; W(s) waits for g(s + 1) at its end.  The second four waves do
+    // all this one turn later.
+    auto request = [&](int s, uint8_t* kn, uint8_t* vn) TM_INLINE {
+      if (s > rounds) return;
+      if (s > 0) feed.load_v(p, vn);
+      if (s < rounds) feed.load_k(p, kn);
+    };
+    // W(s), M(s + 1) with g(s + 1) at kc, vc; g(s + 2) goes to kn, vn.  (The last one's
+    // scores, of a stage that is not there, are not used.)
+    auto round = [&](int s, uint8_t* kc, uint8_t* vc, uint8_t* kn, uint8_t* vn) TM_INLINE {
+      const int kb = begin + 2 * s * kKeys;
+      weigh<DT, HD>(scale_log2, kb, kb + kKeys - 1 > full, r);
+      wait_vm<0>();
+      turn_end();
+      products<DT, HD, true, true>(vc, kc, r);
+      request(s + 2, kn, vn);
+      turn_end();
+    };
+    auto all = [&](uint8_t* ka, uint8_t* va, uint8_t* kb, uint8_t* vb) TM_INLINE {
+      request(0, ka, va);
+      request(1, kb, vb);
+      wait_vm<0>();
+      turn_end();
+      if (second) turn_end();
+      products<DT, HD, false, true>(va, ka, r);
+      turn_end();
+      int s = 0;
+      for (; s + 2 <= rounds; s += 2) {
+        round(s, kb, vb, ka, va);
+        round(s + 1, ka, va, kb, vb);
+      }
+      if (s < rounds) round(s, kb, vb, ka, va);
+    };
+    if (second) {
+      all(s_kb0, s_vb0, s_kb1, s_vb1);
+    } else {
+      all(s_ka0, s_va0, s_ka1, s_va1);
+      turn_end();
+    }
+  }
+  retake<DT, HD, PAGED>(p, it, kvhead, second, 2, n, r);
+  // the second four waves' outputs, each where a buffer was
+  const int w4 = wave & 3;
+  uint8_t* const box = w4 == 0 ? s_ka0 : w4 == 1 ? s_ka1 : w4 == 2 ? s_va0 : s_va1;
+  f32x4_t* const mine = reinterpret_cast<f32x4_t*>(box) + lane;
+  __syncthreads();
+  if (second) {
+#pragma unroll
+    for (int ht = 0; ht < HD / 32; ++ht)
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        mine[64 * (4 * ht + x)] =
+            f32x4_t{r.o[ht][4 * x], r.o[ht][4 * x + 1], r.o[ht][4 * x + 2], r.o[ht][4 * x + 3]};
+    s_stat[w4][lane][0] = r.m;
+    s_stat[w4][lane][1] = r.l;
+  }
+  __syncthreads();
+  if (second) return;
+  const float m1 = s_stat[w4][lane][0], l1 = s_stat[w4][lane][1];
+  const float m = fmaxf(r.m, m1), ref = m == -INFINITY ? 0.0f : m;
+  const float a = __builtin_amdgcn_exp2f(r.m - ref), b = __builtin_amdgcn_exp2f(m1 - ref);
+  r.l = r.l * a + l1 * b;
+  r.m = m;
+#pragma unroll
+  for (int ht = 0; ht < HD / 32; ++ht)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const f32x4_t o = mine[64 * (4 * ht + x)];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r.o[ht][4 * x + e] = r.o[ht][4 * x + e] * a + o[e] * b;
+    }
+  end_rows<DT, HD>(p, it, kvhead, 128, at, r);
+}
+
+// Short tiles: four waves of 32 rows, two workgroups a CU, which drift apart by themselves.
+template <int DT, int HD, bool PAGED>
+__global__ void __launch_bounds__(kThreads, 2) tm_prompt_short_kernel(PromptParams p) {
+  typedef Shape<HD> S;
+  __shared__ __attribute__((aligned(1024))) uint8_t s_k0[S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_v0[S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_k1[S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_v1[S::kTile];
+
+  const int kvhead = (int)blockIdx.x % p.kvh;
+  const Item it = item_of(p, (int)blockIdx.x / p.kvh, 128);
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int n = it.end > it.begin ? (it.end - it.begin + kKeys - 1) / kKeys : 0;
+  const float scale_log2 = p.scale_log2;
+  Rows<HD> r;
+  const Place at = begin_rows<HD>(p, it, kvhead, it.tile * 128 + wave * 32, r);
+  const int full = at.full;
+  if (n > 0) {
+    Feed<HD, PAGED, 4> feed;
+    feed.start(p, it, kvhead, it.begin, kKeys);
+    auto step = [&](int s, const uint8_t* kc, const uint8_t* vc, uint8_t* kn, uint8_t* vn) TM_INLINE {
+      wait_vm<0>();      // this wave's loads of stage s
+      tm_lds_barrier();  // everyone's; and the reads of stage s - 1 are over
+      const int kb = it.begin + s * kKeys;
+      if (s + 1 < n) {
+        feed.load_k(p, kn);
+        feed.load_v(p, vn);
+      }
+      products<DT, HD, false, true>(vc, kc, r);
+      weigh<DT, HD>(scale_log2, kb, kb + kKeys - 1 > full, r);
+      products<DT, HD, true, false>(vc, kc, r);
+    };
+    feed.load_k(p, s_k0);
+    feed.load_v(p, s_v0);
+    for (int s = 0; s < n; s += 2) {
+      step(s, s_k0, s_v0, s_k1, s_v1);
+      if (s + 1 < n) step(s + 1, s_k1, s_v1, s_k0, s_v0);
+    }
+  }
+  retake<DT, HD, PAGED>(p, it, kvhead, 0, 1, n, r);
+  end_rows<DT, HD>(p, it, kvhead, 128, at, r);
+}
+
 // Few rows (a decoded token's heads): a tile of 32, and the four waves take the stages
 // of the range in turn, each with its own part of LDS and no barrier between them, so
 // that a CU has 128 KB of keys under way.  A wave asks for its next K when it has the
@@ -603,7 +861,6 @@ __global__ void __launch_bounds__(64 * NW, 2) tm_prompt_attn_kernel(PromptParams
 template <int DT, int HD, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 1) tm_prompt_few_kernel(PromptParams p) {
   typedef Shape<HD> S;
-  constexpr int kLoads = Loader<HD, PAGED, 1, false>::kLoads;
   __shared__ __attribute__((aligned(1024))) uint8_t s_k[4][S::kTile];
   __shared__ __attribute__((aligned(1024))) uint8_t s_v[4][S::kTile];
   __shared__ float s_stat[4][32][2];
@@ -612,58 +869,33 @@ __global__ void __launch_bounds__(kThreads, 1) tm_prompt_few_kernel(PromptParams
   const Item it = item_of(p, (int)blockIdx.x / p.kvh, 32);
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, c32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int past = it.k_len - it.q_len;
   const int all_rows = it.q_len * p.group;
 
   // row c32 of the tile, in every wave
   const int first = it.tile * 32;
-  const bool ok = first + c32 < all_rows;
-  const int token = ok ? (first + c32) / p.group : 0;
-  const int head = kvhead * p.group + (ok ? first + c32 - token * p.group : 0);
   Rows<HD> r;
   const int n = it.end > it.begin ? (it.end - it.begin + kKeys - 1) / kKeys : 0;
-  Loader<HD, PAGED, 1, false> lk;
-  Loader<HD, PAGED, 1, true> lv;
+  Feed<HD, PAGED, 1> feed;
+  constexpr int kLoads = Feed<HD, PAGED, 1>::kLoads;
   uint8_t* const kt = s_k[wave];
   uint8_t* const vt = s_v[wave];
   if (wave < n) {
-    const int64_t k0 = (int64_t)kvhead * HD + (PAGED ? 0 : (int64_t)it.k0 * p.k_stride);
-    const int64_t v0 = (int64_t)kvhead * HD + (PAGED ? 0 : (int64_t)it.k0 * p.v_stride);
-    const int begin = it.begin + wave * kKeys;
-    lk.start(p, p.k + k0, p.k_stride, begin, it.k_len - 1, 4 * kKeys);
-    lk.load(p, kt);
-    lv.start(p, p.v + v0, p.v_stride, begin, it.k_len - 1, 4 * kKeys);
-    lv.load(p, vt);
+    feed.start(p, it, kvhead, it.begin + wave * kKeys, 4 * kKeys);
+    feed.load_k(p, kt);
+    feed.load_v(p, vt);
   }
-  {
-    const uint16_t* const qr =
-        p.q + (int64_t)(it.q0 + token) * p.q_stride + (int64_t)head * HD + 8 * half;
-#pragma unroll
-    for (int ks = 0; ks < HD / 16; ++ks) {
-      const u32x4_t x = *reinterpret_cast<const u32x4_t*>(qr + 16 * ks);
-      const u32x4_t zero = {0u, 0u, 0u, 0u};
-      r.q[ks] = ok ? x : zero;
-    }
-  }
-#pragma unroll
-  for (int ht = 0; ht < HD / 32; ++ht)
-#pragma unroll
-    for (int x = 0; x < 16; ++x) r.o[ht][x] = 0.0f;
-  r.m = -INFINITY;
-  r.l = 0.0f;
-  r.seen = min(ok ? past + token : -1, it.end - 1);
-  const int full = min(first + 32 <= all_rows ? past + first / p.group : -1, it.end - 1);
+  const int full = begin_rows<HD>(p, it, kvhead, first, r).full;
 
   for (int s = wave; s < n; s += 4) {
     const int kb = it.begin + s * kKeys;
     const bool more = s + 4 < n;
     if (s == wave)
-      wait_vm<0>();  // K and V, the query rows and the pages
+      wait_vm<0>();  // K and V, and the query rows
     else
       wait_vm<kLoads>();  // K: V is behind it
     products<DT, HD, false, true>(vt, kt, r);
     __builtin_amdgcn_sched_barrier(0);
-    if (more) lk.load(p, kt);
+    if (more) feed.load_k(p, kt);
     weigh<DT, HD>(p.scale_log2, kb, kb + kKeys - 1 > full, r);
     if (more)
       wait_vm<kLoads>();
@@ -671,8 +903,9 @@ __global__ void __launch_bounds__(kThreads, 1) tm_prompt_few_kernel(PromptParams
       wait_vm<0>();
     products<DT, HD, true, false>(vt, kt, r);
     __builtin_amdgcn_sched_barrier(0);
-    if (more) lv.load(p, vt);
+    if (more) feed.load_v(p, vt);
   }
+  retake<DT, HD, PAGED>(p, it, kvhead, wave, 4, n, r);
   const float l = r.l + __shfl_xor(r.l, 32);
 
   // each wave's O [32][HD] where its K was
@@ -781,8 +1014,6 @@ __global__ void __launch_bounds__(kThreads) tm_prompt_join_kernel(PromptParams p
 // ------------------------------------------------------------------- host --
 
 constexpr int64_t kMaxStride = 1 << 24;  // of a key's row: 64 of them from 32-bit offsets
-constexpr int64_t kSlotsPerCU = 2;   // workgroups of 128 rows a CU holds
-
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Keys of tile `tile` of a sequence: those before the border of its last row.
@@ -791,22 +1022,29 @@ int64_t tile_keys(int64_t q_len, int64_t k_len, int64_t tile, int64_t rows, int6
   return k_len - q_len + last + 1;
 }
 
-// Rows of a tile, by the rows of the longest sequence and the tiles of 128 of all:
-//   32   where no sequence has more: a decoded token's heads;
-//   256  where tiles of 128 would fill the chip's slots four times over;
-//   128  otherwise.
-int64_t rows_of(int64_t longest, int64_t units128) {
-  return longest <= 32 ? 32 : units128 >= 4 * kCUs * kSlotsPerCU ? 256 : 128;
+// How the rows are tiled, by the rows of the longest sequence, the tiles of 128 of all, and
+// their stages of 64 keys:
+//   few    no sequence has more than 32 rows: a decoded token's heads;
+//   tall   tiles of 128 would fill the chip three and a half times;
+//   pair   tiles of 128 have eight stages or more on average;
+//   short  otherwise.
+enum Kind { kFew, kShort, kPair, kTall, kKinds };
+constexpr int64_t kTileRows[kKinds] = {32, 128, 128, 256};
+// Keys that a workgroup takes in one step, and workgroups that the chip holds.
+constexpr int64_t kStepKeys[kKinds] = {4 * kKeys, kKeys, 2 * kKeys, kKeys};
+constexpr int64_t kSlots[kKinds] = {kCUs, 2 * kCUs, kCUs, kCUs};
+// Keys of a stage that one wave loads.
+constexpr int64_t kWaveKeys[kKinds] = {kKeys, kKeys / 4, kKeys / 4, kKeys / 8};
+
+Kind kind_of(int64_t longest, int64_t units128, int64_t stages128) {
+  if (longest <= 32) return kFew;
+  if (2 * units128 >= 7 * kCUs) return kTall;
+  return stages128 >= 8 * units128 ? kPair : kShort;
 }
 
-// Keys of a workgroup's step: a stage, or one of each of the four waves.
-int64_t step_of(int64_t rows) { return rows == 32 ? 4 * kKeys : kKeys; }
-
-// Key ranges of one sequence's tiles: as many as fill the chip's workgroup slots (one a
-// CU for tiles of 32 rows), at least one step or four stages each.
-int64_t chunks_of(int64_t rows, int64_t units, int64_t keys) {
-  const int64_t slots = rows == 32 ? kCUs : kCUs * kSlotsPerCU;
-  const int64_t want = std::min<int64_t>(slots / std::max<int64_t>(units, 1), kMaxChunks);
+// Key ranges of one sequence's tiles: as many as fill the chip, at least four stages each.
+int64_t chunks_of(Kind kind, int64_t units, int64_t keys) {
+  const int64_t want = std::min<int64_t>(kSlots[kind] / std::max<int64_t>(units, 1), kMaxChunks);
   return std::max<int64_t>(1, std::min(want, ceil_div(keys, 4 * kKeys)));
 }
 
@@ -817,6 +1055,7 @@ int check_heads(int64_t Hq, int64_t kvh, int64_t hd) {
 }
 
 struct OnePlan {
+  Kind kind;
   int64_t rows, tiles, chunks, chunk_len, bytes;
 };
 
@@ -824,10 +1063,16 @@ int plan_one(int64_t T, int64_t S, int64_t Hq, int64_t kvh, int64_t hd, OnePlan*
   const int64_t group = Hq / kvh;
   if (T < 0 || S < T || S > TM_MAX_PROMPT_KEYS || T * group > INT32_MAX - 1024)
     return TM_ERR_SHAPE;
-  o->rows = rows_of(T * group, ceil_div(T * group, 128) * kvh);
+  const int64_t tiles128 = ceil_div(T * group, 128);
+  int64_t stages = 0;  // of the tiles of 128, at their mean
+  if (T > 0)
+    stages = tiles128 * ceil_div(tile_keys(T, S, 0, 128, group) +
+                                     tile_keys(T, S, tiles128 - 1, 128, group), 2 * kKeys);
+  o->kind = kind_of(T * group, tiles128 * kvh, stages * kvh);
+  o->rows = kTileRows[o->kind];
   o->tiles = ceil_div(T * group, o->rows);
-  o->chunks = chunks_of(o->rows, o->tiles * kvh, S);
-  const int64_t step = step_of(o->rows);
+  o->chunks = chunks_of(o->kind, o->tiles * kvh, S);
+  const int64_t step = kStepKeys[o->kind];
   o->chunk_len = std::max(step, ceil_div(ceil_div(S, o->chunks), step) * step);
   o->chunks = std::max<int64_t>(1, ceil_div(S, o->chunk_len));
   o->bytes = o->chunks > 1 ? o->tiles * o->chunks * kvh * o->rows * (hd + 2) * 4 : 0;
@@ -835,34 +1080,36 @@ int plan_one(int64_t T, int64_t S, int64_t Hq, int64_t kvh, int64_t hd, OnePlan*
 }
 
 template <int DT, int HD, bool PAGED>
-void launch_rows(const PromptParams& p, int64_t rows, int64_t blocks, int64_t joins,
+void launch_kind(const PromptParams& p, Kind kind, int64_t blocks, int64_t joins,
                  int64_t join_rows, hipStream_t st) {
   const dim3 grid((unsigned)blocks), block(kThreads);
-  if (rows == 32)
+  if (kind == kFew)
     hipLaunchKernelGGL((tm_prompt_few_kernel<DT, HD, PAGED>), grid, block, 0, st, p);
-  else if (rows == 256)
-    hipLaunchKernelGGL((tm_prompt_attn_kernel<DT, HD, 8, PAGED>), grid, dim3(512), 0, st, p);
+  else if (kind == kShort)
+    hipLaunchKernelGGL((tm_prompt_short_kernel<DT, HD, PAGED>), grid, block, 0, st, p);
+  else if (kind == kPair)
+    hipLaunchKernelGGL((tm_prompt_pair_kernel<DT, HD, PAGED>), grid, dim3(512), 0, st, p);
   else
-    hipLaunchKernelGGL((tm_prompt_attn_kernel<DT, HD, 4, PAGED>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((tm_prompt_tall_kernel<DT, HD, PAGED>), grid, dim3(512), 0, st, p);
   if (joins > 0)
     hipLaunchKernelGGL((tm_prompt_join_kernel<DT, HD>),
                        dim3((unsigned)ceil_div(joins * p.kvh * join_rows, 4)), block, 0, st, p,
-                       (int)rows, (int)join_rows);
+                       (int)kTileRows[kind], (int)join_rows);
 }
 
 template <bool PAGED>
-void launch(const PromptParams& p, int dtype, int64_t hd, int64_t rows, int64_t blocks,
+void launch(const PromptParams& p, int dtype, int64_t hd, Kind kind, int64_t blocks,
             int64_t joins, int64_t join_rows, hipStream_t st) {
   if (dtype == TM_DTYPE_F16) {
     if (hd == 128)
-      launch_rows<TM_DTYPE_F16, 128, PAGED>(p, rows, blocks, joins, join_rows, st);
+      launch_kind<TM_DTYPE_F16, 128, PAGED>(p, kind, blocks, joins, join_rows, st);
     else
-      launch_rows<TM_DTYPE_F16, 64, PAGED>(p, rows, blocks, joins, join_rows, st);
+      launch_kind<TM_DTYPE_F16, 64, PAGED>(p, kind, blocks, joins, join_rows, st);
   } else {
     if (hd == 128)
-      launch_rows<TM_DTYPE_BF16, 128, PAGED>(p, rows, blocks, joins, join_rows, st);
+      launch_kind<TM_DTYPE_BF16, 128, PAGED>(p, kind, blocks, joins, join_rows, st);
     else
-      launch_rows<TM_DTYPE_BF16, 64, PAGED>(p, rows, blocks, joins, join_rows, st);
+      launch_kind<TM_DTYPE_BF16, 64, PAGED>(p, kind, blocks, joins, join_rows, st);
   }
 }
 
@@ -880,7 +1127,7 @@ extern "C" int tm_prompt_plan(const int64_t* q_lens, const int64_t* k_lens, int6
   if (sizes == nullptr || B < 0 || (B > 0 && (q_lens == nullptr || k_lens == nullptr)))
     return TM_ERR_ARG;
   const int64_t group = Hq / kvh;
-  int64_t units = 0, q_rows = 0, k_rows = 0, longest = 0;
+  int64_t units = 0, stages = 0, q_rows = 0, k_rows = 0, longest = 0;
   for (int64_t b = 0; b < B; ++b) {
     if (q_lens[b] < 0 || k_lens[b] < q_lens[b] || k_lens[b] > TM_MAX_PROMPT_KEYS)
       return TM_ERR_SHAPE;
@@ -889,16 +1136,18 @@ extern "C" int tm_prompt_plan(const int64_t* q_lens, const int64_t* k_lens, int6
     if (q_rows * group > INT32_MAX - 1024 || k_rows > INT32_MAX) return TM_ERR_SHAPE;
     units += ceil_div(q_lens[b] * group, 128) * kvh;
     longest = std::max(longest, q_lens[b] * group);
+    for (int64_t t = 0; t * 128 < q_lens[b] * group; ++t)
+      stages += ceil_div(tile_keys(q_lens[b], k_lens[b], t, 128, group), kKeys) * kvh;
   }
-  const int64_t rows = rows_of(longest, units);
-  const int64_t step = step_of(rows);
+  const Kind kind = kind_of(longest, units, stages);
+  const int64_t rows = kTileRows[kind], step = kStepKeys[kind];
   // stages of all workgroups, and how many one of them may have before its keys are
   // split: twice an even share of the chip's slots
-  int64_t stages = 0;
+  stages = 0;
   for (int64_t b = 0; b < B; ++b)
     for (int64_t t = 0; t * rows < q_lens[b] * group; ++t)
       stages += ceil_div(tile_keys(q_lens[b], k_lens[b], t, rows, group), kKeys) * kvh;
-  const int64_t share = std::max<int64_t>(4, ceil_div(stages, kCUs * (rows == 32 ? 1 : kSlotsPerCU)));
+  const int64_t share = std::max<int64_t>(4, ceil_div(stages, kSlots[kind]));
   std::vector<std::pair<int64_t, Item>> list;  // (keys, item)
   std::vector<Join> jlist;
   int64_t q0 = 0, k0 = 0, slots = 0;
@@ -938,9 +1187,10 @@ extern "C" int tm_prompt_plan(const int64_t* q_lens, const int64_t* k_lens, int6
   sizes[0] = (int64_t)list.size();
   sizes[1] = (int64_t)jlist.size();
   sizes[2] = slots;
-  sizes[3] = rows;
+  sizes[3] = kind;
   sizes[4] = q_rows;
   sizes[5] = k_rows;
+  sizes[6] = rows;
   if (items == nullptr && joins == nullptr) return TM_OK;
   if (max_items < sizes[0] || max_joins < sizes[1]) return TM_ERR_SHAPE;
   std::stable_sort(list.begin(), list.end(),
@@ -954,7 +1204,7 @@ extern "C" int tm_prompt_plan(const int64_t* q_lens, const int64_t* k_lens, int6
 extern "C" int tm_prompt_attention(const void* q, int64_t q_stride, const void* k,
                                    int64_t k_stride, const void* v, int64_t v_stride,
                                    const int32_t* items, int64_t num_items, const int32_t* joins,
-                                   int64_t num_joins, int64_t num_slots, int64_t tile_rows,
+                                   int64_t num_joins, int64_t num_slots, int64_t tiling,
                                    int64_t Hq, int64_t kvh, int64_t hd, float scale, int dtype,
                                    void* out, int64_t out_stride, void* workspace,
                                    int64_t workspace_bytes, void* stream) {
@@ -962,7 +1212,9 @@ extern "C" int tm_prompt_attention(const void* q, int64_t q_stride, const void* 
   if (rc) return rc;
   if ((dtype != TM_DTYPE_BF16 && dtype != TM_DTYPE_F16) || !(scale > 0.0f) || scale == INFINITY)
     return TM_ERR_ARG;
-  if ((tile_rows != 32 && tile_rows != 128 && tile_rows != 256) || num_items < 0 || num_joins < 0 || num_slots < 0 ||
+  if (tiling < 0 || tiling >= kKinds) return TM_ERR_ARG;
+  const int64_t tile_rows = kTileRows[tiling];
+  if (num_items < 0 || num_joins < 0 || num_slots < 0 ||
       num_items * kvh > INT32_MAX || num_joins * kvh * tile_rows / 4 > INT32_MAX ||
       num_slots > INT32_MAX)
     return TM_ERR_SHAPE;
@@ -991,7 +1243,7 @@ extern "C" int tm_prompt_attention(const void* q, int64_t q_stride, const void* 
   p.kvh = (int)kvh;
   p.group = (int)(Hq / kvh);
   p.scale_log2 = scale * 1.4426950408889634f;
-  launch<false>(p, dtype, hd, tile_rows, num_items * kvh, num_joins, tile_rows,
+  launch<false>(p, dtype, hd, (Kind)tiling, num_items * kvh, num_joins, tile_rows,
                 (hipStream_t)stream);
   TM_HIP_CHECK_LAUNCH();
   return TM_OK;
@@ -1063,8 +1315,9 @@ extern "C" int tm_prompt_attention_cached(const void* q, int64_t q_stride, int64
   p.page_shift = shift;
   p.table_pages = (int)num_table_pages;
   p.cache_pages = (int)cache_pages;
+  p.wide = page_size >= kWaveKeys[o.kind] ? 1 : 0;
   p.scale_log2 = scale * 1.4426950408889634f;
-  launch<true>(p, dtype, hd, o.rows, o.tiles * o.chunks * kvh, o.chunks > 1 ? o.tiles : 0,
+  launch<true>(p, dtype, hd, o.kind, o.tiles * o.chunks * kvh, o.chunks > 1 ? o.tiles : 0,
                std::min(o.rows, T * p.group), (hipStream_t)stream);
   TM_HIP_CHECK_LAUNCH();
   return TM_OK;

@@ -40,14 +40,14 @@ class PromptPlan:
             raise ValueError("num_heads must be a multiple of num_kv_heads")
         n = len(q_lens)
         ql, kl = (ctypes.c_int64 * n)(*q_lens), (ctypes.c_int64 * n)(*k_lens)
-        sizes = (ctypes.c_int64 * 6)()
+        sizes = (ctypes.c_int64 * 7)()
         _capi.call("tm_prompt_plan", ql, kl, n, num_heads, num_kv_heads, None, 0, None, 0, sizes)
         items = torch.zeros(max(1, sizes[0]), 8, dtype=torch.int32)
         joins = torch.zeros(max(1, sizes[1]), 8, dtype=torch.int32)
         _capi.call("tm_prompt_plan", ql, kl, n, num_heads, num_kv_heads, items.data_ptr(),
                    sizes[0], joins.data_ptr(), sizes[1], sizes)
-        self.num_items, self.num_joins, self.num_slots, self.tile_rows, self.q_rows, \
-            self.k_rows = list(sizes)
+        self.num_items, self.num_joins, self.num_slots, self.tiling, self.q_rows, \
+            self.k_rows, self.tile_rows = list(sizes)
         self.num_heads, self.num_kv_heads = num_heads, num_kv_heads
         self.items, self.joins = items.to(device), joins.to(device)
         self.device = self.items.device
@@ -121,7 +121,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pr
     _capi.launch("tm_prompt_attention", index, q.data_ptr(), qs, k.data_ptr(),
                  k.stride(0) if s > 1 else kvh * hd, v.data_ptr(),
                  v.stride(0) if s > 1 else kvh * hd, plan.items.data_ptr(), plan.num_items,
-                 plan.joins.data_ptr(), plan.num_joins, plan.num_slots, plan.tile_rows, hq, kvh,
+                 plan.joins.data_ptr(), plan.num_joins, plan.num_slots, plan.tiling, hq, kvh,
                  hd, scale, dt, out.data_ptr(), os, ptr(ws), nbytes)
     return out
 
