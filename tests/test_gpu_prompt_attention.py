@@ -102,16 +102,31 @@ def test_packed(q_lens, k_lens, hq, kvh, hd):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_large_tiles(dtype):
-    """Enough rows for the 256-row tiles."""
-    from treemoe_spec_amd.kernels.prompt_attention import PromptPlan
-
+    """Large batches: several tiles a compute unit."""
     _say(f"large tiles {dtype}")
     lens = [1900, 2300, 777]
-    assert PromptPlan(lens, num_heads=64, num_kv_heads=16).tile_rows == 256
     _packed(lens, lens, 64, 16, 64, dtype, 5)
     lens = [900, 2, 4000, 0, 3400]
-    assert PromptPlan(lens, num_heads=32, num_kv_heads=8).tile_rows == 256
     _packed(lens, lens, 32, 8, 128, dtype, 6)
+
+
+@pytest.mark.parametrize("q_lens,k_lens,hq,kvh,tiling", [
+    ([7, 1, 0], [100, 1, 0], 8, 2, 0),
+    ([8] * 3, [3000, 8, 8], 8, 2, 0),
+    ([9, 300], [9, 300], 8, 2, 1),
+    ([60] * 100, [60] * 100, 8, 2, 1),
+    ([700, 3], [1300, 900], 8, 2, 2),
+    ([3500, 4000, 1], [3500, 4100, 4000], 32, 8, 3),
+])
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 128), (torch.float16, 64)])
+def test_every_tiling(q_lens, k_lens, hq, kvh, tiling, dtype, hd):
+    """Few rows, short, pair and tall tiles, each with a sequence that leaves parts of
+    its tiles without rows."""
+    from treemoe_spec_amd.kernels.prompt_attention import PromptPlan
+
+    _say(f"tiling {tiling} {dtype} hd={hd}")
+    assert PromptPlan(q_lens, k_lens, num_heads=hq, num_kv_heads=kvh).tiling == tiling
+    _packed(q_lens, k_lens, hq, kvh, hd, dtype, tiling + hd)
 
 
 def _cache(s, kvh, hd, dtype, page, seed, layers=2):

@@ -1022,12 +1022,18 @@ int64_t tile_keys(int64_t q_len, int64_t k_len, int64_t tile, int64_t rows, int6
   return k_len - q_len + last + 1;
 }
 
-// How the rows are tiled, by the rows of the longest sequence, the tiles of 128 of all, and
-// their stages of 64 keys:
+// How the rows are tiled, by the rows of the longest sequence, the tiles of 128 rows of all
+// sequences, and their stages of 64 keys on average:
 //   few    no sequence has more than 32 rows: a decoded token's heads;
-//   tall   tiles of 128 would fill the chip three and a half times;
-//   pair   tiles of 128 have eight stages or more on average;
+//   tall   3.5 tiles a CU or more, of 24 stages or more;
+//   pair   fewer tiles, of 8 stages or more;
 //   short  otherwise.
+// Measured, 32 query heads over 8 of 128 elements, the three tilings in us: one prompt of
+// 517 tokens short 21, pair 21; 1000 tokens 35, 25, tall 38; 2048 59, 52, 63; 4000 164, 160,
+// 150; 8192 pair 554, tall 520; 12 prompts of 1-2048 tokens (fp16) short 77, pair 102, tall
+// 85; 20 of 100 short 18, pair 27, tall 22; 300 tokens over 1000 cached short 32, pair
+// 30.  Where a CU goes through several tiles of few stages, the two workgroups of `short`
+// hide each other's first loads and last stores.
 enum Kind { kFew, kShort, kPair, kTall, kKinds };
 constexpr int64_t kTileRows[kKinds] = {32, 128, 128, 256};
 // Keys that a workgroup takes in one step, and workgroups that the chip holds.
@@ -1038,7 +1044,7 @@ constexpr int64_t kWaveKeys[kKinds] = {kKeys, kKeys / 4, kKeys / 4, kKeys / 8};
 
 Kind kind_of(int64_t longest, int64_t units128, int64_t stages128) {
   if (longest <= 32) return kFew;
-  if (2 * units128 >= 7 * kCUs) return kTall;
+  if (2 * units128 >= 7 * kCUs) return stages128 >= 24 * units128 ? kTall : kShort;
   return stages128 >= 8 * units128 ? kPair : kShort;
 }
 

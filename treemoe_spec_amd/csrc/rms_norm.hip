@@ -71,6 +71,33 @@ __device__ __forceinline__ uint32_t pack_e4m3(float lo, float hi) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, 0, false) & 0xffffu;
 }
 
+// The largest of v over the lane's group of `group` / 8 lanes (a power of two, 4 .. 64).
+__device__ __forceinline__ uint32_t top_of_group(uint32_t v, int group) {
+#define TM_MAX(ctrl) \
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, ctrl, 0xf, 0xf, false))
+  TM_MAX(0xb1);   // lane ^ 1
+  TM_MAX(0x4e);   // lane ^ 2
+  if (group >= 64) TM_MAX(0x141);   // the other four of eight
+  if (group >= 128) TM_MAX(0x140);  // the other eight of sixteen
+#undef TM_MAX
+  if (group >= 256) v = max(v, (uint32_t)__shfl_xor((int)v, 16));
+  if (group >= 512) v = max(v, (uint32_t)__shfl_xor((int)v, 32));
+  return v;
+}
+
+// v over `scale`, by its inverse: off by three roundings in 32 bits at most, against
+// e4m3's half step of 2^-4.  An inverse would be infinite below 2^-126 or so.
+__device__ __forceinline__ void divide(float (&v)[8], float scale) {
+  if (scale > 1e-37f) {
+    const float inv = 1.0f / scale;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= inv;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] /= scale;
+  }
+}
+
 // NC chunks of 8 elements a thread; W waves a row.  With W = 1 the four waves of a
 // workgroup take a row each and no barrier is needed.
 template <int DT, int NC, int W, bool FP8>
@@ -152,14 +179,12 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) tm_rms_norm_kernel(Norm
       for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(s[c][e]) & 0x7fffffffu);
       if (p.group != 0) {
         // a group is group / 8 consecutive lanes of one chunk
-        uint32_t g = top;
-        for (int m = p.group >> 4; m > 0; m >>= 1) g = max(g, (uint32_t)__shfl_xor((int)g, m));
+        const uint32_t g = top_of_group(top, p.group);
         const float scale = g == 0u ? 1.0f : __uint_as_float(g) / 448.0f;
         if (i < p.hidden) {
           if ((i & (p.group - 1)) == 0)
             p.scales[row * p.scale_stride + i / p.group] = scale;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) s[c][e] = s[c][e] / scale;
+          divide(s[c], scale);
         }
         top = 0u;
       }
@@ -184,14 +209,11 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) tm_rms_norm_kernel(Norm
     for (int c = 0; c < NC; ++c) {
       const int i = (c * kThreads + t) * 8;
       if (i >= p.hidden) continue;
+      if (p.group == 0) divide(s[c], scale);
       uint32_t q[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float a = s[c][2 * j], b = s[c][2 * j + 1];
-        if (p.group == 0) {
-          a = a / scale;
-          b = b / scale;
-        }
         // |y| / (amax / 448) can pass 448 by a rounding only; NaN stays NaN
         a = a > 448.0f ? 448.0f : a < -448.0f ? -448.0f : a;
         b = b > 448.0f ? 448.0f : b < -448.0f ? -448.0f : b;
