@@ -51,6 +51,7 @@ extern "C" {
 #define TM_MAX_NORM_HIDDEN 65536  /* columns of tm_rms_norm */
 #define TM_MAX_PROMPT_KEYS (1 << 24)  /* keys of one sequence of prompt attention */
 #define TM_MAX_SAMPLE_VOCAB 262144  /* columns of tm_sample_tokens */
+#define TM_MAX_ROWS (1 << 21)  /* rows or tokens of one norm, rotary or sampling call */
 
 /* ABI version (major*10000 + minor*100 + patch): 5.0.0.  Version 2 added
  * num_edges to tm_op4_argmax_walk / tm_op4_sample_walk and softmax_argmax to
@@ -438,7 +439,8 @@ int tm_tree_mask_pack(const uint8_t* mask, int64_t N, int64_t row_stride,
  * (treemoe/model/mixtral.py:268-340).  x, out: dtype.  residual may be NULL; it
  * and res_out (which may be the same memory) have res_dtype, weight has
  * weight_dtype, each `dtype` or fp32.  Strides in elements, rows contiguous,
- * H <= TM_MAX_NORM_HIDDEN.  16-byte aligned rows with H % 8 == 0 take vector
+ * H <= TM_MAX_NORM_HIDDEN, T <= TM_MAX_ROWS.  out may be x's memory; otherwise
+ * outputs lie apart from the inputs and from each other.  16-byte aligned rows with H % 8 == 0 take vector
  * loads; any other alignment and width is served too.
  */
 int tm_rms_norm(const void* x, int64_t x_stride, const void* residual,
@@ -469,7 +471,8 @@ int tm_rms_norm_fp8(const void* x, int64_t x_stride, const void* residual,
  * elements (i, i + part / 2), or (2 i, 2 i + 1) when interleaved.  Elements from
  * `part` on are copied.  positions: [T] int32, or int64 with long_positions.
  * Heads contiguous, token strides in elements; hd and part multiples of 16,
- * 16-byte aligned tokens.  The outputs may be the inputs' memory.
+ * 16-byte aligned tokens; T <= TM_MAX_ROWS.  An output is its input's memory, element
+ * for element, or lies apart from both inputs.
  */
 int tm_rotary(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
               void* q_out, int64_t q_out_stride, void* k_out,
@@ -514,7 +517,7 @@ int tm_rotary_append(const void* q, int64_t q_stride, const void* k, int64_t k_s
  *
  * temperatures, top_ks, top_ps, min_ps: one value a row, or NULL for the scalar
  * beside it.  A row value out of its range acts as the nearest one in it.
- * V <= TM_MAX_SAMPLE_VOCAB.
+ * V <= TM_MAX_SAMPLE_VOCAB, N <= TM_MAX_ROWS.  probs lies apart from the logits.
  */
 int tm_sample_tokens(const void* logits, int dtype, int64_t N, int64_t V,
                      int64_t row_stride, const float* uniforms,
@@ -545,8 +548,9 @@ int tm_prompt_plan(const int64_t* q_lens, const int64_t* k_lens, int64_t B,
  * [Sk, kvh, hd], bf16 or fp16, heads contiguous, token strides in elements, 16-byte
  * aligned; hd 64 or 128.  items, joins (device memory, 32-byte aligned) and the four
  * numbers come from tm_prompt_plan for sequences that fit Tq and Sk.  Rows of
- * out behind the last sequence are not written.  workspace: num_slots * kvh *
- * tile_rows * (hd + 2) * 4 bytes.
+ * out behind the last sequence are not written.  out lies apart from q, k and v.
+ * workspace: num_slots * kvh * tile_rows * (hd + 2) * 4 bytes, of this call alone
+ * until it has ended on the stream.
  */
 int tm_prompt_attention(const void* q, int64_t q_stride, const void* k,
                         int64_t k_stride, const void* v, int64_t v_stride,
@@ -566,7 +570,8 @@ int tm_prompt_cached_workspace(int64_t T, int64_t seq_len, int64_t Hq, int64_t k
  * (treemoe/model/kv_cache.py:110-123) and the causal
  * `F.scaled_dot_product_attention` behind it.  Keys are read in place through the
  * block table (position p: page block_table[p / page_size], slot p % page_size;
- * page_size a power of two).  Page ids are clamped to [0, cache_pages).
+ * page_size a power of two).  Page ids are clamped to [0, cache_pages).  out and the
+ * workspace as above.
  */
 int tm_prompt_attention_cached(const void* q, int64_t q_stride, int64_t T,
                                const void* k_cache, const void* v_cache,

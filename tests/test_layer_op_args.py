@@ -27,6 +27,26 @@ def calls(monkeypatch):
 
 # ------------------------------------------------------------------- Python --
 
+def test_rows_are_bounded(calls):
+    n = _capi.TM_MAX_ROWS + 1
+    with pytest.raises(ValueError, match="at most"):
+        rn.rms_norm(torch.zeros(1, 8).expand(n, 8), torch.zeros(8))
+    plan = ro.RotaryPlan(16, 1e4, device="cpu")
+    q = torch.zeros(1, 1, 16).expand(n, 1, 16)
+    with pytest.raises(ValueError, match="at most"):
+        ro.rotary_embed(q, None, torch.zeros(1, dtype=torch.int32).expand(n), plan)
+    with pytest.raises(ValueError, match="at most"):
+        st.sample_tokens(torch.zeros(1, 8).expand(n, 8), torch.zeros(1).expand(n))
+    assert not calls
+
+
+def test_probs_over_the_logits_are_refused(calls):
+    x = torch.zeros(2, 8)
+    with pytest.raises(ValueError, match="apart"):
+        st.sample_tokens(x, torch.zeros(2), return_probs=True, probs_out=x)
+    assert not calls
+
+
 def test_cpu_tensors_raise():
     x, w = torch.zeros(2, 8), torch.zeros(8)
     with pytest.raises(RuntimeError, match="ROCm"):

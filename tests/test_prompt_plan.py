@@ -116,6 +116,14 @@ def test_prompt_attention_refuses(calls, kw):
     assert not calls
 
 
+def test_out_over_the_queries_is_refused(calls):
+    q = torch.zeros(5, 8, 64, dtype=BF)
+    k = torch.zeros(7, 2, 64, dtype=BF)
+    with pytest.raises(ValueError, match="apart"):
+        pa.prompt_attention(q, k, k, _plan([3, 2], [4, 3]), out=q.view(5, 512))
+    assert not calls
+
+
 def test_prompt_attention_arguments(calls):
     plan = _plan([3, 2], [4, 3])
     q = torch.zeros(6, 12, 64, dtype=BF)[:, :8]
@@ -179,11 +187,33 @@ PACKED = dict(q=0, qs=512, k=0, ks=128, v=0, vs=128, items=0, n=1, joins=0, nj=0
     ({"scale": 0.0}, 1003), ({"scale": math.nan}, 1003), ({"scale": math.inf}, 1003),
     ({"tiling": 4}, 1003), ({"tiling": -1}, 1003), ({"n": -1}, 1001), ({"n": 1 << 31}, 1001),
     ({"qs": 500}, 1001), ({"ks": 120}, 1001), ({"vs": 1 << 25}, 1001), ({"os": 8}, 1001),
-    ({"slots": 2}, 1001), ({"n": 0}, 0), ({"q": 8}, 1002), ({"ks": 132}, 1002), ({"items": 16}, 1002),
+    ({"slots": 2}, 1001), ({"n": 0}, 0),
+    ({"n": 1 << 23, "kvh": 8}, 1001), ({"n": 1 << 23, "hq": 1, "kvh": 1, "tiling": 3}, 1001),
+    ({"nj": 2}, 1001), ({}, 1003), ({"items": 32, "n": 1, "nj": 1}, 1003), ({"q": 8}, 1002), ({"ks": 132}, 1002), ({"items": 16}, 1002),
     ({"ws": 8}, 1002),
 ])
 def test_prompt_attention_entry_point(kw, expect):
     assert _c("tm_prompt_attention", PACKED, kw) == expect
+
+
+def test_plan_entry_point():
+    plan = _capi.lib().tm_prompt_plan
+    one = (ctypes.c_int64 * 1)(8)
+    long = (ctypes.c_int64 * 1)(50000)
+    sizes = (ctypes.c_int64 * 7)()
+    items, joins = (ctypes.c_int32 * 4096)(), (ctypes.c_int32 * 4096)()
+    assert plan(one, long, 1, 8, 2, None, 0, None, 0, sizes) == 0
+    assert sizes[0] > 1 and sizes[1] > 0
+    assert plan(one, long, 1, 8, 2, items, 512, joins, 512, sizes) == 0
+    assert plan(one, long, 1, 8, 2, None, 512, joins, 512, sizes) == 1003
+    assert plan(one, long, 1, 8, 2, items, 512, None, 512, sizes) == 1003
+    assert plan(one, long, 1, 8, 2, items, sizes[0] - 1, joins, 512, sizes) == 1001
+    assert plan(one, long, 1, 8, 2, items, 512, joins, 0, sizes) == 1001
+    assert plan(one, one, 1, 8, 2, items, 1, None, 0, sizes) == 0 and sizes[1] == 0
+    assert plan(long, one, 1, 8, 2, items, 1, None, 0, sizes) == 1001
+    assert plan(None, None, 1, 8, 2, items, 1, None, 0, sizes) == 1003
+    assert plan(None, None, 0, 8, 2, items, 1, None, 0, sizes) == 0 and sizes[0] == 0
+    assert plan(one, one, 1, 8, 2, None, 0, None, 0, None) == 1003
 
 
 CACHED = dict(q=0, qs=512, T=4, k=0, v=0, sp=16 * 128, ss=128, page=16, pages=4, table=0, n_table=4,

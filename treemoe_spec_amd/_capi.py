@@ -71,6 +71,7 @@ TM_OP4_NOALLOC_MAX_NODES = 2048
 TM_MAX_NORM_HIDDEN = 65536
 TM_MAX_SAMPLE_VOCAB = 262144
 TM_MAX_PROMPT_KEYS = 1 << 24
+TM_MAX_ROWS = 1 << 21
 
 _lib = None
 

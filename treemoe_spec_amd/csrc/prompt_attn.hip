@@ -29,6 +29,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <new>
 #include <utility>
 #include <vector>
 
@@ -1119,6 +1120,12 @@ void launch(const PromptParams& p, int dtype, int64_t hd, Kind kind, int64_t blo
   }
 }
 
+// A grid counts its threads in 32 bits.
+bool grids_ok(Kind kind, int64_t blocks, int64_t joins_rows) {
+  const int64_t threads = kind == kPair || kind == kTall ? 512 : kThreads;
+  return blocks <= UINT32_MAX / threads && joins_rows <= UINT32_MAX / 64;
+}
+
 bool vec_ok(const void* p, int64_t stride, int64_t tokens) {
   return (uintptr_t)p % 16 == 0 && (tokens <= 1 || stride % 8 == 0);
 }
@@ -1127,7 +1134,7 @@ bool vec_ok(const void* p, int64_t stride, int64_t tokens) {
 
 extern "C" int tm_prompt_plan(const int64_t* q_lens, const int64_t* k_lens, int64_t B, int64_t Hq,
                               int64_t kvh, int32_t* items, int64_t max_items, int32_t* joins,
-                              int64_t max_joins, int64_t* sizes) {
+                              int64_t max_joins, int64_t* sizes) try {
   int rc = check_heads(Hq, kvh, 128);
   if (rc) return rc;
   if (sizes == nullptr || B < 0 || (B > 0 && (q_lens == nullptr || k_lens == nullptr)))
@@ -1199,12 +1206,16 @@ extern "C" int tm_prompt_plan(const int64_t* q_lens, const int64_t* k_lens, int6
   sizes[6] = rows;
   if (items == nullptr && joins == nullptr) return TM_OK;
   if (max_items < sizes[0] || max_joins < sizes[1]) return TM_ERR_SHAPE;
+  if ((items == nullptr && !list.empty()) || (joins == nullptr && !jlist.empty()))
+    return TM_ERR_ARG;
   std::stable_sort(list.begin(), list.end(),
                    [](const auto& a, const auto& b) { return a.first > b.first; });
   for (size_t i = 0; i < list.size(); ++i)
     memcpy(items + 8 * i, &list[i].second, sizeof(Item));
   if (!jlist.empty()) memcpy(joins, jlist.data(), jlist.size() * sizeof(Join));
   return TM_OK;
+} catch (const std::bad_alloc&) {
+  return TM_ERR_SHAPE;  // more work items than the host has memory for
 }
 
 extern "C" int tm_prompt_attention(const void* q, int64_t q_stride, const void* k,
@@ -1220,9 +1231,9 @@ extern "C" int tm_prompt_attention(const void* q, int64_t q_stride, const void* 
     return TM_ERR_ARG;
   if (tiling < 0 || tiling >= kKinds) return TM_ERR_ARG;
   const int64_t tile_rows = kTileRows[tiling];
-  if (num_items < 0 || num_joins < 0 || num_slots < 0 ||
-      num_items * kvh > INT32_MAX || num_joins * kvh * tile_rows / 4 > INT32_MAX ||
-      num_slots > INT32_MAX)
+  if (num_items < 0 || num_joins < 0 || num_slots < 0 || num_items > INT32_MAX ||
+      num_joins > num_items || num_slots > num_items ||
+      !grids_ok((Kind)tiling, num_items * kvh, num_joins * kvh * tile_rows))
     return TM_ERR_SHAPE;
   if (q_stride < Hq * hd || out_stride < Hq * hd || k_stride < kvh * hd || v_stride < kvh * hd ||
       k_stride > kMaxStride || v_stride > kMaxStride)
@@ -1233,6 +1244,8 @@ extern "C" int tm_prompt_attention(const void* q, int64_t q_stride, const void* 
       !vec_ok(out, out_stride, 2) || (uintptr_t)items % 32 || (uintptr_t)joins % 32 ||
       (uintptr_t)workspace % 16)
     return TM_ERR_ALIGN;
+  // (without lists the kernels would take one sequence by arithmetic)
+  if (items == nullptr || (num_joins > 0 && joins == nullptr)) return TM_ERR_ARG;
   PromptParams p = {};
   p.q = (const uint16_t*)q;
   p.k = (const uint16_t*)k;
@@ -1291,8 +1304,8 @@ extern "C" int tm_prompt_attention_cached(const void* q, int64_t q_stride, int64
   if ((T > 1 && (q_stride < Hq * hd || out_stride < Hq * hd)) || stride_slot < kvh * hd ||
       stride_slot > kMaxStride || stride_page < page_size * stride_slot)
     return TM_ERR_SHAPE;
-  if (o.bytes > workspace_bytes || o.tiles * o.chunks * kvh > INT32_MAX ||
-      o.tiles * kvh * o.rows / 4 > INT32_MAX)
+  if (o.bytes > workspace_bytes ||
+      !grids_ok(o.kind, o.tiles * o.chunks * kvh, o.chunks > 1 ? o.tiles * kvh * o.rows : 0))
     return TM_ERR_SHAPE;
   if (!vec_ok(q, q_stride, T) || !vec_ok(out, out_stride, T) || !vec_ok(k_cache, stride_slot, 2) ||
       !vec_ok(v_cache, stride_page, 2) || (uintptr_t)block_table % 4 || (uintptr_t)workspace % 16)

@@ -264,7 +264,7 @@ int rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t res_
   if (weight_dtype != dtype && weight_dtype != TM_DTYPE_F32) return TM_ERR_ARG;
   if (residual != nullptr && res_dtype != dtype && res_dtype != TM_DTYPE_F32) return TM_ERR_ARG;
   if (!(eps >= 0.0f)) return TM_ERR_ARG;
-  if (T < 0 || T > INT32_MAX || H < 1 || H > TM_MAX_NORM_HIDDEN) return TM_ERR_SHAPE;
+  if (T < 0 || T > TM_MAX_ROWS || H < 1 || H > TM_MAX_NORM_HIDDEN) return TM_ERR_SHAPE;
   if (T == 0) return TM_OK;
   if (T > 1 && (x_stride < H || out_stride < H)) return TM_ERR_SHAPE;
   if (residual != nullptr && (res_out == nullptr || (T > 1 && (res_stride < H ||

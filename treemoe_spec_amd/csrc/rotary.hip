@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(256) tm_rotary_kernel(RotaryParams p) {
 }
 
 template <bool APPEND>
-void launch(const RotaryParams& p, int dtype, bool inter, hipStream_t st) {
+int launch(const RotaryParams& p, int dtype, bool inter, hipStream_t st) {
   const int64_t threads = (int64_t)p.tokens * p.slots * p.units;
   const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
 #define TM_ROT(DT)                                                                         \
@@ -178,6 +178,8 @@ void launch(const RotaryParams& p, int dtype, bool inter, hipStream_t st) {
     TM_ROT(TM_DTYPE_F32);
   }
 #undef TM_ROT
+  TM_HIP_CHECK_LAUNCH();
+  return TM_OK;
 }
 
 // Head slots of a token: one head a thread at few tokens, 8 slots (five heads each
@@ -188,7 +190,7 @@ int head_slots(int64_t tokens, int heads) {
 
 int check(int64_t T, int64_t hd, int64_t part, int64_t q_heads, int64_t kv_heads, int dtype) {
   if (!tm_dtype_ok(dtype)) return TM_ERR_ARG;
-  if (T < 0 || T > (1 << 24) || hd < 16 || hd > 1024 || hd % 16 != 0 || part < 16 || part > hd ||
+  if (T < 0 || T > TM_MAX_ROWS || hd < 16 || hd > 1024 || hd % 16 != 0 || part < 16 || part > hd ||
       part % 16 != 0 || q_heads < 0 || kv_heads < 0 || q_heads > 1024 || kv_heads > 1024)
     return TM_ERR_SHAPE;
   return TM_OK;
@@ -239,9 +241,7 @@ extern "C" int tm_rotary(const void* q, int64_t q_stride, const void* k, int64_t
   p.part = (int)part;
   p.long_positions = long_positions ? 1 : 0;
   p.magnitude = magnitude;
-  launch<false>(p, dtype, interleaved != 0, (hipStream_t)stream);
-  TM_HIP_CHECK_LAUNCH();
-  return TM_OK;
+  return launch<false>(p, dtype, interleaved != 0, (hipStream_t)stream);
 }
 
 extern "C" int tm_rotary_append(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
@@ -299,7 +299,5 @@ extern "C" int tm_rotary_append(const void* q, int64_t q_stride, const void* k, 
   p.table_pages = (int)num_table_pages;
   p.cache_pages = (int)cache_pages;
   p.magnitude = magnitude;
-  launch<true>(p, dtype, interleaved != 0, (hipStream_t)stream);
-  TM_HIP_CHECK_LAUNCH();
-  return TM_OK;
+  return launch<true>(p, dtype, interleaved != 0, (hipStream_t)stream);
 }

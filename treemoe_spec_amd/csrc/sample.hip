@@ -794,7 +794,7 @@ extern "C" int tm_sample_tokens(const void* logits, int dtype, int64_t N, int64_
   if (!top_ks && top_k < 0) return TM_ERR_ARG;
   if (!top_ps && !(top_p >= 0.0 && top_p <= 1.0)) return TM_ERR_ARG;
   if (!min_ps && !(min_p >= 0.0 && min_p <= 1.0)) return TM_ERR_ARG;
-  if (N < 0 || N > INT32_MAX || V < 1 || V > TM_MAX_SAMPLE_VOCAB) return TM_ERR_SHAPE;
+  if (N < 0 || N > TM_MAX_ROWS || V < 1 || V > TM_MAX_SAMPLE_VOCAB) return TM_ERR_SHAPE;
   if (N == 0) return TM_OK;
   if (N > 1 && (row_stride < 0 || (probs && probs_stride < V))) return TM_ERR_SHAPE;
   const int64_t es = tm_dtype_bytes(dtype);

@@ -68,13 +68,15 @@ def _check_q(q: torch.Tensor, out: torch.Tensor | None):
     if st[2] != 1 or (st[1] != hd and hq > 1):
         raise ValueError("q must have contiguous heads")
     width = hq * hd
-    os = width
+    ost = width
     if out is not None:
         if out.shape != (t, width) or out.dtype != q.dtype or out.stride(1) != 1:
             raise ValueError("out must be [T, Hq * hd] of q's dtype")
-        os = out.stride(0) if t > 1 else width
+        ost = out.stride(0) if t > 1 else width
+        if out.data_ptr() == q.data_ptr() and t:
+            raise ValueError("out must lie apart from q, k and v")
     # (the stride of one token says nothing)
-    return dt, t, hq, hd, st[0] if t > 1 else width, os
+    return dt, t, hq, hd, st[0] if t > 1 else width, ost
 
 
 def _check_scale(scale: float | None, hd: int) -> float:
@@ -92,8 +94,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pr
     heads contiguous): ``plan``'s sequences one after the other.  A query attends to
     its sequence's keys up to its own position.  Returns [T, Hq * hd]; T and S may
     exceed the plan's rows (a padded batch): in a new result the rows behind the last
-    sequence are 0, in ``out`` they stay as they were."""
-    dt, t, hq, hd, qs, os = _check_q(q, out)
+    sequence are 0, in ``out`` they stay as they were.  ``out`` shares no memory with
+    q, k and v."""
+    dt, t, hq, hd, qs, ost = _check_q(q, out)
     index = q.get_device()
     if index < 0 or k.get_device() != index or v.get_device() != index \
             or plan.items.get_device() != index or out is not None or q.requires_grad \
@@ -122,7 +125,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pr
                  k.stride(0) if s > 1 else kvh * hd, v.data_ptr(),
                  v.stride(0) if s > 1 else kvh * hd, plan.items.data_ptr(), plan.num_items,
                  plan.joins.data_ptr(), plan.num_joins, plan.num_slots, plan.tiling, hq, kvh,
-                 hd, scale, dt, out.data_ptr(), os, ptr(ws), nbytes)
+                 hd, scale, dt, out.data_ptr(), ost, ptr(ws), nbytes)
     return out
 
 
@@ -145,8 +148,9 @@ def prompt_attention_cached(q: torch.Tensor, kv, layer: int, *, scale: float | N
     the cache holds already (``rotary_append``, ``append``).  Query t attends to
     positions 0 .. seq_len - T + t of ``layer``, read in place through the block table.
     The cache is [L, pages, page, kv_heads, head_dim] of q's dtype, page size a power of
-    two.  Returns [T, Hq * hd]."""
-    dt, t, hq, hd, qs, os = _check_q(q, out)
+    two.  Returns [T, Hq * hd].  A captured call repeats the length and pages that it was
+    captured with."""
+    dt, t, hq, hd, qs, ost = _check_q(q, out)
     kc, vc = kv.k, kv.v
     index = q.get_device()
     if index < 0 or kc.get_device() != index or vc.get_device() != index or out is not None \
@@ -180,6 +184,6 @@ def prompt_attention_cached(q: torch.Tensor, kv, layer: int, *, scale: float | N
     off = kc.element_size() * cst[0] * (layer % layers)
     _capi.launch("tm_prompt_attention_cached", index, q.data_ptr(), qs, t, kc.data_ptr() + off,
                  vc.data_ptr() + off, cst[1], cst[2], page, pages, table.data_ptr(),
-                 len(kv.block_table), seq_len, hq, kvh, hd, scale, dt, out.data_ptr(), os,
+                 len(kv.block_table), seq_len, hq, kvh, hd, scale, dt, out.data_ptr(), ost,
                  ptr(ws), nbytes)
     return out

@@ -31,6 +31,8 @@ def _checked(what, x, weight, eps, residual, residual_out):
         raise ValueError("weight must have x's dtype or float32")
     if h < 1 or h > _capi.TM_MAX_NORM_HIDDEN:
         raise ValueError(f"H must be 1..{_capi.TM_MAX_NORM_HIDDEN}, got {h}")
+    if t > _capi.TM_MAX_ROWS:
+        raise ValueError(f"T must be at most {_capi.TM_MAX_ROWS}, got {t}")
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
     index = x.get_device()
@@ -66,19 +68,21 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *,
     x's dtype, and with a residual the pair of that and ``s`` in the residual's
     dtype.  x [T, H] float32, bfloat16 or float16, rows at any stride; weight [H] and
     residual [T, H] in x's dtype or float32.  The norm takes ``s`` before it is
-    rounded.  ``out`` may be ``x`` and ``residual_out`` may be ``residual``."""
+    rounded.  ``out`` may be ``x`` and ``residual_out`` may be ``residual``;
+    otherwise outputs share no memory with inputs or each other."""
     index, t, h, xs, dt, wdt, rdt = _checked("rms_norm", x, weight, eps, residual, residual_out)
     if out is None:
         out = torch.empty_like(x, memory_format=_ROWS)
-        os = h
+        ost = h
     else:
         if out.shape != x.shape or out.dtype != x.dtype or out.stride(1) != 1 \
                 or out.get_device() != index:
             raise ValueError("out must be [T, H] of x's dtype, on x's device")
-        os = out.stride(0)
+        ost = out.stride(0)
+        _capi.require("rms_norm", x.device, out=out)
     if residual is None:
         _capi.launch("tm_rms_norm", index, x.data_ptr(), xs, 0, 0, dt, weight.data_ptr(), wdt,
-                     t, h, eps, dt, out.data_ptr(), os, 0, 0)
+                     t, h, eps, dt, out.data_ptr(), ost, 0, 0)
         return out
     if residual_out is None:
         residual_out = torch.empty_like(residual, memory_format=_ROWS)
@@ -86,7 +90,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *,
     else:
         ros = residual_out.stride(0)
     _capi.launch("tm_rms_norm", index, x.data_ptr(), xs, residual.data_ptr(), residual.stride(0),
-                 rdt, weight.data_ptr(), wdt, t, h, eps, dt, out.data_ptr(), os,
+                 rdt, weight.data_ptr(), wdt, t, h, eps, dt, out.data_ptr(), ost,
                  residual_out.data_ptr(), ros)
     return out, residual_out
 

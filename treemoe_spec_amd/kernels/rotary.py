@@ -131,6 +131,7 @@ def _output(name: str, out: torch.Tensor | None, x: torch.Tensor, heads: int, hd
     n, stride = _heads_of(name, out, hd, x.dtype, x.shape[0])
     if n != heads or out.get_device() != index:
         raise ValueError(f"{name} must have the shape of its input, on the same device")
+    _capi.require(name, x.device, **{name: out})
     return out, stride
 
 
@@ -140,7 +141,7 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     """q [T, Hq, hd] and k [T, kvh, hd] (or None) rotated by ``positions`` [T] (int32
     or int64); returns (q', k').  float32, bfloat16 or float16, heads contiguous,
     tokens at any 16-byte aligned stride.  ``q_out`` may be ``q``, ``k_out`` may be
-    ``k``."""
+    ``k``; otherwise outputs share no memory with inputs or each other."""
     dtype, hd = q.dtype, plan.head_dim
     dt = dtype_code(dtype)
     if dt is None:
@@ -152,6 +153,8 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
                                                       or k.requires_grad)):
         _capi.require("rotary_embed", q.device, q=q, k=k, positions=positions, plan=turns)
     t = q.shape[0]
+    if t > _capi.TM_MAX_ROWS:
+        raise ValueError(f"T must be at most {_capi.TM_MAX_ROWS}, got {t}")
     heads, qs = _heads_of("q", q, hd, dtype, t)
     wide = positions.dtype == torch.int64
     if positions.shape != (t,) or not (wide or positions.dtype == torch.int32) \
@@ -176,7 +179,8 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Rotar
     """Tokens at positions start_pos .. start_pos + T - 1: returns q [T, Hq, hd]
     rotated, and stores the rotated k and v [T, kvh, hd] at those positions of the
     paged cache ``kv``, mapping pages as ``append`` does (treemoe/model/kv_cache.py:
-    62-78); ``kv.seq_len`` grows to cover them."""
+    62-78); ``kv.seq_len`` grows to cover them.  A captured call repeats the positions
+    and pages that it was captured with."""
     dtype, hd = q.dtype, plan.head_dim
     dt = dtype_code(dtype)
     if dt is None:
@@ -190,6 +194,8 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Rotar
         _capi.require("rotary_append", q.device, q=q, k=k, v=v, plan=turns, k_cache=kc,
                       v_cache=vc)
     t = q.shape[0]
+    if t > _capi.TM_MAX_ROWS:
+        raise ValueError(f"T must be at most {_capi.TM_MAX_ROWS}, got {t}")
     heads, qs = _heads_of("q", q, hd, dtype, t)
     kvh, ks = _heads_of("k", k, hd, dtype, t)
     vh, vs = _heads_of("v", v, hd, dtype, t)

@@ -61,6 +61,8 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *,
         raise ValueError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
     if not 1 <= v <= _capi.TM_MAX_SAMPLE_VOCAB:
         raise ValueError(f"V must be 1..{_capi.TM_MAX_SAMPLE_VOCAB}, got {v}")
+    if n > _capi.TM_MAX_ROWS:
+        raise ValueError(f"N must be at most {_capi.TM_MAX_ROWS}, got {n}")
     if uniforms.shape != (n,) or uniforms.dtype != torch.float32 \
             or (n > 1 and uniforms.stride(0) != 1):
         raise ValueError("uniforms must be a contiguous float32 tensor of N entries")
@@ -85,6 +87,8 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *,
         elif probs.shape != shape or probs.dtype != torch.float32 \
                 or (v > 1 and probs.stride(1) != 1):
             raise ValueError("probs_out must be float32 [N, V] with unit stride along V")
+        elif probs.data_ptr() == logits.data_ptr() and n:
+            raise ValueError("probs_out must lie apart from the logits")
         pp, pst = probs.data_ptr(), probs.stride(0)
     elif probs_out is not None:
         raise ValueError("probs_out without return_probs")
