@@ -116,7 +116,8 @@ class Decoder:
             qr, kr = rotary_embed(q, k, pos.cuda(), self.plan)
             self.rotated(qr, q, pos)
             self.rotated(kr, k, pos)
-            return tree_attention(qr, kr, v.contiguous(), kv, li, mask)
+            v = v.clone(memory_format=torch.contiguous_format)  # kr's strides
+            return tree_attention(qr, kr, v, kv, li, mask)
         return attention
 
 
@@ -156,8 +157,7 @@ def test_prompt_speculative_step_and_decode(seed):
     grand, probs1 = _sample(heads[1:2].expand(2, -1), torch.rand(2, generator=g).cuda(),
                             temperature=0.7)
     tokens = torch.cat([root, kids, grand])
-    draft = torch.cat([probs0[:1], probs1[:1], probs1.new_full((4, cfg.vocab_size),
-                                                               1.0 / cfg.vocab_size)])
+    draft = torch.cat([probs0[:1], probs0, probs1])  # a node's: what it was drawn from
     target = model.run(tokens, model.tree(kv, depth, mask))
     children = [[1, 2, 3], [4, 5], [], [], [], []]
     res = fused_verify_commit(target, draft, tokens, None, children, kv=kv, temperature=0.7,
