@@ -143,8 +143,9 @@ template <int HD, bool PAGED, int NW>
 struct Feed {
   typedef Shape<HD> S;
   static constexpr int kLoads = S::kTile / (1024 * NW);  // loads of a wave per tile
-  // of K and V of a stage, and of the look-up behind them
-  static constexpr int kGroup = 2 * kLoads + (PAGED ? 1 : 0);
+  // of K and V of a stage (a look-up behind them is not counted: a wait for what came
+  // before may then take a load too many, never one too few)
+  static constexpr int kGroup = 2 * kLoads;
   const uint16_t *k, *v;   // the next stage's first row (paged: the cache)
   int64_t k_step, v_step;  // from stage to stage
   int k_stride, v_stride;  // of a key, or of a page's slot
@@ -495,13 +496,14 @@ __device__ __forceinline__ Place begin_rows(const PromptParams& p, const Item& i
 template <int DT, int HD, bool PAGED>
 __device__ __forceinline__ void retake(const PromptParams& p, const Item& it, int kvhead, int s0,
                                        int step, int n, Rows<HD>& r) {
-  float bad = 0.0f;
+  float bad[8] = {r.l * 0.0f};  // 0 times what is not finite is NaN
 #pragma unroll
   for (int ht = 0; ht < HD / 32; ++ht)
 #pragma unroll
-    for (int x = 0; x < 16; ++x) bad += r.o[ht][x] * 0.0f;
-  bad += r.l * 0.0f;
-  if (!__any(bad != 0.0f)) return;  // 0 times what is not finite is NaN
+    for (int x = 0; x < 16; ++x) bad[x & 7] = fmaf(r.o[ht][x], 0.0f, bad[x & 7]);
+  if (!__any(((bad[0] + bad[1]) + (bad[2] + bad[3])) +
+                 ((bad[4] + bad[5]) + (bad[6] + bad[7])) != 0.0f))
+    return;
   const int half = (int)(threadIdx.x & 63) >> 5;
   float m = -INFINITY, l = 0.0f;
 #pragma unroll

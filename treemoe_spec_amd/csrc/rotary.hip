@@ -17,7 +17,9 @@
 //
 // Bound by HBM at many tokens, by the launch at few.  A thread owns 8 pairs, two
 // 16-byte pieces, of the same place in several heads of one token, so its 8 sines
-// and cosines (about 250 instructions) serve all of them.
+// and cosines (about 250 instructions) serve all of them.  Measured (bf16, 32 + 8 heads of
+// 128): 5003 tokens rotated and appended, 123 MB from a cold cache, 24.5 us, 5.0 TB/s of the
+// 4.9 that a large copy reaches; 64 tokens 3.0 us of kernel.
 #include "tm_vec.h"
 
 namespace {
@@ -182,10 +184,13 @@ int launch(const RotaryParams& p, int dtype, bool inter, hipStream_t st) {
   return TM_OK;
 }
 
-// Head slots of a token: one head a thread at few tokens, 8 slots (five heads each
-// of a token's 40 rows) from 1024 tokens on, where the angles are then a small part.
+// Head slots of a token: one head a thread at few tokens, 16 slots (two or three heads
+// each of a token's 40 rows) from 1024 tokens on, where the angles are then a smaller part.
+// Measured (bf16, 32 + 8 heads of 128), one head, 16 slots and 8 slots in us: 64 tokens
+// 3.0, 3.8, 4.7; 512 tokens 4.3, 4.5, 5.4; 1024 5.8, 5.5, 5.9; 2048 9.5, 8.5, 9.3; 5003
+// 18.9, 17.8, 17.8.
 int head_slots(int64_t tokens, int heads) {
-  return tokens < 1024 ? heads : (heads < 8 ? heads : 8);
+  return tokens < 1024 ? heads : (heads < 16 ? heads : 16);
 }
 
 int check(int64_t T, int64_t hd, int64_t part, int64_t q_heads, int64_t kv_heads, int dtype) {

@@ -41,7 +41,11 @@ constexpr int kRound = kThreads * 4;            // logits of one round: 4 consec
 constexpr int kRegRounds = 8;                   // rounds held in registers
 constexpr int kBins = 2048;
 constexpr int kList = 1024;                     // logits of a wave that the list holds
-constexpr int kRank = 256;                      // up to so many in all are ranked by counting
+// Up to so many elements of the list in all are ranked by counting, up to 64 of them by one
+// wave.  Measured (fp32, 32000 logits), in us: 64 rows, top-k 50, ranked 11.2, by the
+// histograms 15.0; top-k 200 and top-p 16.6, 20.5; 1 row, top-k 50 and top-p, by one wave
+// 10.6, by the workgroup 12.7.
+constexpr int kRank = 256;
 constexpr int kRankStep = 8;                    // so many at a time
 constexpr float kSpan = 31.25f;                 // (l_max - l) / temperature of the last bin's end
 constexpr double kUnit = 17592186044416.0;      // 2^44
