@@ -145,7 +145,7 @@ def _cache(s, kvh, hd, dtype, page, seed, layers=2):
 
 @pytest.mark.parametrize("t,s,page", [(1, 1, 16), (1, 5, 16), (1, 64, 16), (1, 65, 64),
                                       (1, 7777, 16), (2, 1000, 64), (63, 64, 16), (64, 64, 1),
-                                      (100, 2500, 16), (517, 1100, 64), (700, 700, 256)])
+                                      (100, 2500, 16), (517, 1100, 64), (700, 700, 256), (520, 3600, 16)])
 @pytest.mark.parametrize("hq,kvh,hd,dtype", [(32, 8, 128, torch.bfloat16),
                                              (8, 2, 64, torch.float16)])
 def test_cached(t, s, page, hq, kvh, hd, dtype):

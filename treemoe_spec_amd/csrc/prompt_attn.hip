@@ -7,12 +7,23 @@
 //
 // Decomposition.  The rows of a KV head are its sequence's (token, head of the group)
 // pairs, token major, so neighbouring rows share every key and the causal border
-// crosses a tile of 128 rows within 128 / group tokens.  A workgroup of 4 waves takes
-// 128 QT such rows against one range of keys, 64 keys a stage; K and V rows go
+// crosses a tile of 128 rows within 128 / group tokens.  A workgroup takes a tile of 32, 128
+// or 256 such rows, 32 a wave, against one range of keys, 64 keys a stage; K and V rows go
 // straight from memory to LDS (16 bytes a lane, no registers between), V transposed
 // as it is read from there.  Few rows over many keys are split over key ranges; each
 // leaves its sum, maximum and unnormalised output in fp32 in the workspace, which a
-// second kernel joins in key order.
+// second kernel joins in key order.  Four kernels (the rule between them: kind_of):
+//   few    32 rows; four waves take the stages in turn, no barrier between them
+//   short  128 rows, two workgroups a CU
+//   pair   128 rows; eight waves, half of them on every other stage
+//   tall   256 rows; eight waves
+// In pair and tall one wave of a SIMD is in the matrix products while the other weighs.
+//
+// Bound by the matrix pipe, the exponentials and the power limit at many rows: 8192 tokens,
+// 32 heads over 8 of 128 in bf16, 549 GFLOP in 525 us, 1.05 PFLOP/s, where a plain 16384^3
+// product reaches 1.39; 4.0 k tokens 0.87 PFLOP/s.  By HBM at few rows: one token over 40000
+// keys 32 us, 5.2 TB/s; over 7777 14.3 us, of which 2.5 are the second launch and about 6
+// the latency of one stage.
 //
 // Per wave and stage (v_mfma_f32_32x32x16):
 //   S^T = K Q^T   lane l holds S^T[key 32 kt + 8 (v / 4) + 4 (l / 32) + v % 4][query l % 32]
@@ -71,7 +82,7 @@ struct PromptParams {
   const int32_t* table;        // block table (paged)
   const Item* items;           // NULL: one sequence, items by arithmetic
   const Join* joins;
-  float* part;                 // [slot][kvh][tile rows][hd]
+  float* part;                 // [slot][kvh][tile rows][hd], 32 rows as end_rows lays them
   float* stats;                // [slot][kvh][tile rows][2]
   int64_t q_stride, k_stride, v_stride, out_stride;  // paged: k_stride is the slot's
   int64_t stride_page;
@@ -557,7 +568,8 @@ __device__ __forceinline__ void retake(const PromptParams& p, const Item& it, in
   r.l = half == 0 ? l : 0.0f;
 }
 
-// The wave's rows as the output, or as a partial of a tile of `tile_rows`.
+// The wave's rows as the output, or as a partial of a tile of `tile_rows`: 32 rows as
+// they lie in the registers, [HD / 8][64 lanes][4], 1024 bytes a store.
 template <int DT, int HD>
 __device__ __forceinline__ void end_rows(const PromptParams& p, const Item& it, int kvhead,
                                          int tile_rows, const Place& at, const Rows<HD>& r) {
@@ -581,12 +593,13 @@ __device__ __forceinline__ void end_rows(const PromptParams& p, const Item& it, 
   } else {
     const int64_t slot =
         ((int64_t)it.slot * p.kvh + kvhead) * tile_rows + (at.row - it.tile * tile_rows);
-    float* const o = p.part + slot * HD + 4 * half;
+    const int lane = threadIdx.x & 63;
+    f32x4_t* const o = reinterpret_cast<f32x4_t*>(p.part + (slot - (lane & 31)) * HD) + lane;
 #pragma unroll
     for (int ht = 0; ht < HD / 32; ++ht)
 #pragma unroll
       for (int x = 0; x < 4; ++x)
-        *reinterpret_cast<f32x4_t*>(o + 32 * ht + 8 * x) =
+        o[64 * (4 * ht + x)] =
             f32x4_t{r.o[ht][4 * x], r.o[ht][4 * x + 1], r.o[ht][4 * x + 2], r.o[ht][4 * x + 3]};
     if (half == 0) {
       p.stats[slot * 2] = r.m;
@@ -956,7 +969,63 @@ __global__ void __launch_bounds__(kThreads, 1) tm_prompt_few_kernel(PromptParams
 
 constexpr int kMaxChunks = 512;  // of one tile's keys
 
-// Joins the partials of one row, a wave each: the maximum and the sum over the chunks
+// The tile that a join's unit `at` stands for.
+__device__ __forceinline__ Join join_of(const PromptParams& p, int at) {
+  if (p.joins != nullptr) return p.joins[at];
+  Join j;
+  j.q0 = 0;
+  j.q_len = p.q_len;
+  j.tile = at;
+  j.slot0 = at * p.chunks;
+  j.count = p.chunks;
+  return j;
+}
+
+// Joins the partials of 32 rows' 32 columns, a wave each, in chunk order: lane l has row
+// l % 32 and the columns that the partials' layout gives it.  `blocks`: of 32 rows in a tile
+// that may hold some.
+template <int DT, int HD>
+__global__ void __launch_bounds__(kThreads) tm_prompt_join_tiles_kernel(PromptParams p,
+                                                                        int tile_rows,
+                                                                        int blocks) {
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  int unit = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6);
+  const int ht = unit % (HD / 32);
+  unit /= HD / 32;
+  const int first = unit % blocks * 32 + (lane & 31);
+  unit /= blocks;
+  const int kvhead = unit % p.kvh, at = unit / p.kvh;
+  if (p.joins == nullptr && at >= p.tiles) return;
+  const Join j = join_of(p, at);
+  const int row = j.tile * tile_rows + first;
+  if (row >= j.q_len * p.group) return;
+  const int64_t slot0 = ((int64_t)j.slot0 * p.kvh + kvhead) * tile_rows + first;
+  const int64_t step = (int64_t)p.kvh * tile_rows;  // from chunk to chunk
+  const float* const stats = p.stats + slot0 * 2;
+  const float* const from = p.part + (slot0 - (lane & 31)) * HD + 1024 * ht + 4 * lane;
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int c = 0; c < j.count; ++c) m = fmaxf(m, stats[c * step * 2]);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float sum = 0.0f;
+  f32x4_t o[4] = {};
+#pragma unroll 4
+  for (int c = 0; c < j.count; ++c) {
+    const float a = __builtin_amdgcn_exp2f(stats[c * step * 2] - ref);
+    sum += stats[c * step * 2 + 1] * a;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const f32x4_t v = *reinterpret_cast<const f32x4_t*>(from + c * step * HD + 256 * x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[x][e] = fmaf(v[e], a, o[x][e]);
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    store_row<DT>(p, j.q0, row, kvhead, HD, 32 * ht + 8 * x + 4 * half, o[x], sum);
+}
+
+// Joins the partials of one row of few, a wave each: the maximum and the sum over the chunks
 // first, a lane per chunk, then the weighted outputs in chunk order, four elements a
 // lane and the lanes' groups a chunk each.
 template <int DT, int HD>
@@ -968,17 +1037,8 @@ __global__ void __launch_bounds__(kThreads) tm_prompt_join_kernel(PromptParams p
   const int r = unit % rows;          // of the tile's `rows` that may hold some
   const int kv = unit / rows;
   const int kvhead = kv % p.kvh, at = kv / p.kvh;
-  Join j;
-  if (p.joins != nullptr) {
-    j = p.joins[at];
-  } else {
-    if (at >= p.tiles) return;
-    j.q0 = 0;
-    j.q_len = p.q_len;
-    j.tile = at;
-    j.slot0 = at * p.chunks;
-    j.count = p.chunks;
-  }
+  if (p.joins == nullptr && at >= p.tiles) return;
+  const Join j = join_of(p, at);
   const int row = j.tile * tile_rows + r;
   if (row >= j.q_len * p.group) return;
   const int64_t slot0 = ((int64_t)j.slot0 * p.kvh + kvhead) * tile_rows + r;
@@ -1077,10 +1137,19 @@ int plan_one(int64_t T, int64_t S, int64_t Hq, int64_t kvh, int64_t hd, OnePlan*
   if (T > 0)
     stages = tiles128 * ceil_div(tile_keys(T, S, 0, 128, group) +
                                      tile_keys(T, S, tiles128 - 1, 128, group), 2 * kKeys);
-  o->kind = kind_of(T * group, tiles128 * kvh, stages * kvh);
+  const int64_t units = tiles128 * kvh;
+  o->kind = kind_of(T * group, units, stages * kvh);
+  // Tiles that leave many CUs without one, in their only turn or in the last of two: a CU
+  // each to `short` workgroups over a third of the keys, where the keys are many enough to
+  // pay for the join.  Measured, 32 heads over 8 of 128, whole tiles and thirds in us: 517
+  // tokens of 2000 36, 37; of 4613 72, 62; of 10000 147, 115; 1100 of 9000 249, 201; but 700
+  // of 6000, whose thirds do not fit one turn, 91, 113.
+  const bool thirds = o->kind == kPair && units > kCUs / 2 &&
+                      3 * units <= 2 * kCUs * ceil_div(units, kCUs) && stages >= 48 * tiles128;
+  if (thirds) o->kind = kShort;
   o->rows = kTileRows[o->kind];
   o->tiles = ceil_div(T * group, o->rows);
-  o->chunks = chunks_of(o->kind, o->tiles * kvh, S);
+  o->chunks = thirds ? 3 : chunks_of(o->kind, o->tiles * kvh, S);
   const int64_t step = kStepKeys[o->kind];
   o->chunk_len = std::max(step, ceil_div(ceil_div(S, o->chunks), step) * step);
   o->chunks = std::max<int64_t>(1, ceil_div(S, o->chunk_len));
@@ -1100,10 +1169,19 @@ void launch_kind(const PromptParams& p, Kind kind, int64_t blocks, int64_t joins
     hipLaunchKernelGGL((tm_prompt_pair_kernel<DT, HD, PAGED>), grid, dim3(512), 0, st, p);
   else
     hipLaunchKernelGGL((tm_prompt_tall_kernel<DT, HD, PAGED>), grid, dim3(512), 0, st, p);
-  if (joins > 0)
+  if (joins == 0) return;
+  const int tile_rows = (int)kTileRows[kind];
+  if (kind == kFew) {
     hipLaunchKernelGGL((tm_prompt_join_kernel<DT, HD>),
                        dim3((unsigned)ceil_div(joins * p.kvh * join_rows, 4)), block, 0, st, p,
-                       (int)kTileRows[kind], (int)join_rows);
+                       tile_rows, (int)join_rows);
+  } else {
+    // (whole tiles, as packed sequences have them, make whole workgroups)
+    const int64_t blocks32 = ceil_div(join_rows, 32);
+    hipLaunchKernelGGL((tm_prompt_join_tiles_kernel<DT, HD>),
+                       dim3((unsigned)ceil_div(joins * p.kvh * blocks32 * (HD / 32), 4)), block,
+                       0, st, p, tile_rows, (int)blocks32);
+  }
 }
 
 template <bool PAGED>
