@@ -5,6 +5,11 @@ and op4 (greedy tree verify + paged KV commit).
 Module layout mirrors the reference package:
   treemoe_spec_amd.kernels.op1_tree_moe   tree_moe_forward, route_experts, Routing, ...
   treemoe_spec_amd.kernels.op4_commit     fused_verify_commit, VerifyResult
+  treemoe_spec_amd.kernels.tree_attention    tree_attention
+  treemoe_spec_amd.kernels.rms_norm          rms_norm, rms_norm_fp8
+  treemoe_spec_amd.kernels.rotary            RotaryPlan, rotary_embed, rotary_append
+  treemoe_spec_amd.kernels.prompt_attention  PromptPlan, prompt_attention, prompt_attention_cached
+  treemoe_spec_amd.kernels.sample_tokens     sample_tokens
   treemoe_spec_amd.kv_cache               PagedKVCache (page size configurable)
 The GPU work lives in libtreemoe_amd.so (C ABI: include/treemoe_amd.h).
 """
