@@ -88,7 +88,7 @@ struct PromptParams {
   int64_t stride_page;
   int kvh, group, q_len, k_len, tiles, chunks, chunk_len;  // one sequence's
   int page_shift, table_pages, cache_pages;
-  int wide;                    // the keys that a wave loads of a stage lie in one page
+  int wide;                    // the keys of each part that a wave loads lie in one page
   float scale_log2;
 };
 
@@ -154,9 +154,11 @@ template <int HD, bool PAGED, int NW>
 struct Feed {
   typedef Shape<HD> S;
   static constexpr int kLoads = S::kTile / (1024 * NW);  // loads of a wave per tile
-  // of K and V of a stage (a look-up behind them is not counted: a wait for what came
-  // before may then take a load too many, never one too few)
-  static constexpr int kGroup = 2 * kLoads;
+  static constexpr int kGroup = 2 * kLoads;  // of K and V of a stage
+  static constexpr int kWaveKeys = kLoads * S::kKeysPerLoad;  // of a stage, by one wave
+  // a wave's keys in parts of at most 16, each within a page of 16 or more
+  static constexpr int kParts = kWaveKeys > 16 ? kWaveKeys / 16 : 1;
+  static constexpr int kPartKeys = kWaveKeys / kParts;
   const uint16_t *k, *v;   // the next stage's first row (paged: the cache)
   int64_t k_step, v_step;  // from stage to stage
   int k_stride, v_stride;  // of a key, or of a page's slot
@@ -165,14 +167,14 @@ struct Feed {
   int first, left, step;   // the next stage's first key, the last key from there on, and
                            // the keys to the stage behind
   int v_first, v_left;     // of the stage whose K came last
-  int64_t off;             // its wave's first row in the cache
-  int page;                // the next stage's page of the wave, asked for a stage ahead
+  int64_t off[kParts];     // what its parts' rows in the cache lie past those of one page
+  int page[kParts];        // the next stage's pages of the wave, asked for a stage ahead
 
   // of the NW waves that load a stage together
   static __device__ __forceinline__ int wave() {
     return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) & (NW - 1);
   }
-  static __device__ __forceinline__ int wave_key() { return wave() * kLoads * S::kKeysPerLoad; }
+  static __device__ __forceinline__ int wave_key() { return wave() * kWaveKeys; }
   static __device__ __forceinline__ int key_in(int i) {  // within the stage
     return wave_key() + i * S::kKeysPerLoad + (int)(threadIdx.x & 63) / S::kChunks;
   }
@@ -186,7 +188,17 @@ struct Feed {
                                      (lds_void*)(tile + (wave() * kLoads + i) * 1024), 16, 0, 0);
   }
   __device__ __forceinline__ void look_up(const PromptParams& p) {
-    if constexpr (PAGED) page = p.table[(first + min(wave_key(), left)) >> p.page_shift];
+    if constexpr (PAGED) {
+      // by scalar loads, which the waits for K and V do not count: the table does not change
+      // during a launch
+      const auto table =
+          (const __attribute__((address_space(4))) int32_t*)reinterpret_cast<uintptr_t>(p.table);
+      page[0] = table[(first + min(wave_key(), left)) >> p.page_shift];
+      if (kParts > 1 && (1 << p.page_shift) < kWaveKeys)
+#pragma unroll
+        for (int j = 1; j < kParts; ++j)
+          page[j] = table[(first + min(wave_key() + j * kPartKeys, left)) >> p.page_shift];
+    }
   }
   // From key `begin` on of the item's sequence, `step` keys from stage to stage.
   __device__ __forceinline__ void start(const PromptParams& p, const Item& it, int kvhead,
@@ -201,7 +213,8 @@ struct Feed {
     first = begin;
     left = it.k_len - 1 - begin;
     v_first = v_left = 0;
-    off = 0;
+#pragma unroll
+    for (int j = 0; j < kParts; ++j) off[j] = page[j] = 0;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int key = key_in(i) - (PAGED ? wave_key() : 0);
@@ -237,12 +250,23 @@ struct Feed {
   }
   __device__ __forceinline__ void load_k(const PromptParams& p, uint8_t* tile) {
     if (whole(p, left)) {
-      if constexpr (PAGED)
-        off = (int64_t)min(max(__builtin_amdgcn_readfirstlane(page), 0), p.cache_pages - 1) *
-                  p.stride_page +
-              (int64_t)((first + wave_key()) & ((1 << p.page_shift) - 1)) * k_stride;
+      if constexpr (PAGED) {
+        auto off_of = [&](int j) TM_INLINE {
+          const int pg = min(max(__builtin_amdgcn_readfirstlane(page[j]), 0), p.cache_pages - 1);
+          const int slot = (first + wave_key() + j * kPartKeys) & ((1 << p.page_shift) - 1);
+          return (int64_t)pg * p.stride_page + (int64_t)(slot - j * kPartKeys) * k_stride;
+        };
+        off[0] = off_of(0);
+        const bool one = kParts == 1 || (1 << p.page_shift) >= kWaveKeys;  // one page
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) to_lds(k + off + (uint32_t)k_lane[i], tile, i);
+        for (int j = 1; j < kParts; ++j) off[j] = off[0];
+        if (!one)
+#pragma unroll
+          for (int j = 1; j < kParts; ++j) off[j] = off_of(j);
+      }
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        to_lds(k + off[i * kParts / kLoads] + (uint32_t)k_lane[i], tile, i);
     } else {
       load_rows<false>(p, first, left, tile);
     }
@@ -256,7 +280,8 @@ struct Feed {
   __device__ __forceinline__ void load_v(const PromptParams& p, uint8_t* tile) {
     if (whole(p, v_left)) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) to_lds(v + off + (uint32_t)v_lane[i], tile, i);
+      for (int i = 0; i < kLoads; ++i)
+        to_lds(v + off[i * kParts / kLoads] + (uint32_t)v_lane[i], tile, i);
     } else {
       load_rows<true>(p, v_first, v_left, tile);
     }
@@ -1102,8 +1127,8 @@ constexpr int64_t kTileRows[kKinds] = {32, 128, 128, 256};
 // Keys that a workgroup takes in one step, and workgroups that the chip holds.
 constexpr int64_t kStepKeys[kKinds] = {4 * kKeys, kKeys, 2 * kKeys, kKeys};
 constexpr int64_t kSlots[kKinds] = {kCUs, 2 * kCUs, kCUs, kCUs};
-// Keys of a stage that one wave loads.
-constexpr int64_t kWaveKeys[kKinds] = {kKeys, kKeys / 4, kKeys / 4, kKeys / 8};
+// Keys of a stage that a wave takes from one page (of few, one of four parts).
+constexpr int64_t kPartKeys[kKinds] = {kKeys / 4, kKeys / 4, kKeys / 4, kKeys / 8};
 
 Kind kind_of(int64_t longest, int64_t units128, int64_t stages128) {
   if (longest <= 32) return kFew;
@@ -1414,7 +1439,7 @@ extern "C" int tm_prompt_attention_cached(const void* q, int64_t q_stride, int64
   p.page_shift = shift;
   p.table_pages = (int)num_table_pages;
   p.cache_pages = (int)cache_pages;
-  p.wide = page_size >= kWaveKeys[o.kind] ? 1 : 0;
+  p.wide = page_size >= kPartKeys[o.kind] ? 1 : 0;
   p.scale_log2 = scale * 1.4426950408889634f;
   launch<true>(p, dtype, hd, o.kind, o.tiles * o.chunks * kvh, o.chunks > 1 ? o.tiles : 0,
                std::min(o.rows, T * p.group), (hipStream_t)stream);
