@@ -24,7 +24,8 @@ from treemoe_spec_amd.kv_cache import device_tables_of
 class PromptPlan:
     """The work list of ``prompt_attention`` for one batch, made once and used by
     every layer.  ``q_lens``: each sequence's queries; ``k_lens`` (default: the same):
-    its keys, of which the queries are the last."""
+    its keys, of which the queries are the last.  A graph that captured a call reads the
+    plan's lists on every replay: keep the plan as long as the graph."""
 
     def __init__(self, q_lens, k_lens=None, *, num_heads: int, num_kv_heads: int,
                  device="cuda"):

@@ -80,7 +80,8 @@ class RotaryPlan:
     head_dim and rotary_dim (default: the whole head) are multiples of 16.
     ``interleaved``: pairs are elements (2i, 2i+1), else (i, i + rotary_dim / 2).
     ``inv_freq``: radians a position of the rotary_dim / 2 pairs in place of
-    theta's and the scaling's."""
+    theta's and the scaling's.  Keep the plan as long as a graph that captured a call
+    with it."""
 
     def __init__(self, head_dim: int, theta: float = 1e6, *, rotary_dim: int | None = None,
                  interleaved: bool = False, scaling: dict | None = None, inv_freq=None,
