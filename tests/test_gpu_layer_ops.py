@@ -331,3 +331,26 @@ def test_two_streams_and_two_threads():
         t.join()
     torch.cuda.synchronize()
     assert not errors and all(_same(g, want[n]) for n, g in results)
+
+
+def test_a_cache_of_the_reference_layout():
+    """rotary_append and prompt_attention_cached on a cache without device tables: the
+    same bits as on this package's."""
+    from tests.ref_layout_cache import RefLayoutKVCache
+    from treemoe_spec_amd.kernels.prompt_attention import prompt_attention_cached
+    from treemoe_spec_amd.kernels.rotary import RotaryPlan, rotary_append
+
+    _say("cache of the reference layout")
+    plan = RotaryPlan(128, 1e6)
+    ours, ref = t_rot._cache(2, 128, BF, 64, 20), RefLayoutKVCache(2, 2, 128, 20)
+    start = 0
+    for t in (100, 30, 1):
+        q, k, v = (x.cuda() for x in t_rot._qkv(t, 8, 2, 128, BF, t))
+        outs = []
+        for kv in (ours, ref):
+            for layer in (0, 1):
+                qr = rotary_append(q, k, v, plan, kv, layer, start)
+                outs.append(prompt_attention_cached(qr, kv, layer))
+        start += t
+        assert ref.seq_len == ours.seq_len == start
+        assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3])
