@@ -198,3 +198,22 @@ def test_frequencies():
     p = torch.softmax(row.double(), 0)
     share = torch.bincount(got.cpu(), minlength=5) / n
     assert bool(((share - p).abs() <= 5 * (p * (1 - p) / n).sqrt()).all())
+
+
+@pytest.mark.parametrize("v", [32000, 100001])
+@pytest.mark.parametrize("kw", [{"top_k": 2000}, {"top_k": 30000, "top_p": 0.7}, {"top_p": 0.5},
+                                {"top_p": 0.97, "min_p": 0.3}])
+def test_flat_rows(v, kw):
+    """Cuts through thousands of equal or nearly equal logits, more than a list holds,
+    and through rows that a list of the cut's step serves."""
+    from treemoe_spec_amd.kernels.sample_tokens import sample_tokens
+
+    _say(f"sample flat v={v} {kw}")
+    g = torch.Generator().manual_seed(v)
+    rows = [torch.zeros(v), torch.randint(0, 3, (v,), generator=g).float(),
+            torch.randn(v, generator=g) * 0.01, torch.randn(v, generator=g),
+            torch.randn(v, generator=g) * 2]
+    logits, u = torch.stack(rows), torch.rand(len(rows), generator=g)
+    got, probs = sample_tokens(logits.cuda(), u.cuda(), return_probs=True, **kw)
+    torch.cuda.synchronize()
+    _check(logits, u, got, probs, **kw)
