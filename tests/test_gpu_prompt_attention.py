@@ -117,6 +117,8 @@ def test_large_tiles(dtype):
     ([60] * 100, [60] * 100, 8, 2, 1),
     ([700, 3], [1300, 900], 8, 2, 2),
     ([3500, 4000, 1], [3500, 4100, 4000], 32, 8, 3),
+    ([60] * 100 + [1], [60] * 100 + [50000], 8, 2, 1),   # short and tall tiles with joins
+    ([4000, 1], [4000, 100000], 32, 8, 3),
 ])
 @pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 128), (torch.float16, 64)])
 def test_every_tiling(q_lens, k_lens, hq, kvh, tiling, dtype, hd):

@@ -60,7 +60,8 @@ def _check_plan(q_lens, k_lens, hq, kvh):
     ([1], [1], 8, 2, 0), ([8], [5000], 8, 2, 0), ([9], [9], 8, 2, 1), ([1], [100000], 33, 1, 2),
     ([8192], [8192], 32, 8, 3), ([600], [5000], 32, 8, 2), ([100] * 50, [100] * 50, 32, 8, 1),
     ([0, 0, 5], [0, 4, 5], 4, 4, 0), ([1] * 300, [4000] * 300, 32, 8, 0),
-    ([1], [1 << 24], 1, 1, 0),
+    ([1], [1 << 24], 1, 1, 0), ([60] * 100 + [1], [60] * 100 + [50000], 8, 2, 1),
+    ([4000, 1], [4000, 100000], 32, 8, 3),
 ])
 def test_plans(q_lens, k_lens, hq, kvh, tiling):
     assert _check_plan(q_lens, k_lens, hq, kvh).tiling == tiling
