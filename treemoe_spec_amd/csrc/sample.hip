@@ -54,6 +54,7 @@ constexpr int kList = 1024;                     // logits of a wave that the lis
 constexpr int kRank = 256;
 constexpr int kRankStep = 8;                    // so many at a time
 constexpr float kSpan = 31.25f;                 // (l_max - l) / temperature of the last bin's end
+constexpr float kMaxF32 = 3.402823466e38f;      // the largest finite float
 constexpr double kUnit = 17592186044416.0;      // 2^44
 constexpr double kTwo52 = 4503599627370496.0;   // where doubles are integers
 
@@ -526,7 +527,7 @@ __device__ __forceinline__ float max_block(Shared& s, float v) {
 // covers the roundings here and in step_of, a few 2^-24 of them.  Above -infinity.
 __device__ __forceinline__ float below(const Row& row, float depth) {
   const float d = depth / row.inv_t;
-  return fmaxf(row.top - d - 1.9e-6f * (d + fabsf(row.top)), -3.402823466e38f);
+  return fmaxf(row.top - d - 1.9e-6f * (d + fabsf(row.top)), -kMaxF32);
 }
 
 // A value that at least `k` (<= 1024) of the threads' `most` reach, the lowest one where
@@ -536,7 +537,7 @@ __device__ __forceinline__ float reached_by(Shared& s, const Row& row, float mos
   const int step = step_of(row, most);
   if (step >= 0) atomicAdd(&s.count[step], 1u);
   find_bin<false>(s, (uint64_t)k, 1.0);
-  if (s.found < 0) return -3.402823466e38f;
+  if (s.found < 0) return -kMaxF32;
   return below(row, (float)(s.found + 1) * (kSpan / (float)kBins));
 }
 
@@ -553,7 +554,10 @@ __global__ void __launch_bounds__(kThreads) tm_sample_kernel(SampleParams p) {
   lg.aligned = p.aligned != 0;
   const double power = kPowers[t & 31];
   lg.hold();
-  double temp = p.temperatures ? (double)p.temperatures[n] : p.temperature;
+  // (a row's infinite one as the largest; NaN stays, which takes the largest logit)
+  const float row_temp = p.temperatures ? p.temperatures[n] : 0.0f;
+  double temp = p.temperatures ? (double)(row_temp > kMaxF32 ? kMaxF32 : row_temp)
+                               : p.temperature;
   const float u = p.uniforms[n];
   const int top_k = p.top_ks ? p.top_ks[n] : p.top_k;
   const double top_p = p.top_ps ? (double)p.top_ps[n] : p.top_p;
@@ -587,7 +591,9 @@ __global__ void __launch_bounds__(kThreads) tm_sample_kernel(SampleParams p) {
       for (int i = t; i < p.vocab; i += kThreads) probs[i] = i == token ? 1.0f : 0.0f;
     return;
   }
-  temp = fmax(temp, 1e-300);  // its inverse finite
+  // its inverse finite, and 32.5 of it: from 1e300 on all finite logits weigh the same, while
+  // an infinite `deepest` would make NaN of the weight of -inf
+  temp = fmin(fmax(temp, 1e-300), 1e300);
   row.inv_t = (float)(1.0 / temp);
   if (row.top == INFINITY) {
     lg.make_infinite();
