@@ -40,3 +40,23 @@ def test_infinite_and_largest(v, dtype, kw):
                                    **kw)
         torch.cuda.synchronize()
         t_samp._check(logits, u, got, probs, temperature=temp, **kw)
+
+
+@pytest.mark.parametrize("v", [3000, 40000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kw", [{}, {"top_k": 50}, {"top_k": 2000}, {"top_p": 0.9},
+                                {"min_p": 0.05}])
+def test_logits_further_apart_than_the_largest_float(v, dtype, kw):
+    """Logits whose difference passes the type's range, at temperatures that leave them
+    a weight."""
+    from treemoe_spec_amd.kernels.sample_tokens import sample_tokens
+
+    _say(f"sample far logits v={v} {dtype} {kw}")
+    g = torch.Generator().manual_seed(v)
+    logits = ((torch.rand(4, v, generator=g) * 2 - 1) * 3.2e38).to(dtype)
+    u = torch.rand(4, generator=g)
+    temps = torch.tensor([F32_MAX, 1e38, 3e37, 1e38])
+    got, probs = sample_tokens(logits.cuda(), u.cuda(), temperature=temps.cuda(),
+                               return_probs=True, **kw)
+    torch.cuda.synchronize()
+    t_samp._check(logits, u, got, probs, temperature=temps, **kw)

@@ -86,6 +86,7 @@ struct SampleParams {
 
 struct Row {
   float top;       // largest logit
+  float half_top;  // half of it
   float inv_t;     // 1 / temperature
   double inv_y;    // 32 log2(e) / temperature
   double deepest;  // l_max - l at which the weight is 0 for long
@@ -108,10 +109,11 @@ __device__ __forceinline__ float logit_of(uint64_t key) {
 __device__ __forceinline__ int index_of(uint64_t key) { return (int)~(uint32_t)key; }
 
 // The step of a logit, from (l_max - l) / temperature in fp32, monotone in l; -1 for
-// one too far below to weigh anything.
+// one too far below to weigh anything.  By half of that: finite logits can lie further
+// apart than the largest float, and have a weight at temperatures near it.
 __device__ __forceinline__ int step_of(const Row& r, float l) {
-  const float d = l == r.top ? 0.0f : (r.top - l) * r.inv_t;
-  return d < kSpan ? min(kBins - 1, (int)(d * ((float)kBins / kSpan))) : -1;
+  const float half = l == r.top ? 0.0f : fmaf(l, -0.5f, r.half_top) * r.inv_t;
+  return half < 0.5f * kSpan ? min(kBins - 1, (int)(half * (2.0f * (float)kBins / kSpan))) : -1;
 }
 
 // 2^44 times the weight of a logit, in 64 bits: with d = l_max - l and t = 32 d log2(e) /
@@ -600,6 +602,7 @@ __global__ void __launch_bounds__(kThreads) tm_sample_kernel(SampleParams p) {
     most = most == INFINITY ? 0.0f : -INFINITY;
     row.top = 0.0f;
   }
+  row.half_top = 0.5f * row.top;
   row.inv_y = 46.166241308446828384 / temp;
   row.deepest = 32.5 * temp;  // 2^44 e^-32.5 < 0.14
   row.powers = s.powers;
