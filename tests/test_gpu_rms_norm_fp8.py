@@ -48,3 +48,20 @@ def test_values_at_the_border_of_two_steps(t, h, group):
         torch.cuda.synchronize()
         assert torch.equal(sc.cpu().view(t, -1), scale)
         assert torch.equal(q.float().cpu(), want)
+
+
+@pytest.mark.parametrize("group", [32, None])
+def test_magnitudes_whose_scale_underflows(group):
+    """A largest magnitude that leaves 0 when divided by 448 has scale 1, like 0."""
+    from treemoe_spec_amd.kernels.rms_norm import rms_norm_fp8
+
+    _say(f"rms_norm_fp8 underflow group={group}")
+    x = _signs(3, 256, 2)
+    for top in (1.4e-45, 1e-43, 2.8e-43, 7e-43, 1e-40):
+        w = torch.zeros(256)
+        w[::7] = top
+        want, scale = _want(x * w, group or 256)
+        q, sc = rms_norm_fp8(x.cuda(), w.cuda(), 0.0, scale_group=group)
+        torch.cuda.synchronize()
+        assert torch.equal(sc.cpu().view(3, -1), scale)
+        assert torch.equal(q.float().cpu(), want), top

@@ -5,7 +5,7 @@
 //
 // s, the sum of squares and y in fp32, each output rounded once.  The 8-bit
 // form scales y by the largest magnitude of a row or of a group of columns:
-// scale = amax / 448 (1 where amax is 0), q = e4m3(y / scale), 448 being
+// scale = amax / 448 (1 where that is 0), q = e4m3(y / scale), 448 being
 // e4m3's largest value.
 //
 // Bound by HBM: every input is read once and every output written once, a
@@ -87,6 +87,12 @@ __device__ __forceinline__ uint32_t top_of_group(uint32_t v, int group) {
   if (group >= 256) v = max(v, (uint32_t)__shfl_xor((int)v, 16));
   if (group >= 512) v = max(v, (uint32_t)__shfl_xor((int)v, 32));
   return v;
+}
+
+// The scale of a largest magnitude, given as bits: over 448, or 1 where that leaves 0.
+__device__ __forceinline__ float scale_of(uint32_t top) {
+  const float scale = __uint_as_float(top) / 448.0f;
+  return scale == 0.0f ? 1.0f : scale;
 }
 
 // v over `scale`, each quotient rounded to 32 bits as a division rounds it: a product with
@@ -182,8 +188,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) tm_rms_norm_kernel(Norm
       for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(s[c][e]) & 0x7fffffffu);
       if (p.group != 0) {
         // a group is group / 8 consecutive lanes of one chunk
-        const uint32_t g = top_of_group(top, p.group);
-        const float scale = g == 0u ? 1.0f : __uint_as_float(g) / 448.0f;
+        const float scale = scale_of(top_of_group(top, p.group));
         if (i < p.hidden) {
           if ((i & (p.group - 1)) == 0)
             p.scales[row * p.scale_stride + i / p.group] = scale;
@@ -204,7 +209,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) tm_rms_norm_kernel(Norm
 #pragma unroll
         for (int w = 0; w < W; ++w) top = max(top, s_max[w]);
       }
-      scale = top == 0u ? 1.0f : __uint_as_float(top) / 448.0f;
+      scale = scale_of(top);
       if (t == 0) p.scales[row * p.scale_stride] = scale;
     }
     uint8_t* const orow = reinterpret_cast<uint8_t*>(p.out) + row * p.out_stride;
