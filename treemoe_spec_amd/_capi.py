@@ -153,10 +153,11 @@ def dtype_code(dtype) -> int | None:
 
 def require(what: str, device, **tensors) -> None:
     """All given tensors on ``device``, a ROCm device, and none that a gradient is
-    asked of: these operators have no backward pass.  (Callers look for the common
-    case themselves and come here for the error: host time is what bounds their
-    smallest calls.)"""
+    asked of or that carries a forward-mode tangent: these operators have no
+    derivatives.  (Callers look for the common case themselves and come here for the
+    error: host time is what bounds their smallest calls.)"""
     import torch
+    from torch.autograd import forward_ad
 
     if device.type != "cuda":
         raise RuntimeError(f"treemoe_spec_amd {what} runs on ROCm devices only; "
@@ -170,6 +171,9 @@ def require(what: str, device, **tensors) -> None:
         if grad and t.requires_grad:
             raise RuntimeError(f"{what} has no backward pass, but {name} requires a gradient; "
                                "call it under torch.no_grad()")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no forward derivative, but {name} carries a tangent; "
+                               "call it on the primal")
 
 
 def check(rc: int, what: str) -> None:

@@ -15,6 +15,7 @@ import ctypes
 import operator
 
 import torch
+from torch.autograd import forward_ad
 
 from treemoe_spec_amd import _capi
 from treemoe_spec_amd._capi import dtype_code, ptr
@@ -101,7 +102,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pr
     index = q.get_device()
     if index < 0 or k.get_device() != index or v.get_device() != index \
             or plan.items.get_device() != index or out is not None or q.requires_grad \
-            or k.requires_grad or v.requires_grad:
+            or k.requires_grad or v.requires_grad or forward_ad._current_level >= 0:
         _capi.require("prompt_attention", q.device, q=q, k=k, v=v, plan=plan.items, out=out)
     for name, x in (("k", k), ("v", v)):
         if x.dim() != 3 or x.shape[2] != hd or x.dtype != q.dtype or x.shape != k.shape:
@@ -155,7 +156,8 @@ def prompt_attention_cached(q: torch.Tensor, kv, layer: int, *, scale: float | N
     kc, vc = kv.k, kv.v
     index = q.get_device()
     if index < 0 or kc.get_device() != index or vc.get_device() != index or out is not None \
-            or q.requires_grad or kc.requires_grad or vc.requires_grad:
+            or q.requires_grad or kc.requires_grad or vc.requires_grad \
+            or forward_ad._current_level >= 0:
         _capi.require("prompt_attention_cached", q.device, q=q, k_cache=kc, v_cache=vc, out=out)
     cshape, cst = kc.shape, kc.stride()
     if kc.dtype != q.dtype or vc.dtype != q.dtype or vc.shape != cshape or vc.stride() != cst \

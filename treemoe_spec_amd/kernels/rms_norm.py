@@ -10,6 +10,7 @@ an 8-bit product.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from treemoe_spec_amd import _capi
 from treemoe_spec_amd._capi import dtype_code
@@ -39,7 +40,7 @@ def _checked(what, x, weight, eps, residual, residual_out):
     if index < 0 or weight.get_device() != index or residual_out is not None \
             or (residual is not None and (residual.get_device() != index
                                           or residual.requires_grad)) \
-            or x.requires_grad or weight.requires_grad:
+            or x.requires_grad or weight.requires_grad or forward_ad._current_level >= 0:
         _capi.require(what, x.device, x=x, weight=weight, residual=residual,
                       residual_out=residual_out)
     xs, step = x.stride()

@@ -16,6 +16,7 @@ import operator
 from fractions import Fraction
 
 import torch
+from torch.autograd import forward_ad
 
 from treemoe_spec_amd import _capi
 from treemoe_spec_amd._capi import dtype_code
@@ -151,7 +152,8 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     turns = plan.turns
     if index < 0 or positions.get_device() != index or turns.get_device() != index \
             or q.requires_grad or (k is not None and (k.get_device() != index
-                                                      or k.requires_grad)):
+                                                      or k.requires_grad)) \
+            or forward_ad._current_level >= 0:
         _capi.require("rotary_embed", q.device, q=q, k=k, positions=positions, plan=turns)
     t = q.shape[0]
     if t > _capi.TM_MAX_ROWS:
@@ -191,7 +193,8 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Rotar
     if index < 0 or k.get_device() != index or v.get_device() != index \
             or turns.get_device() != index or kc.get_device() != index \
             or vc.get_device() != index or q.requires_grad or k.requires_grad \
-            or v.requires_grad or kc.requires_grad or vc.requires_grad:
+            or v.requires_grad or kc.requires_grad or vc.requires_grad \
+            or forward_ad._current_level >= 0:
         _capi.require("rotary_append", q.device, q=q, k=k, v=v, plan=turns, k_cache=kc,
                       v_cache=vc)
     t = q.shape[0]

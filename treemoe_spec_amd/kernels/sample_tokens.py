@@ -14,6 +14,7 @@ import operator
 import sys
 
 import torch
+from torch.autograd import forward_ad
 
 from treemoe_spec_amd import _capi
 from treemoe_spec_amd._capi import dtype_code, ptr
@@ -76,6 +77,7 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, *,
     index = logits.get_device()
     if index < 0 or uniforms.get_device() != index or logits.requires_grad \
             or uniforms.requires_grad or probs_out is not None \
+            or forward_ad._current_level >= 0 \
             or not (temps is ks is ps is ms is None):
         _capi.require("sample_tokens", logits.device, logits=logits, uniforms=uniforms,
                       temperature=temps, top_k=ks, top_p=ps, min_p=ms, probs_out=probs_out)
