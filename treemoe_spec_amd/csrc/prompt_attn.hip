@@ -87,7 +87,7 @@ struct PromptParams {
   int64_t q_stride, k_stride, v_stride, out_stride;  // paged: k_stride is the slot's
   int64_t stride_page;
   int kvh, group, q_len, k_len, tiles, chunks, chunk_len;  // one sequence's
-  int page_shift, table_pages, cache_pages;
+  int page_shift, cache_pages;
   int wide;                    // the keys of each part that a wave loads lie in one page
   float scale_log2;
 };
@@ -1437,7 +1437,6 @@ extern "C" int tm_prompt_attention_cached(const void* q, int64_t q_stride, int64
   int shift = 0;
   while ((int64_t(1) << shift) < page_size) ++shift;
   p.page_shift = shift;
-  p.table_pages = (int)num_table_pages;
   p.cache_pages = (int)cache_pages;
   p.wide = page_size >= kPartKeys[o.kind] ? 1 : 0;
   p.scale_log2 = scale * 1.4426950408889634f;

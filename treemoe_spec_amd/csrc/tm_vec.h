@@ -4,15 +4,6 @@
 #include "tm_common.h"
 
 template <int DT>
-struct Elem {  // TM_DTYPE_BF16 or TM_DTYPE_F16
-  typedef uint16_t type;
-};
-template <>
-struct Elem<TM_DTYPE_F32> {
-  typedef float type;
-};
-
-template <int DT>
 __device__ __forceinline__ float tm_load1(const void* p, int64_t i) {
   if constexpr (DT == TM_DTYPE_F32)
     return reinterpret_cast<const float*>(p)[i];
