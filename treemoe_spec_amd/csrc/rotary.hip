@@ -9,11 +9,13 @@
 //
 // The angle.  f_i comes as a 64-bit fixed-point fraction of a turn, F = f 2^64.  The
 // integer product position * F wraps at whole turns, so its 64 bits are the angle
-// mod 1 turn, off by position 2^-65 turns at most: no table of cosines is read
-// and none limits the position.  The top two bits after rounding to the nearest
-// quarter turn pick the quadrant, the rest is a remainder of at most 1/8 turn whose
-// sine and cosine come from their Taylor polynomials in fp32 (degree 9 and 10 on
-// |x| <= pi / 4: truncation below 2e-9).
+// mod 1 turn, off by |position| 2^-65 turns for F's rounding and |position| f 2^-52 for that
+// of the frequency, a double (2^-49 where `part` is no power of two: 2 i / part is rounded
+// too): no table of cosines is read and none limits the position.  The top two bits after
+// rounding to the nearest quarter turn pick the quadrant, the rest is a remainder of at most
+// 1/8 turn, cut to 2^-34 turn (all in all under 2^-33 up to position 2^20, 2^-24 at 2^30; for
+// other parts to 2^17, and 2^-21), whose sine and cosine come from their Taylor polynomials in
+// fp32 (degree 9 and 10 on |x| <= pi / 4: truncation below 2e-9).
 //
 // Bound by HBM at many tokens, by the launch at few.  A thread owns 8 pairs, two
 // 16-byte pieces, of the same place in several heads of one token, so its 8 sines
@@ -186,8 +188,8 @@ int launch(const RotaryParams& p, int dtype, bool inter, hipStream_t st) {
 
 // Head slots of a token: one head a thread at few tokens, 16 slots (two or three heads
 // each of a token's 40 rows) from 1024 tokens on, where the angles are then a smaller part.
-// Measured (bf16, 32 + 8 heads of 128), one head, 16 slots and 8 slots in us: 64 tokens
-// 3.0, 3.8, 4.7; 512 tokens 4.3, 4.5, 5.4; 1024 5.8, 5.5, 5.9; 2048 9.5, 8.5, 9.3; 5003
+// Measured on one head shape (bf16, 32 + 8 heads of 128), one head, 16 slots and 8 slots in
+// us: 64 tokens 3.0, 3.8, 4.7; 512 tokens 4.3, 4.5, 5.4; 1024 5.8, 5.5, 5.9; 2048 9.5, 8.5, 9.3; 5003
 // 18.9, 17.8, 17.8.
 int head_slots(int64_t tokens, int heads) {
   return tokens < 1024 ? heads : (heads < 16 ? heads : 16);
