@@ -96,8 +96,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pr
     heads contiguous): ``plan``'s sequences one after the other.  A query attends to
     its sequence's keys up to its own position.  Returns [T, Hq * hd]; T and S may
     exceed the plan's rows (a padded batch): in a new result the rows behind the last
-    sequence are 0, in ``out`` they stay as they were.  ``out`` shares no memory with
-    q, k and v."""
+    sequence are 0 (a fill by torch), in ``out`` they stay as they were.  ``out``
+    shares no memory with q, k and v."""
     dt, t, hq, hd, qs, ost = _check_q(q, out)
     index = q.get_device()
     if index < 0 or k.get_device() != index or v.get_device() != index \
@@ -150,8 +150,8 @@ def prompt_attention_cached(q: torch.Tensor, kv, layer: int, *, scale: float | N
     the cache holds already (``rotary_append``, ``append``).  Query t attends to
     positions 0 .. seq_len - T + t of ``layer``, read in place through the block table.
     The cache is [L, pages, page, kv_heads, head_dim] of q's dtype, page size a power of
-    two.  Returns [T, Hq * hd].  A captured call repeats the length and pages that it was
-    captured with."""
+    two.  Returns [T, Hq * hd].  A replay of a captured call repeats the length of the
+    capture, in the pages that the cache's device table then holds."""
     dt, t, hq, hd, qs, ost = _check_q(q, out)
     kc, vc = kv.k, kv.v
     index = q.get_device()

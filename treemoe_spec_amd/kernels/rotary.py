@@ -182,8 +182,10 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Rotar
     """Tokens at positions start_pos .. start_pos + T - 1: returns q [T, Hq, hd]
     rotated, and stores the rotated k and v [T, kvh, hd] at those positions of the
     paged cache ``kv``, mapping pages as ``append`` does (treemoe/model/kv_cache.py:
-    62-78); ``kv.seq_len`` grows to cover them.  A captured call repeats the positions
-    and pages that it was captured with."""
+    62-78); ``kv.seq_len`` grows to cover them.  A call that maps a page copies the block
+    table to the device and waits for it, so a capture needs its pages mapped by an
+    eager call before; a replay repeats the positions of the capture, in the pages that
+    the device table then holds."""
     dtype, hd = q.dtype, plan.head_dim
     dt = dtype_code(dtype)
     if dt is None:
