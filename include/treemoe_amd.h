@@ -434,8 +434,9 @@ int tm_tree_mask_pack(const uint8_t* mask, int64_t N, int64_t row_stride,
 /*
  * Root-mean-square norm of T rows of H elements, with the residual's addition:
  *   s = x (+ residual),  out = s / sqrt(mean(s^2) + eps) * weight,  res_out = s,
- * computed in fp32 and rounded once per output.  Replaces `rms_norm` and the
- * residual additions around it in the reference's decoder layer
+ * computed in fp32 and rounded once per output; the sum of the squares has to fit
+ * fp32 (a root mean square above 1.8e19 / sqrt(H) gives zeros).  Replaces `rms_norm`
+ * and the residual additions around it in the reference's decoder layer
  * (treemoe/model/mixtral.py:268-340).  x, out: dtype.  residual may be NULL; it
  * and res_out (which may be the same memory) have res_dtype, weight has
  * weight_dtype, each `dtype` or fp32.  Strides in elements, rows contiguous,
@@ -516,7 +517,8 @@ int tm_rotary_append(const void* q, int64_t q_stride, const void* k, int64_t k_s
  * -infinity gives token -1 and zero probabilities.  Weights below 2^-45 are 0.
  *
  * temperatures, top_ks, top_ps, min_ps: one value a row, or NULL for the scalar
- * beside it.  A row value out of its range acts as the nearest one in it.
+ * beside it.  A row value out of its range acts as the nearest one in it; NaN as a
+ * temperature of 0, and as no top-p or min-p.
  * V <= TM_MAX_SAMPLE_VOCAB, N <= TM_MAX_ROWS.  probs lies apart from the logits.
  */
 int tm_sample_tokens(const void* logits, int dtype, int64_t N, int64_t V,

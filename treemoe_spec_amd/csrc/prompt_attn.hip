@@ -19,11 +19,13 @@
 //   tall   256 rows; eight waves
 // In pair and tall one wave of a SIMD is in the matrix products while the other weighs.
 //
-// Bound by the matrix pipe, the exponentials and the power limit at many rows: 8192 tokens,
-// 32 heads over 8 of 128 in bf16, 549 GFLOP in 525 us, 1.05 PFLOP/s, where a plain 16384^3
-// product reaches 1.39; 4.0 k tokens 0.87 PFLOP/s.  By HBM at few rows: one token over 40000
-// keys 32 us, 5.2 TB/s; over 7777 14.3 us, of which 2.5 are the second launch and about 6
-// the latency of one stage.
+// Bound by the power limit and the turns of products and exponentials at many rows: 8192
+// tokens, 32 heads over 8 of 128 in bf16, 549 GFLOP in 525 us, 1.05 PFLOP/s, where a plain
+// 16384^3 product reaches 1.39; the matrix pipe is busy in 48 % of the cycles, of a clock that
+// power holds at 1.78 GHz.  4.0 k tokens 0.87 PFLOP/s.  Through pages of 16, in a graph: 8192
+// tokens 579 us, packed 545; 4000 162, 147.  By HBM at few rows: one token over 40000 keys
+// 32 us, 5.2 TB/s; over 7777 14.3 us, of which 2.5 are the second launch and about 6 the
+// latency of one stage.
 //
 // Per wave and stage (v_mfma_f32_32x32x16):
 //   S^T = K Q^T   lane l holds S^T[key 32 kt + 8 (v / 4) + 4 (l / 32) + v % 4][query l % 32]
@@ -34,9 +36,11 @@
 //                 in k-step (kt, m) stands for key 32 kt + 16 m + 8 (j / 4) + 4 h + j % 4,
 //                 and V^T is read with the same map, four keys of a column by each
 //                 transposing LDS read.
-// The weights are rounded to the inputs' 16-bit type for the product; the sums are
-// taken over the rounded weights in fp32, so that the roundings weigh alike above and
-// below the division.
+// The weights are rounded to the inputs' 16-bit type, which the product takes: a second
+// product with what the rounding left would cost half as many products again.  The sums are
+// taken over the rounded weights in fp32, so that the roundings weigh alike above and below the
+// division.  The whole output is off by 0.0021 of its norm in bf16 over 8192 tokens, where
+// its own rounding alone is 0.0016 (fp16, packed prompts: 0.00024, 0.00020).
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -1116,7 +1120,8 @@ int64_t tile_keys(int64_t q_len, int64_t k_len, int64_t tile, int64_t rows, int6
 //   tall   3.5 tiles a CU or more, of 24 stages or more;
 //   pair   fewer tiles, of 8 stages or more;
 //   short  otherwise.
-// Measured, 32 query heads over 8 of 128 elements, the three tilings in us: one prompt of
+// Measured on one head shape, 32 query heads over 8 of 128 elements (heads of 64, whose stages
+// are half the work, take the same thresholds), the three tilings in us: one prompt of
 // 517 tokens short 21, pair 21; 1000 tokens 35, 25, tall 38; 2048 59, 52, 63; 4000 164, 160,
 // 150; 8192 pair 554, tall 520; 12 prompts of 1-2048 tokens (fp16) short 77, pair 102, tall
 // 85; 20 of 100 short 18, pair 27, tall 22; 300 tokens over 1000 cached short 32, pair

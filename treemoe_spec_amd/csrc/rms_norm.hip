@@ -16,7 +16,9 @@
 //
 // Measured in bf16 with a residual of the same type: 6011 rows of 4096, 40 us from a cold
 // cache, 4.9 TB/s of the 4.9 TB/s that a 2 GiB copy reaches; 8 bits with scales of 128,
-// 2048 rows, 13.5 us, 4.4 TB/s; one row 2.7 us of kernel, which is its launch.
+// 2048 rows, 14.4 us, 4.1 TB/s; one row 2.7 us of kernel, which is its launch.  Rows that
+// do not start on 16 bytes, or whose width is no multiple of 8, take eight narrow loads for
+// a wide one: 2048 rows of 4096 in a graph 37.8 us in place of 11.5, of 4100 44.3.
 #include "tm_vec.h"
 
 namespace {

@@ -28,12 +28,15 @@
 // list in LDS, in index order, and the rest runs on the list: up to 256 elements are
 // ranked by counting, more are cut by histograms.  top-p without top-k needs the weight
 // of the whole row, one pass of 64-bit exponentials; where the list turns out to hold
-// too little of it, or overflows, the row itself is cut by histograms.
+// too little of it, or overflows, the row itself is cut by histograms.  The form with a row
+// in registers spills 16 of 128 a thread (52 bytes) beside its 32 logits.
 //
 // Bound by latency at few rows and by passes over a row on one CU: 1 row of 32000, top-k 50
 // and top-p, 10.7 us; 64 rows with top-p, min-p and their distributions 21.7; 256 rows of
 // 131072 with top-p 92 us, 29 of them the first reading (HBM, 4.7 TB/s), 18 the second, 14
-// the 64-bit exponentials.
+// the 64-bit exponentials.  Rows that do not start on four logits, as with a vocabulary that
+// is no multiple of 4, take a load a logit: 64 rows in a graph, top-k 50, of 32000 11.6 us,
+// of 32001 16.4; of 131072 26.4, of 131073 64.3.
 #include <cmath>
 #include <type_traits>
 

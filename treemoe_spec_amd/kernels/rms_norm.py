@@ -102,7 +102,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *,
     """The norm as ``float8_e4m3fn`` [T, H] and float32 scales: one for every row
     ([T], the default) or for every ``scale_group`` columns (32, 64, 128, 256 or
     512; [T, H / scale_group]).  A scale is the largest magnitude over 448 (1 where
-    that is 0), a value the norm over its scale, rounded to the nearest.  Returns
+    that is 0), a value the norm over its scale, rounded to the nearest e4m3.  Returns
     (values, scales), with a residual (values, scales, sum)."""
     if scale_group is not None and (scale_group not in _SCALE_GROUPS
                                     or x.shape[-1] % scale_group != 0):
