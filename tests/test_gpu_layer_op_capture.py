@@ -66,3 +66,35 @@ def test_replay_follows_the_table(make):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+def test_a_plan_dropped_behind_a_call_on_another_stream():
+    """The lists of a plan stay its own until the calls that read them have ended."""
+    from treemoe_spec_amd.kernels.prompt_attention import PromptPlan, prompt_attention
+    from treemoe_spec_amd.kernels.rotary import RotaryPlan, rotary_embed
+
+    _say("plans dropped early")
+    q, k, v = (x.cuda() for x in t_attn._qkv(70, 900, 8, 2, 128, BF, 3))
+    pos = torch.arange(70, device="cuda")
+
+    def plans():
+        return PromptPlan([70], [900], num_heads=8, num_kv_heads=2), RotaryPlan(128, 1e6)
+
+    plan, rope = plans()
+    want = prompt_attention(q, k, v, plan), rotary_embed(q, None, pos, rope)[0]
+    busy = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(60):
+            busy = busy @ busy * 1e-3     # the calls wait behind it
+        got = prompt_attention(q, k, v, plan), rotary_embed(q, None, pos, rope)[0]
+        ended = torch.cuda.Event()
+        ended.record()
+    held = {t.data_ptr() for t in (plan.items, plan.joins, rope.turns)}
+    del plan, rope
+    others = [plans() for _ in range(3)]
+    assert not ended.query()
+    assert not held & {t.data_ptr() for a, b in others for t in (a.items, a.joins, b.turns)}
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

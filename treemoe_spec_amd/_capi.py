@@ -142,6 +142,25 @@ def launch(name: str, index: int, *args) -> None:
         check(rc, name)
 
 
+def stream_made_on(device) -> int | None:
+    """torch's current raw stream of ``device``, None for one that has none."""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(device.index) if device.type == "cuda" else None
+
+
+def used_by(index: int, made_on: int | None, *tensors) -> None:
+    """A call on torch's current stream of device ``index`` reads ``tensors``, which a plan
+    allocated on the raw stream ``made_on``: where the streams differ their memory is not
+    given away, once the plan is gone, before that call has ended."""
+    import torch
+
+    if made_on is not None and torch._C._cuda_getCurrentRawStream(index) != made_on:
+        stream = torch.cuda.current_stream(index)
+        for t in tensors:
+            t.record_stream(stream)
+
+
 @functools.cache
 def dtype_code(dtype) -> int | None:
     """TM_DTYPE_* of a torch dtype, None for one that the kernels do not take."""

@@ -53,6 +53,7 @@ class PromptPlan:
         self.num_heads, self.num_kv_heads = num_heads, num_kv_heads
         self.items, self.joins = items.to(device), joins.to(device)
         self.device = self.items.device
+        self.made_on = _capi.stream_made_on(self.device)
 
 
 def _check_q(q: torch.Tensor, out: torch.Tensor | None):
@@ -128,6 +129,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Pr
                  v.stride(0) if s > 1 else kvh * hd, plan.items.data_ptr(), plan.num_items,
                  plan.joins.data_ptr(), plan.num_joins, plan.num_slots, plan.tiling, hq, kvh,
                  hd, scale, dt, out.data_ptr(), ost, ptr(ws), nbytes)
+    _capi.used_by(index, plan.made_on, plan.items, plan.joins)
     return out
 
 

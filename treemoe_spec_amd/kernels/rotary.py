@@ -110,6 +110,7 @@ class RotaryPlan:
             turns.append(u - 2 ** 64 if u >= 2 ** 63 else u)  # the same 64 bits, signed
         self.turns = torch.tensor(turns, dtype=torch.int64).to(device)
         self.device = self.turns.device
+        self.made_on = _capi.stream_made_on(self.device)
 
 
 def _heads_of(name: str, t: torch.Tensor, hd: int, dtype, tokens: int) -> tuple[int, int]:
@@ -174,6 +175,7 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     _capi.launch("tm_rotary", index, q.data_ptr(), qs, kp, ks, q_out.data_ptr(), qos, kop, kos,
                  positions.data_ptr(), 1 if wide else 0, turns.data_ptr(), plan.magnitude, t,
                  heads, kvh, hd, plan.rotary_dim, plan.interleaved, dt)
+    _capi.used_by(index, plan.made_on, turns)
     return q_out, k_out
 
 
@@ -230,5 +232,6 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Rotar
                  cshape[2], cshape[1], table.data_ptr(), len(kv.block_table), start_pos,
                  turns.data_ptr(), plan.magnitude, t, heads, kvh, hd, plan.rotary_dim,
                  plan.interleaved, dt)
+    _capi.used_by(index, plan.made_on, turns)
     kv.seq_len = max(kv.seq_len, end)
     return q_out
