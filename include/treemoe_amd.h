@@ -51,6 +51,7 @@ extern "C" {
 #define TM_MAX_NORM_HIDDEN 65536  /* columns of tm_rms_norm */
 #define TM_MAX_PROMPT_KEYS (1 << 24)  /* keys of one sequence of prompt attention */
 #define TM_MAX_SAMPLE_VOCAB 262144  /* columns of tm_sample_tokens */
+#define TM_MAX_BEAMS 64  /* beams of a group, and candidates of tm_beam_select */
 #define TM_MAX_ROWS (1 << 21)  /* rows or tokens of one norm, rotary or sampling call */
 
 /* ABI version (major*10000 + minor*100 + patch): 5.0.0.  Version 2 added
@@ -584,6 +585,101 @@ int tm_prompt_attention_cached(const void* q, int64_t q_stride, int64_t T,
                                float scale, int dtype, void* out, int64_t out_stride,
                                void* workspace, int64_t workspace_bytes,
                                void* stream);
+
+/*
+ * Lists of tm_branch_attention for branches that add different numbers of tokens,
+ * counts[b] >= 0 by branch b, made once per batch on the host and used by every layer.
+ * Writes num_units x 4 int32 to `units` and total x 4 to `tokens` (host memory, to be
+ * copied to the device), and sizes[0..2] = num_units, total, the largest count.  With
+ * both NULL it only writes sizes.
+ */
+int tm_branch_plan(const int64_t* counts, int64_t B, int64_t Hq, int64_t kvh,
+                   int32_t* units, int64_t max_units, int32_t* tokens,
+                   int64_t max_tokens, int64_t* sizes);
+
+/* Workspace bytes of tm_branch_attention for these sizes. */
+int tm_branch_workspace(int64_t T, int64_t units, int64_t max_count, int64_t seq_len,
+                        int64_t longest, int64_t Hq, int64_t kvh, int64_t hd,
+                        int64_t* bytes);
+
+/*
+ * Attention of T tokens of many branches of one sequence (requests behind a shared
+ * prompt, beams, drafted chains), one launch per part of the keys: the shared ones
+ * are taken once for all branches.  The reference continues one sequence at a time
+ * (treemoe/model/mixtral.py:208-250); for one branch this is its append, gather and
+ * causal `F.scaled_dot_product_attention`.
+ *
+ * q, out [T, Hq, hd] and k, v [T, kvh, hd], bf16 or fp16, hd 64 or 128, heads
+ * contiguous, token strides in elements, 16-byte aligned: branch after branch, with
+ * units and tokens NULL max_count tokens of each (T = rows * max_count, num_units =
+ * rows * ceil(max_count * Hq / kvh / tile), tile 32 where max_count * Hq / kvh <= 32,
+ * else 128), otherwise as tm_branch_plan laid them down (device memory).  Token i of branch
+ * b sees the seq_len positions of the pages (k_cache .. seq_len as in
+ * tm_prompt_attention_cached; seq_len may be 0) and the branch's own lengths[b] + i + 1
+ * keys: position t < lengths[b] is row origin[b * origin_stride + t] (row b with origin
+ * NULL), place t of the layer's branch cache k_rows, v_rows [rows, capacity, kvh, hd]
+ * (strides in elements); the others are the call's, which are also stored there in row
+ * b, at places lengths[b] + i below capacity.  lengths [rows] int32 and origin are device
+ * memory, their values clamped to 0..capacity and to the rows; `longest`, at least
+ * the largest of them, only sets how the work is split.  out lies apart from all else;
+ * the workspace is this call's until it has ended on the stream.
+ */
+int tm_branch_attention(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                        const void* v, int64_t v_stride, int64_t T, const void* k_cache,
+                        const void* v_cache, int64_t stride_page, int64_t stride_slot,
+                        int64_t page_size, int64_t cache_pages,
+                        const int32_t* block_table, int64_t num_table_pages,
+                        int64_t seq_len, void* k_rows, void* v_rows, int64_t stride_row,
+                        int64_t stride_pos, int64_t rows, int64_t capacity,
+                        const int32_t* origin, int64_t origin_stride,
+                        const int32_t* lengths, int64_t longest, const int32_t* units,
+                        int64_t num_units, const int32_t* tokens, int64_t max_count,
+                        int64_t Hq, int64_t kvh, int64_t hd, float scale, int dtype,
+                        void* out, int64_t out_stride, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+
+/*
+ * lengths[b] += counts[b], or `count` with counts NULL, up to capacity: after a step's
+ * last layer.
+ */
+int tm_branch_advance(int32_t* lengths, const int32_t* counts, int64_t count,
+                      int64_t rows, int64_t capacity, void* stream);
+
+/* Workspace bytes of tm_beam_select for these sizes. */
+int tm_beam_workspace(int64_t G, int64_t K, int64_t V, int64_t num, int64_t* bytes);
+
+/*
+ * Beam search's selection: for each of G groups of K beams the `num` best of
+ *   scores[b] + l_b[v] - log sum_u exp l_b[u]     (l_b: row g K + b of logits)
+ * and, for a beam b with finished[b], of (scores[b], pad_token) alone.  Larger
+ * scores first; of equal ones the lower beam, then the larger logit, then the lower
+ * token.  Scores are formed in 64 bits and written in fp32.  The reference decodes one
+ * continuation (greedy or sampled) and has no counterpart.
+ *
+ * logits [G K, V] of dtype, row stride in elements; scores fp32 [G, K]; finished [G, K]
+ * bytes, or NULL.  NaN logits count as -infinity; of a row with infinite logits those
+ * share the weight.  A score of -infinity or NaN, or a row without a logit above
+ * -infinity, gives no candidates; where fewer than num are left the rest are score
+ * -infinity, parent -1 and token -1.  out_scores fp32, parents int32 (the beam within the
+ * group) and tokens int64, each [G, num].  K, num <= TM_MAX_BEAMS, V <=
+ * TM_MAX_SAMPLE_VOCAB, G K <= TM_MAX_ROWS.  The workspace (8-byte aligned) is this call's
+ * until it has ended on the stream.
+ */
+int tm_beam_select(const void* logits, int dtype, int64_t G, int64_t K, int64_t V,
+                   int64_t row_stride, const float* scores, const uint8_t* finished,
+                   int64_t pad_token, int64_t num, float* out_scores, int32_t* parents,
+                   int64_t* tokens, void* workspace, int64_t workspace_bytes,
+                   void* stream);
+
+/*
+ * What beams hold, reordered: row g K + i of out becomes row g K + parents[g, i] of x,
+ * `width` bytes of each (row strides in bytes, parents_stride in elements).  A parent
+ * outside 0..K-1 stands for the beam itself.  out is x, with the same stride, or lies
+ * apart from it.  K <= TM_MAX_BEAMS, G <= 65535.
+ */
+int tm_reorder_rows(const void* x, int64_t x_stride, void* out, int64_t out_stride,
+                    int64_t width, const int32_t* parents, int64_t parents_stride,
+                    int64_t G, int64_t K, void* stream);
 
 #ifdef __cplusplus
 }

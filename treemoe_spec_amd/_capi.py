@@ -59,6 +59,15 @@ SIGNATURES: dict[str, list] = {
     "tm_prompt_cached_workspace": [I64] * 5 + [P],
     "tm_prompt_attention_cached": [P, I64, I64, P, P, I64, I64, I64, I64, P, I64, I64, I64, I64,
                                    I64, F32, I32, P, I64, P, I64, P],
+    "tm_branch_plan": [P, I64, I64, I64, P, I64, P, I64, P],
+    "tm_branch_workspace": [I64] * 8 + [P],
+    "tm_branch_attention": [P, I64] * 3 + [I64, P, P, I64, I64, I64, I64, P, I64, I64, P, P]
+                           + [I64] * 4 + [P, I64, P, I64, P, I64, P] + [I64] * 4
+                           + [F32, I32, P, I64, P, I64, P],
+    "tm_branch_advance": [P, P, I64, I64, I64, P],
+    "tm_beam_workspace": [I64] * 4 + [P],
+    "tm_beam_select": [P, I32] + [I64] * 4 + [P, P, I64, I64, P, P, P, P, I64, P],
+    "tm_reorder_rows": [P, I64, P, I64, I64, P, I64, I64, I64, P],
 }
 
 TM_OBJECTIVE = {"mass": 0, "critical_path": 1}
@@ -71,6 +80,7 @@ TM_OP4_NOALLOC_MAX_NODES = 2048
 TM_MAX_NORM_HIDDEN = 65536
 TM_MAX_SAMPLE_VOCAB = 262144
 TM_MAX_PROMPT_KEYS = 1 << 24
+TM_MAX_BEAMS = 64
 TM_MAX_ROWS = 1 << 21
 
 _lib = None

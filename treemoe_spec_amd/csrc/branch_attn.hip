@@ -1,0 +1,600 @@
+// Attention of branches of one sequence: requests behind a shared prompt, beams, drafts.
+// Branch b's tokens attend to all S positions of the sequence, in the pages of its cache,
+// and causally to what the branch itself holds: len_b keys in the branch cache and the
+// tokens of this call, whose keys and values come as k and v and are stored behind them:
+//
+//   out[t, h] = sum_j softmax_j(scale q[t, h] . k[j, h / group]) v[j, h / group].
+//
+// Decomposition.  The softmax over a row's keys splits into parts that leave their sum,
+// maximum and unnormalised output in fp32.  The shared keys are taken once for all
+// branches: their (token, head of the group) pairs are one long list of rows for prompt
+// attention's kernels, without a causal border.  A branch's own keys are taken by
+// workgroups of its own, few rows against one range of keys.  A last kernel joins a row's
+// parts, the shared ones first, each in key order, so results are the same on every run.
+//
+// Position t of branch b lies in row origin[b][t] of the branch cache, the row of the
+// ancestor that stored it (without a table of origins, in row b).  So beams are reordered
+// by their tables, and no key moves.
+#include <algorithm>
+#include <new>
+
+#include "attn_tile.h"
+#include "prompt_parts.h"
+
+namespace {
+
+struct BranchParams : PromptParams {   // k, v: the layer's [rows, capacity, kvh, hd]
+  const uint16_t *new_k, *new_v;       // of the call's tokens
+  int64_t new_k_stride, new_v_stride;
+  int64_t row_stride;                  // of the branch cache; k_stride is a position's
+  const int32_t* origin;               // [rows, origin_stride], or NULL
+  int64_t origin_stride;
+  const int32_t* lengths;              // [rows]
+  const int4* units;                   // (branch, tile, first token, tokens), or NULL:
+  int count, unit_tiles;               // `count` tokens of every branch
+  int rows, capacity;
+  int parts;                           // leaves partials even where one part has all own keys
+};
+
+// Stages of a branch's own keys into LDS by NW waves, as Feed has them.  A key's row
+// stands alone: the lanes look the origins of the wave's keys up, a stage ahead, and
+// pass them to each other.
+template <int HD, int NW>
+struct BranchFeed {
+  typedef Shape<HD> S;
+  typedef BranchParams Params;
+  static constexpr int kLoads = S::kTile / (1024 * NW);
+  static constexpr int kWaveKeys = kLoads * S::kKeysPerLoad;
+  static_assert(kWaveKeys <= 64, "a lane looks up one key");
+  const uint16_t *k, *v, *new_k, *new_v;  // the head's first element
+  int b, len;              // the branch, and the keys that it held before the call
+  int first, left, step;   // the next stage's first key, the last key from there on, and
+                           // the keys to the stage behind
+  int row;                 // the row of one of the wave's keys in the next stage
+  int v_first, v_left, v_row;  // of the stage whose K came last
+
+  static __device__ __forceinline__ int wave() {
+    return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) & (NW - 1);
+  }
+  static __device__ __forceinline__ int wave_key() { return wave() * kWaveKeys; }
+  static __device__ __forceinline__ int row_of(const BranchParams& p, int b, int len, int key) {
+    if (p.origin == nullptr || key >= len) return b;
+    return min(max(p.origin[(int64_t)b * p.origin_stride + key], 0), p.rows - 1);
+  }
+  __device__ __forceinline__ void look_up(const BranchParams& p) {
+    const int j = wave_key() + ((int)threadIdx.x & (kWaveKeys - 1));
+    row = row_of(p, b, len, first + min(j, left));
+  }
+  static __device__ __forceinline__ void key_at(const BranchParams& p, const Item& it, int key,
+                                                const uint16_t*& kr, const uint16_t*& vr) {
+    const int len = it.k_len - it.q_len;
+    if (key < len) {
+      const int64_t at = (int64_t)row_of(p, it.k0, len, key) * p.row_stride + key * p.k_stride;
+      kr = p.k + at;
+      vr = p.v + at;
+    } else {
+      kr = p.new_k + (int64_t)(it.q0 + key - len) * p.new_k_stride;
+      vr = p.new_v + (int64_t)(it.q0 + key - len) * p.new_v_stride;
+    }
+  }
+  __device__ __forceinline__ void start(const BranchParams& p, const Item& it, int kvhead,
+                                        int begin, int step_) {
+    b = it.k0;
+    len = it.k_len - it.q_len;
+    k = p.k + kvhead * HD;
+    v = p.v + kvhead * HD;
+    new_k = p.new_k + kvhead * HD + (int64_t)(it.q0 - len) * p.new_k_stride;
+    new_v = p.new_v + kvhead * HD + (int64_t)(it.q0 - len) * p.new_v_stride;
+    step = step_;
+    first = begin;
+    left = it.k_len - 1 - begin;
+    v_first = v_left = v_row = 0;
+    look_up(p);
+  }
+  template <bool V>
+  __device__ __forceinline__ void load(const BranchParams& p, int first_, int left_, int row_,
+                                       uint8_t* tile) const {
+    const int lane = threadIdx.x & 63, mine = lane / S::kChunks;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int in = i * S::kKeysPerLoad + mine;  // among the wave's keys
+      const int j = wave_key() + in;
+      const int key = first_ + min(j, left_);
+      const int at = __shfl(row_, in);
+      const uint16_t* const held = (V ? v : k) + (int64_t)at * p.row_stride + key * p.k_stride;
+      const uint16_t* const fresh_ =
+          V ? new_v + (int64_t)key * p.new_v_stride : new_k + (int64_t)key * p.new_k_stride;
+      const int chunk = (lane & (S::kChunks - 1)) ^ (V ? S::swz_v(j) : S::swz_k(j));
+      __builtin_amdgcn_global_load_lds((glb_void*)((key < len ? held : fresh_) + chunk * 8),
+                                       (lds_void*)(tile + (wave() * kLoads + i) * 1024), 16, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void load_k(const BranchParams& p, uint8_t* tile) {
+    load<false>(p, first, left, row, tile);
+    v_first = first;
+    v_left = left;
+    v_row = row;
+    first += step;
+    left -= step;
+    look_up(p);
+  }
+  __device__ __forceinline__ void load_v(const BranchParams& p, uint8_t* tile) {
+    load<true>(p, v_first, v_left, v_row, tile);
+  }
+};
+
+// A workgroup's part of a branch: its rows against a range of its keys.
+struct Work {
+  Item it;
+  int kvhead;
+  int lo, hi;  // the new keys of the range that this workgroup stores
+};
+__device__ __forceinline__ Work work_of(const BranchParams& p, int block, int tile_rows) {
+  Work w;
+  w.kvhead = block % p.kvh;
+  const int at = block / p.kvh, chunk = at % p.chunks, unit = at / p.chunks;
+  Item& it = w.it;
+  if (p.units != nullptr) {
+    const int4 u = p.units[unit];
+    it.k0 = u.x;
+    it.tile = u.y;
+    it.q0 = u.z;
+    it.q_len = u.w;
+  } else {
+    it.k0 = unit / p.unit_tiles;
+    it.tile = unit % p.unit_tiles;
+    it.q0 = it.k0 * p.count;
+    it.q_len = p.count;
+  }
+  const int len = min(max(__builtin_amdgcn_readfirstlane(p.lengths[it.k0]), 0), p.capacity);
+  it.k_len = len + it.q_len;
+  // ranges by the branch's own length: they hold all its keys whatever the host took it for
+  const int per = (it.k_len + p.chunks - 1) / p.chunks;
+  const int span = (per + kKeys - 1) / kKeys * kKeys;
+  const int last_token = min(it.q_len - 1, (it.tile * tile_rows + tile_rows - 1) / p.group);
+  it.begin = min(chunk * span, it.k_len);
+  const int end = min(it.begin + span, it.k_len);
+  it.end = min(end, len + last_token + 1);
+  it.slot = p.parts ? unit * p.chunks + chunk : -1;
+  w.lo = it.tile == 0 ? max(it.begin, len) : end;
+  w.hi = end;
+  return w;
+}
+
+// The new keys and values lo .. hi - 1 of the head into the branch's own row.
+template <int HD>
+__device__ __forceinline__ void store_new(const BranchParams& p, const Work& w) {
+  constexpr int kPieces = HD / 8;
+  const int len = w.it.k_len - w.it.q_len, hi = min(w.hi, p.capacity);
+  for (int x = threadIdx.x; x < (hi - w.lo) * kPieces; x += kThreads) {
+    const int key = w.lo + x / kPieces, e = w.kvhead * HD + x % kPieces * 8;
+    const int64_t from = w.it.q0 + key - len;
+    const int64_t to = (int64_t)w.it.k0 * p.row_stride + key * p.k_stride + e;
+    *reinterpret_cast<u32x4_t*>(const_cast<uint16_t*>(p.k) + to) =
+        *reinterpret_cast<const u32x4_t*>(p.new_k + from * p.new_k_stride + e);
+    *reinterpret_cast<u32x4_t*>(const_cast<uint16_t*>(p.v) + to) =
+        *reinterpret_cast<const u32x4_t*>(p.new_v + from * p.new_v_stride + e);
+  }
+}
+
+// A branch's own keys, few rows (a decoded token's heads).
+template <int DT, int HD>
+__global__ void __launch_bounds__(kThreads, 1) tm_branch_few_kernel(BranchParams p) {
+  typedef Shape<HD> S;
+  __shared__ __attribute__((aligned(1024))) uint8_t s_k[4][S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_v[4][S::kTile];
+  __shared__ float s_stat[4][32][2];
+  const Work w = work_of(p, blockIdx.x, 32);
+  store_new<HD>(p, w);
+  few_body<DT, HD, BranchFeed<HD, 1>>(p, w.it, w.kvhead, s_k, s_v, s_stat);
+}
+
+// Its own keys, tiles of 128 rows.
+template <int DT, int HD>
+__global__ void __launch_bounds__(kThreads, 2) tm_branch_short_kernel(BranchParams p) {
+  typedef Shape<HD> S;
+  __shared__ __attribute__((aligned(1024))) uint8_t s_k0[S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_v0[S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_k1[S::kTile];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_v1[S::kTile];
+  const Work w = work_of(p, blockIdx.x, 128);
+  store_new<HD>(p, w);
+  short_body<DT, HD, BranchFeed<HD, 4>>(p, w.it, w.kvhead, s_k0, s_v0, s_k1, s_v1);
+}
+
+// Branches whose call has ended hold `count` more keys, or counts[b].
+__global__ void __launch_bounds__(kThreads) tm_branch_advance_kernel(int32_t* lengths,
+                                                                     const int32_t* counts,
+                                                                     int count, int rows,
+                                                                     int capacity) {
+  const int b = (int)(blockIdx.x * kThreads + threadIdx.x);
+  if (b < rows)
+    lengths[b] = min(max(lengths[b], 0) + max(counts != nullptr ? counts[b] : count, 0), capacity);
+}
+
+// Parts of one kind: `chunks` of every tile, as `few` lays rows down or as whole tiles.
+struct Parts {
+  const float* part;
+  const float* stats;
+  int chunks, tile_rows, part_rows;
+  int tiled;
+};
+struct BranchJoin {
+  Parts shared, own;
+  const int4* tokens;  // (branch, place in it, its first unit), or NULL:
+  int count, unit_tiles;
+  int T, Hq, kvh, group;
+  uint16_t* out;
+  int64_t out_stride;
+};
+constexpr int kMaxParts = 512;  // of each kind
+
+// Where a row's parts lie: chunk c's statistics at (first + c * step) * 2, its output at
+// o + c * step * HD.
+struct RowParts {
+  const float *stats, *o;
+  int64_t step;
+};
+// elements e .. e + 3 of row `row` of a KV head; tile0: its rows' first tile
+template <int HD>
+__device__ __forceinline__ RowParts parts_of(const Parts& s, int kvh, int kvhead, int tile0,
+                                             int row, int e) {
+  const int tile = row / s.tile_rows, in = row - tile * s.tile_rows;
+  const int64_t slot =
+      ((int64_t)(tile0 + tile) * s.chunks * kvh + kvhead) * s.part_rows + in;
+  RowParts r;
+  r.step = (int64_t)kvh * s.part_rows;
+  r.stats = s.stats + slot * 2;
+  r.o = s.tiled ? s.part + (slot - (in & 31)) * HD + (e >> 3) * 256 + ((e >> 2) & 1) * 128 +
+                      (in & 31) * 4
+                : s.part + slot * HD + e;
+  return r;
+}
+
+// A wave joins the parts of one row: the maximum and the sum over the parts first, a lane
+// per part, then the weighted outputs in their order, four elements a lane.
+template <int DT, int HD>
+__global__ void __launch_bounds__(kThreads) tm_branch_join_kernel(BranchJoin p) {
+  __shared__ float s_a[4][2 * kMaxParts];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + wave;
+  if (unit >= (int64_t)p.T * p.Hq) return;
+  const int t = (int)(unit / p.Hq), head = (int)(unit - (int64_t)t * p.Hq);
+  const int kvhead = head / p.group, g = head - kvhead * p.group;
+  constexpr int kLanes = HD / 4, kGroups = 64 / kLanes;
+  const int e = 4 * (lane % kLanes);
+  int place, unit0;
+  if (p.tokens != nullptr) {
+    const int4 x = p.tokens[t];
+    place = x.y;
+    unit0 = x.z;
+  } else {
+    place = t % p.count;
+    unit0 = t / p.count * p.unit_tiles;
+  }
+  const RowParts r[2] = {parts_of<HD>(p.shared, p.kvh, kvhead, 0, t * p.group + g, e),
+                         parts_of<HD>(p.own, p.kvh, kvhead, unit0, place * p.group + g, e)};
+  const int n[2] = {p.shared.chunks, p.own.chunks};
+  float m = -INFINITY;
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+    for (int c = lane; c < n[s]; c += 64) m = fmaxf(m, r[s].stats[c * r[s].step * 2]);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float sum = 0.0f;
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+    for (int c = lane; c < n[s]; c += 64) {
+      const float a = __builtin_amdgcn_exp2f(r[s].stats[c * r[s].step * 2] - ref);
+      sum += r[s].stats[c * r[s].step * 2 + 1] * a;
+      s_a[wave][(s ? n[0] : 0) + c] = a;
+    }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll 8
+    for (int c = lane / kLanes; c < n[s]; c += kGroups) {
+      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(r[s].o + c * r[s].step * HD);
+      const float a = s_a[wave][(s ? n[0] : 0) + c];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = fmaf(x[i], a, o[i]);
+    }
+#pragma unroll
+  for (int d = 32; d >= kLanes; d >>= 1)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], d);
+  if (lane >= kLanes) return;
+  const float inv = sum > 0.0f ? 1.0f / sum : sum;  // 0 where nothing was seen; NaN stays
+  u32x2_t w;
+  w.x = tm_pack2<DT>(o[0] * inv, o[1] * inv);
+  w.y = tm_pack2<DT>(o[2] * inv, o[3] * inv);
+  *reinterpret_cast<u32x2_t*>(p.out + (int64_t)t * p.out_stride + (int64_t)head * HD + e) = w;
+}
+
+// ------------------------------------------------------------------- host --
+
+constexpr int64_t kMaxStride = 1 << 24;
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+int check_heads(int64_t Hq, int64_t kvh, int64_t hd) {
+  if (kvh < 1 || Hq < kvh || Hq % kvh != 0 || Hq > 1024 || (hd != 64 && hd != 128))
+    return TM_ERR_SHAPE;
+  return TM_OK;
+}
+
+// Rows of a tile of a branch: 32 where no branch has more, else 128.
+int64_t own_tile_rows(int64_t max_count, int64_t group) { return max_count * group <= 32 ? 32 : 128; }
+
+struct BranchPlan {
+  PrefixPlan prefix;
+  bool few;
+  int64_t units, chunks;           // of the branches' own keys
+  int64_t own_rows;                // rows of one of their partials
+  int64_t prefix_slots, own_slots; // (of one KV head)
+  int64_t prefix_floats, floats;   // of the workspace
+};
+
+// T tokens, at most max_count of one branch, in `units` tiles of branches; S shared keys, at
+// most `longest` held by a branch.
+int plan_branches(int64_t T, int64_t units, int64_t max_count, int64_t S, int64_t longest,
+                  int64_t Hq, int64_t kvh, int64_t hd, BranchPlan* o) {
+  const int64_t group = Hq / kvh;
+  if (units < 0 || max_count < 0 || max_count > T || longest < 0 || longest > TM_MAX_PROMPT_KEYS)
+    return TM_ERR_SHAPE;
+  *o = {};
+  if (S > 0) {
+    const int rc = tm_prefix_plan(T, S, Hq, kvh, &o->prefix);
+    if (rc) return rc;
+  } else if (S < 0 || T < 0 || T * group > INT32_MAX - 1024) {
+    return TM_ERR_SHAPE;
+  }
+  const int64_t rows = own_tile_rows(max_count, group);
+  o->few = rows == 32;
+  o->units = units;
+  const int64_t keys = longest + max_count;
+  const int64_t want = std::min<int64_t>((o->few ? kCUs : 2 * kCUs) / std::max<int64_t>(units * kvh, 1),
+                                         kMaxParts);
+  o->chunks = std::max<int64_t>(1, std::min(want, ceil_div(keys, 4 * kKeys)));
+  o->own_rows = o->few ? std::min<int64_t>(32, max_count * group) : rows;
+  o->prefix_slots = S > 0 ? o->prefix.tiles * o->prefix.chunks : 0;
+  const bool joined = S > 0 || o->chunks > 1;
+  o->own_slots = joined ? units * o->chunks : 0;
+  if (o->own_slots > INT32_MAX || units * o->chunks * kvh > UINT32_MAX / kThreads ||
+      T * Hq > UINT32_MAX / 64)
+    return TM_ERR_SHAPE;
+  o->prefix_floats = S > 0 ? kvh * (hd + 2) * o->prefix_slots * o->prefix.part_rows : 0;
+  o->prefix_floats = ceil_div(o->prefix_floats, 4) * 4;  // (16-byte stores behind them)
+  o->floats = o->prefix_floats + kvh * (hd + 2) * o->own_slots * o->own_rows;
+  return TM_OK;
+}
+
+bool vec_ok(const void* p, int64_t stride) { return (uintptr_t)p % 16 == 0 && stride % 8 == 0; }
+
+template <int DT, int HD>
+void launch_own(const BranchParams& p, const BranchPlan& o, hipStream_t st) {
+  const dim3 grid((unsigned)(o.units * o.chunks * p.kvh)), block(kThreads);
+  if (o.few)
+    hipLaunchKernelGGL((tm_branch_few_kernel<DT, HD>), grid, block, 0, st, p);
+  else
+    hipLaunchKernelGGL((tm_branch_short_kernel<DT, HD>), grid, block, 0, st, p);
+}
+template <int DT, int HD>
+void launch_join(const BranchJoin& j, hipStream_t st) {
+  hipLaunchKernelGGL((tm_branch_join_kernel<DT, HD>),
+                     dim3((unsigned)ceil_div((int64_t)j.T * j.Hq, 4)), dim3(kThreads), 0, st, j);
+}
+
+}  // namespace
+
+extern "C" int tm_branch_plan(const int64_t* counts, int64_t B, int64_t Hq, int64_t kvh,
+                              int32_t* units, int64_t max_units, int32_t* tokens,
+                              int64_t max_tokens, int64_t* sizes) {
+  int rc = check_heads(Hq, kvh, 128);
+  if (rc) return rc;
+  if (sizes == nullptr || B < 0 || (B > 0 && counts == nullptr)) return TM_ERR_ARG;
+  if (B > INT32_MAX) return TM_ERR_SHAPE;
+  const int64_t group = Hq / kvh;
+  int64_t total = 0, longest = 0;
+  for (int64_t b = 0; b < B; ++b) {
+    if (counts[b] < 0 || counts[b] > TM_MAX_PROMPT_KEYS) return TM_ERR_SHAPE;
+    total += counts[b];
+    if (total * group > INT32_MAX - 1024) return TM_ERR_SHAPE;
+    longest = std::max(longest, counts[b]);
+  }
+  const int64_t rows = own_tile_rows(longest, group);
+  int64_t n = 0;
+  for (int64_t b = 0; b < B; ++b) n += ceil_div(counts[b] * group, rows);
+  sizes[0] = n;
+  sizes[1] = total;
+  sizes[2] = longest;
+  if (units == nullptr && tokens == nullptr) return TM_OK;
+  if (max_units < n || max_tokens < total) return TM_ERR_SHAPE;
+  if ((units == nullptr && n > 0) || (tokens == nullptr && total > 0)) return TM_ERR_ARG;
+  int64_t at = 0, first = 0;
+  for (int64_t b = 0; b < B; ++b) {
+    const int64_t tiles = ceil_div(counts[b] * group, rows);
+    for (int64_t t = 0; t < tiles; ++t) {
+      int32_t* const u = units + 4 * (at + t);
+      u[0] = (int32_t)b;
+      u[1] = (int32_t)t;
+      u[2] = (int32_t)first;
+      u[3] = (int32_t)counts[b];
+    }
+    for (int64_t i = 0; i < counts[b]; ++i) {
+      int32_t* const x = tokens + 4 * (first + i);
+      x[0] = (int32_t)b;
+      x[1] = (int32_t)i;
+      x[2] = (int32_t)at;
+      x[3] = 0;
+    }
+    at += tiles;
+    first += counts[b];
+  }
+  return TM_OK;
+}
+
+extern "C" int tm_branch_workspace(int64_t T, int64_t units, int64_t max_count, int64_t seq_len,
+                                   int64_t longest, int64_t Hq, int64_t kvh, int64_t hd,
+                                   int64_t* bytes) {
+  int rc = check_heads(Hq, kvh, hd);
+  if (rc) return rc;
+  if (bytes == nullptr) return TM_ERR_ARG;
+  BranchPlan o;
+  rc = plan_branches(T, units, max_count, seq_len, longest, Hq, kvh, hd, &o);
+  if (rc) return rc;
+  *bytes = 4 * o.floats;
+  return TM_OK;
+}
+
+extern "C" int tm_branch_attention(
+    const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+    int64_t v_stride, int64_t T, const void* k_cache, const void* v_cache, int64_t stride_page,
+    int64_t stride_slot, int64_t page_size, int64_t cache_pages, const int32_t* block_table,
+    int64_t num_table_pages, int64_t seq_len, void* k_rows, void* v_rows, int64_t stride_row,
+    int64_t stride_pos, int64_t rows, int64_t capacity, const int32_t* origin,
+    int64_t origin_stride, const int32_t* lengths, int64_t longest, const int32_t* units,
+    int64_t num_units, const int32_t* tokens, int64_t max_count, int64_t Hq, int64_t kvh,
+    int64_t hd, float scale, int dtype, void* out, int64_t out_stride, void* workspace,
+    int64_t workspace_bytes, void* stream) {
+  int rc = check_heads(Hq, kvh, hd);
+  if (rc) return rc;
+  if ((dtype != TM_DTYPE_BF16 && dtype != TM_DTYPE_F16) || !(scale > 0.0f) || scale == INFINITY)
+    return TM_ERR_ARG;
+  const int64_t group = Hq / kvh;
+  if (T < 0 || rows < 0 || rows > INT32_MAX || capacity < 0 || capacity > TM_MAX_PROMPT_KEYS ||
+      longest > capacity)
+    return TM_ERR_SHAPE;
+  if (T == 0) return TM_OK;
+  if ((units == nullptr) != (tokens == nullptr)) return TM_ERR_ARG;
+  int64_t unit_tiles = 1;
+  if (units == nullptr) {
+    if (max_count < 1 || rows < 1 || T != rows * max_count) return TM_ERR_SHAPE;
+    unit_tiles = ceil_div(max_count * group, own_tile_rows(max_count, group));
+    if (num_units != rows * unit_tiles) return TM_ERR_SHAPE;
+  } else if (num_units < 1 || num_units > T) {
+    return TM_ERR_SHAPE;
+  }
+  BranchPlan o;
+  rc = plan_branches(T, num_units, max_count, seq_len, longest, Hq, kvh, hd, &o);
+  if (rc) return rc;
+  if (seq_len > 0 &&
+      (page_size < 1 || page_size > (1 << 24) || (page_size & (page_size - 1)) != 0 ||
+       cache_pages < 1 || cache_pages > INT32_MAX || num_table_pages > INT32_MAX ||
+       ceil_div(seq_len, page_size) > num_table_pages || stride_slot < kvh * hd ||
+       stride_slot > kMaxStride || stride_page < page_size * stride_slot))
+    return TM_ERR_SHAPE;
+  if ((T > 1 && (q_stride < Hq * hd || out_stride < Hq * hd || k_stride < kvh * hd ||
+                 v_stride < kvh * hd)) ||
+      k_stride > kMaxStride || v_stride > kMaxStride || stride_pos < kvh * hd ||
+      stride_pos > kMaxStride || stride_row < capacity * stride_pos ||
+      (origin != nullptr && origin_stride < capacity))
+    return TM_ERR_SHAPE;
+  if (4 * o.floats > workspace_bytes) return TM_ERR_SHAPE;
+  if (!vec_ok(q, T > 1 ? q_stride : 0) || !vec_ok(out, T > 1 ? out_stride : 0) ||
+      !vec_ok(k, T > 1 ? k_stride : 0) || !vec_ok(v, T > 1 ? v_stride : 0) ||
+      !vec_ok(k_rows, stride_row) || !vec_ok(v_rows, stride_pos) ||
+      (seq_len > 0 && (!vec_ok(k_cache, stride_slot) || !vec_ok(v_cache, stride_page))) ||
+      (uintptr_t)units % 16 || (uintptr_t)tokens % 16 || (uintptr_t)block_table % 4 ||
+      (uintptr_t)origin % 4 || (uintptr_t)lengths % 4 || (uintptr_t)workspace % 16)
+    return TM_ERR_ALIGN;
+  const hipStream_t st = (hipStream_t)stream;
+  BranchParams p = {};
+  p.q = (const uint16_t*)q;
+  p.out = (uint16_t*)out;
+  p.q_stride = q_stride;
+  p.out_stride = out_stride;
+  p.kvh = (int)kvh;
+  p.group = (int)group;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  float* at = (float*)workspace;
+  BranchJoin j = {};
+  if (seq_len > 0) {
+    PromptParams s = p;
+    s.k = (const uint16_t*)k_cache;
+    s.v = (const uint16_t*)v_cache;
+    s.table = block_table;
+    s.k_stride = s.v_stride = stride_slot;
+    s.stride_page = stride_page;
+    s.q_len = (int)T;
+    s.k_len = (int)seq_len;
+    while ((int64_t(1) << s.page_shift) < page_size) ++s.page_shift;
+    s.cache_pages = (int)cache_pages;
+    const int64_t part_rows = o.prefix_slots * kvh * o.prefix.part_rows;
+    s.part = at;
+    s.stats = at + part_rows * hd;
+    at += o.prefix_floats;
+    tm_prefix_launch(s, o.prefix, dtype, hd, page_size, st);
+    j.shared = {s.part, s.stats, (int)o.prefix.chunks, (int)o.prefix.tile_rows,
+                (int)o.prefix.part_rows, o.prefix.kind != 0};
+  } else {
+    j.shared.tile_rows = 1;
+  }
+  p.k = (const uint16_t*)k_rows;
+  p.v = (const uint16_t*)v_rows;
+  p.k_stride = p.v_stride = stride_pos;
+  p.row_stride = stride_row;
+  p.new_k = (const uint16_t*)k;
+  p.new_v = (const uint16_t*)v;
+  p.new_k_stride = k_stride;
+  p.new_v_stride = v_stride;
+  p.origin = origin;
+  p.origin_stride = origin_stride;
+  p.lengths = lengths;
+  p.units = (const int4*)units;
+  p.count = (int)max_count;
+  p.unit_tiles = (int)unit_tiles;
+  p.rows = (int)rows;
+  p.capacity = (int)capacity;
+  p.chunks = (int)o.chunks;
+  p.parts = o.own_slots > 0;
+  p.part_rows = (int)o.own_rows;
+  p.part = at;
+  p.stats = at + o.own_slots * kvh * o.own_rows * hd;
+  j.own = {p.part, p.stats, (int)o.chunks, o.few ? 32 : 128, (int)o.own_rows, !o.few};
+  j.tokens = (const int4*)tokens;
+  j.count = (int)max_count;
+  j.unit_tiles = (int)unit_tiles;
+  j.T = (int)T;
+  j.Hq = (int)Hq;
+  j.kvh = (int)kvh;
+  j.group = (int)group;
+  j.out = (uint16_t*)out;
+  j.out_stride = out_stride;
+#define TM_BRANCH(DT, HD)                             \
+  do {                                                \
+    launch_own<DT, HD>(p, o, st);                     \
+    if (p.parts) launch_join<DT, HD>(j, st);          \
+  } while (0)
+  if (dtype == TM_DTYPE_F16) {
+    if (hd == 128)
+      TM_BRANCH(TM_DTYPE_F16, 128);
+    else
+      TM_BRANCH(TM_DTYPE_F16, 64);
+  } else {
+    if (hd == 128)
+      TM_BRANCH(TM_DTYPE_BF16, 128);
+    else
+      TM_BRANCH(TM_DTYPE_BF16, 64);
+  }
+#undef TM_BRANCH
+  TM_HIP_CHECK_LAUNCH();
+  return TM_OK;
+}
+
+extern "C" int tm_branch_advance(int32_t* lengths, const int32_t* counts, int64_t count,
+                                 int64_t rows, int64_t capacity, void* stream) {
+  if (rows < 0 || rows > INT32_MAX - kThreads || capacity < 0 || capacity > TM_MAX_PROMPT_KEYS ||
+      count < 0 || count > TM_MAX_PROMPT_KEYS)
+    return TM_ERR_SHAPE;
+  if (rows == 0) return TM_OK;
+  if ((uintptr_t)lengths % 4 || (uintptr_t)counts % 4) return TM_ERR_ALIGN;
+  hipLaunchKernelGGL(tm_branch_advance_kernel, dim3((unsigned)ceil_div(rows, kThreads)),
+                     dim3(kThreads), 0, (hipStream_t)stream, lengths, counts, (int)count,
+                     (int)rows, (int)capacity);
+  TM_HIP_CHECK_LAUNCH();
+  return TM_OK;
+}

@@ -1,5 +1,6 @@
 // _tmlayer: CPython calls of the entry points that a forward makes once or more per
-// layer (norm, rotary positions, prompt attention) and per step (sampling).  Each
+// layer (norm, rotary positions, attention of prompts and branches) and per step
+// (sampling).  Each
 // function takes the entry point's arguments in order, addresses as integers, and
 // returns its status; conversions follow the C parameter types.  ctypes spends
 // ~3.5 us on a call of twenty arguments, this ~0.5 us.  The interpreter lock is
@@ -67,6 +68,19 @@ PyObject* cached_workspace(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return Py_BuildValue("iL", rc, (long long)bytes);
 }
 
+// branch_workspace(T, units, max_count, seq_len, longest, Hq, kvh, hd) -> (status, bytes)
+PyObject* branch_workspace(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 8) {
+    PyErr_SetString(PyExc_TypeError, "expected 8 arguments");
+    return nullptr;
+  }
+  int64_t a[8], bytes = 0;
+  for (int i = 0; i < 8; ++i) a[i] = convert<int64_t>(args[i]);
+  if (PyErr_Occurred()) return nullptr;
+  const int rc = tm_branch_workspace(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], &bytes);
+  return Py_BuildValue("iL", rc, (long long)bytes);
+}
+
 #define TM_ENTRY(name) \
   {#name, (PyCFunction)(void (*)(void))entry<name>, METH_FASTCALL, nullptr}
 
@@ -80,6 +94,11 @@ PyMethodDef kMethods[] = {
     {"prompt_cached_workspace", (PyCFunction)(void (*)(void))cached_workspace, METH_FASTCALL,
      nullptr},
     TM_ENTRY(tm_prompt_attention_cached),
+    {"branch_workspace", (PyCFunction)(void (*)(void))branch_workspace, METH_FASTCALL, nullptr},
+    TM_ENTRY(tm_branch_attention),
+    TM_ENTRY(tm_branch_advance),
+    TM_ENTRY(tm_beam_select),
+    TM_ENTRY(tm_reorder_rows),
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -251,3 +251,107 @@ def device_tables_of(kv, device) -> tuple[torch.Tensor, torch.Tensor]:
     if t.entries != kv.block_table:
         t.fill(kv.block_table)
     return t.table, t.scratch
+
+
+class BranchCache:
+    """What many branches of one sequence hold behind it: requests that share a prompt,
+    beams, drafted chains.  k and v are [layers, rows, capacity, kv_heads, head_dim], a
+    row for every branch; ``lengths`` (int32 on the device, mirrored in
+    ``host_lengths``) says how many keys each branch holds.
+
+    With ``beams`` > 1, neighbouring branches in groups of that many are the beams of one
+    search: position t of branch b lies in row ``origin[b, t]``, the row of the beam
+    that stored it, and ``reorder`` moves entries of this table instead of keys."""
+
+    def __init__(self, config, rows: int, capacity: int, device: str = "cuda",
+                 dtype: torch.dtype = torch.bfloat16, beams: int = 1):
+        if rows < 1 or capacity < 1:
+            raise ValueError("rows and capacity must be at least 1")
+        if beams < 1 or rows % beams:
+            raise ValueError("rows must be a multiple of beams")
+        self.config, self.beams = config, beams
+        shape = (config.num_layers, rows, capacity, config.num_kv_heads, config.head_dim)
+        self.k = torch.zeros(shape, device=device, dtype=dtype)
+        self.v = torch.zeros(shape, device=device, dtype=dtype)
+        self.lengths = torch.zeros(rows, device=device, dtype=torch.int32)
+        self.host_lengths = [0] * rows
+        self.longest = 0
+        self.origin = None
+        if beams > 1:
+            own = torch.arange(rows, device=device, dtype=torch.int32)
+            self.origin = own[:, None].repeat(1, capacity)
+
+    @property
+    def rows(self) -> int:
+        return self.k.shape[1]
+
+    @property
+    def capacity(self) -> int:
+        return self.k.shape[2]
+
+    def advance(self, counts=1) -> None:
+        """After the last layer of a step in which every branch has added ``counts``
+        tokens (a number, or the step's ``BranchPlan``): they now hold them.  A replay of
+        a captured call advances ``lengths`` alone; ``read_lengths`` brings the host's
+        up to it."""
+        from treemoe_spec_amd import _capi
+
+        uniform = isinstance(counts, int)
+        added = [counts] * self.rows if uniform else counts.counts
+        if len(added) != self.rows or (uniform and counts < 0):
+            raise ValueError(f"counts must be a number or a plan for {self.rows} branches")
+        now = [a + b for a, b in zip(self.host_lengths, added)]
+        if max(now) > self.capacity:
+            raise ValueError(f"a branch would hold {max(now)} keys, over the capacity of "
+                             f"{self.capacity}")
+        dev = self.lengths.device
+        _capi.require("BranchCache.advance", dev, lengths=self.lengths)
+        table = None if uniform else counts.device_counts
+        _capi.launch("tm_branch_advance", dev.index, self.lengths.data_ptr(), _capi.ptr(table),
+                     counts if uniform else 0, self.rows, self.capacity)
+        if not uniform:
+            _capi.used_by(dev.index, counts.made_on, table)
+        self.host_lengths, self.longest = now, max(now)
+
+    def read_lengths(self) -> None:
+        """The host's lengths from the device's (waits for them)."""
+        self.host_lengths = self.lengths.tolist()
+        self.longest = max(self.host_lengths)
+
+    def set_lengths(self, lengths) -> None:
+        """Cuts branches back to ``lengths`` keys (0 for a new request; a chain whose
+        last tokens were rejected).  The beams of a group are cut alike."""
+        lengths = [int(n) for n in lengths]
+        if len(lengths) != self.rows or any(not 0 <= n <= m for n, m in
+                                            zip(lengths, self.host_lengths)):
+            raise ValueError("lengths must be 0 .. the branches' present ones, one for each")
+        if self.origin is not None:
+            self._check_groups(lengths)
+            own = torch.arange(self.rows, dtype=torch.int32)[:, None].to(self.origin.device)
+            at = torch.arange(self.capacity).to(self.origin.device)
+            new = torch.tensor(lengths).to(self.origin.device)
+            self.origin.copy_(torch.where(at[None, :] < new[:, None], self.origin, own))
+        self.lengths.copy_(torch.tensor(lengths, dtype=torch.int32))
+        self.host_lengths, self.longest = lengths, max(lengths)
+
+    def reset(self) -> None:
+        """All branches hold nothing."""
+        self.set_lengths([0] * self.rows)
+
+    def _check_groups(self, lengths) -> None:
+        n = self.beams
+        if any(len(set(lengths[i:i + n])) > 1 for i in range(0, len(lengths), n)):
+            raise ValueError("the beams of a group must hold the same number of keys")
+
+    def reorder(self, parents: torch.Tensor) -> None:
+        """Beam i of group g goes on from what beam ``parents[g, i]`` holds (int32
+        [groups, beams], as ``beam_select`` gives them; one outside the group
+        leaves the beam as it is).  Moves entries of ``origin``, all layers at once."""
+        from treemoe_spec_amd.kernels.beam_search import reorder_rows
+
+        if self.origin is None:
+            raise ValueError("reorder needs a cache made with beams > 1")
+        if tuple(parents.shape) != (self.rows // self.beams, self.beams):
+            raise ValueError(f"parents must be [{self.rows // self.beams}, {self.beams}]")
+        self._check_groups(self.host_lengths)
+        reorder_rows(self.origin, parents, out=self.origin, columns=self.longest)
