@@ -681,6 +681,59 @@ int tm_reorder_rows(const void* x, int64_t x_stride, void* out, int64_t out_stri
                     int64_t width, const int32_t* parents, int64_t parents_stride,
                     int64_t G, int64_t K, void* stream);
 
+/* Workspace bytes of tm_attention_mass for these sizes. */
+int tm_mass_workspace(int64_t T, int64_t seq_len, int64_t Hq, int64_t kvh, int64_t hd,
+                      int64_t* bytes);
+
+/*
+ * What the last T of one sequence's seq_len cached positions give to every key:
+ *   mass[h, j] = before[h, j] + sum softmax_j(scale q[t, hq] . k_j)
+ * over the tokens t that see position j (causally, as in tm_prompt_attention_cached) and
+ * the query heads hq of KV head h; before may be NULL, for zeros.  A row whose scores
+ * are all -infinity gives nothing.  In fp32.  The attention itself is the reference's
+ * (treemoe/model/mixtral.py:208-250), which keeps no such sums.  Cache and q as in
+ * tm_prompt_attention_cached; before and mass fp32 [kvh, >= seq_len], row strides in
+ * elements, mass the same memory as before or apart from it.  The workspace (8-byte
+ * aligned) is this call's until it has ended on the stream.
+ */
+int tm_attention_mass(const void* q, int64_t q_stride, int64_t T, const void* k_cache,
+                      int64_t stride_page, int64_t stride_slot, int64_t page_size,
+                      int64_t cache_pages, const int32_t* block_table,
+                      int64_t num_table_pages, int64_t seq_len, int64_t Hq,
+                      int64_t kvh, int64_t hd, float scale, int dtype,
+                      const float* before, int64_t before_stride, float* mass,
+                      int64_t mass_stride, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+
+/* Workspace bytes of tm_evict for these sizes. */
+int tm_evict_workspace(int64_t L, int64_t kvh, int64_t seq_len, int64_t keep,
+                       int64_t* bytes);
+
+/*
+ * Cuts every (layer, KV head) of a paged cache from seq_len to `keep` keys.  Slot s has
+ * position positions[l, h, s] for s < recorded, else next_position - seq_len + s.  Positions
+ * below `sinks` and from next_position - recent on stay; of the others those with the
+ * largest mass, the lower slot first among equals, NaN last.  Kept keys in slots from
+ * `keep` on move, with their values, into the slots below that have become free, the i-th
+ * into the i-th; nothing else in the cache changes.  mass_out [L, kvh, columns]: the
+ * mass of what each slot then holds, 0 from `keep` on; positions_out [L, kvh, keep]: its
+ * position.  The reference's cache (treemoe/model/kv_cache.py) only grows.
+ *
+ * k_cache, v_cache: [L, pages, page_size, kvh, hd] of elem_bytes (1, 2 or 4), strides in
+ * elements, a key's row a multiple of 16 bytes, 16-byte aligned.  mass: fp32, rows
+ * of `columns` >= seq_len, strides mass_layer and mass_head; positions int32, strides
+ * pos_layer and pos_head.  The outputs lie apart from the inputs.
+ */
+int tm_evict(void* k_cache, void* v_cache, int64_t elem_bytes, int64_t L,
+             int64_t stride_layer, int64_t stride_page, int64_t stride_slot,
+             int64_t kvh, int64_t hd, int64_t page_size, int64_t cache_pages,
+             const int32_t* block_table, int64_t num_table_pages, int64_t seq_len,
+             int64_t keep, const float* mass, int64_t mass_layer, int64_t mass_head,
+             int64_t columns, const int32_t* positions, int64_t pos_layer,
+             int64_t pos_head, int64_t recorded, int64_t next_position, int64_t recent,
+             int64_t sinks, float* mass_out, int32_t* positions_out, void* workspace,
+             int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

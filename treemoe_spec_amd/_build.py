@@ -24,7 +24,7 @@ ORACLE_LIB = ROOT / "oracle" / "liboracle_c.so"
 
 HIP_SOURCES = ["capi.hip", "op1_route.hip", "op1_gemm.hip", "op1_prefill.hip", "op4_verify.hip",
                "tree_attn.hip", "rms_norm.hip", "rotary.hip", "sample.hip",
-               "prompt_attn.hip", "branch_attn.hip", "beam.hip"]
+               "prompt_attn.hip", "branch_attn.hip", "beam.hip", "evict.hip"]
 ARCH = os.environ.get("TREEMOE_AMD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [

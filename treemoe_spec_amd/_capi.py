@@ -68,6 +68,12 @@ SIGNATURES: dict[str, list] = {
     "tm_beam_workspace": [I64] * 4 + [P],
     "tm_beam_select": [P, I32] + [I64] * 4 + [P, P, I64, I64, P, P, P, P, I64, P],
     "tm_reorder_rows": [P, I64, P, I64, I64, P, I64, I64, I64, P],
+    "tm_mass_workspace": [I64] * 5 + [P],
+    "tm_attention_mass": [P, I64, I64, P, I64, I64, I64, I64, P, I64, I64, I64, I64, I64, F32, I32,
+                          P, I64, P, I64, P, I64, P],
+    "tm_evict_workspace": [I64] * 4 + [P],
+    "tm_evict": [P, P] + [I64] * 9 + [P, I64, I64, I64, P, I64, I64, I64, P] + [I64] * 6
+                + [P, P, P, I64, P],
 }
 
 TM_OBJECTIVE = {"mass": 0, "critical_path": 1}

@@ -68,6 +68,19 @@ PyObject* cached_workspace(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return Py_BuildValue("iL", rc, (long long)bytes);
 }
 
+// mass_workspace(T, seq_len, Hq, kvh, hd) -> (status, bytes)
+PyObject* mass_workspace(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 5) {
+    PyErr_SetString(PyExc_TypeError, "expected 5 arguments");
+    return nullptr;
+  }
+  int64_t a[5], bytes = 0;
+  for (int i = 0; i < 5; ++i) a[i] = convert<int64_t>(args[i]);
+  if (PyErr_Occurred()) return nullptr;
+  const int rc = tm_mass_workspace(a[0], a[1], a[2], a[3], a[4], &bytes);
+  return Py_BuildValue("iL", rc, (long long)bytes);
+}
+
 // branch_workspace(T, units, max_count, seq_len, longest, Hq, kvh, hd) -> (status, bytes)
 PyObject* branch_workspace(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 8) {
@@ -99,6 +112,9 @@ PyMethodDef kMethods[] = {
     TM_ENTRY(tm_branch_advance),
     TM_ENTRY(tm_beam_select),
     TM_ENTRY(tm_reorder_rows),
+    {"mass_workspace", (PyCFunction)(void (*)(void))mass_workspace, METH_FASTCALL, nullptr},
+    TM_ENTRY(tm_attention_mass),
+    TM_ENTRY(tm_evict),
     {nullptr, nullptr, 0, nullptr},
 };
 
