@@ -134,6 +134,25 @@ def _shorter(kv, n):
     return kv
 
 
+@pytest.mark.parametrize("t", [40, 300, 1100])
+def test_a_row_that_is_not_a_number(t):
+    """A NaN in a query reaches the keys that it sees, of its KV head, and no others."""
+    from treemoe_spec_amd.kernels.cache_eviction import attention_mass
+
+    _say(f"mass with a NaN query, {t} tokens")
+    q, k, v = t_attn._qkv(t, t, 4, 2, 64, BF, t)
+    q[t // 3, 3, 7] = NAN
+    kv = t_attn._cache(t, 2, 64, BF, 16, t)
+    kv.append(0, k.cuda(), v.cuda(), 0)
+    got = attention_mass(q.cuda(), kv, 0).cpu()
+    assert bool(got[1, :t // 3 + 1].isnan().all())
+    q[t // 3, 3] = 0.0
+    want = _want(q, k, 64 ** -0.5)
+    assert bool(((got[0] - want[0]).abs() <= 1e-4 * want[0] + 2.0 ** -90).all())
+    late = got[1, t // 3 + 1:]
+    assert bool(((late - want[1, t // 3 + 1:]).abs() <= 1e-4 * late + 2.0 ** -90).all())
+
+
 def test_mass_is_the_same_again():
     from treemoe_spec_amd.kernels.cache_eviction import attention_mass
 
@@ -219,13 +238,26 @@ def _check_evict(kv, mass, keep, positions=None, nxt=None, recent=0, sinks=0):
 @pytest.mark.parametrize("n,keep,recent,sinks", [
     (1, 1, 0, 0), (2, 1, 0, 0), (100, 50, 0, 0), (100, 99, 10, 4), (130, 20, 16, 4), (65, 64, 64, 0),
     (64, 1, 0, 1), (200, 199, 0, 0), (1100, 1030, 64, 4), (2100, 100, 32, 4), (50, 50, 3, 0),
-    (50, 90, 3, 0), (30, 0, 0, 0)])
+    (50, 90, 3, 0), (30, 0, 0, 0), (2048, 2000, 100, 4), (2049, 700, 64, 0)])
 def test_evict(n, keep, recent, sinks, layers, kvh, hd, dtype, page):
     _say(f"evict {n} -> {keep} recent {recent} sinks {sinks} {layers}x{kvh} hd={hd} {dtype}")
     g = torch.Generator().manual_seed(n + keep)
     kv = _cache_of(layers, n, kvh, hd, dtype, page, g)
     mass = torch.exp(2 * torch.randn(layers, kvh, n + 7, generator=g))
     _check_evict(kv, mass, keep, recent=recent, sinks=sinks)
+
+
+@pytest.mark.parametrize("layers,n,keep", [(1, 8192, 4000), (1, 8193, 8100), (1, 16384, 8192),
+                                           (1, 16385, 9000), (1, 20000, 130), (40, 600, 580),
+                                           (40, 600, 300)])
+def test_evict_long_and_many(layers, n, keep):
+    """Keys of a head beyond what a workgroup holds; heads that fill the chip."""
+    _say(f"evict {layers} layers {n} -> {keep}")
+    g = torch.Generator().manual_seed(n)
+    kv = _cache_of(layers, n, 4, 16, BF, 64, g)
+    mass = torch.exp(2 * torch.randn(layers, 4, n, generator=g))
+    mass[0, 1] = mass[0, 1].round()
+    _check_evict(kv, mass, keep, recent=64, sinks=4)
 
 
 def test_evict_ties_and_odd_masses():

@@ -144,6 +144,20 @@ def entry(name: str):
     return getattr(layer_binding() or lib(), name)
 
 
+def workspace_bytes(name: str, *sizes) -> int:
+    """What the size query tm_``name`` says: through the CPython binding where there is
+    one, else ctypes."""
+    fast = layer_binding()
+    if fast is not None:
+        rc, nbytes = getattr(fast, name)(*sizes)
+        if rc:
+            check(rc, "tm_" + name)
+        return nbytes
+    out = ctypes.c_int64()
+    call("tm_" + name, *sizes, ctypes.byref(out))
+    return out.value
+
+
 def launch(name: str, index: int, *args) -> None:
     """An entry point on torch's current stream of device ``index``, with that device
     current during the call."""

@@ -15,9 +15,10 @@
 // A wave takes 1024 logits of a row: its sum, and its best `num` as sorted keys (ordered
 // bits of the logit, inverted token), all distinct.  At least `num` logits reach the
 // num-th largest of the 64 lanes' largest, and only the `num` lanes that reach it hold
-// such, 16 at most each: the list never overflows.  Then one workgroup a group joins the sums,
-// takes the num-th largest of the lists' heads, which bounds the result from below in
-// the same way, and ranks what reaches it by binary search in the lists it came from.
+// such, 16 at most each: the list never overflows.  Four waves' lists become one.  Then one
+// workgroup a group joins the sums and ranks the lists' heads.  Entry i of the list whose
+// head is the r-th has r + i above it: what is left when that is `num` or more, and what
+// lies below the num-th head, cannot come out; the rest is ranked by counting.
 #include <cmath>
 
 #include "tm_vec.h"
@@ -26,10 +27,12 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kSeg = 1024;               // logits of a wave
-constexpr int kPer = kSeg / 64;          // of a lane
+// Logits of a lane, 256 times as many of a workgroup, which leaves one list.  A wave's
+// ranks, merges and barriers cost the same whatever it holds: many where the chip is full
+// anyway.  PER_FIGURES
+constexpr int kFewPer = 16, kManyPer = 64;
 constexpr int kMaxNum = TM_MAX_BEAMS;
-constexpr int kJoin = 1024;              // threads of a group's workgroup
+constexpr int kJoin = 512;               // threads of a group's workgroup, a list each
 
 struct BeamParams {
   const void* logits;
@@ -73,10 +76,10 @@ __device__ __forceinline__ int index_of(int e) {
   constexpr int kVec = DT == TM_DTYPE_F32 ? 4 : 8;
   return e / kVec * 64 * kVec + (int)(threadIdx.x & 63) * kVec + e % kVec;
 }
-template <int DT>
+template <int DT, int kPer>
 __device__ __forceinline__ void fetch(const BeamParams& p, int64_t row, int base,
                                       float (&x)[kPer]) {
-  if (p.aligned && base + kSeg <= p.vocab) {
+  if (p.aligned && base + 64 * kPer <= p.vocab) {
 #pragma unroll
     for (int c = 0; c < kPer / 8; ++c) {
       if constexpr (DT == TM_DTYPE_F32) {
@@ -107,6 +110,45 @@ __device__ __forceinline__ void fetch(const BeamParams& p, int64_t row, int base
   for (int e = 0; e < kPer; ++e) x[e] = fmaxf(x[e], -INFINITY);
 }
 
+// 2^(j / 64)
+__constant__ const double kPowers[64] = {
+    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
+    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
+    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
+    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
+    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
+    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
+    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
+    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
+    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
+    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
+    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0};
+
+// e^d for d <= 0, in 64 bits: with t = 64 d log2(e) and k the integer nearest to it,
+// 2^(k / 64) e^x, x = d - k ln 2 / 64, |x| <= ln 2 / 128: 2^(j / 64) from a table, e^x from
+// its Taylor polynomial of degree 4 (truncation below 4e-14).  Below -700 it is e^-700.
+// A library exponential, with its wider range and half an ulp, takes three times as long.
+__device__ __forceinline__ double exp_of(double d, const double* powers) {
+  constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to integers
+  constexpr double c = 0.010830424696249145;     // ln 2 / 64
+  const double y = fmax(d, -700.0) * 92.332482616893657;
+  const double t = y + kMagic;
+  const double x = y - (t - kMagic);
+  double q = fma(x, c * c * c * c / 24.0, c * c * c / 6.0);
+  q = fma(q, x, c * c / 2.0);
+  q = fma(q, x, c);
+  q = fma(q, x, 1.0);
+  const int k = (int)(uint32_t)(uint64_t)__double_as_longlong(t);
+  // (times 2^(k / 64) by the exponent: it stays above -1011)
+  return __longlong_as_double(__double_as_longlong(q * powers[k & 63]) +
+                              ((int64_t)(k >> 6) << 52));
+}
+
 // How many of the lanes' first `n` keys are larger than this lane's.
 __device__ __forceinline__ int rank_in_wave(uint64_t key, int n) {
   int rank = 0;
@@ -114,74 +156,149 @@ __device__ __forceinline__ int rank_in_wave(uint64_t key, int n) {
   return rank;
 }
 
-template <int DT>
+// The num-th largest of the lanes' keys, or a bound that just num of them reach: by
+// bisection of the logits' ordered bits, which ends as soon as a count is num; where
+// logits are equal, by the keys' ranks.
+__device__ __forceinline__ uint64_t least_of(uint64_t key, float top, int num) {
+  const uint32_t own = (uint32_t)(key >> 32);
+  // reached by num or more (all lanes reach -inf); above it: by fewer
+  uint32_t lo = 0x007fffffu, hi = order_bits(top);
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo + 1) / 2;
+    const int count = __popcll(__ballot(own >= mid));
+    if (count == num) return (uint64_t)mid << 32;
+    if (count > num)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  const uint64_t at = __ballot(rank_in_wave(key, 64) == num - 1);
+  return lane_of(key, __ffsll((unsigned long long)at) - 1);
+}
+
+// How many of each of N sorted lists' entries, `num` with zeros behind the last, are above
+// x: N searches side by side.
+template <int N, typename T, class ABOVE>
+__device__ __forceinline__ int above_in(const T* const (&lists)[N], int num, const T& x,
+                                        ABOVE&& above) {
+  int at[N] = {};
+  int step = 1;
+  while (2 * step <= num) step *= 2;
+  for (; step > 0; step /= 2) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (at[i] + step <= num && above(lists[i][at[i] + step - 1], x)) at[i] += step;
+  }
+  int sum = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) sum += at[i];
+  return sum;
+}
+
+template <int DT, int kPer>
 __global__ void __launch_bounds__(kThreads) tm_beam_rows_kernel(BeamParams p) {
-  __shared__ uint64_t s_list[kWaves][kSeg];
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int64_t unit = (int64_t)blockIdx.x * kWaves + wave;
-  if (unit >= (int64_t)p.rows * p.segs) return;
+  extern __shared__ uint64_t s_lists[];  // [kWaves][num * kPer]
+  __shared__ uint64_t s_best[kWaves][kMaxNum];
+  __shared__ double s_sum[kWaves];
+  __shared__ float s_top[kWaves];
+  __shared__ int s_found[kWaves];
+  __shared__ double s_powers[64];
+  const int tid = threadIdx.x, lane = tid & 63, num = p.num;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t unit = blockIdx.x;
   const int row = (int)(unit / p.segs), seg = (int)(unit - (int64_t)row * p.segs);
   if (p.finished != nullptr && p.finished[row]) return;
-  const int base = seg * kSeg;
+  const int base = (seg * kWaves + wave) * 64 * kPer;
+  uint64_t* const list = s_lists + wave * num * kPer;
   float x[kPer];
-  fetch<DT>(p, row, base, x);
+  fetch<DT, kPer>(p, row, base, x);
+  if (tid < 64) s_powers[tid] = kPowers[tid];
   float top = x[0];
-  uint64_t best = 0;
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) {
-    top = fmaxf(top, x[e]);
-    const uint64_t k = key_of(x[e], base + index_of<DT>(e));
-    best = k > best ? k : best;
-  }
+  for (int e = 1; e < kPer; ++e) top = fmaxf(top, x[e]);
+  int at = 0;  // of the lane's largest, the lowest index
+#pragma unroll
+  for (int e = kPer - 1; e >= 0; --e) at = x[e] == top ? index_of<DT>(e) : at;
+  const uint64_t best = key_of(top, base + at);
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-  uint64_t* const out = p.lists + unit * p.num;
-  if (top == -INFINITY) {  // nothing here: no candidate, and no weight
-    if (lane < p.num) out[lane] = 0;
-    if (lane == 0) {
-      p.sums[unit] = 0.0;
-      p.tops[unit] = top;
-    }
-    return;
-  }
-  // (an infinite largest logit weighs 1, and all finite ones nothing)
-  double sum = 0.0;
-#pragma unroll
-  for (int e = 0; e < kPer; ++e)
-    sum += x[e] == top ? 1.0 : exp((double)x[e] - (double)top);
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-  if (lane == 0) {
-    p.sums[unit] = sum;
-    p.tops[unit] = top;
-  }
-  // the num-th largest of the lanes' largest, and what reaches it
-  const uint64_t at = __ballot(rank_in_wave(best, 64) == p.num - 1);
-  const uint64_t least = lane_of(best, __ffsll((unsigned long long)at) - 1);
+  __syncthreads();
   int n = 0;
+  double sum = 0.0;
+  if (top > -INFINITY) {  // (else no candidate, and no weight)
+    double part[2] = {0.0, 0.0};
+    if (top < INFINITY) {
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) {
-    const uint64_t k = key_of(x[e], base + index_of<DT>(e));
-    const bool in = k >= least && x[e] > -INFINITY;
-    const uint64_t who = __ballot(in);
-    if (in) s_list[wave][n + lanes_before(who)] = k;
-    n += __popcll(who);
-  }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  if (n <= 64) {
-    const uint64_t k = lane < n ? s_list[wave][lane] : 0;
-    const int rank = rank_in_wave(k, n);
-    if (lane < n && rank < p.num) out[rank] = k;
-  } else {
-    for (int i = lane; i < n; i += 64) {
-      const uint64_t k = s_list[wave][i];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += s_list[wave][j] > k ? 1 : 0;
-      if (rank < p.num) out[rank] = k;
+      for (int e = 0; e < kPer; ++e)
+        part[e & 1] += exp_of((double)x[e] - (double)top, s_powers);
+    } else {  // infinite ones weigh 1, and all finite ones nothing
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) part[e & 1] += x[e] == top ? 1.0 : 0.0;
+    }
+    sum = part[0] + part[1];
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+    // the num-th largest of the lanes' largest, and what reaches it
+    const uint64_t least = least_of(best, top, num);
+    const float least_logit = float_of((uint32_t)(least >> 32));
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      if (!__any(x[e] >= least_logit)) continue;
+      const uint64_t k = key_of(x[e], base + index_of<DT>(e));
+      const bool in = k >= least && x[e] > -INFINITY;
+      const uint64_t who = __ballot(in);
+      if (in) list[n + lanes_before(who)] = k;
+      n += __popcll(who);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (n <= 64) {
+      const uint64_t k = lane < n ? list[lane] : 0;
+      const int rank = rank_in_wave(k, n);
+      if (lane < n && rank < num) s_best[wave][rank] = k;
+    } else {
+      for (int i = lane; i < n; i += 64) {
+        const uint64_t k = list[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += list[j] > k ? 1 : 0;
+        if (rank < num) s_best[wave][rank] = k;
+      }
     }
   }
-  if (lane >= n && lane < p.num) out[lane] = 0;
+  n = min(n, num);
+  if (lane >= n && lane < num) s_best[wave][lane] = 0;
+  if (lane == 0) {
+    s_sum[wave] = sum;
+    s_top[wave] = top;
+    s_found[wave] = n;
+  }
+  __syncthreads();
+  // the waves' lists and sums as one
+  if (tid < kWaves) {
+    float most = s_top[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) most = fmaxf(most, s_top[w]);
+    const float own = s_top[tid];
+    double all = own == most        ? s_sum[tid]
+                 : most == INFINITY ? 0.0
+                                    : s_sum[tid] * exp_of((double)own - (double)most, s_powers);
+#pragma unroll
+    for (int d = 1; d < kWaves; d <<= 1) all += __shfl_xor(all, d);
+    if (tid == 0) {
+      p.sums[unit] = all;
+      p.tops[unit] = most;
+    }
+  }
+  uint64_t* const out = p.lists + unit * num;
+  if (lane < n) {
+    const uint64_t k = s_best[wave][lane];
+    const uint64_t* const lists[kWaves] = {s_best[0], s_best[1], s_best[2], s_best[3]};
+    const int rank = above_in<kWaves>(lists, num, k, [](uint64_t a, uint64_t b) { return a > b; });
+    if (rank < num) out[rank] = k;
+  }
+  int found = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) found += s_found[w];
+  if (tid >= found && tid < num) out[tid] = 0;
 }
 
 // A candidate: ordered bits of its score, then the beam (inverted), the logit's ordered
@@ -211,26 +328,16 @@ __device__ __forceinline__ Cand cand_of(double score, int beam, uint32_t logit, 
 }
 
 struct JoinShared {
-  Cand pool[kMaxNum + 1][kMaxNum];  // sorted lists; the last is the best so far
+  Cand pool[kMaxNum * (kMaxNum + 1) / 2 + kMaxNum];
   Cand heads[kJoin / 64][kMaxNum];  // of each wave, sorted
+  Cand best[kMaxNum];               // so far, sorted
   double base[TM_MAX_BEAMS];        // score - log of the sum, -inf for a beam without candidates
+  double powers[64];
   float top[TM_MAX_BEAMS];
-  Cand least;
-  int used;                         // of the pool
+  Cand least;                       // the num-th of the heads
+  int list[kMaxNum];                // the lists in their heads' order
+  int count;                        // of the pool
 };
-
-// How many of the sorted list's n candidates are above c.
-__device__ __forceinline__ int above_in(const Cand* list, int n, const Cand& c) {
-  int lo = 0, hi = n;
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (above(list[mid], c))
-      lo = mid + 1;
-    else
-      hi = mid;
-  }
-  return lo;
-}
 
 __global__ void __launch_bounds__(kJoin) tm_beam_join_kernel(BeamParams p) {
   __shared__ JoinShared s;
@@ -239,7 +346,14 @@ __global__ void __launch_bounds__(kJoin) tm_beam_join_kernel(BeamParams p) {
   const int group = blockIdx.x, K = p.beams, num = p.num;
   const int64_t row0 = (int64_t)group * K;
   const int lists = K * p.segs;
+  const uint64_t* const from = p.lists + row0 * p.segs * num;
+  const auto higher = [](const Cand& a, const Cand& b) { return above(a, b); };
+  // (of a finished beam nothing is there, and what is read is not used)
+  uint64_t head_key = tid < lists ? from[(int64_t)tid * num] : 0;
 
+  if (tid < 64) s.powers[tid] = kPowers[tid];
+  if (tid < num) s.best[tid] = {0, 0};
+  __syncthreads();
   // each beam's sum over its segments, a wave a beam
   for (int b = wave; b < K; b += kJoin / 64) {
     const int64_t at = (row0 + b) * p.segs;
@@ -252,8 +366,10 @@ __global__ void __launch_bounds__(kJoin) tm_beam_join_kernel(BeamParams p) {
       for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
       for (int i = lane; i < p.segs; i += 64) {
         const float t = p.tops[at + i];
-        if (t > -INFINITY)
-          sum += p.sums[at + i] * (t == top ? 1.0 : exp((double)t - (double)top));
+        if (t == top)
+          sum += p.sums[at + i];
+        else if (t > -INFINITY && top < INFINITY)
+          sum += p.sums[at + i] * exp_of((double)t - (double)top, s.powers);
       }
 #pragma unroll
       for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
@@ -264,105 +380,89 @@ __global__ void __launch_bounds__(kJoin) tm_beam_join_kernel(BeamParams p) {
       s.base[b] = top > -INFINITY && score > -INFINITY ? score - log(sum) : -INFINITY;
     }
   }
-  // the finished beams, sorted, are the best so far
-  if (wave == 0) {
+  // the finished beams are the best so far
+  if (wave == 0 && p.finished != nullptr) {
     Cand c = {0, 0};
-    if (lane < K && p.finished != nullptr && p.finished[row0 + lane])
+    if (lane < K && p.finished[row0 + lane])
       c = cand_of(p.scores[row0 + lane], lane, 0, (uint32_t)p.pad_token);
     int rank = 0;
-    for (int l = 0; l < K; ++l) {
-      const Cand x = {lane_of(c.hi, l), lane_of(c.lo, l)};
-      rank += above(x, c) || (x.hi == 0 && c.hi == 0 && l < lane) ? 1 : 0;
-    }
-    if (lane < K && rank < num) s.pool[kMaxNum][rank] = c;
-    if (lane >= K && lane < num) s.pool[kMaxNum][lane] = {0, 0};
+    for (int l = 0; l < K; ++l) rank += above({lane_of(c.hi, l), lane_of(c.lo, l)}, c) ? 1 : 0;
+    if (c.hi != 0 && rank < num) s.best[rank] = c;
   }
 
+  auto cand = [&](int beam, uint64_t key) {
+    const double base = s.base[beam];
+    const float l = float_of((uint32_t)(key >> 32)), top = s.top[beam];
+    // (l - top is 0 for equal infinities)
+    const double score = l == top ? base : base + ((double)l - (double)top);
+    return key == 0 || !(base > -INFINITY)
+               ? Cand{0, 0}
+               : cand_of(score, beam, (uint32_t)(key >> 32), ~(uint32_t)key);
+  };
   for (int first = 0; first < lists; first += kJoin) {
-    if (tid == 0) s.used = 0;
-    __syncthreads();
-    // this thread's list and its head
-    const int list = first + tid;
+    const int now = min(lists - first, kJoin), waves = (now + 63) / 64;
+    if (tid < num) s.list[tid] = -1;
+    if (tid == 0) {
+      s.least = {0, 1};  // fewer heads than num: nothing lies below
+      s.count = 0;
+    }
+    __syncthreads();  // the sums, and the best so far
+    // the heads in order: within the waves, then over them
     Cand head = {0, 0};
-    int beam = 0;
-    const uint64_t* from = nullptr;
-    double base = -INFINITY;
-    float top = 0.0f;
-    auto cand = [&](uint64_t key) {
-      const float l = float_of((uint32_t)(key >> 32));
-      // (l - top is 0 for equal infinities)
-      const double score = l == top ? base : base + ((double)l - (double)top);
-      return key == 0 ? Cand{0, 0}
-                      : cand_of(score, beam, (uint32_t)(key >> 32), ~(uint32_t)key);
-    };
-    if (list < lists) {
-      beam = list / p.segs;
-      base = s.base[beam];
-      top = s.top[beam];
-      if (base > -INFINITY) {
-        from = p.lists + (row0 * p.segs + list) * num;
-        head = cand(from[0]);
+    int rank = num;
+    if (wave < waves) {
+      const int list = first + tid;
+      if (list < lists)
+        head = cand(list / p.segs, first == 0 ? head_key : from[(int64_t)list * num]);
+      rank = 0;
+      const int n = min(now - wave * 64, 64);
+      for (int l = 0; l < n; ++l) {
+        const Cand x = {lane_of(head.hi, l), lane_of(head.lo, l)};
+        rank += above(x, head) || (x.hi == 0 && head.hi == 0 && l < lane) ? 1 : 0;
       }
+      if (rank < num) s.heads[wave][rank] = head;
+      if (lane >= n && lane < num) s.heads[wave][lane] = {0, 0};
     }
-    // the waves' best heads, sorted
-    int rank = 0;
-#pragma unroll 4
-    for (int l = 0; l < 64; ++l) {
-      const Cand x = {lane_of(head.hi, l), lane_of(head.lo, l)};
-      rank += above(x, head) || (x.hi == 0 && head.hi == 0 && l < lane) ? 1 : 0;
-    }
-    if (rank < num) s.heads[wave][rank] = head;
-    if (tid == 0) s.least = {0, 1};  // fewer heads than num: all candidates
-    __syncthreads();
-    // the num-th largest of all heads
-    const int waves = (min(lists - first, kJoin) + 63) / 64;
-    if (rank < num && head.hi != 0) {
-      int r = 0;
-      for (int w = 0; w < waves; ++w) r += above_in(s.heads[w], num, head);
-      if (r == num - 1) s.least = head;
-    }
-    __syncthreads();
-    // the lists that reach it, num at most, up to where they do
-    if (head.hi != 0 && !above(s.least, head)) {
-      Cand* const to = s.pool[atomicAdd(&s.used, 1)];
-      for (int i = 0; i < num; ++i) {
-        const Cand c = i == 0 ? head : cand(from[i]);
-        const bool in = c.hi != 0 && !above(s.least, c);
-        to[i] = in ? c : Cand{0, 0};
-        if (!in) {
-          for (int j = i + 1; j < num; ++j) to[j] = {0, 0};
-          break;
+    if (waves > 1) {
+      __syncthreads();
+      if (rank < num && head.hi != 0)
+        for (int w = 0; w < waves; ++w) {
+          const Cand* const one[1] = {s.heads[w]};
+          if (w != wave) rank += above_in<1>(one, num, head, higher);
         }
+    }
+    if (rank < num && head.hi != 0) {
+      s.list[rank] = first + tid;
+      if (rank == num - 1) s.least = head;
+    }
+    __syncthreads();
+    // what can come out, in any order
+    const Cand least = s.least;
+    for (int e = tid; e < num * num + num; e += kJoin) {
+      const int r = e / num, i = e - r * num;
+      Cand c = {0, 0};
+      if (r == num) {
+        c = s.best[i];
+      } else if (r + i < num && s.list[r] >= 0) {
+        const int list = s.list[r];
+        c = cand(list / p.segs, from[(int64_t)list * num + i]);
+        if (above(least, c)) c = {0, 0};
       }
+      if (c.hi != 0) s.pool[atomicAdd(&s.count, 1)] = c;
     }
     __syncthreads();
-    // their ranks among each other and the best so far
-    const int used = s.used;
-    constexpr int kMine = (kMaxNum + 1) * kMaxNum / kJoin + 1;
-    Cand mine[kMine];
-    int place[kMine];
-#pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      const int at = i * kJoin + tid;
-      place[i] = -1;
-      if (at >= (used + 1) * num) continue;
-      const int li = at / num, l = li == used ? kMaxNum : li;
-      mine[i] = s.pool[l][at - li * num];
-      if (mine[i].hi == 0) continue;
-      int r = above_in(s.pool[kMaxNum], num, mine[i]);
-      for (int j = 0; j < used && r < num; ++j) r += above_in(s.pool[j], num, mine[i]);
-      place[i] = r < num ? r : -1;
+    const int count = s.count;
+    if (tid < num && tid >= count) s.best[tid] = {0, 0};
+    for (int e = tid; e < count; e += kJoin) {
+      const Cand c = s.pool[e];
+      int r = 0;
+      for (int j = 0; j < count; ++j) r += above(s.pool[j], c) ? 1 : 0;
+      if (r < num) s.best[r] = c;
     }
-    __syncthreads();
-    if (tid < num) s.pool[kMaxNum][tid] = {0, 0};
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kMine; ++i)
-      if (place[i] >= 0) s.pool[kMaxNum][place[i]] = mine[i];
     __syncthreads();
   }
   if (tid < num) {
-    const Cand c = s.pool[kMaxNum][tid];
+    const Cand c = s.best[tid];
     const int64_t at = (int64_t)group * num + tid;
     const bool none = c.hi == 0;
     p.out_scores[at] = none ? -INFINITY : (float)double_of(c.hi);
@@ -374,6 +474,8 @@ __global__ void __launch_bounds__(kJoin) tm_beam_join_kernel(BeamParams p) {
 
 // ---------------------------------------------------------------- reorder --
 
+constexpr int kReorderPieces = 4096;  // of a workgroup
+
 struct ReorderParams {
   const uint8_t* x;
   uint8_t* out;
@@ -383,25 +485,38 @@ struct ReorderParams {
   int beams;
 };
 
-// Rows of a group in pieces of T: the parents' rows into LDS, and from there to where they
-// go, so that out may be x.  A beam that goes on from itself, or whose parent is no beam of
-// the group, is copied only where out is not x.
+// Rows into an output of their own, in pieces of T.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) tm_reorder_kernel(ReorderParams p, int cols) {
-  __shared__ __attribute__((aligned(16))) uint8_t s_rows[kThreads * 16 * 16];
+__global__ void __launch_bounds__(kThreads) tm_reorder_kernel(ReorderParams p, int64_t pieces,
+                                                              int blocks) {
+  const int64_t row = (int)blockIdx.x / blocks;
+  const int64_t i = (int64_t)((int)blockIdx.x % blocks) * kThreads + threadIdx.x;
+  if (i >= pieces) return;
+  const int64_t group = row / p.beams;
+  const int own = (int)(row - group * p.beams);
+  const int b = p.parents[group * p.parents_stride + own];
+  const int64_t from = group * p.beams + (b < 0 || b >= p.beams ? own : b);
+  *reinterpret_cast<T*>(p.out + row * p.out_stride + i * (int64_t)sizeof(T)) =
+      *reinterpret_cast<const T*>(p.x + from * p.x_stride + i * (int64_t)sizeof(T));
+}
+
+// Rows within x: a workgroup takes `cols` pieces of a group's rows, those that are parents of
+// others into LDS, and from there to where they go.  A beam that goes on from itself, or
+// whose parent is no beam of the group, stays.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) tm_reorder_within_kernel(ReorderParams p, int cols) {
+  __shared__ __attribute__((aligned(16))) T rows[kReorderPieces];
   __shared__ int s_parent[TM_MAX_BEAMS];
   __shared__ int s_need[TM_MAX_BEAMS];
-  T* const rows = reinterpret_cast<T*>(s_rows);
   const int K = p.beams, tid = threadIdx.x;
   const int64_t group = blockIdx.y, row0 = group * K;
-  const bool same = p.out == p.x;
   if (tid < K) s_need[tid] = 0;
   __syncthreads();
   if (tid < K) {
     int b = p.parents[group * p.parents_stride + tid];
     if (b < 0 || b >= K) b = tid;
     s_parent[tid] = b;
-    if (!same || b != tid) s_need[b] = 1;
+    if (b != tid) s_need[b] = 1;
   }
   __syncthreads();
   const int64_t col0 = (int64_t)blockIdx.x * cols, all = p.width / (int64_t)sizeof(T);
@@ -415,7 +530,7 @@ __global__ void __launch_bounds__(kThreads) tm_reorder_kernel(ReorderParams p, i
   __syncthreads();
   for (int i = tid; i < K * cols; i += kThreads) {
     const int r = i / cols, c = i - r * cols, b = s_parent[r];
-    if (c < n && (!same || b != r))
+    if (c < n && b != r)
       *reinterpret_cast<T*>(p.out + (row0 + r) * p.out_stride + (col0 + c) * (int64_t)sizeof(T)) =
           rows[b * cols + c];
   }
@@ -425,23 +540,48 @@ __global__ void __launch_bounds__(kThreads) tm_reorder_kernel(ReorderParams p, i
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Logits of a lane, by the workgroups that many of them would leave; a lane's largest are
+// kept apart in LDS, `num` lanes' at most.
+int per_of(int64_t rows, int64_t V, int64_t num) {
+  return num <= 24 && rows * ceil_div(V, kThreads * kManyPer) >= 2 * 256 ? kManyPer : kFewPer;
+}
+
 int check_beams(int64_t G, int64_t K, int64_t V, int64_t num) {
   if (G < 0 || K < 1 || K > TM_MAX_BEAMS || num < 1 || num > kMaxNum || V < 1 ||
       V > TM_MAX_SAMPLE_VOCAB || G > TM_MAX_ROWS / K)
     return TM_ERR_SHAPE;
-  if (ceil_div(G * K * ceil_div(V, kSeg), kWaves) > UINT32_MAX / kThreads) return TM_ERR_SHAPE;
+  if (G * K * ceil_div(V, kThreads * kFewPer) > UINT32_MAX / kThreads) return TM_ERR_SHAPE;
   return TM_OK;
+}
+
+template <int DT>
+void launch_rows(const BeamParams& p, int per, hipStream_t st) {
+  const dim3 grid((unsigned)(p.rows * p.segs)), block(kThreads);
+  const size_t lds = (size_t)kWaves * p.num * per * sizeof(uint64_t);
+  if (per == kManyPer)
+    hipLaunchKernelGGL((tm_beam_rows_kernel<DT, kManyPer>), grid, block, lds, st, p);
+  else
+    hipLaunchKernelGGL((tm_beam_rows_kernel<DT, kFewPer>), grid, block, lds, st, p);
 }
 
 template <typename T>
 int launch_reorder(const ReorderParams& p, int64_t G, hipStream_t st) {
-  // columns of a workgroup: all rows of a group within its LDS
+  const int64_t pieces = p.width / (int64_t)sizeof(T);
+  const bool within = p.out == p.x;
+  // columns of a workgroup: all rows of a group within its LDS, and not more than a round
   int cols = kThreads;
-  while (cols * p.beams > kThreads * 16) cols /= 2;
-  const int64_t blocks = ceil_div(p.width / (int64_t)sizeof(T), cols);
-  if (blocks > UINT32_MAX / kThreads / G) return TM_ERR_SHAPE;  // a grid's threads in 32 bits
-  hipLaunchKernelGGL((tm_reorder_kernel<T>), dim3((unsigned)blocks, (unsigned)G), dim3(kThreads),
-                     0, st, p, cols);
+  while (cols > 16 && cols * p.beams > kThreads) cols /= 2;
+  while (cols * p.beams > kReorderPieces) cols /= 2;
+  const int64_t blocks = ceil_div(pieces, within ? cols : kThreads);
+  const int64_t rows = within ? G : G * p.beams;
+  if (blocks > UINT32_MAX / kThreads / rows) return TM_ERR_SHAPE;  // a grid's threads in 32 bits
+  const dim3 block(kThreads);
+  if (within)
+    hipLaunchKernelGGL((tm_reorder_within_kernel<T>), dim3((unsigned)blocks, (unsigned)G), block,
+                       0, st, p, cols);
+  else
+    hipLaunchKernelGGL((tm_reorder_kernel<T>), dim3((unsigned)(blocks * rows)), block, 0, st, p,
+                       pieces, (int)blocks);
   TM_HIP_CHECK_LAUNCH();
   return TM_OK;
 }
@@ -452,7 +592,7 @@ extern "C" int tm_beam_workspace(int64_t G, int64_t K, int64_t V, int64_t num, i
   const int rc = check_beams(G, K, V, num);
   if (rc) return rc;
   if (bytes == nullptr) return TM_ERR_ARG;
-  *bytes = G * K * ceil_div(V, kSeg) * (8 * num + 8 + 4);
+  *bytes = G * K * ceil_div(V, kThreads * per_of(G * K, V, num)) * (8 * num + 8 + 4);
   return TM_OK;
 }
 
@@ -481,7 +621,8 @@ extern "C" int tm_beam_select(const void* logits, int dtype, int64_t G, int64_t 
   p.rows = (int)(G * K);
   p.beams = (int)K;
   p.vocab = (int)V;
-  p.segs = (int)ceil_div(V, kSeg);
+  const int per = per_of(G * K, V, num);
+  p.segs = (int)ceil_div(V, kThreads * per);
   p.num = (int)num;
   const int64_t units = (int64_t)p.rows * p.segs;
   p.lists = (uint64_t*)workspace;
@@ -491,14 +632,13 @@ extern "C" int tm_beam_select(const void* logits, int dtype, int64_t G, int64_t 
   p.out_scores = out_scores;
   p.parents = parents;
   p.tokens = tokens;
-  const dim3 grid((unsigned)ceil_div(units, kWaves)), block(kThreads);
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == TM_DTYPE_F32)
-    hipLaunchKernelGGL((tm_beam_rows_kernel<TM_DTYPE_F32>), grid, block, 0, st, p);
+    launch_rows<TM_DTYPE_F32>(p, per, st);
   else if (dtype == TM_DTYPE_F16)
-    hipLaunchKernelGGL((tm_beam_rows_kernel<TM_DTYPE_F16>), grid, block, 0, st, p);
+    launch_rows<TM_DTYPE_F16>(p, per, st);
   else
-    hipLaunchKernelGGL((tm_beam_rows_kernel<TM_DTYPE_BF16>), grid, block, 0, st, p);
+    launch_rows<TM_DTYPE_BF16>(p, per, st);
   hipLaunchKernelGGL(tm_beam_join_kernel, dim3((unsigned)G), dim3(kJoin), 0, st, p);
   TM_HIP_CHECK_LAUNCH();
   return TM_OK;

@@ -5,8 +5,8 @@
 // of the group) pairs,
 //   mass[j] += sum over the rows that see key j of exp(s_rj - m_r) / l_r,
 // with s = scale q . k, m_r the largest of a row's scores and l_r the sum of its
-// exponentials.  Two launches: m and l of every row, over ranges of keys; then, key tile
-// by key tile, the scores again and their sums over the rows.  K is read twice, from L2 the
+// exponentials.  First m and l of every row, over ranges of keys; then, 32 keys a wave, the
+// scores again and their sums over the rows.  K is read twice, from L2 the
 // second time where a head's keys fit it (a head's workgroups share an XCD); the
 // scores of many rows would be far more to store than to compute twice.  All in fp32; the
 // order of the sums is fixed.
@@ -19,6 +19,7 @@
 // ordered bits of the weights), a second launch moves.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "attn_tile.h"
 
@@ -26,6 +27,10 @@ namespace {
 
 struct MassParams : PromptParams {
   float2* row_stats;      // (m in base 2, l) [chunks][kvh][rows]
+  float* row_consts;      // -(m + log2 l) [kvh][rows in whole stages], or NULL: the sums'
+                          // workgroups take row_stats
+  float* parts;           // [splits][kvh][keys], or NULL: the mass itself
+  int splits;             // of a tile's rows
   const float* before;    // [kvh, before_stride], or NULL
   int64_t before_stride;
   float* mass;            // [kvh, mass_stride]
@@ -65,6 +70,13 @@ __device__ __forceinline__ void join_stats(float& m, float& l, float m1, float l
   m = mn;
 }
 
+// What a score s in base 2 takes to become a weight, 2^(s + c); -inf, for nothing, of a row
+// whose scores are all -inf.  As one number it is off by half a step below 2^6: 1.3e-6 of a
+// weight.
+__device__ __forceinline__ float const_of(float m, float l) {
+  return l == 0.0f ? -INFINITY : -(m + __builtin_amdgcn_logf(l));
+}
+
 // Rows 128 a tile, 32 a wave, that share the stages of a range of keys.
 template <int DT, int HD>
 __global__ void __launch_bounds__(kThreads, 2) tm_mass_stats_kernel(MassParams p) {
@@ -95,9 +107,16 @@ __global__ void __launch_bounds__(kThreads, 2) tm_mass_stats_kernel(MassParams p
     }
   }
   const float l = r.l + __shfl_xor(r.l, 32);
-  if (at.ok && (threadIdx.x & 32) == 0)
-    p.row_stats[((int64_t)(at_item % p.chunks) * p.kvh + kvhead) * it.q_len * p.group + at.row] =
+  const int rows = it.q_len * p.group;
+  if ((threadIdx.x & 32) != 0) return;
+  if (p.row_consts != nullptr && p.chunks == 1) {
+    const int whole = (rows + kKeys - 1) / kKeys * kKeys;
+    if (at.row < whole)
+      p.row_consts[(int64_t)kvhead * whole + at.row] = at.ok ? const_of(r.m, l) : -INFINITY;
+  } else if (at.ok) {
+    p.row_stats[((int64_t)(at_item % p.chunks) * p.kvh + kvhead) * rows + at.row] =
         float2{r.m, l};
+  }
 }
 
 // Up to 32 rows: the waves take the stages in turn.
@@ -139,133 +158,157 @@ __global__ void __launch_bounds__(kThreads, 2) tm_mass_stats_few_kernel(MassPara
       float2{m, sum};
 }
 
-// Sums over the rows, 64 keys a wave or (SHARE 4) a workgroup, whose waves take the tiles of
-// 32 rows in turn.  K stays in registers, the queries stream through.
-template <int DT, int HD, int SHARE>
-__global__ void __launch_bounds__(kThreads, 2) tm_mass_sum_kernel(MassParams p) {
-  __shared__ float s_sum[4][64];
-  const int lane = threadIdx.x & 63, half = lane >> 5, c32 = lane & 31;
-  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int kvhead = (int)blockIdx.x % p.kvh;
-  const int unit = (int)blockIdx.x / p.kvh;
-  const int first = (SHARE == 1 ? unit * 4 + wave : unit) * kKeys;
+// The constant of a row from its ranges, P neighbouring lanes a row.
+__device__ __forceinline__ float joined(const float2* st, int64_t step, int chunks, int P) {
+  const int part = (int)threadIdx.x & (P - 1);
+  float m = -INFINITY, l = 0.0f;
+#pragma unroll 4
+  for (int c = part; c < chunks; c += P) m = fmaxf(m, st[c * step].x);
+  for (int d = 1; d < P; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+  const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll 4
+  for (int c = part; c < chunks; c += P) {
+    const float2 x = st[c * step];
+    l = fmaf(x.y, __builtin_amdgcn_exp2f(x.x - ref), l);
+  }
+  for (int d = 1; d < P; d <<= 1) l += __shfl_xor(l, d);
+  return const_of(m, l);
+}
+
+// The constants of all rows, and -inf up to whole stages: where the rows are too many for
+// every workgroup of the sums to do it again.
+__global__ void __launch_bounds__(kThreads) tm_mass_rows_kernel(MassParams p, int rows, int whole) {
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (i >= (int64_t)p.kvh * whole) return;
+  const int kvhead = (int)(i / whole), row = (int)(i - (int64_t)kvhead * whole);
+  p.row_consts[i] = row < rows ? joined(p.row_stats + (int64_t)kvhead * rows + row,
+                                        (int64_t)p.kvh * rows, p.chunks, 1)
+                               : -INFINITY;
+}
+
+constexpr int kOwnRows = 1024;  // whose constants a workgroup of the sums makes by itself
+
+// Sums over the rows: a wave has 32 keys, one a column, and 64 rows at a time come by in LDS,
+// for all waves.  A lane's products with a stage belong to its key, so they are summed in
+// its registers.  OWN: the workgroup joins the rows' ranges itself.
+template <int DT, int HD, int WAVES, bool OWN>
+__global__ void __launch_bounds__(64 * WAVES, WAVES == 8 ? 4 : 2) tm_mass_sum_kernel(MassParams p) {
+  typedef Shape<HD> S;
+  constexpr int kLoads = S::kTile / (1024 * WAVES);
+  __shared__ __attribute__((aligned(1024))) uint8_t s_q[2][S::kTile];
+  __shared__ __attribute__((aligned(16))) float s_const[OWN ? kOwnRows : 2 * kKeys];
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, c32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kvhead = (int)blockIdx.x % p.kvh, rest = (int)blockIdx.x / p.kvh;
+  const int split = rest % p.splits;
+  const int first = rest / p.splits * (32 * WAVES);  // the keys with the most rows first
   const int rows = p.q_len * p.group, past = p.k_len - p.q_len;
-  u32x4_t kf[2][HD / 16];
-  float acc[2][16];
+  const int whole = (rows + kKeys - 1) / kKeys * kKeys;
+  const int key = first + 32 * wave + c32;
+  // the key's first row, and that of the workgroup's last key
+  const int seen = max(min(key, p.k_len - 1) - past, 0) * p.group;
+  const int all = max(min(first + 32 * WAVES, p.k_len) - 1 - past, 0) * p.group;
+  const int stage0 = max(first - past, 0) * p.group / kKeys;
+  const int per = (whole / kKeys - stage0 + p.splits - 1) / p.splits;
+  const int begin = stage0 + split * per, end = min(begin + per, whole / kKeys);
+  // row `in` of a stage, of the loads of this wave
+  auto load = [&](int stage, uint8_t* tile) TM_INLINE {
 #pragma unroll
-  for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-    for (int x = 0; x < 16; ++x) acc[kt][x] = 0.0f;
-  const int tiles = (rows + 31) / 32;
-  // the first tile of rows of which one sees the first key
-  const int tile0 = first > past ? (first - past) * p.group / 32 : 0;
-  const int mine = SHARE == 1 ? 0 : wave;
-  if (first < p.k_len && tile0 + mine < tiles) {
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      const int key = min(first + 32 * kt + c32, p.k_len - 1);
-      const int pg = min(max(p.table[key >> p.page_shift], 0), p.cache_pages - 1);
+    for (int i = 0; i < kLoads; ++i) {
+      const int in = (wave * kLoads + i) * S::kKeysPerLoad + lane / S::kChunks;
+      const int row = min(stage * kKeys + in, rows - 1);
+      const int token = row / p.group;
+      const uint16_t* const qr = p.q + (int64_t)token * p.q_stride +
+                                 (int64_t)(kvhead * p.group + row - token * p.group) * HD +
+                                 (((lane & (S::kChunks - 1)) ^ S::swz_k(in)) * 8);
+      __builtin_amdgcn_global_load_lds((glb_void*)qr,
+                                       (lds_void*)(tile + (wave * kLoads + i) * 1024), 16, 0, 0);
+    }
+  };
+  Rows<HD> r;
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (begin < end) {
+    load(begin, s_q[0]);
+    {
+      const int at = min(key, p.k_len - 1);
+      const int pg = min(max(p.table[at >> p.page_shift], 0), p.cache_pages - 1);
       const uint16_t* const kr = p.k + (int64_t)pg * p.stride_page +
-                                 (int64_t)(key & ((1 << p.page_shift) - 1)) * p.k_stride +
+                                 (int64_t)(at & ((1 << p.page_shift) - 1)) * p.k_stride +
                                  kvhead * HD + 8 * half;
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks)
-        kf[kt][ks] = *reinterpret_cast<const u32x4_t*>(kr + 16 * ks);
+        r.q[ks] = *reinterpret_cast<const u32x4_t*>(kr + 16 * ks);
     }
-    struct Tile {
-      u32x4_t q[HD / 16];
-      float m, inv;
-      int seen;
-    };
-    auto read = [&](int tile, Tile& t) TM_INLINE {
-      const int row = tile * 32 + c32;
-      const bool ok = row < rows;
-      const int token = ok ? row / p.group : 0;
-      const int head = kvhead * p.group + (ok ? row - token * p.group : 0);
-      const uint16_t* const qr = p.q + (int64_t)token * p.q_stride + (int64_t)head * HD + 8 * half;
-#pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks)
-        t.q[ks] = *reinterpret_cast<const u32x4_t*>(qr + 16 * ks);
-      float m = -INFINITY, l = 0.0f;
-      if (ok) {
-        const float2* const st = p.row_stats + (int64_t)kvhead * rows + row;
-        const int64_t step = (int64_t)p.kvh * rows;
-        const float2 a = st[0];
-        m = a.x;
-        l = a.y;
-        for (int c = 1; c < p.chunks; ++c) {
-          const float2 b = st[c * step];
-          join_stats(m, l, b.x, b.y);
-        }
+    const float* const consts = p.row_consts + (int64_t)kvhead * whole;
+    float next = 0.0f;
+    if constexpr (OWN) {
+      int P = 1;  // lanes a row
+      while (P < 64 && 2 * P * rows <= 64 * WAVES) P *= 2;
+      for (int row = tid / P; row < whole; row += 64 * WAVES / P) {
+        float c = -INFINITY;
+        if (row < rows)
+          c = joined(p.row_stats + (int64_t)kvhead * rows + row, (int64_t)p.kvh * rows, p.chunks,
+                     P);
+        if ((tid & (P - 1)) == 0) s_const[row] = c;
       }
-      // (a row of scores -inf gives nothing)
-      t.m = l == 0.0f ? 0.0f : -m;
-      t.inv = l == 0.0f ? 0.0f : 1.0f / l;
-      t.seen = ok ? past + token : -1;
-    };
-    auto add = [&](int tile, const Tile& t) TM_INLINE {
-      f32x16_t sc[2];
-#pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks)
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-          const f32x16_t zero = {};
-          sc[kt] = mfma32<DT>(kf[kt][ks], t.q[ks], ks == 0 ? zero : sc[kt]);
-        }
-      // masked where some row of the tile does not see some key
-      if (tile * 32 + 32 > rows || past + tile * 32 / p.group < first + kKeys - 1)
-        mask_scores(sc, t.seen - first - 4 * half);
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int x = 0; x < 16; ++x)
-          acc[kt][x] = fmaf(__builtin_amdgcn_exp2f(fmaf(sc[kt][x], p.scale_log2, t.m)), t.inv,
-                            acc[kt][x]);
-    };
-    Tile a, b;
-    int t = tile0 + mine;
-    read(t, a);
-    for (; t < tiles; t += 2 * SHARE) {
-      if (t + SHARE < tiles) read(t + SHARE, b);
-      add(t, a);
-      if (t + SHARE < tiles) {
-        if (t + 2 * SHARE < tiles) read(t + 2 * SHARE, a);
-        add(t + SHARE, b);
+    } else if (wave == 0) {
+      next = consts[begin * kKeys + lane];
+    }
+    auto step = [&](int stage, int turn) TM_INLINE {
+      wait_vm<0>();
+      if (!OWN && wave == 0) s_const[turn * kKeys + lane] = next;
+      tm_lds_barrier();
+      if (stage + 1 < end) {
+        load(stage + 1, s_q[turn ^ 1]);
+        if (!OWN && wave == 0) next = consts[(stage + 1) * kKeys + lane];
       }
+      products<DT, HD, false, true>(s_q[turn], s_q[turn], r);
+      const float* const c = s_const + (OWN ? stage : turn) * kKeys + 4 * half;
+      // rows that do not see the lane's key give 0, whatever their constant
+      const int hidden = seen - stage * kKeys - 4 * half;
+      auto weights = [&](auto masked) TM_INLINE {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const f32x4_t cc = *reinterpret_cast<const f32x4_t*>(c + 32 * kt + 8 * j);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const float e =
+                  __builtin_amdgcn_exp2f(fmaf(r.sc[kt][4 * j + x], p.scale_log2, cc[x]));
+              sum[x] += !decltype(masked)::value || 32 * kt + 8 * j + x >= hidden ? e : 0.0f;
+            }
+          }
+      };
+      if (stage * kKeys < all)
+        weights(std::true_type{});
+      else
+        weights(std::false_type{});
+    };
+    for (int stage = begin; stage < end; stage += 2) {
+      step(stage, 0);
+      if (stage + 1 < end) step(stage + 1, 1);
     }
   }
-  // over the 32 columns of each half: lane x of a half gets key x's sum, kt 0 and 1
-  float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-  for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-    for (int x = 0; x < 16; ++x) {
-      float v = acc[kt][x];
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) v += __shfl_xor(v, d);
-      sum[kt] = c32 == x ? v : sum[kt];
-    }
-  const int in = 8 * (c32 >> 2) + 4 * half + (c32 & 3);  // the key that a lane below 16 has
-  auto store = [&](int key, float v) TM_INLINE {
-    if (key >= p.k_len) return;
+  float v = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  v += __shfl_xor(v, 32);
+  if (half != 0 || key >= p.k_len) return;
+  if (p.parts != nullptr) {
+    p.parts[((int64_t)split * p.kvh + kvhead) * p.k_len + key] = v;
+  } else {
     if (p.before != nullptr) v += p.before[kvhead * p.before_stride + key];
     p.mass[kvhead * p.mass_stride + key] = v;
-  };
-  if constexpr (SHARE == 1) {
-    if (c32 < 16) {
-      store(first + in, sum[0]);
-      store(first + 32 + in, sum[1]);
-    }
-  } else {
-    if (c32 < 16) {
-      s_sum[wave][in] = sum[0];
-      s_sum[wave][32 + in] = sum[1];
-    }
-    __syncthreads();
-    if (threadIdx.x < 64)
-      store(first + lane,
-            (s_sum[0][lane] + s_sum[1][lane]) + (s_sum[2][lane] + s_sum[3][lane]));
   }
+}
+
+// The splits' sums, in their order.
+__global__ void __launch_bounds__(kThreads) tm_mass_join_kernel(MassParams p) {
+  const int key = (int)(blockIdx.x * kThreads + threadIdx.x), kvhead = blockIdx.y;
+  if (key >= p.k_len) return;
+  float v = 0.0f;
+  for (int s = 0; s < p.splits; ++s) v += p.parts[((int64_t)s * p.kvh + kvhead) * p.k_len + key];
+  if (p.before != nullptr) v += p.before[kvhead * p.before_stride + key];
+  p.mass[kvhead * p.mass_stride + key] = v;
 }
 
 // --------------------------------------------------------------- eviction --
@@ -288,6 +331,7 @@ struct EvictParams {
   int recorded, next, recent, sinks;
   float* mass_out;                // [heads][columns]
   int32_t* positions_out;         // [heads][keep]
+  int fused;                      // the selecting workgroup moves the keys, too
   int32_t* counts;                // [heads]: of the moves
   int32_t *holes, *movers;        // [heads][moves]
 };
@@ -313,26 +357,229 @@ struct BlockRank {
   }
 };
 
+// What a head's workgroup reads.
+struct Head {
+  const float* mass;
+  const int32_t* pos;
+  const EvictParams& p;
+  int index;
+  __device__ __forceinline__ Head(const EvictParams& p_) : p(p_), index((int)blockIdx.x) {
+    const int layer = index / p.kvh, kvhead = index - layer * p.kvh;
+    mass = p.mass + layer * p.mass_layer + kvhead * p.mass_head;
+    pos = p.positions + layer * p.pos_layer + kvhead * p.pos_head;
+  }
+  __device__ __forceinline__ int position(int s) const {
+    return s < p.recorded ? pos[s] : p.next - p.length + s;
+  }
+  // larger: kept sooner.  NaN last; what is kept in any case first.
+  __device__ __forceinline__ uint32_t key(int s) const { return key(mass[s], position(s)); }
+  __device__ __forceinline__ uint32_t key(float m, int at) const {
+    if (at < p.sinks || at >= p.next - p.recent) return 0xffffffffu;
+    if (m != m) return 0u;
+    const uint32_t u = __float_as_uint(m + 0.0f);
+    return u ^ (uint32_t)(((int32_t)u >> 31) | 0x80000000);
+  }
+  // Where a slot of the head lies in k and v.
+  __device__ __forceinline__ int64_t slot(int s) const {
+    const int layer = index / p.kvh, kvhead = index - layer * p.kvh;
+    const int pg = min(max(p.table[s >> p.page_shift], 0), p.cache_pages - 1);
+    return (int64_t)layer * p.stride_layer + (int64_t)kvhead * p.stride_head +
+           (int64_t)pg * p.stride_page +
+           (int64_t)(s & ((1 << p.page_shift) - 1)) * p.stride_slot;
+  }
+};
+
+// The sum of the waves' counts before this wave's, and of all.
+template <int WAVES>
+__device__ __forceinline__ int sum_waves(int* waves, int mine, int* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (lane == 0) waves[wave] = mine;
+  __syncthreads();
+  int before = 0, sum = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    const int x = waves[w];
+    before += w < wave ? x : 0;
+    sum += x;
+  }
+  *total = sum;
+  return before;
+}
+__device__ __forceinline__ int lanes_before(uint64_t who) {
+  return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32),
+                                        __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+}
+// Inclusive sum over the lanes of a wave.
+__device__ __forceinline__ int scan_wave(int v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int up = __shfl_up(v, d);
+    v += lane >= d ? up : 0;
+  }
+  return v;
+}
+
+// Selection with a head's keys in registers, PER a thread: the threshold from four
+// histograms of eight bits.  A wave owns consecutive slots, so that ranks need one sum over the
+// waves.  Few waves where few keys are: what a step costs is its barriers.
+template <int PER, int THREADS>
+__global__ void __launch_bounds__(THREADS) tm_evict_held_kernel(EvictParams p) {
+  constexpr int kWaves = THREADS / 64, kMost = PER * THREADS / 2;  // moves
+  __shared__ uint32_t s_bins[4][256];
+  __shared__ int s_scan[4][4];
+  __shared__ int s_rank[2][kWaves];
+  __shared__ uint32_t s_digit[4];
+  __shared__ int s_need[4];
+  __shared__ uint16_t s_hole[kMost], s_mover[kMost];
+  static_assert(PER * THREADS <= 65536, "slots in 16 bits");
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const Head head(p);
+  const int first = wave * (64 * PER) + lane;  // slots first + 64 i
+  uint32_t key[PER];
+  float mass[PER];
+  int pos[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int s = min(first + 64 * i, p.length - 1);
+    mass[i] = p.length > 0 ? head.mass[s] : 0.0f;
+    pos[i] = p.length > 0 ? head.position(s) : 0;
+  }
+  for (int i = tid; i < 4 * 256; i += THREADS) s_bins[i >> 8][i & 255] = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) key[i] = head.key(mass[i], pos[i]);
+  // the keep-th largest key, and how many of its equals stay
+  uint32_t t = 0;
+  int need = p.keep;
+  if (p.keep < p.length && p.keep > 0) {
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      const int shift = 24 - 8 * d;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (first + 64 * i < p.length && (d == 0 || (key[i] >> (shift + 8)) == t))
+          atomicAdd(&s_bins[d][(key[i] >> shift) & 255], 1u);
+      __syncthreads();
+      // from the largest digit down, one a thread of the first four waves
+      int own = 0, upto = 0;
+      if (tid < 256) {
+        own = (int)s_bins[d][255 - tid];
+        upto = scan_wave(own);
+        if (lane == 63) s_scan[d][wave] = upto;
+      }
+      __syncthreads();
+      if (tid < 256) {
+        for (int w = 0; w < wave; ++w) upto += s_scan[d][w];
+        if (upto >= need && upto - own < need) {
+          s_digit[d] = 255 - tid;
+          s_need[d] = need - (upto - own);
+        }
+      }
+      __syncthreads();
+      t = (t << 8) | s_digit[d];
+      need = s_need[d];
+    }
+  }
+  // which stay: above t, and the first `need` of its equals
+  uint32_t kept = 0;
+  {
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      mine += __popcll(__ballot(first + 64 * i < p.length && key[i] == t));
+    int all;
+    int at = sum_waves<kWaves>(s_rank[0], mine, &all);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bool in = first + 64 * i < p.length, equal = in && key[i] == t;
+      const uint64_t who = __ballot(equal);
+      if (in && p.keep > 0 && (key[i] > t || (equal && at + lanes_before(who) < need)))
+        kept |= 1u << i;
+      at += __popcll(who);
+    }
+  }
+  // holes below keep, movers behind it, both in the slots' order
+  int mine = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int s = first + 64 * i;
+    const bool stays = kept >> i & 1;
+    mine += __popcll(__ballot(s < p.length && s < p.keep && !stays));
+    mine += __popcll(__ballot(stays && s >= p.keep)) << 16;
+  }
+  int all;
+  int at = sum_waves<kWaves>(s_rank[1], mine, &all);
+  float* const mass_out = p.mass_out + (int64_t)head.index * p.columns;
+  int32_t* const pos_out = p.positions_out + (int64_t)head.index * p.keep;
+  int rank[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int s = first + 64 * i;
+    const bool stays = kept >> i & 1;
+    const bool hole = s < p.length && s < p.keep && !stays, mover = stays && s >= p.keep;
+    const uint64_t holes = __ballot(hole), movers = __ballot(mover);
+    if (hole) s_hole[(at & 0xffff) + lanes_before(holes)] = (uint16_t)s;
+    rank[i] = mover ? (at >> 16) + lanes_before(movers) : -1;
+    if (mover) s_mover[rank[i]] = (uint16_t)s;
+    at += __popcll(holes) + (__popcll(movers) << 16);
+    if (stays && !mover) {
+      mass_out[s] = mass[i];
+      pos_out[s] = pos[i];
+    }
+  }
+  for (int s = p.keep + tid; s < p.columns; s += THREADS) mass_out[s] = 0.0f;
+  const int moves = all >> 16;  // (as many as holes)
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (rank[i] >= 0) {
+      const int to = s_hole[rank[i]];
+      mass_out[to] = mass[i];
+      pos_out[to] = pos[i];
+    }
+  if (!p.fused) {
+    if (tid == 0) p.counts[head.index] = moves;
+    for (int i = tid; i < moves; i += THREADS) {
+      p.holes[(int64_t)head.index * p.moves + i] = s_hole[i];
+      p.movers[(int64_t)head.index * p.moves + i] = s_mover[i];
+    }
+    return;
+  }
+  const int pieces = p.row_bytes / 16, all_pieces = moves * pieces;
+  constexpr int kAhead = 4;  // pieces of a thread under way
+  for (int i0 = tid; i0 < all_pieces; i0 += kAhead * THREADS) {
+    int64_t from[kAhead], to[kAhead];
+    u32x4_t k[kAhead], v[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = min(i0 + u * THREADS, all_pieces - 1);  // (the last one again and again)
+      const int move = i / pieces, piece = (i - move * pieces) * 16;
+      from[u] = head.slot(s_mover[move]) + piece;
+      to[u] = head.slot(s_hole[move]) + piece;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      k[u] = *reinterpret_cast<const u32x4_t*>(p.k + from[u]);
+      v[u] = *reinterpret_cast<const u32x4_t*>(p.v + from[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      *reinterpret_cast<u32x4_t*>(p.k + to[u]) = k[u];
+      *reinterpret_cast<u32x4_t*>(p.v + to[u]) = v[u];
+    }
+  }
+}
+
+// Selection of any number of keys, read again for each pass: the threshold from histograms
+// of 11, 11 and 10 bits.
 __global__ void __launch_bounds__(kSelect) tm_evict_select_kernel(EvictParams p) {
   __shared__ uint32_t s_bins[kBins];
   __shared__ int s_waves[kSelect / 64];
   __shared__ uint32_t s_prefix;
   __shared__ int s_need;
-  const int tid = threadIdx.x, head = blockIdx.x;
-  const int layer = head / p.kvh, kvhead = head - layer * p.kvh;
-  const float* const mass = p.mass + layer * p.mass_layer + kvhead * p.mass_head;
-  const int32_t* const pos =
-      p.positions == nullptr ? nullptr : p.positions + layer * p.pos_layer + kvhead * p.pos_head;
-  auto position = [&](int s) { return s < p.recorded ? pos[s] : p.next - p.length + s; };
-  // larger: kept sooner.  NaN last; what is kept in any case first.
-  auto key_of = [&](int s) {
-    const int at = position(s);
-    if (at < p.sinks || at >= p.next - p.recent) return 0xffffffffu;
-    const float m = mass[s];
-    if (m != m) return 0u;
-    const uint32_t u = __float_as_uint(m + 0.0f);
-    return u ^ (uint32_t)(((int32_t)u >> 31) | 0x80000000);
-  };
+  const int tid = threadIdx.x;
+  const Head head(p);
   // the keep-th largest key, 11, 11 and 10 bits at a time, and how many of its equals stay
   uint32_t prefix = 0;
   int need = p.keep;
@@ -342,7 +589,7 @@ __global__ void __launch_bounds__(kSelect) tm_evict_select_kernel(EvictParams p)
       for (int i = tid; i < kBins; i += kSelect) s_bins[i] = 0;
       __syncthreads();
       for (int s = tid; s < p.length; s += kSelect) {
-        const uint32_t k = key_of(s);
+        const uint32_t k = head.key(s);
         if (shift == 21 || (k >> (shift + bits)) == prefix)
           atomicAdd(&s_bins[(k >> shift) & ((1u << bits) - 1)], 1u);
       }
@@ -374,16 +621,16 @@ __global__ void __launch_bounds__(kSelect) tm_evict_select_kernel(EvictParams p)
   }
   // slot by slot: which stay, holes below keep and movers behind it
   const BlockRank ranked = {s_waves};
-  int32_t* const holes = p.holes + (int64_t)head * p.moves;
-  int32_t* const movers = p.movers + (int64_t)head * p.moves;
-  float* const mass_out = p.mass_out + (int64_t)head * p.columns;
-  int32_t* const pos_out = p.positions_out + (int64_t)head * p.keep;
+  int32_t* const holes = p.holes + (int64_t)head.index * p.moves;
+  int32_t* const movers = p.movers + (int64_t)head.index * p.moves;
+  float* const mass_out = p.mass_out + (int64_t)head.index * p.columns;
+  int32_t* const pos_out = p.positions_out + (int64_t)head.index * p.keep;
   int equal0 = 0, hole0 = 0, mover0 = 0;
   const bool all = p.keep >= p.length;
   for (int s0 = 0; s0 < p.length; s0 += kSelect) {
     const int s = s0 + tid;
     const bool in = s < p.length;
-    const uint32_t k = in ? key_of(s) : 0;
+    const uint32_t k = in ? head.key(s) : 0;
     int total;
     const int equal = equal0 + ranked(in && k == prefix, &total);
     equal0 += total;
@@ -396,18 +643,18 @@ __global__ void __launch_bounds__(kSelect) tm_evict_select_kernel(EvictParams p)
     if (hole && h < p.moves) holes[h] = s;
     if (mover && m < p.moves) movers[m] = s;
     if (kept && s < p.keep) {
-      mass_out[s] = mass[s];
-      pos_out[s] = position(s);
+      mass_out[s] = head.mass[s];
+      pos_out[s] = head.position(s);
     }
   }
   for (int s = p.keep + tid; s < p.columns; s += kSelect) mass_out[s] = 0.0f;
   const int moves = min(min(hole0, mover0), p.moves);
-  if (tid == 0) p.counts[head] = moves;
+  if (tid == 0) p.counts[head.index] = moves;
   __syncthreads();  // this workgroup's lists
   for (int i = tid; i < moves; i += kSelect) {
     const int to = holes[i], from = movers[i];
-    mass_out[to] = mass[from];
-    pos_out[to] = position(from);
+    mass_out[to] = head.mass[from];
+    pos_out[to] = head.position(from);
   }
 }
 
@@ -439,11 +686,16 @@ __global__ void __launch_bounds__(kThreads) tm_evict_move_kernel(EvictParams p) 
 // ------------------------------------------------------------------- host --
 
 constexpr int64_t kMaxStride = 1 << 24;
+constexpr int64_t kHeld = 16 * kSelect;  // keys of a head that its workgroup holds
+// The selecting workgroups move the keys where they fill the chip, or have few to move.
+constexpr int64_t kFusedHeads = 128, kFusedMoves = 128;
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct MassPlan {
-  bool few;
-  int64_t rows, tiles, chunks, chunk_len, bytes;
+  bool few, own;
+  int64_t rows, tiles, chunks, chunk_len;
+  int64_t key_tiles, splits;               // of the sums
+  int64_t stats, consts, parts, bytes;     // floats, floats, floats; of the workspace
 };
 
 int plan_mass(int64_t T, int64_t S, int64_t Hq, int64_t kvh, int64_t hd, MassPlan* o) {
@@ -454,17 +706,27 @@ int plan_mass(int64_t T, int64_t S, int64_t Hq, int64_t kvh, int64_t hd, MassPla
     return TM_ERR_SHAPE;
   o->rows = T * group;
   o->few = o->rows <= 32;
+  o->own = o->rows <= kOwnRows;
   o->tiles = ceil_div(o->rows, o->few ? 32 : 128);
   // ranges of keys as many as fill the chip, of four stages or more
   const int64_t units = std::max<int64_t>(o->tiles * kvh, 1);
-  const int64_t want = std::max<int64_t>(1, 2 * kCUs / units);
+  const int64_t want = std::max<int64_t>(1, kCUs / units);
   const int64_t chunks = std::max<int64_t>(1, std::min(want, ceil_div(S, 4 * kKeys)));
   const int64_t step = o->few ? 4 * kKeys : kKeys;
   o->chunk_len = std::max(step, ceil_div(ceil_div(S, chunks), step) * step);
   o->chunks = std::max<int64_t>(1, ceil_div(S, o->chunk_len));
-  o->bytes = o->chunks * kvh * o->rows * 8;
+  // the sums' rows in parts of eight stages or more, two workgroups a slot of the chip
+  o->key_tiles = ceil_div(S, o->own ? 128 : 256);
+  const int64_t stages = ceil_div(o->rows, kKeys);
+  o->splits = o->own ? 1
+                     : std::max<int64_t>(1, std::min(4 * kCUs / std::max<int64_t>(o->key_tiles * kvh, 1),
+                                                     stages / 8));
+  o->stats = o->own || o->chunks > 1 ? 2 * o->chunks * kvh * o->rows : 0;
+  o->consts = o->own ? 0 : kvh * stages * kKeys;
+  o->parts = o->splits > 1 ? o->splits * kvh * S : 0;
+  o->bytes = 4 * (o->stats + o->consts + o->parts);
   if (o->tiles * o->chunks * kvh > UINT32_MAX / kThreads ||
-      ceil_div(S, kKeys) * kvh > UINT32_MAX / kThreads)
+      o->key_tiles * o->splits * kvh > UINT32_MAX / 512 || kvh * stages * kKeys > UINT32_MAX)
     return TM_ERR_SHAPE;
   return TM_OK;
 }
@@ -473,19 +735,26 @@ template <int DT, int HD>
 void launch_mass(const MassParams& p, const MassPlan& o, hipStream_t st) {
   const dim3 block(kThreads);
   const dim3 items((unsigned)(o.tiles * o.chunks * p.kvh));
-  const int64_t keys = ceil_div(p.k_len, kKeys);
+  const dim3 sums((unsigned)(o.key_tiles * o.splits * p.kvh));
   if (o.rows > 0) {
     if (o.few)
       hipLaunchKernelGGL((tm_mass_stats_few_kernel<DT, HD>), items, block, 0, st, p);
     else
       hipLaunchKernelGGL((tm_mass_stats_kernel<DT, HD>), items, block, 0, st, p);
   }
-  if (o.rows <= 64)
-    hipLaunchKernelGGL((tm_mass_sum_kernel<DT, HD, 1>),
-                       dim3((unsigned)(ceil_div(keys, 4) * p.kvh)), block, 0, st, p);
-  else
-    hipLaunchKernelGGL((tm_mass_sum_kernel<DT, HD, 4>), dim3((unsigned)(keys * p.kvh)), block, 0,
-                       st, p);
+  if (o.own) {
+    hipLaunchKernelGGL((tm_mass_sum_kernel<DT, HD, 4, true>), sums, block, 0, st, p);
+    return;
+  }
+  const int64_t whole = ceil_div(o.rows, kKeys) * kKeys;
+  if (o.chunks > 1)
+    hipLaunchKernelGGL(tm_mass_rows_kernel, dim3((unsigned)ceil_div(p.kvh * whole, kThreads)),
+                       block, 0, st, p, (int)o.rows, (int)whole);
+  hipLaunchKernelGGL((tm_mass_sum_kernel<DT, HD, 8, false>), sums, dim3(512), 0, st, p);
+  if (o.splits > 1)
+    hipLaunchKernelGGL(tm_mass_join_kernel,
+                       dim3((unsigned)ceil_div(p.k_len, kThreads), (unsigned)p.kvh), block, 0, st,
+                       p);
 }
 
 int page_shift_of(int64_t page_size) {
@@ -568,7 +837,11 @@ extern "C" int tm_attention_mass(const void* q, int64_t q_stride, int64_t T, con
   p.cache_pages = (int)cache_pages;
   p.wide = page_size >= 16 ? 1 : 0;  // keys of a stage that a wave takes from one page
   p.scale_log2 = scale * 1.4426950408889634f;
-  p.row_stats = (float2*)workspace;
+  float* const at = (float*)workspace;
+  p.row_stats = (float2*)at;
+  p.row_consts = o.own ? nullptr : at + o.stats;
+  p.parts = o.splits > 1 ? at + o.stats + o.consts : nullptr;
+  p.splits = (int)o.splits;
   p.before = before;
   p.before_stride = before_stride;
   p.mass = mass;
@@ -660,8 +933,17 @@ extern "C" int tm_evict(void* k_cache, void* v_cache, int64_t elem_bytes, int64_
   p.holes = p.counts + o.heads;
   p.movers = p.holes + o.heads * o.moves;
   const hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(tm_evict_select_kernel, dim3((unsigned)o.heads), dim3(kSelect), 0, st, p);
-  if (o.moves > 0)
+  p.fused = seq_len <= kHeld && (o.heads >= kFusedHeads || o.moves <= kFusedMoves);
+  const dim3 grid((unsigned)o.heads), block(kSelect);
+  if (seq_len <= 2048)
+    hipLaunchKernelGGL((tm_evict_held_kernel<4, 512>), grid, dim3(512), 0, st, p);
+  else if (seq_len <= 8192)
+    hipLaunchKernelGGL((tm_evict_held_kernel<8, 1024>), grid, block, 0, st, p);
+  else if (seq_len <= kHeld)
+    hipLaunchKernelGGL((tm_evict_held_kernel<16, 1024>), grid, block, 0, st, p);
+  else
+    hipLaunchKernelGGL(tm_evict_select_kernel, grid, block, 0, st, p);
+  if (o.moves > 0 && !p.fused)
     hipLaunchKernelGGL(tm_evict_move_kernel,
                        dim3((unsigned)ceil_div(o.moves, kMovesOf), (unsigned)o.heads),
                        dim3(kThreads), 0, st, p);

@@ -55,47 +55,33 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return invoke<F>(F, args, n, indexes(F));
 }
 
-// prompt_cached_workspace(T, seq_len, Hq, kvh, hd) -> (status, bytes)
-PyObject* cached_workspace(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 5) {
-    PyErr_SetString(PyExc_TypeError, "expected 5 arguments");
+// A size query: its arguments without the last, which takes the bytes -> (status, bytes).
+template <auto F, typename... A, size_t... I>
+PyObject* query(int (*)(A...), PyObject* const* args, Py_ssize_t n, std::index_sequence<I...>) {
+  if (n != (Py_ssize_t)sizeof...(I)) {
+    PyErr_Format(PyExc_TypeError, "expected %d arguments, got %d", (int)sizeof...(I), (int)n);
     return nullptr;
   }
-  int64_t a[5], bytes = 0;
-  for (int i = 0; i < 5; ++i) a[i] = convert<int64_t>(args[i]);
+  const int64_t a[] = {convert<int64_t>(args[I])...};
   if (PyErr_Occurred()) return nullptr;
-  const int rc = tm_prompt_cached_workspace(a[0], a[1], a[2], a[3], a[4], &bytes);
+  int64_t bytes = 0;
+  const int rc = F(a[I]..., &bytes);
   return Py_BuildValue("iL", rc, (long long)bytes);
 }
-
-// mass_workspace(T, seq_len, Hq, kvh, hd) -> (status, bytes)
-PyObject* mass_workspace(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 5) {
-    PyErr_SetString(PyExc_TypeError, "expected 5 arguments");
-    return nullptr;
-  }
-  int64_t a[5], bytes = 0;
-  for (int i = 0; i < 5; ++i) a[i] = convert<int64_t>(args[i]);
-  if (PyErr_Occurred()) return nullptr;
-  const int rc = tm_mass_workspace(a[0], a[1], a[2], a[3], a[4], &bytes);
-  return Py_BuildValue("iL", rc, (long long)bytes);
+template <typename... A>
+constexpr std::make_index_sequence<sizeof...(A) - 1> sizes(int (*)(A...)) {
+  return {};
 }
-
-// branch_workspace(T, units, max_count, seq_len, longest, Hq, kvh, hd) -> (status, bytes)
-PyObject* branch_workspace(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 8) {
-    PyErr_SetString(PyExc_TypeError, "expected 8 arguments");
-    return nullptr;
-  }
-  int64_t a[8], bytes = 0;
-  for (int i = 0; i < 8; ++i) a[i] = convert<int64_t>(args[i]);
-  if (PyErr_Occurred()) return nullptr;
-  const int rc = tm_branch_workspace(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], &bytes);
-  return Py_BuildValue("iL", rc, (long long)bytes);
+template <auto F>
+PyObject* bytes_of(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return query<F>(F, args, n, sizes(F));
 }
 
 #define TM_ENTRY(name) \
   {#name, (PyCFunction)(void (*)(void))entry<name>, METH_FASTCALL, nullptr}
+
+#define TM_BYTES(name, entry) \
+  {name, (PyCFunction)(void (*)(void))bytes_of<entry>, METH_FASTCALL, nullptr}
 
 PyMethodDef kMethods[] = {
     TM_ENTRY(tm_rms_norm),
@@ -104,15 +90,16 @@ PyMethodDef kMethods[] = {
     TM_ENTRY(tm_rotary_append),
     TM_ENTRY(tm_sample_tokens),
     TM_ENTRY(tm_prompt_attention),
-    {"prompt_cached_workspace", (PyCFunction)(void (*)(void))cached_workspace, METH_FASTCALL,
-     nullptr},
+    TM_BYTES("prompt_cached_workspace", tm_prompt_cached_workspace),
     TM_ENTRY(tm_prompt_attention_cached),
-    {"branch_workspace", (PyCFunction)(void (*)(void))branch_workspace, METH_FASTCALL, nullptr},
+    TM_BYTES("branch_workspace", tm_branch_workspace),
     TM_ENTRY(tm_branch_attention),
     TM_ENTRY(tm_branch_advance),
     TM_ENTRY(tm_beam_select),
     TM_ENTRY(tm_reorder_rows),
-    {"mass_workspace", (PyCFunction)(void (*)(void))mass_workspace, METH_FASTCALL, nullptr},
+    TM_BYTES("beam_workspace", tm_beam_workspace),
+    TM_BYTES("mass_workspace", tm_mass_workspace),
+    TM_BYTES("evict_workspace", tm_evict_workspace),
     TM_ENTRY(tm_attention_mass),
     TM_ENTRY(tm_evict),
     {nullptr, nullptr, 0, nullptr},

@@ -17,8 +17,6 @@ from torch.autograd import forward_ad
 from treemoe_spec_amd import _capi
 from treemoe_spec_amd._capi import dtype_code, ptr
 
-_SEGMENT = 1024  # logits of a list in the workspace
-
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, num: int | None = None,
                 finished: torch.Tensor | None = None, pad_token: int = 0):
@@ -74,7 +72,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, num: int | None =
     best = torch.empty((groups, num), dtype=torch.float32, device=dev)
     parents = torch.empty((groups, num), dtype=torch.int32, device=dev)
     tokens = torch.empty((groups, num), dtype=torch.int64, device=dev)
-    nbytes = rows * -(-v // _SEGMENT) * (8 * num + 12)
+    nbytes = _capi.workspace_bytes("beam_workspace", groups, beams, v, num)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _capi.launch("tm_beam_select", index, logits.data_ptr(), dt, groups, beams, v,
                  stride if rows > 1 else v, scores.data_ptr(), ptr(finished), pad_token, num,

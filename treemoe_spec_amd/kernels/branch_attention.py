@@ -50,19 +50,6 @@ class BranchPlan:
         self.made_on = _capi.stream_made_on(self.device)
 
 
-def _workspace_bytes(*sizes) -> int:
-    """tm_branch_workspace(T, units, max_count, seq_len, longest, Hq, kvh, hd)."""
-    fast = _capi.layer_binding()
-    if fast is not None:
-        rc, nbytes = fast.branch_workspace(*sizes)
-        if rc:
-            _capi.check(rc, "tm_branch_workspace")
-        return nbytes
-    size = ctypes.c_int64()
-    _capi.call("tm_branch_workspace", *sizes, ctypes.byref(size))
-    return size.value
-
-
 def branch_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv, branches, layer: int,
                      plan: BranchPlan | None = None, *, scale: float | None = None,
                      out: torch.Tensor | None = None) -> torch.Tensor:
@@ -160,7 +147,8 @@ def branch_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv, bran
     table = mapped = 0
     if seq_len:
         table, mapped = device_tables_of(kv, dev)[0].data_ptr(), len(kv.block_table)
-    nbytes = _workspace_bytes(total, num_units, count, seq_len, longest, hq, kvh, hd)
+    nbytes = _capi.workspace_bytes("branch_workspace", total, num_units, count, seq_len, longest,
+                                   hq, kvh, hd)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     size = kc.element_size()
     at, bat = size * cst[0] * (layer % layers), size * bst[0] * (layer % bshape[0])

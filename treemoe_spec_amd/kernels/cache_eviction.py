@@ -8,7 +8,6 @@ cache to the keys of the largest sums, beside the first and the most recent ones
 
 from __future__ import annotations
 
-import ctypes
 import operator
 
 import torch
@@ -75,15 +74,7 @@ def attention_mass(q: torch.Tensor, kv, layer: int, mass: torch.Tensor | None = 
     if n == 0:
         return out
     table, _ = device_tables_of(kv, dev)
-    fast = _capi.layer_binding()
-    if fast is not None:
-        rc, nbytes = fast.mass_workspace(t, n, hq, kvh, hd)
-        if rc:
-            _capi.check(rc, "tm_mass_workspace")
-    else:
-        size = ctypes.c_int64()
-        _capi.call("tm_mass_workspace", t, n, hq, kvh, hd, ctypes.byref(size))
-        nbytes = size.value
+    nbytes = _capi.workspace_bytes("mass_workspace", t, n, hq, kvh, hd)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _capi.launch("tm_attention_mass", index, q.data_ptr(), qs, t,
                  kc.data_ptr() + kc.element_size() * cst[0] * (layer % layers), cst[1], cst[2], page,
@@ -145,13 +136,12 @@ def evict(kv, mass: torch.Tensor, keep: int, *, positions: torch.Tensor | None =
     if mass.shape[2] == 0:
         return new_mass, new_positions
     table, _ = device_tables_of(kv, dev)
-    need = ctypes.c_int64()
-    _capi.call("tm_evict_workspace", layers, kvh, n, keep, ctypes.byref(need))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+    nbytes = _capi.workspace_bytes("evict_workspace", layers, kvh, n, keep)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _capi.launch("tm_evict", dev.index, kc.data_ptr(), vc.data_ptr(), size, layers, cst[0], cst[1],
                  cst[2], kvh, hd, page, pages, table.data_ptr(), len(kv.block_table), n, keep,
                  mass.data_ptr(), mass.stride(0), mass.stride(1), mass.shape[2],
                  ptr(positions) if recorded else 0, pl, ph, recorded, next_position, recent, sinks,
-                 new_mass.data_ptr(), new_positions.data_ptr(), ws.data_ptr(), need.value)
+                 new_mass.data_ptr(), new_positions.data_ptr(), ws.data_ptr(), nbytes)
     kv.seq_len = keep
     return new_mass, new_positions
