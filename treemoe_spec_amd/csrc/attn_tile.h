@@ -131,14 +131,14 @@ struct Shape {
   }
 };
 
-// Stages of 64 keys into LDS by NW waves, one after the other, V of a stage at any time
+// Stages of KEYS keys into LDS by NW waves, one after the other, V of a stage at any time
 // between its K and the next one's.  Keys past the sequence's last are that one again:
 // their scores are masked.
-template <int HD, bool PAGED, int NW>
+template <int HD, bool PAGED, int NW, int KEYS = kKeys>
 struct Feed {
   typedef Shape<HD> S;
   typedef PromptParams Params;
-  static constexpr int kLoads = S::kTile / (1024 * NW);  // loads of a wave per tile
+  static constexpr int kLoads = KEYS * S::kRow / (1024 * NW);  // loads of a wave per tile
   static constexpr int kGroup = 2 * kLoads;  // of K and V of a stage
   static constexpr int kWaveKeys = kLoads * S::kKeysPerLoad;  // of a stage, by one wave
   // a wave's keys in parts of at most 16, each within a page of 16 or more
@@ -245,7 +245,7 @@ struct Feed {
     }
   }
   __device__ __forceinline__ bool whole(const PromptParams& p, int left_) const {
-    return left_ >= kKeys - 1 && (!PAGED || p.wide);
+    return left_ >= KEYS - 1 && (!PAGED || p.wide);
   }
   __device__ __forceinline__ void load_k(const PromptParams& p, uint8_t* tile) {
     if (whole(p, left)) {
@@ -411,21 +411,22 @@ __device__ __forceinline__ void products(const uint8_t* vt, const uint8_t* kt_, 
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// The weights of the stage's keys kb .. against the running maximum.  mask: some key
+// The weights of the stage's 32 KT keys kb .. against the running maximum.  mask: some key
 // lies past the last one that some row sees.
-template <int DT, int HD>
+template <int DT, int HD, int KT = 2>
 __device__ __forceinline__ void weigh(float scale_log2, int kb, bool mask, Rows<HD>& r) {
   if (mask) {
     const int left = r.seen - kb - 4 * ((int)(threadIdx.x & 63) >> 5);
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
       for (int x = 0; x < 16; ++x)
         r.sc[kt][x] = 32 * kt + 8 * (x >> 2) + (x & 3) <= left ? r.sc[kt][x] : -INFINITY;
   }
-  float mx[2] = {fmaxf(r.sc[0][0], r.sc[1][0]), fmaxf(r.sc[0][1], r.sc[1][1])};
+  constexpr int kLast = KT - 1;  // (of one tile of keys, the maximum of itself)
+  float mx[2] = {fmaxf(r.sc[0][0], r.sc[kLast][0]), fmaxf(r.sc[0][1], r.sc[kLast][1])};
 #pragma unroll
-  for (int x = 2; x < 16; ++x) mx[x & 1] = fmaxf(fmaxf(mx[x & 1], r.sc[0][x]), r.sc[1][x]);
+  for (int x = 2; x < 16; ++x) mx[x & 1] = fmaxf(fmaxf(mx[x & 1], r.sc[0][x]), r.sc[kLast][x]);
   const float cand = max_halves(fmaxf(mx[0], mx[1])) * scale_log2;
   const bool bump = cand > r.m + 8.0f;
   if (__any(bump)) {
@@ -441,7 +442,7 @@ __device__ __forceinline__ void weigh(float scale_log2, int kb, bool mask, Rows<
   const float base = r.m == -INFINITY ? 0.0f : -r.m;
   float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-  for (int s = 0; s < 4; ++s)
+  for (int s = 0; s < 2 * KT; ++s)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int x = 8 * (s & 1) + 2 * j;
@@ -529,7 +530,7 @@ __device__ __forceinline__ Place begin_rows(const PromptParams& p, const Item& i
 // its value, by the products.  Rows whose output is not finite are therefore taken again,
 // key by key over what each sees: stages s0, s0 + step, ... of the range.  Slow, and
 // only reached where an input is not finite or a product overflows.
-template <int DT, int HD, class FEED>
+template <int DT, int HD, class FEED, int KEYS = kKeys>
 __device__ __forceinline__ void retake(const typename FEED::Params& p, const Item& it, int kvhead,
                                        int s0, int step, int n, Rows<HD>& r) {
   float bad[8] = {r.l * 0.0f};  // 0 times what is not finite is NaN
@@ -547,7 +548,7 @@ __device__ __forceinline__ void retake(const typename FEED::Params& p, const Ite
 #pragma unroll
     for (int x = 0; x < 16; ++x) r.o[ht][x] = 0.0f;
   for (int s = s0; s < n; s += step) {
-    const int first = it.begin + s * kKeys, end = min(first + kKeys, it.end);
+    const int first = it.begin + s * KEYS, end = min(first + KEYS, it.end);
 #pragma unroll 1
     for (int key = first; key < end; ++key) {
       const uint16_t *kr, *vr;

@@ -39,11 +39,11 @@ struct BranchParams : PromptParams {   // k, v: the layer's [rows, capacity, kvh
 // Stages of a branch's own keys into LDS by NW waves, as Feed has them.  A key's row
 // stands alone: the lanes look the origins of the wave's keys up, a stage ahead, and
 // pass them to each other.
-template <int HD, int NW>
+template <int HD, int NW, int KEYS = kKeys>
 struct BranchFeed {
   typedef Shape<HD> S;
   typedef BranchParams Params;
-  static constexpr int kLoads = S::kTile / (1024 * NW);
+  static constexpr int kLoads = KEYS * S::kRow / (1024 * NW);
   static constexpr int kWaveKeys = kLoads * S::kKeysPerLoad;
   static_assert(kWaveKeys <= 64, "a lane looks up one key");
   const uint16_t *k, *v, *new_k, *new_v;  // the head's first element
@@ -177,16 +177,149 @@ __device__ __forceinline__ void store_new(const BranchParams& p, const Work& w) 
   }
 }
 
-// A branch's own keys, few rows (a decoded token's heads).
+// Up to 32 rows against a range of keys, 32 keys a stage, the four waves in turn, each with
+// its own part of LDS and no barrier between them.  Stages of 32 keys leave room for two
+// workgroups a CU: most ranges are a few stages long, and one's first loads and last stores
+// run under the other's products.
+constexpr int kLean = 32;
+template <int HD>
+struct LeanShared {
+  uint8_t tiles[4][2 * kLean * Shape<HD>::kRow];  // of each wave, K and V
+  float stat[4][32][2];
+};
+
+// S^T = K Q^T of the stage at kt_.
 template <int DT, int HD>
-__global__ void __launch_bounds__(kThreads, 1) tm_branch_few_kernel(BranchParams p) {
-  typedef Shape<HD> S;
-  __shared__ __attribute__((aligned(1024))) uint8_t s_k[4][S::kTile];
-  __shared__ __attribute__((aligned(1024))) uint8_t s_v[4][S::kTile];
-  __shared__ float s_stat[4][32][2];
-  const Work w = work_of(p, blockIdx.x, 32);
+__device__ __forceinline__ void lean_scores(const uint8_t* kt_, Rows<HD>& r) {
+  const int at = k_offset<HD>();
+  u32x4_t f[HD / 16];
+#pragma unroll
+  for (int ks = 0; ks < HD / 16; ++ks)
+    f[ks] = *reinterpret_cast<const u32x4_t*>(kt_ + (at ^ (32 * ks)));
+  f32x16_t sc = {};
+#pragma unroll
+  for (int ks = 0; ks < HD / 16; ++ks) sc = mfma32<DT>(f[ks], r.q[ks], sc);
+  r.sc[0] = sc;
+}
+// O^T += V^T P^T of the stage at vt.
+template <int DT, int HD>
+__device__ __forceinline__ void lean_outputs(const uint8_t* vt, Rows<HD>& r) {
+  int lo, hi;
+  v_offsets<HD>(lo, hi);
+#pragma unroll
+  for (int s = 0; s < kLean / 16; ++s) {
+    u32x4_t vf[HD / 32];
+    read_v<HD>(vt, fresh(lo), fresh(hi), s, vf);
+#pragma unroll
+    for (int ht = 0; ht < HD / 32; ++ht) r.o[ht] = mfma32<DT>(vf[ht], r.pw[s], r.o[ht]);
+  }
+}
+
+template <int DT, int HD, class FEED>
+__device__ __forceinline__ void lean_body(const typename FEED::Params& p, const Item& it,
+                                          int kvhead, LeanShared<HD>& lds) {
+  constexpr int kLoads = FEED::kLoads;
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, c32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int first = it.tile * 32, rows = min(it.q_len * p.group - first, 32);
+  const int n = it.end > it.begin ? (it.end - it.begin + kLean - 1) / kLean : 0;
+  uint8_t* const kt = lds.tiles[wave];
+  uint8_t* const vt = kt + kLean * Shape<HD>::kRow;
+  FEED feed;
+  if (wave < n) {
+    feed.start(p, it, kvhead, it.begin + wave * kLean, 4 * kLean);
+    feed.load_k(p, kt);
+    feed.load_v(p, vt);
+  }
+  Rows<HD> r;
+  const int full = begin_rows<HD>(p, it, kvhead, first, r).full;
+  for (int s = wave; s < n; s += 4) {
+    const int kb = it.begin + s * kLean;
+    const bool more = s + 4 < n;
+    if (s == wave)
+      wait_vm<0>();  // K and V, and the query rows
+    else
+      wait_vm<kLoads>();  // K: V is behind it
+    lean_scores<DT, HD>(kt, r);
+    __builtin_amdgcn_sched_barrier(0);
+    if (more) feed.load_k(p, kt);
+    weigh<DT, HD, 1>(p.scale_log2, kb, kb + kLean - 1 > full, r);
+    if (more)
+      wait_vm<kLoads>();
+    else
+      wait_vm<0>();
+    lean_outputs<DT, HD>(vt, r);
+    __builtin_amdgcn_sched_barrier(0);
+    if (more) feed.load_v(p, vt);
+  }
+  retake<DT, HD, FEED, kLean>(p, it, kvhead, wave, 4, n, r);
+  const float l = r.l + __shfl_xor(r.l, 32);
+  // each wave's O [32][HD] where its K and V were
+  if (c32 < rows) {
+    float* const mine = reinterpret_cast<float*>(kt) + c32 * HD + 4 * half;
+#pragma unroll
+    for (int ht = 0; ht < HD / 32; ++ht)
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        *reinterpret_cast<f32x4_t*>(mine + 32 * ht + 8 * x) =
+            f32x4_t{r.o[ht][4 * x], r.o[ht][4 * x + 1], r.o[ht][4 * x + 2], r.o[ht][4 * x + 3]};
+    if (half == 0) {
+      lds.stat[wave][c32][0] = r.m;
+      lds.stat[wave][c32][1] = l;
+    }
+  }
+  __syncthreads();
+  constexpr int kLanes = HD / 4;  // of a row, four elements each
+  for (int row = tid / kLanes; row < rows; row += kThreads / kLanes) {
+    float m = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) m = fmaxf(m, lds.stat[w][row][0]);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float a = __builtin_amdgcn_exp2f(lds.stat[w][row][0] - ref);
+      sum += lds.stat[w][row][1] * a;
+      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(
+          reinterpret_cast<const float*>(lds.tiles[w]) + row * HD + 4 * (tid % kLanes));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += x[e] * a;
+    }
+    if (it.slot < 0) {
+      store_row<DT>(p, it.q0, first + row, kvhead, HD, 4 * (tid % kLanes), o, sum);
+    } else {
+      const int64_t slot = ((int64_t)it.slot * p.kvh + kvhead) * p.part_rows + row;
+      *reinterpret_cast<f32x4_t*>(p.part + slot * HD + 4 * (tid % kLanes)) = o;
+      if (tid % kLanes == 0) {
+        p.stats[slot * 2] = m;
+        p.stats[slot * 2 + 1] = sum;
+      }
+    }
+  }
+}
+
+// Shared keys and the branches' own, where no branch adds more than 32 rows, in one launch:
+// the shared ones' workgroups first, tiles of 32 rows (where that is all) or of 128.  The
+// products over the shared keys run beside the reading of the others.
+enum Shared { kNone, kLeanTile, kShortTile };
+template <int DT, int HD, int SHARED>
+__global__ void __launch_bounds__(kThreads, 2) tm_branch_kernel(PromptParams s, BranchParams p,
+                                                               int shared_blocks) {
+  __shared__ __attribute__((aligned(1024))) LeanShared<HD> lds;
+  static_assert(sizeof(lds.tiles) == 4 * Shape<HD>::kTile, "two stages of 64 keys");
+  if (SHARED != kNone && (int)blockIdx.x < shared_blocks) {
+    const int kvhead = (int)blockIdx.x % s.kvh, at = (int)blockIdx.x / s.kvh;
+    if constexpr (SHARED == kLeanTile) {
+      lean_body<DT, HD, Feed<HD, true, 1, kLean>>(s, item_of(s, at, 32), kvhead, lds);
+    } else {
+      short_body<DT, HD, Feed<HD, true, 4>>(s, item_of(s, at, 128), kvhead, lds.tiles[0],
+                                            lds.tiles[1], lds.tiles[2], lds.tiles[3]);
+    }
+    return;
+  }
+  const Work w = work_of(p, (int)blockIdx.x - shared_blocks, 32);
   store_new<HD>(p, w);
-  few_body<DT, HD, BranchFeed<HD, 1>>(p, w.it, w.kvhead, s_k, s_v, s_stat);
+  lean_body<DT, HD, BranchFeed<HD, 1, kLean>>(p, w.it, w.kvhead, lds);
 }
 
 // Its own keys, tiles of 128 rows.
@@ -317,6 +450,12 @@ __global__ void __launch_bounds__(kThreads) tm_branch_join_kernel(BranchJoin p) 
 
 // ------------------------------------------------------------------- host --
 
+#ifndef TM_C1
+#define TM_C1 128
+#endif
+#ifndef TM_C2
+#define TM_C2 256
+#endif
 constexpr int64_t kMaxStride = 1 << 24;
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -330,8 +469,9 @@ int check_heads(int64_t Hq, int64_t kvh, int64_t hd) {
 int64_t own_tile_rows(int64_t max_count, int64_t group) { return max_count * group <= 32 ? 32 : 128; }
 
 struct BranchPlan {
-  PrefixPlan prefix;
-  bool few;
+  PrefixPlan prefix;               // the shared keys
+  Shared shared;
+  bool few;                        // one launch for both kinds of keys
   int64_t units, chunks;           // of the branches' own keys
   int64_t own_rows;                // rows of one of their partials
   int64_t prefix_slots, own_slots; // (of one KV head)
@@ -343,27 +483,42 @@ struct BranchPlan {
 int plan_branches(int64_t T, int64_t units, int64_t max_count, int64_t S, int64_t longest,
                   int64_t Hq, int64_t kvh, int64_t hd, BranchPlan* o) {
   const int64_t group = Hq / kvh;
-  if (units < 0 || max_count < 0 || max_count > T || longest < 0 || longest > TM_MAX_PROMPT_KEYS)
+  if (units < 0 || max_count < 0 || max_count > T || longest < 0 || longest > TM_MAX_PROMPT_KEYS ||
+      S < 0 || S > TM_MAX_PROMPT_KEYS || T < 0 || T * group > INT32_MAX - 1024)
     return TM_ERR_SHAPE;
   *o = {};
-  if (S > 0) {
-    const int rc = tm_prefix_plan(T, S, Hq, kvh, &o->prefix);
-    if (rc) return rc;
-  } else if (S < 0 || T < 0 || T * group > INT32_MAX - 1024) {
-    return TM_ERR_SHAPE;
-  }
   const int64_t rows = own_tile_rows(max_count, group);
   o->few = rows == 32;
   o->units = units;
+  if (S > 0 && o->few) {
+    // ranges of shared keys: FIGURES
+    const int64_t all = T * group;
+    o->shared = all <= 32 ? kLeanTile : kShortTile;
+    PrefixPlan& f = o->prefix;
+    f.kind = o->shared == kLeanTile ? 0 : 1;
+    f.tile_rows = o->shared == kLeanTile ? 32 : 128;
+    f.tiles = ceil_div(all, f.tile_rows);
+    f.part_rows = o->shared == kLeanTile ? all : 128;
+    const int64_t step = o->shared == kLeanTile ? 4 * kLean : kKeys;
+    const int64_t want = std::max<int64_t>(1, TM_C1 / std::max<int64_t>(f.tiles * kvh, 1));
+    const int64_t chunks = std::max<int64_t>(
+        1, std::min(std::min<int64_t>(want, kMaxParts),
+                    ceil_div(S, o->shared == kLeanTile ? 4 * kLean : 4 * kKeys)));
+    f.chunk_len = std::max(step, ceil_div(ceil_div(S, chunks), step) * step);
+    f.chunks = ceil_div(S, f.chunk_len);
+  } else if (S > 0) {
+    const int rc = tm_prefix_plan(T, S, Hq, kvh, &o->prefix);
+    if (rc) return rc;
+  }
   const int64_t keys = longest + max_count;
-  const int64_t want = std::min<int64_t>((o->few ? kCUs : 2 * kCUs) / std::max<int64_t>(units * kvh, 1),
-                                         kMaxParts);
-  o->chunks = std::max<int64_t>(1, std::min(want, ceil_div(keys, 4 * kKeys)));
+  const int64_t want = std::min<int64_t>(2 * kCUs / std::max<int64_t>(units * kvh, 1), kMaxParts);
+  o->chunks = std::max<int64_t>(1, std::min(want, ceil_div(keys, o->few ? TM_C2 : 4 * kKeys)));
   o->own_rows = o->few ? std::min<int64_t>(32, max_count * group) : rows;
   o->prefix_slots = S > 0 ? o->prefix.tiles * o->prefix.chunks : 0;
   const bool joined = S > 0 || o->chunks > 1;
   o->own_slots = joined ? units * o->chunks : 0;
-  if (o->own_slots > INT32_MAX || units * o->chunks * kvh > UINT32_MAX / kThreads ||
+  if (o->own_slots > INT32_MAX ||
+      (o->prefix_slots + units * o->chunks) * kvh > UINT32_MAX / kThreads ||
       T * Hq > UINT32_MAX / 64)
     return TM_ERR_SHAPE;
   o->prefix_floats = S > 0 ? kvh * (hd + 2) * o->prefix_slots * o->prefix.part_rows : 0;
@@ -375,12 +530,21 @@ int plan_branches(int64_t T, int64_t units, int64_t max_count, int64_t S, int64_
 bool vec_ok(const void* p, int64_t stride) { return (uintptr_t)p % 16 == 0 && stride % 8 == 0; }
 
 template <int DT, int HD>
-void launch_own(const BranchParams& p, const BranchPlan& o, hipStream_t st) {
-  const dim3 grid((unsigned)(o.units * o.chunks * p.kvh)), block(kThreads);
-  if (o.few)
-    hipLaunchKernelGGL((tm_branch_few_kernel<DT, HD>), grid, block, 0, st, p);
+void launch_own(const PromptParams& s, const BranchParams& p, const BranchPlan& o,
+                hipStream_t st) {
+  const int64_t own = o.units * o.chunks * p.kvh, shared = o.prefix_slots * p.kvh;
+  const dim3 block(kThreads);
+  if (!o.few)
+    hipLaunchKernelGGL((tm_branch_short_kernel<DT, HD>), dim3((unsigned)own), block, 0, st, p);
+  else if (o.shared == kNone)
+    hipLaunchKernelGGL((tm_branch_kernel<DT, HD, kNone>), dim3((unsigned)own), block, 0, st, s, p,
+                       0);
+  else if (o.shared == kLeanTile)
+    hipLaunchKernelGGL((tm_branch_kernel<DT, HD, kLeanTile>), dim3((unsigned)(own + shared)),
+                       block, 0, st, s, p, (int)shared);
   else
-    hipLaunchKernelGGL((tm_branch_short_kernel<DT, HD>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((tm_branch_kernel<DT, HD, kShortTile>), dim3((unsigned)(own + shared)),
+                       block, 0, st, s, p, (int)shared);
 }
 template <int DT, int HD>
 void launch_join(const BranchJoin& j, hipStream_t st) {
@@ -512,8 +676,8 @@ extern "C" int tm_branch_attention(
   p.scale_log2 = scale * 1.4426950408889634f;
   float* at = (float*)workspace;
   BranchJoin j = {};
+  PromptParams s = p;
   if (seq_len > 0) {
-    PromptParams s = p;
     s.k = (const uint16_t*)k_cache;
     s.v = (const uint16_t*)v_cache;
     s.table = block_table;
@@ -527,7 +691,16 @@ extern "C" int tm_branch_attention(
     s.part = at;
     s.stats = at + part_rows * hd;
     at += o.prefix_floats;
-    tm_prefix_launch(s, o.prefix, dtype, hd, page_size, st);
+    if (o.few) {
+      s.tiles = (int)o.prefix.tiles;
+      s.chunks = (int)o.prefix.chunks;
+      s.chunk_len = (int)o.prefix.chunk_len;
+      s.part_rows = (int)o.prefix.part_rows;
+      s.whole = 1;
+      s.wide = page_size >= 16 ? 1 : 0;  // keys of a stage that a wave takes from one page
+    } else {
+      tm_prefix_launch(s, o.prefix, dtype, hd, page_size, st);
+    }
     j.shared = {s.part, s.stats, (int)o.prefix.chunks, (int)o.prefix.tile_rows,
                 (int)o.prefix.part_rows, o.prefix.kind != 0};
   } else {
@@ -566,7 +739,7 @@ extern "C" int tm_branch_attention(
   j.out_stride = out_stride;
 #define TM_BRANCH(DT, HD)                             \
   do {                                                \
-    launch_own<DT, HD>(p, o, st);                     \
+    launch_own<DT, HD>(s, p, o, st);                    \
     if (p.parts) launch_join<DT, HD>(j, st);          \
   } while (0)
   if (dtype == TM_DTYPE_F16) {
