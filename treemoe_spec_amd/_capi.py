@@ -200,6 +200,24 @@ def dtype_code(dtype) -> int | None:
             torch.float16: TM_DTYPE_F16}.get(dtype)
 
 
+@functools.cache
+def _forward_ad():
+    from torch.autograd import forward_ad
+
+    return forward_ad
+
+
+def ready(index: int, *tensors) -> bool:
+    """Whether all given tensors (None for none) are on the ROCm device ``index``, and none
+    is one that ``require`` refuses."""
+    if index < 0 or _forward_ad()._current_level >= 0:
+        return False
+    for t in tensors:
+        if t is not None and (t.get_device() != index or t.requires_grad):
+            return False
+    return True
+
+
 def require(what: str, device, **tensors) -> None:
     """All given tensors on ``device``, a ROCm device, and none that a gradient is
     asked of or that carries a forward-mode tangent: these operators have no

@@ -12,7 +12,6 @@ from __future__ import annotations
 import operator
 
 import torch
-from torch.autograd import forward_ad
 
 from treemoe_spec_amd import _capi
 from treemoe_spec_amd._capi import dtype_code, ptr
@@ -64,16 +63,14 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, num: int | None =
     if step != 1 and v > 1:
         raise ValueError("logits must have unit stride along V")
     index = logits.get_device()
-    if index < 0 or scores.get_device() != index or logits.requires_grad or scores.requires_grad \
-            or finished is not None or forward_ad._current_level >= 0:
+    if not _capi.ready(index, logits, scores, finished):
         _capi.require("beam_select", logits.device, logits=logits, scores=scores,
                       finished=finished)
-    dev = logits.device
-    best = torch.empty((groups, num), dtype=torch.float32, device=dev)
-    parents = torch.empty((groups, num), dtype=torch.int32, device=dev)
-    tokens = torch.empty((groups, num), dtype=torch.int64, device=dev)
+    best = scores.new_empty(groups, num)
+    parents = scores.new_empty((groups, num), dtype=torch.int32)
+    tokens = scores.new_empty((groups, num), dtype=torch.int64)
     nbytes = _capi.workspace_bytes("beam_workspace", groups, beams, v, num)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    ws = scores.new_empty(nbytes // 4)
     _capi.launch("tm_beam_select", index, logits.data_ptr(), dt, groups, beams, v,
                  stride if rows > 1 else v, scores.data_ptr(), ptr(finished), pad_token, num,
                  best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), ws.data_ptr(), nbytes)
@@ -100,11 +97,12 @@ def reorder_rows(x: torch.Tensor, parents: torch.Tensor, *, out: torch.Tensor | 
         raise ValueError(f"x must have a row for each of {groups * beams} beams")
     rows = x.shape[0]
     index = x.get_device()
-    _capi.require("reorder_rows", x.device, x=x, parents=parents, out=out)
+    if not _capi.ready(index, x, parents, out):
+        _capi.require("reorder_rows", x.device, x=x, parents=parents, out=out)
     if out is None:
         if columns is not None:
             raise ValueError("columns without out")
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        out = x.new_empty(*x.shape)
     elif out.shape != x.shape or out.dtype != x.dtype:
         raise ValueError("out must have x's shape and type")
     size, width = x.element_size(), 1

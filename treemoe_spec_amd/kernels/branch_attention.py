@@ -14,7 +14,6 @@ import ctypes
 import operator
 
 import torch
-from torch.autograd import forward_ad
 
 from treemoe_spec_amd import _capi
 from treemoe_spec_amd._capi import ptr
@@ -71,16 +70,11 @@ def branch_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv, bran
     lengths, origin = branches.lengths, branches.origin
     dtype = q.dtype
     index = q.get_device()
-    if index < 0 or k.get_device() != index or v.get_device() != index \
-            or kc.get_device() != index or vc.get_device() != index \
-            or bk.get_device() != index or bv.get_device() != index \
-            or lengths.get_device() != index or out is not None or q.requires_grad \
-            or k.requires_grad or v.requires_grad or kc.requires_grad or vc.requires_grad \
-            or bk.requires_grad or bv.requires_grad or origin is not None or plan is not None \
-            or forward_ad._current_level >= 0:
+    if not _capi.ready(index, q, k, v, kc, vc, bk, bv, lengths, origin, out,
+                       plan and plan.lists):
         _capi.require("branch_attention", q.device, q=q, k=k, v=v, k_cache=kc, v_cache=vc,
                       branch_k=bk, branch_v=bv, lengths=lengths, origin=origin,
-                      plan=None if plan is None else plan.lists, out=out)
+                      plan=plan and plan.lists, out=out)
     kshape, ks, vs = k.shape, k.stride(), v.stride()
     if len(kshape) != 3 or kshape[0] != t or kshape[2] != hd or v.shape != kshape \
             or k.dtype != dtype or v.dtype != dtype:
@@ -136,9 +130,8 @@ def branch_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv, bran
     if most > capacity:
         raise ValueError(f"a branch would hold {most} keys, over the capacity of {capacity}")
     scale = _check_scale(scale, hd)
-    dev = q.device
     if out is None:
-        out = torch.empty((t, hq * hd), dtype=dtype, device=dev)
+        out = q.new_empty(t, hq * hd)
         if t > total:
             out[total:].zero_()
     if total == 0:
@@ -146,10 +139,10 @@ def branch_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv, bran
     seq_len = kv.seq_len
     table = mapped = 0
     if seq_len:
-        table, mapped = device_tables_of(kv, dev)[0].data_ptr(), len(kv.block_table)
+        table, mapped = device_tables_of(kv, q.device)[0].data_ptr(), len(kv.block_table)
     nbytes = _capi.workspace_bytes("branch_workspace", total, num_units, count, seq_len, longest,
                                    hq, kvh, hd)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    ws = q.new_empty(nbytes // 2) if nbytes else None
     size = kc.element_size()
     at, bat = size * cst[0] * (layer % layers), size * bst[0] * (layer % bshape[0])
     _capi.launch("tm_branch_attention", index, q.data_ptr(), qs, k.data_ptr(),

@@ -11,7 +11,6 @@ from __future__ import annotations
 import operator
 
 import torch
-from torch.autograd import forward_ad
 
 from treemoe_spec_amd import _capi
 from treemoe_spec_amd._capi import ptr
@@ -43,8 +42,7 @@ def attention_mass(q: torch.Tensor, kv, layer: int, mass: torch.Tensor | None = 
     dt, t, hq, hd, qs, _ = _check_q(q, None)
     kc, vc = kv.k, kv.v
     index = q.get_device()
-    if index < 0 or kc.get_device() != index or q.requires_grad or kc.requires_grad \
-            or mass is not None or out is not None or forward_ad._current_level >= 0:
+    if not _capi.ready(index, q, kc, mass, out):
         _capi.require("attention_mass", q.device, q=q, k_cache=kc, mass=mass, out=out)
     shape, cst = _cache_layout(kv, kc, vc)
     layers, pages, page, kvh, chd = shape
@@ -59,9 +57,8 @@ def attention_mass(q: torch.Tensor, kv, layer: int, mass: torch.Tensor | None = 
     if t > n:
         raise ValueError(f"{t} queries over a cache of {n} positions")
     scale = _check_scale(scale, hd)
-    dev = q.device
     if out is None:
-        out = torch.empty((kvh, n), dtype=torch.float32, device=dev)
+        out = q.new_empty((kvh, n), dtype=torch.float32)
     for name, x in (("mass", mass), ("out", out)):
         if x is not None and (x.dtype != torch.float32 or x.dim() != 2 or x.shape[0] != kvh
                               or x.shape[1] < n or (x.stride(1) != 1 and x.shape[1] > 1)
@@ -73,9 +70,9 @@ def attention_mass(q: torch.Tensor, kv, layer: int, mass: torch.Tensor | None = 
         raise ValueError("out must be mass, or lie apart from it")
     if n == 0:
         return out
-    table, _ = device_tables_of(kv, dev)
+    table, _ = device_tables_of(kv, q.device)
     nbytes = _capi.workspace_bytes("mass_workspace", t, n, hq, kvh, hd)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    ws = out.new_empty(nbytes // 4) if nbytes else None
     _capi.launch("tm_attention_mass", index, q.data_ptr(), qs, t,
                  kc.data_ptr() + kc.element_size() * cst[0] * (layer % layers), cst[1], cst[2], page,
                  pages, table.data_ptr(), len(kv.block_table), n, hq, kvh, hd, scale, dt,
@@ -103,7 +100,9 @@ def evict(kv, mass: torch.Tensor, keep: int, *, positions: torch.Tensor | None =
     Every attention over the whole cache goes on as before, since it does not depend on
     the order of the slots."""
     kc, vc = kv.k, kv.v
-    _capi.require("evict", kc.device, k_cache=kc, v_cache=vc, mass=mass, positions=positions)
+    index = kc.get_device()
+    if not _capi.ready(index, kc, vc, mass, positions):
+        _capi.require("evict", kc.device, k_cache=kc, v_cache=vc, mass=mass, positions=positions)
     shape, cst = _cache_layout(kv, kc, vc)
     layers, pages, page, kvh, hd = shape
     size, n = kc.element_size(), kv.seq_len
@@ -130,17 +129,17 @@ def evict(kv, mass: torch.Tensor, keep: int, *, positions: torch.Tensor | None =
     next_position = n if next_position is None else operator.index(next_position)
     if not n <= next_position < 2 ** 31:
         raise ValueError(f"next_position must be seq_len .. 2^31 - 1, got {next_position}")
-    dev = kc.device
-    new_mass = torch.empty(mass.shape, dtype=torch.float32, device=dev)
-    new_positions = torch.empty((layers, kvh, keep), dtype=torch.int32, device=dev)
-    if mass.shape[2] == 0:
+    columns = mass.shape[2]
+    new_mass = mass.new_empty(layers, kvh, columns)
+    new_positions = mass.new_empty((layers, kvh, keep), dtype=torch.int32)
+    if columns == 0:
         return new_mass, new_positions
-    table, _ = device_tables_of(kv, dev)
+    table, _ = device_tables_of(kv, kc.device)
     nbytes = _capi.workspace_bytes("evict_workspace", layers, kvh, n, keep)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _capi.launch("tm_evict", dev.index, kc.data_ptr(), vc.data_ptr(), size, layers, cst[0], cst[1],
+    ws = mass.new_empty(nbytes // 4)
+    _capi.launch("tm_evict", index, kc.data_ptr(), vc.data_ptr(), size, layers, cst[0], cst[1],
                  cst[2], kvh, hd, page, pages, table.data_ptr(), len(kv.block_table), n, keep,
-                 mass.data_ptr(), mass.stride(0), mass.stride(1), mass.shape[2],
+                 mass.data_ptr(), mass.stride(0), mass.stride(1), columns,
                  ptr(positions) if recorded else 0, pl, ph, recorded, next_position, recent, sinks,
                  new_mass.data_ptr(), new_positions.data_ptr(), ws.data_ptr(), nbytes)
     kv.seq_len = keep
