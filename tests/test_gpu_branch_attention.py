@@ -139,8 +139,20 @@ def test_ragged(counts, prefix, page, pad):
         assert not bool(out[sum(counts):].any())
 
 
+@pytest.mark.parametrize("prefix,page", [(0, 16), (63, 16), (64, 16), (65, 1), (300, 64), (1000, 16),
+                                         (2500, 64)])
+@pytest.mark.parametrize("counts", [[64], [32, 96, 31], [30, 0, 62, 128], [200, 150]])
+@pytest.mark.parametrize("hq,kvh,hd,dtype", [(8, 2, 128, BF), (32, 8, 64, F16)])
+def test_branches_that_fill_tiles(counts, prefix, page, hq, kvh, hd, dtype):
+    """Shared and own keys as one sequence, in one range or several."""
+    _say(f"branches: {counts} that fill tiles over {prefix} page {page} {hq}/{kvh} hd={hd}")
+    s = Setup(prefix, [(37 * i) % 150 for i in range(len(counts))], hq, kvh, hd, dtype, page,
+              seed=prefix + 1, capacity=400)
+    _run(s, counts)
+
+
 @pytest.mark.parametrize("beams,groups", [(2, 3), (4, 1), (5, 2), (8, 9)])
-@pytest.mark.parametrize("count", [1, 3, 20])
+@pytest.mark.parametrize("count", [1, 3, 20, 32])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_beams_share_rows(beams, groups, count, hd):
     _say(f"branches: {groups} x {beams} beams, {count} tokens, hd={hd}")
@@ -161,6 +173,8 @@ def test_long_own_keys():
     """Own keys over several ranges."""
     _say("branches: long own keys")
     _run(Setup(40, [3000, 1, 2049], 8, 2, 128, BF, seed=3, spare=5), [1, 1, 1])
+    _run(Setup(40, [20000, 9000], 8, 2, 128, BF, seed=3, spare=5), [1, 1])
+    _run(Setup(0, [9000], 8, 2, 64, F16, seed=3, spare=5), [3])
     _run(Setup(0, [3000, 700], 8, 2, 128, BF, seed=4, spare=60), [50, 50])
 
 
@@ -169,9 +183,11 @@ def test_longest_may_be_too_small():
     grown."""
     _say("branches: device lengths beyond the host's")
     for host in (0, 3):
-        s = Setup(100, [900, 3, 333], 8, 2, 128, BF, seed=host)
-        s.br.longest = host
-        _run(s, [1, 1, 1])
+        for counts in ([1, 1, 1], [40, 64, 1]):
+            s = Setup(100, [900, 3, 333], 8, 2, 128, BF, seed=host, spare=70)
+            s.br.longest = host
+            s.br.host_lengths = [host] * 3
+            _run(s, counts)
 
 
 def test_strides_scale_and_out():
@@ -210,26 +226,27 @@ def test_rows_behind_the_plan_stay():
 
 
 @pytest.mark.parametrize("where", ["shared", "own", "new"])
-def test_not_finite(where):
+@pytest.mark.parametrize("n", [3, 64])
+def test_not_finite(where, n):
     """Infinities in a value that is seen reach the output of those that see it, alone."""
     from treemoe_spec_amd.kernels.branch_attention import branch_attention
 
-    _say(f"branches: not finite, {where}")
-    s = Setup(90, [20, 70], 8, 2, 128, BF, seed=9)
-    q, k, v = s.new(6)
+    _say(f"branches: not finite, {where}, {n} tokens each")
+    s = Setup(90, [20, 70], 8, 2, 128, BF, seed=9, spare=70)
+    q, k, v = s.new(2 * n, scale=1.0)
     if where == "shared":
         page, off = s.kv.slot_of(80)
         s.kv.v[1, page, off, 1, 5] = float("inf")
     elif where == "own":
         s.br.v[1, 1, 69, 1, 5] = float("inf")
     else:
-        v[4, 1, 5] = float("inf")      # the second branch's second token
+        v[n + 1, 1, 5] = float("inf")      # the second branch's second token
     out = branch_attention(q.cuda(), k.cuda(), v.cuda(), s.kv, s.br, 1)
     torch.cuda.synchronize()
-    hit = torch.zeros(6, 8, 128, dtype=torch.bool)
-    hit[{"shared": 0, "own": 3, "new": 4}[where]:, 4:, 5] = True
-    assert bool((out.view(6, 8, 128).cpu().isinf() == hit).all())
-    assert bool(out.view(6, 8, 128).cpu()[~hit].isfinite().all())
+    hit = torch.zeros(2 * n, 8, 128, dtype=torch.bool)
+    hit[{"shared": 0, "own": n, "new": n + 1}[where]:, 4:, 5] = True
+    assert bool((out.view(2 * n, 8, 128).cpu().isinf() == hit).all())
+    assert bool(out.view(2 * n, 8, 128).cpu()[~hit].isfinite().all())
 
 
 def test_hidden_scores():

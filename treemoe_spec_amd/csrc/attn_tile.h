@@ -185,6 +185,10 @@ struct Feed {
           page[j] = table[(first + min(wave_key() + j * kPartKeys, left)) >> p.page_shift];
     }
   }
+  // The last key that can be seen in the stage at kb, where `last` is the range's.
+  static __device__ __forceinline__ int last_of(const PromptParams&, int, int last) {
+    return last;
+  }
   // The first head's K and V of one key.
   static __device__ __forceinline__ void key_at(const PromptParams& p, const Item& it, int key,
                                                 const uint16_t*& kr, const uint16_t*& vr) {
@@ -414,9 +418,10 @@ __device__ __forceinline__ void products(const uint8_t* vt, const uint8_t* kt_, 
 // The weights of the stage's 32 KT keys kb .. against the running maximum.  mask: some key
 // lies past the last one that some row sees.
 template <int DT, int HD, int KT = 2>
-__device__ __forceinline__ void weigh(float scale_log2, int kb, bool mask, Rows<HD>& r) {
+__device__ __forceinline__ void weigh(float scale_log2, int kb, bool mask, int seen,
+                                      Rows<HD>& r) {
   if (mask) {
-    const int left = r.seen - kb - 4 * ((int)(threadIdx.x & 63) >> 5);
+    const int left = seen - kb - 4 * ((int)(threadIdx.x & 63) >> 5);
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -454,6 +459,14 @@ __device__ __forceinline__ void weigh(float scale_log2, int kb, bool mask, Rows<
       r.pw[s][j] = w;
     }
   r.l += sum[0] + sum[1];
+}
+
+// The same for a stage of a Feed: full, the last key that every row sees.
+template <int DT, int HD, class FEED, int KT = 2>
+__device__ __forceinline__ void weigh_stage(const typename FEED::Params& p, int kb, int full,
+                                            Rows<HD>& r) {
+  weigh<DT, HD, KT>(p.scale_log2, kb, kb + 32 * KT - 1 > FEED::last_of(p, kb, full),
+                    FEED::last_of(p, kb, r.seen), r);
 }
 
 // What a workgroup works on.
@@ -549,6 +562,7 @@ __device__ __forceinline__ void retake(const typename FEED::Params& p, const Ite
     for (int x = 0; x < 16; ++x) r.o[ht][x] = 0.0f;
   for (int s = s0; s < n; s += step) {
     const int first = it.begin + s * KEYS, end = min(first + KEYS, it.end);
+    const int seen = FEED::last_of(p, first, r.seen);
 #pragma unroll 1
     for (int key = first; key < end; ++key) {
       const uint16_t *kr, *vr;
@@ -565,7 +579,7 @@ __device__ __forceinline__ void retake(const typename FEED::Params& p, const Ite
         for (int e = 0; e < 8; ++e) dot = fmaf(a[e], b[e], dot);
       }
       dot += __shfl_xor(dot, 32);
-      if (key > r.seen) continue;
+      if (key > seen) continue;
       const float x = dot * p.scale_log2;
       const float mn = fmaxf(m, x);
       const float a = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -626,6 +640,120 @@ __device__ __forceinline__ void end_rows(const PromptParams& p, const Item& it, 
   }
 }
 
+// The end of a turn: no wave of the workgroup goes on before all have come here.  What
+// a turn read from LDS its products have used, so no reads are waited for.
+__device__ __forceinline__ void turn_end() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_barrier" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// The same turns on tiles of 128 rows: waves w and w + 4 have the same 32 rows, waves 0-3
+// take the even stages and waves 4-7 the odd ones, each four with buffers of their own.
+// At the end the two outputs of a row are joined through LDS.
+template <int HD>
+struct PairShared {
+  __attribute__((aligned(1024))) uint8_t tiles[8][Shape<HD>::kTile];
+  float stat[4][64][2];
+};
+template <int DT, int HD, class FEED>
+__device__ __forceinline__ void pair_body(const typename FEED::Params& p, const Item& it,
+                                          int kvhead, PairShared<HD>& lds) {
+  uint8_t *const s_ka0 = lds.tiles[0], *const s_va0 = lds.tiles[1], *const s_ka1 = lds.tiles[2],
+          *const s_va1 = lds.tiles[3], *const s_kb0 = lds.tiles[4], *const s_vb0 = lds.tiles[5],
+          *const s_kb1 = lds.tiles[6], *const s_vb1 = lds.tiles[7];
+  float(*const s_stat)[64][2] = lds.stat;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int second = wave >> 2;
+  Rows<HD> r;
+  const Place at = begin_rows<HD>(p, it, kvhead, it.tile * 128 + (wave & 3) * 32, r);
+  const int full = at.full;
+  const int n = it.end > it.begin ? (it.end - it.begin + kKeys - 1) / kKeys : 0;
+  // stages of the first four waves; the last of the second four may lie past the range,
+  // all of it masked
+  const int rounds = (n + 1) / 2;
+  if (n > 0) {
+    FEED feed;
+    const int begin = it.begin + second * kKeys;
+    feed.start(p, it, kvhead, begin, 2 * kKeys);
+    // Load group g(s), in slot s % 2: K of round s and V of round s - 1, what the products
+    // M(s) = {O += V P of s - 1, S = K Q of s} read.  Round s: W(s) weighs its scores, then
+    // M(s + 1), and behind it g(s + 2) is requested, whose slot all four waves left with
+    // M(s) two turns before; W(s) waits for g(s + 1) at its end.  The second four waves do
+    // all this one turn later.
+    auto request = [&](int s, uint8_t* kn, uint8_t* vn) TM_INLINE {
+      if (s > rounds) return;
+      if (s > 0) feed.load_v(p, vn);
+      if (s < rounds) feed.load_k(p, kn);
+    };
+    // W(s), M(s + 1) with g(s + 1) at kc, vc; g(s + 2) goes to kn, vn.  (The last one's
+    // scores, of a stage that is not there, are not used.)
+    auto round = [&](int s, uint8_t* kc, uint8_t* vc, uint8_t* kn, uint8_t* vn) TM_INLINE {
+      const int kb = begin + 2 * s * kKeys;
+      weigh_stage<DT, HD, FEED>(p, kb, full, r);
+      wait_vm<0>();
+      turn_end();
+      products<DT, HD, true, true>(vc, kc, r);
+      request(s + 2, kn, vn);
+      turn_end();
+    };
+    auto all = [&](uint8_t* ka, uint8_t* va, uint8_t* kb, uint8_t* vb) TM_INLINE {
+      request(0, ka, va);
+      request(1, kb, vb);
+      wait_vm<0>();
+      turn_end();
+      if (second) turn_end();
+      products<DT, HD, false, true>(va, ka, r);
+      turn_end();
+      int s = 0;
+      for (; s + 2 <= rounds; s += 2) {
+        round(s, kb, vb, ka, va);
+        round(s + 1, ka, va, kb, vb);
+      }
+      if (s < rounds) round(s, kb, vb, ka, va);
+    };
+    if (second) {
+      all(s_kb0, s_vb0, s_kb1, s_vb1);
+    } else {
+      all(s_ka0, s_va0, s_ka1, s_va1);
+      turn_end();
+    }
+  }
+  retake<DT, HD, FEED>(p, it, kvhead, second, 2, n, r);
+  // the second four waves' outputs, each where a buffer was
+  const int w4 = wave & 3;
+  uint8_t* const box = w4 == 0 ? s_ka0 : w4 == 1 ? s_ka1 : w4 == 2 ? s_va0 : s_va1;
+  f32x4_t* const mine = reinterpret_cast<f32x4_t*>(box) + lane;
+  __syncthreads();
+  if (second) {
+#pragma unroll
+    for (int ht = 0; ht < HD / 32; ++ht)
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        mine[64 * (4 * ht + x)] =
+            f32x4_t{r.o[ht][4 * x], r.o[ht][4 * x + 1], r.o[ht][4 * x + 2], r.o[ht][4 * x + 3]};
+    s_stat[w4][lane][0] = r.m;
+    s_stat[w4][lane][1] = r.l;
+  }
+  __syncthreads();
+  if (second) return;
+  const float m1 = s_stat[w4][lane][0], l1 = s_stat[w4][lane][1];
+  const float m = fmaxf(r.m, m1), ref = m == -INFINITY ? 0.0f : m;
+  const float a = __builtin_amdgcn_exp2f(r.m - ref), b = __builtin_amdgcn_exp2f(m1 - ref);
+  r.l = r.l * a + l1 * b;
+  r.m = m;
+#pragma unroll
+  for (int ht = 0; ht < HD / 32; ++ht)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const f32x4_t o = mine[64 * (4 * ht + x)];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r.o[ht][4 * x + e] = r.o[ht][4 * x + e] * a + o[e] * b;
+    }
+  end_rows<DT, HD>(p, it, kvhead, 128, at, r);
+}
+
 // Short tiles: four waves of 32 rows, two workgroups a CU, which drift apart by themselves.
 template <int DT, int HD, class FEED>
 __device__ __forceinline__ void short_body(const typename FEED::Params& p, const Item& it,
@@ -633,7 +761,6 @@ __device__ __forceinline__ void short_body(const typename FEED::Params& p, const
                                            uint8_t* s_k1, uint8_t* s_v1) {
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int n = it.end > it.begin ? (it.end - it.begin + kKeys - 1) / kKeys : 0;
-  const float scale_log2 = p.scale_log2;
   Rows<HD> r;
   const Place at = begin_rows<HD>(p, it, kvhead, it.tile * 128 + wave * 32, r);
   const int full = at.full;
@@ -649,7 +776,7 @@ __device__ __forceinline__ void short_body(const typename FEED::Params& p, const
         feed.load_v(p, vn);
       }
       products<DT, HD, false, true>(vc, kc, r);
-      weigh<DT, HD>(scale_log2, kb, kb + kKeys - 1 > full, r);
+      weigh_stage<DT, HD, FEED>(p, kb, full, r);
       products<DT, HD, true, false>(vc, kc, r);
     };
     feed.load_k(p, s_k0);
@@ -702,7 +829,7 @@ __device__ __forceinline__ void few_body(const typename FEED::Params& p, const I
     products<DT, HD, false, true>(vt, kt, r);
     __builtin_amdgcn_sched_barrier(0);
     if (more) feed.load_k(p, kt);
-    weigh<DT, HD>(p.scale_log2, kb, kb + kKeys - 1 > full, r);
+    weigh_stage<DT, HD, FEED>(p, kb, full, r);
     if (more)
       wait_vm<kLoads>();
     else

@@ -17,6 +17,12 @@
 // by their tables, and no key moves.
 #include <algorithm>
 #include <new>
+#ifndef TM_NT
+#define TM_NT 2
+#endif
+#ifndef TM_OWNFIRST
+#define TM_OWNFIRST 0
+#endif
 
 #include "attn_tile.h"
 #include "prompt_parts.h"
@@ -33,6 +39,7 @@ struct BranchParams : PromptParams {   // k, v: the layer's [rows, capacity, kvh
   const int4* units;                   // (branch, tile, first token, tokens), or NULL:
   int count, unit_tiles;               // `count` tokens of every branch
   int rows, capacity;
+  int span;                            // keys of a range
   int parts;                           // leaves partials even where one part has all own keys
 };
 
@@ -53,6 +60,9 @@ struct BranchFeed {
   int row;                 // the row of one of the wave's keys in the next stage
   int v_first, v_left, v_row;  // of the stage whose K came last
 
+  static __device__ __forceinline__ int last_of(const BranchParams&, int, int last) {
+    return last;
+  }
   static __device__ __forceinline__ int wave() {
     return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) & (NW - 1);
   }
@@ -91,7 +101,8 @@ struct BranchFeed {
     v_first = v_left = v_row = 0;
     look_up(p);
   }
-  template <bool V>
+  // AUX 2: non-temporal
+  template <bool V, int AUX>
   __device__ __forceinline__ void load(const BranchParams& p, int first_, int left_, int row_,
                                        uint8_t* tile) const {
     const int lane = threadIdx.x & 63, mine = lane / S::kChunks;
@@ -106,11 +117,11 @@ struct BranchFeed {
           V ? new_v + (int64_t)key * p.new_v_stride : new_k + (int64_t)key * p.new_k_stride;
       const int chunk = (lane & (S::kChunks - 1)) ^ (V ? S::swz_v(j) : S::swz_k(j));
       __builtin_amdgcn_global_load_lds((glb_void*)((key < len ? held : fresh_) + chunk * 8),
-                                       (lds_void*)(tile + (wave() * kLoads + i) * 1024), 16, 0, 0);
+                                       (lds_void*)(tile + (wave() * kLoads + i) * 1024), 16, 0, AUX);
     }
   }
   __device__ __forceinline__ void load_k(const BranchParams& p, uint8_t* tile) {
-    load<false>(p, first, left, row, tile);
+    load_any<false>(p, first, left, row, tile);
     v_first = first;
     v_left = left;
     v_row = row;
@@ -119,56 +130,71 @@ struct BranchFeed {
     look_up(p);
   }
   __device__ __forceinline__ void load_v(const BranchParams& p, uint8_t* tile) {
-    load<true>(p, v_first, v_left, v_row, tile);
+    load_any<true>(p, v_first, v_left, v_row, tile);
+  }
+  // What a branch holds alone is read once; NT_FIGURES
+  template <bool V>
+  __device__ __forceinline__ void load_any(const BranchParams& p, int first_, int left_, int row_,
+                                           uint8_t* tile) const {
+    if (p.origin == nullptr)
+      load<V, TM_NT>(p, first_, left_, row_, tile);
+    else
+      load<V, 0>(p, first_, left_, row_, tile);
   }
 };
 
-// A workgroup's part of a branch: its rows against a range of its keys.
+// A part of a branch: rows of a tile against a range of its keys.
 struct Work {
   Item it;
   int kvhead;
-  int lo, hi;  // the new keys of the range that this workgroup stores
+  int len;     // keys that the branch held
+  int lo, hi;  // the new keys of the range, which are stored with it
 };
-__device__ __forceinline__ Work work_of(const BranchParams& p, int block, int tile_rows) {
+// Part `at` of all.  Ranges are whole stages, and go by the branch's own length, so that
+// they hold all its keys even where it is longer than the host took it for.  Before the
+// branch's keys lie `base` others.
+template <int STAGE>
+__device__ __forceinline__ Work work_of(const BranchParams& p, int kvhead, int at, int tile_rows,
+                                        int base = 0) {
   Work w;
-  w.kvhead = block % p.kvh;
-  const int at = block / p.kvh, chunk = at % p.chunks, unit = at / p.chunks;
+  w.kvhead = kvhead;
+  const int chunk = at % p.chunks, unit = at / p.chunks;
   Item& it = w.it;
   if (p.units != nullptr) {
     const int4 u = p.units[unit];
-    it.k0 = u.x;
-    it.tile = u.y;
-    it.q0 = u.z;
-    it.q_len = u.w;
+    it.k0 = __builtin_amdgcn_readfirstlane(u.x);
+    it.tile = __builtin_amdgcn_readfirstlane(u.y);
+    it.q0 = __builtin_amdgcn_readfirstlane(u.z);
+    it.q_len = __builtin_amdgcn_readfirstlane(u.w);
   } else {
     it.k0 = unit / p.unit_tiles;
-    it.tile = unit % p.unit_tiles;
+    it.tile = unit - it.k0 * p.unit_tiles;
     it.q0 = it.k0 * p.count;
     it.q_len = p.count;
   }
-  const int len = min(max(__builtin_amdgcn_readfirstlane(p.lengths[it.k0]), 0), p.capacity);
-  it.k_len = len + it.q_len;
-  // ranges by the branch's own length: they hold all its keys whatever the host took it for
+  w.len = min(max(__builtin_amdgcn_readfirstlane(p.lengths[it.k0]), 0), p.capacity);
+  it.k_len = base + w.len + it.q_len;
   const int per = (it.k_len + p.chunks - 1) / p.chunks;
-  const int span = (per + kKeys - 1) / kKeys * kKeys;
+  const int span = max((per + STAGE - 1) / STAGE * STAGE, p.span);
   const int last_token = min(it.q_len - 1, (it.tile * tile_rows + tile_rows - 1) / p.group);
-  it.begin = min(chunk * span, it.k_len);
+  it.begin = (int)min((int64_t)chunk * span, (int64_t)it.k_len);
   const int end = min(it.begin + span, it.k_len);
-  it.end = min(end, len + last_token + 1);
+  it.end = min(end, base + w.len + last_token + 1);
   it.slot = p.parts ? unit * p.chunks + chunk : -1;
-  w.lo = it.tile == 0 ? max(it.begin, len) : end;
-  w.hi = end;
+  w.hi = it.tile == 0 ? end - base : 0;
+  w.lo = max(it.begin - base, w.len);
   return w;
 }
 
-// The new keys and values lo .. hi - 1 of the head into the branch's own row.
-template <int HD>
-__device__ __forceinline__ void store_new(const BranchParams& p, const Work& w) {
+// The new keys and values lo .. hi - 1 of the head into the branch's own row, by THREADS
+// threads of which this is the `me`-th.
+template <int HD, int THREADS>
+__device__ __forceinline__ void store_new(const BranchParams& p, const Work& w, int me) {
   constexpr int kPieces = HD / 8;
-  const int len = w.it.k_len - w.it.q_len, hi = min(w.hi, p.capacity);
-  for (int x = threadIdx.x; x < (hi - w.lo) * kPieces; x += kThreads) {
+  const int hi = min(w.hi, p.capacity);
+  for (int x = me; x < (hi - w.lo) * kPieces; x += THREADS) {
     const int key = w.lo + x / kPieces, e = w.kvhead * HD + x % kPieces * 8;
-    const int64_t from = w.it.q0 + key - len;
+    const int64_t from = w.it.q0 + key - w.len;
     const int64_t to = (int64_t)w.it.k0 * p.row_stride + key * p.k_stride + e;
     *reinterpret_cast<u32x4_t*>(const_cast<uint16_t*>(p.k) + to) =
         *reinterpret_cast<const u32x4_t*>(p.new_k + from * p.new_k_stride + e);
@@ -188,31 +214,46 @@ struct LeanShared {
   float stat[4][32][2];
 };
 
-// S^T = K Q^T of the stage at kt_.
-template <int DT, int HD>
-__device__ __forceinline__ void lean_scores(const uint8_t* kt_, Rows<HD>& r) {
+// What comes behind is not begun before the fragments are in their registers.
+template <int N>
+__device__ __forceinline__ void refill_after(u32x4_t (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
+  __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));  // LDS reads
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// S^T = K Q^T of the stage at kt_, whose place is free for `refill` once its fragments are
+// read.
+template <int DT, int HD, class REFILL>
+__device__ __forceinline__ void lean_scores(const uint8_t* kt_, Rows<HD>& r, REFILL&& refill) {
   const int at = k_offset<HD>();
   u32x4_t f[HD / 16];
 #pragma unroll
   for (int ks = 0; ks < HD / 16; ++ks)
     f[ks] = *reinterpret_cast<const u32x4_t*>(kt_ + (at ^ (32 * ks)));
+  refill_after(f);
+  refill();
   f32x16_t sc = {};
 #pragma unroll
   for (int ks = 0; ks < HD / 16; ++ks) sc = mfma32<DT>(f[ks], r.q[ks], sc);
   r.sc[0] = sc;
 }
 // O^T += V^T P^T of the stage at vt.
-template <int DT, int HD>
-__device__ __forceinline__ void lean_outputs(const uint8_t* vt, Rows<HD>& r) {
+template <int DT, int HD, class REFILL>
+__device__ __forceinline__ void lean_outputs(const uint8_t* vt, Rows<HD>& r, REFILL&& refill) {
   int lo, hi;
   v_offsets<HD>(lo, hi);
+  u32x4_t vf[kLean / 16][HD / 32];
 #pragma unroll
-  for (int s = 0; s < kLean / 16; ++s) {
-    u32x4_t vf[HD / 32];
-    read_v<HD>(vt, fresh(lo), fresh(hi), s, vf);
+  for (int s = 0; s < kLean / 16; ++s) read_v<HD>(vt, fresh(lo), fresh(hi), s, vf[s]);
 #pragma unroll
-    for (int ht = 0; ht < HD / 32; ++ht) r.o[ht] = mfma32<DT>(vf[ht], r.pw[s], r.o[ht]);
-  }
+  for (int s = 0; s < kLean / 16; ++s) refill_after(vf[s]);
+  refill();
+#pragma unroll
+  for (int s = 0; s < kLean / 16; ++s)
+#pragma unroll
+    for (int ht = 0; ht < HD / 32; ++ht) r.o[ht] = mfma32<DT>(vf[s][ht], r.pw[s], r.o[ht]);
 }
 
 template <int DT, int HD, class FEED>
@@ -240,17 +281,17 @@ __device__ __forceinline__ void lean_body(const typename FEED::Params& p, const 
       wait_vm<0>();  // K and V, and the query rows
     else
       wait_vm<kLoads>();  // K: V is behind it
-    lean_scores<DT, HD>(kt, r);
-    __builtin_amdgcn_sched_barrier(0);
-    if (more) feed.load_k(p, kt);
-    weigh<DT, HD, 1>(p.scale_log2, kb, kb + kLean - 1 > full, r);
+    lean_scores<DT, HD>(kt, r, [&]() TM_INLINE {
+      if (more) feed.load_k(p, kt);
+    });
+    weigh_stage<DT, HD, FEED, 1>(p, kb, full, r);
     if (more)
       wait_vm<kLoads>();
     else
       wait_vm<0>();
-    lean_outputs<DT, HD>(vt, r);
-    __builtin_amdgcn_sched_barrier(0);
-    if (more) feed.load_v(p, vt);
+    lean_outputs<DT, HD>(vt, r, [&]() TM_INLINE {
+      if (more) feed.load_v(p, vt);
+    });
   }
   retake<DT, HD, FEED, kLean>(p, it, kvhead, wave, 4, n, r);
   const float l = r.l + __shfl_xor(r.l, 32);
@@ -298,28 +339,108 @@ __device__ __forceinline__ void lean_body(const typename FEED::Params& p, const 
   }
 }
 
-// Shared keys and the branches' own, where no branch adds more than 32 rows, in one launch:
-// the shared ones' workgroups first, tiles of 32 rows (where that is all) or of 128.  The
-// products over the shared keys run beside the reading of the others.
-enum Shared { kNone, kLeanTile, kShortTile };
-template <int DT, int HD, int SHARED>
-__global__ void __launch_bounds__(kThreads, 2) tm_branch_kernel(PromptParams s, BranchParams p,
-                                                               int shared_blocks) {
-  __shared__ __attribute__((aligned(1024))) LeanShared<HD> lds;
-  static_assert(sizeof(lds.tiles) == 4 * Shape<HD>::kTile, "two stages of 64 keys");
-  if (SHARED != kNone && (int)blockIdx.x < shared_blocks) {
-    const int kvhead = (int)blockIdx.x % s.kvh, at = (int)blockIdx.x / s.kvh;
-    if constexpr (SHARED == kLeanTile) {
-      lean_body<DT, HD, Feed<HD, true, 1, kLean>>(s, item_of(s, at, 32), kvhead, lds);
-    } else {
-      short_body<DT, HD, Feed<HD, true, 4>>(s, item_of(s, at, 128), kvhead, lds.tiles[0],
-                                            lds.tiles[1], lds.tiles[2], lds.tiles[3]);
+// A branch's own keys, up to 32 rows against one range by one wave: no barrier, and no
+// join within the workgroup.  What such a part costs most is its chain of latencies (the
+// length, the first keys, the last stores), so all of a step's are to run at once.
+template <int DT, int HD>
+__device__ __forceinline__ void wave_body(const BranchParams& p, const Work& w, uint8_t* kt) {
+  typedef BranchFeed<HD, 1, kLean> Own;
+  const Item& it = w.it;
+  const int lane = threadIdx.x & 63, half = lane >> 5, c32 = lane & 31;
+  const int n = it.end > it.begin ? (it.end - it.begin + kLean - 1) / kLean : 0;
+  const int rows = min(it.q_len * p.group, 32);
+  uint8_t* const vt = kt + kLean * Shape<HD>::kRow;
+  if (n == 0) {  // (what the join does not read is not written)
+    if (lane < rows && it.slot >= 0) {
+      float* const st =
+          p.stats + (((int64_t)it.slot * p.kvh + w.kvhead) * p.part_rows + lane) * 2;
+      st[0] = -INFINITY;
+      st[1] = 0.0f;
     }
     return;
   }
-  const Work w = work_of(p, (int)blockIdx.x - shared_blocks, 32);
-  store_new<HD>(p, w);
-  lean_body<DT, HD, BranchFeed<HD, 1, kLean>>(p, w.it, w.kvhead, lds);
+  Own feed;
+  feed.start(p, it, w.kvhead, it.begin, kLean);
+  feed.load_k(p, kt);
+  feed.load_v(p, vt);
+  Rows<HD> r;
+  const int full = begin_rows<HD>(p, it, w.kvhead, 0, r).full;
+  for (int s = 0; s < n; ++s) {
+    const int kb = it.begin + s * kLean;
+    const bool more = s + 1 < n;
+    if (s == 0)
+      wait_vm<0>();  // K and V, and the query rows
+    else
+      wait_vm<Own::kLoads>();  // K: V is behind it
+    lean_scores<DT, HD>(kt, r, [&]() TM_INLINE {
+      if (more) feed.load_k(p, kt);
+    });
+    weigh_stage<DT, HD, Own, 1>(p, kb, full, r);
+    if (more)
+      wait_vm<Own::kLoads>();
+    else
+      wait_vm<0>();
+    lean_outputs<DT, HD>(vt, r, [&]() TM_INLINE {
+      if (more) feed.load_v(p, vt);
+    });
+  }
+  retake<DT, HD, Own, kLean>(p, it, w.kvhead, 0, 1, n, r);
+  const float l = r.l + __shfl_xor(r.l, 32);
+  if (c32 >= rows) return;
+  if (it.slot < 0) {
+#pragma unroll
+    for (int ht = 0; ht < HD / 32; ++ht)
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        store_row<DT>(p, it.q0, c32, w.kvhead, HD, 32 * ht + 8 * x + 4 * half,
+                      f32x4_t{r.o[ht][4 * x], r.o[ht][4 * x + 1], r.o[ht][4 * x + 2],
+                              r.o[ht][4 * x + 3]},
+                      l);
+    return;
+  }
+  const int64_t slot = ((int64_t)it.slot * p.kvh + w.kvhead) * p.part_rows + c32;
+#pragma unroll
+  for (int ht = 0; ht < HD / 32; ++ht)
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      *reinterpret_cast<f32x4_t*>(p.part + slot * HD + 32 * ht + 8 * x + 4 * half) = f32x4_t{
+          r.o[ht][4 * x], r.o[ht][4 * x + 1], r.o[ht][4 * x + 2], r.o[ht][4 * x + 3]};
+  if (half == 0) {
+    p.stats[slot * 2] = r.m;
+    p.stats[slot * 2 + 1] = l;
+  }
+}
+
+// Shared keys and the branches' own, where no branch adds more than 32 rows, in one launch:
+// the shared ones' workgroups first, tiles of 32 rows (where that is all) or of 128; then
+// four parts of the branches' own a workgroup.  The products over the shared keys run
+// beside the reading of the others.
+enum Shared { kNone, kLeanTile, kShortTile };
+template <int DT, int HD, int SHARED>
+__global__ void __launch_bounds__(kThreads, 2) tm_branch_kernel(PromptParams s, BranchParams p,
+                                                               int shared_blocks, int own_parts) {
+  __shared__ __attribute__((aligned(1024))) LeanShared<HD> lds;
+  static_assert(sizeof(lds.tiles) == 4 * Shape<HD>::kTile, "two stages of 64 keys");
+  const int block = TM_OWNFIRST ? ((int)blockIdx.x + shared_blocks) % (int)gridDim.x : (int)blockIdx.x;
+  if (SHARED != kNone && block < shared_blocks) {
+    // (KV heads innermost: with 8 of them a head's workgroups, which share its keys, run
+    // on one XCD)
+    const int kvhead = block % p.kvh, at = block / p.kvh;
+    if constexpr (SHARED == kLeanTile)
+      lean_body<DT, HD, Feed<HD, true, 1, kLean>>(s, item_of(s, at, 32), kvhead, lds);
+    else
+      short_body<DT, HD, Feed<HD, true, 4>>(s, item_of(s, at, 128), kvhead, lds.tiles[0],
+                                            lds.tiles[1], lds.tiles[2], lds.tiles[3]);
+    return;
+  }
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  // (the waves of a workgroup take neighbouring heads of the same keys, which lie side by
+  // side)
+  const int id = (block - shared_blocks) * 4 + wave, at = id / p.kvh;
+  if (at >= own_parts) return;
+  const Work w = work_of<kLean>(p, id - at * p.kvh, at, 32);
+  store_new<HD, 64>(p, w, threadIdx.x & 63);
+  wave_body<DT, HD>(p, w, lds.tiles[wave]);
 }
 
 // Its own keys, tiles of 128 rows.
@@ -330,9 +451,88 @@ __global__ void __launch_bounds__(kThreads, 2) tm_branch_short_kernel(BranchPara
   __shared__ __attribute__((aligned(1024))) uint8_t s_v0[S::kTile];
   __shared__ __attribute__((aligned(1024))) uint8_t s_k1[S::kTile];
   __shared__ __attribute__((aligned(1024))) uint8_t s_v1[S::kTile];
-  const Work w = work_of(p, blockIdx.x, 128);
-  store_new<HD>(p, w);
+  const Work w = work_of<kKeys>(p, (int)blockIdx.x % p.kvh, (int)blockIdx.x / p.kvh, 128);
+  store_new<HD, kThreads>(p, w, threadIdx.x);
   short_body<DT, HD, BranchFeed<HD, 4>>(p, w.it, w.kvhead, s_k0, s_v0, s_k1, s_v1);
+}
+
+// The shared keys and behind them the branch's own as one sequence, for tiles that one
+// branch fills: nothing is left to share between branches, and nothing to join.  The own keys
+// begin with a stage of theirs, `base`, the shared ones in whole stages.
+struct ChainParams : BranchParams {
+  PromptParams shared;
+  int shared_keys, base;
+};
+template <int HD, int NW>
+struct ChainFeed {
+  typedef ChainParams Params;
+  typedef Feed<HD, true, NW> Pages;
+  typedef BranchFeed<HD, NW> Own;
+  static constexpr int kLoads = Pages::kLoads, kGroup = Pages::kGroup;
+  static_assert(kLoads == Own::kLoads, "the waits count either's loads");
+  Pages pages;
+  Own own;
+  int at, step;  // the next stage
+  bool v_own;    // of the stage whose K came last
+
+  static __device__ __forceinline__ int last_of(const ChainParams& p, int kb, int last) {
+    return kb < p.base ? min(last, p.shared_keys - 1) : last;
+  }
+  static __device__ __forceinline__ Item own_of(const ChainParams& p, const Item& it) {
+    Item o = it;
+    o.k_len -= p.base;
+    return o;
+  }
+  static __device__ __forceinline__ void key_at(const ChainParams& p, const Item& it, int key,
+                                                const uint16_t*& kr, const uint16_t*& vr) {
+    if (key < p.base)
+      Pages::key_at(p.shared, it, min(key, p.shared_keys - 1), kr, vr);
+    else
+      Own::key_at(p, own_of(p, it), key - p.base, kr, vr);
+  }
+  __device__ __forceinline__ void start(const ChainParams& p, const Item& it, int kvhead,
+                                        int begin, int step_) {
+    at = begin;
+    step = step_;
+    v_own = false;
+    if (begin < p.base) {
+      Item s = it;
+      s.k_len = p.shared_keys;
+      pages.start(p.shared, s, kvhead, begin, step);
+    }
+    const int first = begin < p.base ? begin + (p.base - begin + step - 1) / step * step : begin;
+    own.start(p, own_of(p, it), kvhead, first - p.base, step);
+  }
+  __device__ __forceinline__ void load_k(const ChainParams& p, uint8_t* tile) {
+    v_own = at >= p.base;
+    if (v_own)
+      own.load_k(p, tile);
+    else
+      pages.load_k(p.shared, tile);
+    at += step;
+  }
+  __device__ __forceinline__ void load_v(const ChainParams& p, uint8_t* tile) {
+    if (v_own)
+      own.load_v(p, tile);
+    else
+      pages.load_v(p.shared, tile);
+  }
+};
+template <int DT, int HD>
+__global__ void __launch_bounds__(512, 2) tm_branch_chain_pair_kernel(ChainParams p) {
+  __shared__ PairShared<HD> lds;
+  const Work w =
+      work_of<kKeys>(p, (int)blockIdx.x % p.kvh, (int)blockIdx.x / p.kvh, 128, p.base);
+  store_new<HD, 512>(p, w, threadIdx.x);
+  pair_body<DT, HD, ChainFeed<HD, 4>>(p, w.it, w.kvhead, lds);
+}
+template <int DT, int HD>
+__global__ void __launch_bounds__(kThreads, 2) tm_branch_chain_short_kernel(ChainParams p) {
+  __shared__ __attribute__((aligned(1024))) uint8_t tiles[4][Shape<HD>::kTile];
+  const Work w =
+      work_of<kKeys>(p, (int)blockIdx.x % p.kvh, (int)blockIdx.x / p.kvh, 128, p.base);
+  store_new<HD, kThreads>(p, w, threadIdx.x);
+  short_body<DT, HD, ChainFeed<HD, 4>>(p, w.it, w.kvhead, tiles[0], tiles[1], tiles[2], tiles[3]);
 }
 
 // Branches whose call has ended hold `count` more keys, or counts[b].
@@ -384,8 +584,9 @@ __device__ __forceinline__ RowParts parts_of(const Parts& s, int kvh, int kvhead
   return r;
 }
 
-// A wave joins the parts of one row: the maximum and the sum over the parts first, a lane
-// per part, then the weighted outputs in their order, four elements a lane.
+// A wave joins the parts of one row: the maximum and the sum over the parts, a lane per
+// part, then the weighted outputs in their order, four elements a lane and the lanes' groups a
+// part each.  The first kAhead parts of a group are asked for before anything is known.
 template <int DT, int HD>
 __global__ void __launch_bounds__(kThreads) tm_branch_join_kernel(BranchJoin p) {
   __shared__ float s_a[4][2 * kMaxParts];
@@ -394,8 +595,8 @@ __global__ void __launch_bounds__(kThreads) tm_branch_join_kernel(BranchJoin p) 
   if (unit >= (int64_t)p.T * p.Hq) return;
   const int t = (int)(unit / p.Hq), head = (int)(unit - (int64_t)t * p.Hq);
   const int kvhead = head / p.group, g = head - kvhead * p.group;
-  constexpr int kLanes = HD / 4, kGroups = 64 / kLanes;
-  const int e = 4 * (lane % kLanes);
+  constexpr int kLanes = HD / 4, kGroups = 64 / kLanes, kAhead = 8;
+  const int e = 4 * (lane % kLanes), group = lane / kLanes;
   int place, unit0;
   if (p.tokens != nullptr) {
     const int4 x = p.tokens[t];
@@ -405,37 +606,58 @@ __global__ void __launch_bounds__(kThreads) tm_branch_join_kernel(BranchJoin p) 
     place = t % p.count;
     unit0 = t / p.count * p.unit_tiles;
   }
-  const RowParts r[2] = {parts_of<HD>(p.shared, p.kvh, kvhead, 0, t * p.group + g, e),
-                         parts_of<HD>(p.own, p.kvh, kvhead, unit0, place * p.group + g, e)};
-  const int n[2] = {p.shared.chunks, p.own.chunks};
-  float m = -INFINITY;
+  // part c: the shared ones first
+  const RowParts r0 = parts_of<HD>(p.shared, p.kvh, kvhead, 0, t * p.group + g, e);
+  const RowParts r1 = parts_of<HD>(p.own, p.kvh, kvhead, unit0, place * p.group + g, e);
+  const int n0 = p.shared.chunks, n = n0 + p.own.chunks;
+  auto out_of = [&](int c) {
+    return c < n0 ? r0.o + c * r0.step * HD : r1.o + (c - n0) * r1.step * HD;
+  };
+  auto stat_of = [&](int c) {
+    return *reinterpret_cast<const float2*>(c < n0 ? r0.stats + c * r0.step * 2
+                                                   : r1.stats + (c - n0) * r1.step * 2);
+  };
+  f32x4_t first[kAhead];
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
-    for (int c = lane; c < n[s]; c += 64) m = fmaxf(m, r[s].stats[c * r[s].step * 2]);
+  for (int i = 0; i < kAhead; ++i)
+    first[i] = *reinterpret_cast<const f32x4_t*>(out_of(min(group + i * kGroups, n - 1)));
+  float m = -INFINITY, sum = 0.0f;
+  if (n <= 64) {
+    const float2 st = lane < n ? stat_of(lane) : float2{-INFINITY, 0.0f};
+    m = st.x;
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-  const float ref = m == -INFINITY ? 0.0f : m;
-  float sum = 0.0f;
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    const float a = __builtin_amdgcn_exp2f(st.x - (m == -INFINITY ? 0.0f : m));
+    sum = st.y * a;
+    s_a[wave][lane] = a;
+  } else {
+    for (int c = lane; c < n; c += 64) m = fmaxf(m, stat_of(c).x);
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
-    for (int c = lane; c < n[s]; c += 64) {
-      const float a = __builtin_amdgcn_exp2f(r[s].stats[c * r[s].step * 2] - ref);
-      sum += r[s].stats[c * r[s].step * 2 + 1] * a;
-      s_a[wave][(s ? n[0] : 0) + c] = a;
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    const float ref = m == -INFINITY ? 0.0f : m;
+    for (int c = lane; c < n; c += 64) {
+      const float2 st = stat_of(c);
+      const float a = __builtin_amdgcn_exp2f(st.x - ref);
+      sum = fmaf(st.y, a, sum);
+      s_a[wave][c] = a;
     }
+  }
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+  auto add = [&](int c, const f32x4_t& x) {
+    const float a = s_a[wave][c];
+    // (a part without keys has no output)
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
+    for (int i = 0; i < 4; ++i) o[i] = a == 0.0f ? o[i] : fmaf(x[i], a, o[i]);
+  };
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (group + i * kGroups < n) add(group + i * kGroups, first[i]);
 #pragma unroll 8
-    for (int c = lane / kLanes; c < n[s]; c += kGroups) {
-      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(r[s].o + c * r[s].step * HD);
-      const float a = s_a[wave][(s ? n[0] : 0) + c];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = fmaf(x[i], a, o[i]);
-    }
+  for (int c = group + kAhead * kGroups; c < n; c += kGroups)
+    add(c, *reinterpret_cast<const f32x4_t*>(out_of(c)));
 #pragma unroll
   for (int d = 32; d >= kLanes; d >>= 1)
 #pragma unroll
@@ -454,7 +676,10 @@ __global__ void __launch_bounds__(kThreads) tm_branch_join_kernel(BranchJoin p) 
 #define TM_C1 128
 #endif
 #ifndef TM_C2
-#define TM_C2 256
+#define TM_C2 128
+#endif
+#ifndef TM_W2
+#define TM_W2 3072
 #endif
 constexpr int64_t kMaxStride = 1 << 24;
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -472,7 +697,8 @@ struct BranchPlan {
   PrefixPlan prefix;               // the shared keys
   Shared shared;
   bool few;                        // one launch for both kinds of keys
-  int64_t units, chunks;           // of the branches' own keys
+  bool chain, pair;                // both as one sequence; with eight waves
+  int64_t units, chunks, span;     // of the branches' own keys
   int64_t own_rows;                // rows of one of their partials
   int64_t prefix_slots, own_slots; // (of one KV head)
   int64_t prefix_floats, floats;   // of the workspace
@@ -506,22 +732,31 @@ int plan_branches(int64_t T, int64_t units, int64_t max_count, int64_t S, int64_
                     ceil_div(S, o->shared == kLeanTile ? 4 * kLean : 4 * kKeys)));
     f.chunk_len = std::max(step, ceil_div(ceil_div(S, chunks), step) * step);
     f.chunks = ceil_div(S, f.chunk_len);
-  } else if (S > 0) {
+  }
+  // Tiles of 128 rows that the branches fill by themselves have nothing to share.  CHAIN_FIGURES
+  const int64_t base = ceil_div(S, kKeys) * kKeys;
+  o->chain = !o->few && 4 * T * group >= 3 * units * 128 && base + longest + max_count < INT32_MAX / 2;
+  if (S > 0 && !o->few && !o->chain) {
     const int rc = tm_prefix_plan(T, S, Hq, kvh, &o->prefix);
     if (rc) return rc;
   }
-  const int64_t keys = longest + max_count;
-  const int64_t want = std::min<int64_t>(2 * kCUs / std::max<int64_t>(units * kvh, 1), kMaxParts);
-  o->chunks = std::max<int64_t>(1, std::min(want, ceil_div(keys, o->few ? TM_C2 : 4 * kKeys)));
+  const int64_t keys = longest + max_count + (o->chain ? base : 0);
+  o->pair = o->chain && keys >= 8 * kKeys;
+  const int64_t slots = o->few ? TM_W2 : o->pair ? kCUs : 2 * kCUs;
+  const int64_t want = std::min<int64_t>(slots / std::max<int64_t>(units * kvh, 1), kMaxParts);
+  const int64_t least = o->few ? TM_C2 : o->pair ? 8 * kKeys : 4 * kKeys;
+  const int64_t stage = o->few ? kLean : o->pair ? 2 * kKeys : kKeys;
+  o->chunks = std::max<int64_t>(1, std::min(want, ceil_div(keys, least)));
+  o->span = ceil_div(ceil_div(keys, o->chunks), stage) * stage;
   o->own_rows = o->few ? std::min<int64_t>(32, max_count * group) : rows;
-  o->prefix_slots = S > 0 ? o->prefix.tiles * o->prefix.chunks : 0;
-  const bool joined = S > 0 || o->chunks > 1;
+  o->prefix_slots = S > 0 && !o->chain ? o->prefix.tiles * o->prefix.chunks : 0;
+  const bool joined = o->prefix_slots > 0 || o->chunks > 1;
   o->own_slots = joined ? units * o->chunks : 0;
   if (o->own_slots > INT32_MAX ||
-      (o->prefix_slots + units * o->chunks) * kvh > UINT32_MAX / kThreads ||
+      (o->prefix_slots + units * o->chunks) * kvh > UINT32_MAX / 512 ||
       T * Hq > UINT32_MAX / 64)
     return TM_ERR_SHAPE;
-  o->prefix_floats = S > 0 ? kvh * (hd + 2) * o->prefix_slots * o->prefix.part_rows : 0;
+  o->prefix_floats = kvh * (hd + 2) * o->prefix_slots * o->prefix.part_rows;
   o->prefix_floats = ceil_div(o->prefix_floats, 4) * 4;  // (16-byte stores behind them)
   o->floats = o->prefix_floats + kvh * (hd + 2) * o->own_slots * o->own_rows;
   return TM_OK;
@@ -532,19 +767,32 @@ bool vec_ok(const void* p, int64_t stride) { return (uintptr_t)p % 16 == 0 && st
 template <int DT, int HD>
 void launch_own(const PromptParams& s, const BranchParams& p, const BranchPlan& o,
                 hipStream_t st) {
-  const int64_t own = o.units * o.chunks * p.kvh, shared = o.prefix_slots * p.kvh;
+  const int64_t parts = o.units * o.chunks, shared = o.prefix_slots * p.kvh;
+  const int64_t own = o.few ? ceil_div(parts * p.kvh, 4) : parts * p.kvh;
   const dim3 block(kThreads);
-  if (!o.few)
+  if (o.chain) {
+    ChainParams c;
+    static_cast<BranchParams&>(c) = p;
+    c.shared = s;
+    c.shared_keys = s.k_len;
+    c.base = (int)(ceil_div(s.k_len, kKeys) * kKeys);
+    if (o.pair)
+      hipLaunchKernelGGL((tm_branch_chain_pair_kernel<DT, HD>), dim3((unsigned)own), dim3(512), 0,
+                         st, c);
+    else
+      hipLaunchKernelGGL((tm_branch_chain_short_kernel<DT, HD>), dim3((unsigned)own), block, 0, st,
+                         c);
+  } else if (!o.few)
     hipLaunchKernelGGL((tm_branch_short_kernel<DT, HD>), dim3((unsigned)own), block, 0, st, p);
   else if (o.shared == kNone)
     hipLaunchKernelGGL((tm_branch_kernel<DT, HD, kNone>), dim3((unsigned)own), block, 0, st, s, p,
-                       0);
+                       0, (int)parts);
   else if (o.shared == kLeanTile)
     hipLaunchKernelGGL((tm_branch_kernel<DT, HD, kLeanTile>), dim3((unsigned)(own + shared)),
-                       block, 0, st, s, p, (int)shared);
+                       block, 0, st, s, p, (int)shared, (int)parts);
   else
     hipLaunchKernelGGL((tm_branch_kernel<DT, HD, kShortTile>), dim3((unsigned)(own + shared)),
-                       block, 0, st, s, p, (int)shared);
+                       block, 0, st, s, p, (int)shared, (int)parts);
 }
 template <int DT, int HD>
 void launch_join(const BranchJoin& j, hipStream_t st) {
@@ -687,6 +935,8 @@ extern "C" int tm_branch_attention(
     s.k_len = (int)seq_len;
     while ((int64_t(1) << s.page_shift) < page_size) ++s.page_shift;
     s.cache_pages = (int)cache_pages;
+    // keys of a stage that a wave takes from one page: 16 (of prompt attention's tallest tiles 8)
+    s.wide = page_size >= 16 ? 1 : 0;
     const int64_t part_rows = o.prefix_slots * kvh * o.prefix.part_rows;
     s.part = at;
     s.stats = at + part_rows * hd;
@@ -697,15 +947,14 @@ extern "C" int tm_branch_attention(
       s.chunk_len = (int)o.prefix.chunk_len;
       s.part_rows = (int)o.prefix.part_rows;
       s.whole = 1;
-      s.wide = page_size >= 16 ? 1 : 0;  // keys of a stage that a wave takes from one page
-    } else {
+    } else if (!o.chain) {
       tm_prefix_launch(s, o.prefix, dtype, hd, page_size, st);
     }
+  }
+  j.shared.tile_rows = 1;
+  if (o.prefix_slots > 0)
     j.shared = {s.part, s.stats, (int)o.prefix.chunks, (int)o.prefix.tile_rows,
                 (int)o.prefix.part_rows, o.prefix.kind != 0};
-  } else {
-    j.shared.tile_rows = 1;
-  }
   p.k = (const uint16_t*)k_rows;
   p.v = (const uint16_t*)v_rows;
   p.k_stride = p.v_stride = stride_pos;
@@ -723,6 +972,7 @@ extern "C" int tm_branch_attention(
   p.rows = (int)rows;
   p.capacity = (int)capacity;
   p.chunks = (int)o.chunks;
+  p.span = (int)o.span;
   p.parts = o.own_slots > 0;
   p.part_rows = (int)o.own_rows;
   p.part = at;

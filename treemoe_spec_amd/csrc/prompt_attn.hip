@@ -38,14 +38,6 @@
 
 namespace {
 
-// The end of a turn: no wave of the workgroup goes on before all have come here.  What
-// a turn read from LDS its products have used, so no reads are waited for.
-__device__ __forceinline__ void turn_end() {
-  __builtin_amdgcn_sched_barrier(0);
-  asm volatile("s_barrier" ::: "memory");
-  __builtin_amdgcn_sched_barrier(0);
-}
-
 // Eight waves, two a SIMD, that take turns: one is in the matrix products of its stage
 // while the other weighs, a barrier between the turns.  Tiles of 256 rows: every wave has
 // 32 rows of its own, and all read the same stages.
@@ -94,7 +86,7 @@ __global__ void __launch_bounds__(512, 2) tm_prompt_tall_kernel(PromptParams p) 
     // one's scores, of a stage that is not there, are not used.)
     auto early = [&](int s, uint8_t* kc, uint8_t* vc, uint8_t* kn, uint8_t* vn) TM_INLINE {
       const int kb = it.begin + s * kKeys;
-      weigh<DT, HD>(scale_log2, kb, kb + kKeys - 1 > full, r);
+      weigh<DT, HD>(scale_log2, kb, kb + kKeys - 1 > full, r.seen, r);
       await(s + 1);
       turn_end();
       products<DT, HD, true, true>(vc, kc, r);
@@ -103,7 +95,7 @@ __global__ void __launch_bounds__(512, 2) tm_prompt_tall_kernel(PromptParams p) 
     };
     auto late = [&](int s, uint8_t* kc, uint8_t* vc, uint8_t* kn, uint8_t* vn) TM_INLINE {
       const int kb = it.begin + s * kKeys;
-      weigh<DT, HD>(scale_log2, kb, kb + kKeys - 1 > full, r);
+      weigh<DT, HD>(scale_log2, kb, kb + kKeys - 1 > full, r.seen, r);
       turn_end();
       products<DT, HD, true, true>(vc, kc, r);
       request(s + 3, kn, vn);
@@ -146,114 +138,11 @@ __global__ void __launch_bounds__(512, 2) tm_prompt_tall_kernel(PromptParams p) 
   end_rows<DT, HD>(p, it, kvhead, 256, at, r);
 }
 
-// The same turns on tiles of 128 rows: waves w and w + 4 have the same 32 rows, waves 0-3
-// take the even stages and waves 4-7 the odd ones, each four with buffers of their own.
-// At the end the two outputs of a row are joined through LDS.
 template <int DT, int HD, bool PAGED>
 __global__ void __launch_bounds__(512, 2) tm_prompt_pair_kernel(PromptParams p) {
-  typedef Shape<HD> S;
-  __shared__ __attribute__((aligned(1024))) uint8_t s_ka0[S::kTile];
-  __shared__ __attribute__((aligned(1024))) uint8_t s_va0[S::kTile];
-  __shared__ __attribute__((aligned(1024))) uint8_t s_ka1[S::kTile];
-  __shared__ __attribute__((aligned(1024))) uint8_t s_va1[S::kTile];
-  __shared__ __attribute__((aligned(1024))) uint8_t s_kb0[S::kTile];
-  __shared__ __attribute__((aligned(1024))) uint8_t s_vb0[S::kTile];
-  __shared__ __attribute__((aligned(1024))) uint8_t s_kb1[S::kTile];
-  __shared__ __attribute__((aligned(1024))) uint8_t s_vb1[S::kTile];
-  __shared__ float s_stat[4][64][2];
-
-  const int kvhead = (int)blockIdx.x % p.kvh;
+  __shared__ PairShared<HD> lds;
   const Item it = item_of(p, (int)blockIdx.x / p.kvh, 128);
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int second = wave >> 2;
-  Rows<HD> r;
-  const Place at = begin_rows<HD>(p, it, kvhead, it.tile * 128 + (wave & 3) * 32, r);
-  const int full = at.full;
-  const int n = it.end > it.begin ? (it.end - it.begin + kKeys - 1) / kKeys : 0;
-  // stages of the first four waves; the last of the second four may lie past the range,
-  // all of it masked
-  const int rounds = (n + 1) / 2;
-  const float scale_log2 = p.scale_log2;
-  if (n > 0) {
-    Feed<HD, PAGED, 4> feed;
-    const int begin = it.begin + second * kKeys;
-    feed.start(p, it, kvhead, begin, 2 * kKeys);
-    // Load group g(s), in slot s % 2: K of round s and V of round s - 1, what the products
-    // M(s) = {O += V P of s - 1, S = K Q of s} read.  Round s: W(s) weighs its scores, then
-    // M(s + 1), and behind it g(s + 2) is requested, whose slot all four waves left with
-    // M(s) two turns before; W(s) waits for g(s + 1) at its end.  The second four waves do
-    // all this one turn later.
-    auto request = [&](int s, uint8_t* kn, uint8_t* vn) TM_INLINE {
-      if (s > rounds) return;
-      if (s > 0) feed.load_v(p, vn);
-      if (s < rounds) feed.load_k(p, kn);
-    };
-    // W(s), M(s + 1) with g(s + 1) at kc, vc; g(s + 2) goes to kn, vn.  (The last one's
-    // scores, of a stage that is not there, are not used.)
-    auto round = [&](int s, uint8_t* kc, uint8_t* vc, uint8_t* kn, uint8_t* vn) TM_INLINE {
-      const int kb = begin + 2 * s * kKeys;
-      weigh<DT, HD>(scale_log2, kb, kb + kKeys - 1 > full, r);
-      wait_vm<0>();
-      turn_end();
-      products<DT, HD, true, true>(vc, kc, r);
-      request(s + 2, kn, vn);
-      turn_end();
-    };
-    auto all = [&](uint8_t* ka, uint8_t* va, uint8_t* kb, uint8_t* vb) TM_INLINE {
-      request(0, ka, va);
-      request(1, kb, vb);
-      wait_vm<0>();
-      turn_end();
-      if (second) turn_end();
-      products<DT, HD, false, true>(va, ka, r);
-      turn_end();
-      int s = 0;
-      for (; s + 2 <= rounds; s += 2) {
-        round(s, kb, vb, ka, va);
-        round(s + 1, ka, va, kb, vb);
-      }
-      if (s < rounds) round(s, kb, vb, ka, va);
-    };
-    if (second) {
-      all(s_kb0, s_vb0, s_kb1, s_vb1);
-    } else {
-      all(s_ka0, s_va0, s_ka1, s_va1);
-      turn_end();
-    }
-  }
-  retake<DT, HD, Feed<HD, PAGED, 4>>(p, it, kvhead, second, 2, n, r);
-  // the second four waves' outputs, each where a buffer was
-  const int w4 = wave & 3;
-  uint8_t* const box = w4 == 0 ? s_ka0 : w4 == 1 ? s_ka1 : w4 == 2 ? s_va0 : s_va1;
-  f32x4_t* const mine = reinterpret_cast<f32x4_t*>(box) + lane;
-  __syncthreads();
-  if (second) {
-#pragma unroll
-    for (int ht = 0; ht < HD / 32; ++ht)
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        mine[64 * (4 * ht + x)] =
-            f32x4_t{r.o[ht][4 * x], r.o[ht][4 * x + 1], r.o[ht][4 * x + 2], r.o[ht][4 * x + 3]};
-    s_stat[w4][lane][0] = r.m;
-    s_stat[w4][lane][1] = r.l;
-  }
-  __syncthreads();
-  if (second) return;
-  const float m1 = s_stat[w4][lane][0], l1 = s_stat[w4][lane][1];
-  const float m = fmaxf(r.m, m1), ref = m == -INFINITY ? 0.0f : m;
-  const float a = __builtin_amdgcn_exp2f(r.m - ref), b = __builtin_amdgcn_exp2f(m1 - ref);
-  r.l = r.l * a + l1 * b;
-  r.m = m;
-#pragma unroll
-  for (int ht = 0; ht < HD / 32; ++ht)
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const f32x4_t o = mine[64 * (4 * ht + x)];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) r.o[ht][4 * x + e] = r.o[ht][4 * x + e] * a + o[e] * b;
-    }
-  end_rows<DT, HD>(p, it, kvhead, 128, at, r);
+  pair_body<DT, HD, Feed<HD, PAGED, 4>>(p, it, (int)blockIdx.x % p.kvh, lds);
 }
 
 template <int DT, int HD, bool PAGED>
