@@ -640,10 +640,11 @@ int tm_branch_attention(const void* q, int64_t q_stride, const void* k, int64_t 
 
 /*
  * lengths[b] += counts[b], or `count` with counts NULL, up to capacity: after a step's
- * last layer.
+ * last layer.  With origin [rows, origin_stride], origin[b, t] = b for the places added.
  */
 int tm_branch_advance(int32_t* lengths, const int32_t* counts, int64_t count,
-                      int64_t rows, int64_t capacity, void* stream);
+                      int64_t rows, int64_t capacity, int32_t* origin,
+                      int64_t origin_stride, void* stream);
 
 /* Workspace bytes of tm_beam_select for these sizes. */
 int tm_beam_workspace(int64_t G, int64_t K, int64_t V, int64_t num, int64_t* bytes);

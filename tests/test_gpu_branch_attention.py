@@ -97,7 +97,8 @@ def _run(s, counts, layer=1, pad=0, scale=None, plan=None, **kw):
     return out
 
 
-HEADS = [(32, 8, 128), (8, 2, 64), (4, 4, 128), (3, 1, 64), (16, 2, 128), (7, 1, 128)]
+HEADS = [(32, 8, 128), (8, 2, 64), (4, 4, 128), (3, 1, 64), (16, 2, 128), (7, 1, 128),
+         (64, 1, 64)]
 
 
 @pytest.mark.parametrize("hq,kvh,hd", HEADS)
@@ -139,8 +140,8 @@ def test_ragged(counts, prefix, page, pad):
         assert not bool(out[sum(counts):].any())
 
 
-@pytest.mark.parametrize("prefix,page", [(0, 16), (63, 16), (64, 16), (65, 1), (300, 64), (1000, 16),
-                                         (2500, 64)])
+@pytest.mark.parametrize("prefix,page", [(0, 16), (63, 16), (64, 16), (65, 1), (300, 64),
+                                         (1000, 16), (2500, 64)])
 @pytest.mark.parametrize("counts", [[64], [32, 96, 31], [30, 0, 62, 128], [200, 150]])
 @pytest.mark.parametrize("hq,kvh,hd,dtype", [(8, 2, 128, BF), (32, 8, 64, F16)])
 def test_branches_that_fill_tiles(counts, prefix, page, hq, kvh, hd, dtype):

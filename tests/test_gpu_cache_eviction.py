@@ -59,7 +59,8 @@ def _mass(t, n, hq, kvh, hd, dtype, page, seed, scale=None, add=False, q_scale=2
     q, k, v = t_attn._qkv(t, n, hq, kvh, hd, dtype, seed, q_scale)
     kv = t_attn._cache(n, kvh, hd, dtype, page, seed)
     kv.append(1, k.cuda(), v.cuda(), 0)
-    before = 3.0 * torch.rand(kvh, n, generator=torch.Generator().manual_seed(seed)) if add else None
+    g = torch.Generator().manual_seed(seed)
+    before = 3.0 * torch.rand(kvh, n, generator=g) if add else None
     got = attention_mass(q.cuda(), kv, 1, None if before is None else before.cuda(), scale=scale)
     torch.cuda.synchronize()
     assert got.shape == (kvh, n) and got.dtype == torch.float32
@@ -68,7 +69,7 @@ def _mass(t, n, hq, kvh, hd, dtype, page, seed, scale=None, add=False, q_scale=2
 
 
 @pytest.mark.parametrize("hq,kvh,hd", [(32, 8, 128), (8, 2, 64), (4, 4, 128), (3, 1, 64),
-                                       (16, 2, 128), (7, 1, 128)])
+                                       (16, 2, 128), (7, 1, 128), (64, 1, 64)])
 @pytest.mark.parametrize("dtype", [BF, F16])
 @pytest.mark.parametrize("t,n,page", [(1, 1, 16), (1, 64, 16), (1, 65, 64), (1, 1000, 16),
                                       (2, 2, 16), (8, 300, 64), (9, 9, 1), (33, 200, 16),
@@ -236,7 +237,8 @@ def _check_evict(kv, mass, keep, positions=None, nxt=None, recent=0, sinks=0):
                                                       (2, 8, 128, BF, 1),
                                                       (2, 2, 16, torch.float32, 16)])
 @pytest.mark.parametrize("n,keep,recent,sinks", [
-    (1, 1, 0, 0), (2, 1, 0, 0), (100, 50, 0, 0), (100, 99, 10, 4), (130, 20, 16, 4), (65, 64, 64, 0),
+    (1, 1, 0, 0), (2, 1, 0, 0), (100, 50, 0, 0), (100, 99, 10, 4), (130, 20, 16, 4),
+    (65, 64, 64, 0),
     (64, 1, 0, 1), (200, 199, 0, 0), (1100, 1030, 64, 4), (2100, 100, 32, 4), (50, 50, 3, 0),
     (50, 90, 3, 0), (30, 0, 0, 0), (2048, 2000, 100, 4), (2049, 700, 64, 0)])
 def test_evict(n, keep, recent, sinks, layers, kvh, hd, dtype, page):
@@ -300,8 +302,8 @@ def test_evict_strided_inputs():
     n, keep = 300, 200
     mass = torch.rand(3, 4, 500, generator=g)
     pos = torch.rand(3, 4, 900, generator=g).argsort(2).to(torch.int32)[:, :, :250]
-    _check_evict(_cache_of(3, n, 2, 64, BF, 16, g), mass[:, 1:3, 60:400], keep, pos[:, 2:, :120], 1000,
-                 recent=30, sinks=2)
+    _check_evict(_cache_of(3, n, 2, 64, BF, 16, g), mass[:, 1:3, 60:400], keep,
+                 pos[:, 2:, :120], 1000, recent=30, sinks=2)
 
 
 def test_attention_after_eviction():

@@ -64,7 +64,7 @@ SIGNATURES: dict[str, list] = {
     "tm_branch_attention": [P, I64] * 3 + [I64, P, P, I64, I64, I64, I64, P, I64, I64, P, P]
                            + [I64] * 4 + [P, I64, P, I64, P, I64, P] + [I64] * 4
                            + [F32, I32, P, I64, P, I64, P],
-    "tm_branch_advance": [P, P, I64, I64, I64, P],
+    "tm_branch_advance": [P, P, I64, I64, I64, P, I64, P],
     "tm_beam_workspace": [I64] * 4 + [P],
     "tm_beam_select": [P, I32] + [I64] * 4 + [P, P, I64, I64, P, P, P, P, I64, P],
     "tm_reorder_rows": [P, I64, P, I64, I64, P, I64, I64, I64, P],

@@ -6,23 +6,27 @@
 //   out[t, h] = sum_j softmax_j(scale q[t, h] . k[j, h / group]) v[j, h / group].
 //
 // Decomposition.  The softmax over a row's keys splits into parts that leave their sum,
-// maximum and unnormalised output in fp32.  The shared keys are taken once for all
-// branches: their (token, head of the group) pairs are one long list of rows for prompt
-// attention's kernels, without a causal border.  A branch's own keys are taken by
-// workgroups of its own, few rows against one range of keys.  A last kernel joins a row's
-// parts, the shared ones first, each in key order, so results are the same on every run.
+// maximum and unnormalised output in fp32, which a last launch joins, the shared keys'
+// first, each in key order, so results are the same on every run.
+//   Few rows a branch (up to 32: decoded tokens, short drafts).  One launch.  The shared keys
+//   are taken once for all branches, whose (token, head of the group) pairs are one long list
+//   of rows: tiles of 32 where that is all, else prompt attention's tiles of 128, without a
+//   causal border.  A branch's own keys are taken by a wave or a workgroup a range.
+//   Many rows a branch (prompts behind a shared one).  Where the branches fill tiles of 128
+//   rows, shared and own keys are one sequence for a tile, and nothing is joined but the tiles
+//   of a last partial round.  Otherwise (drafts of 9 tokens, say) the shared keys go through
+//   prompt attention's kernels for all branches, the own ones through tiles of 128 rows.
 //
 // Position t of branch b lies in row origin[b][t] of the branch cache, the row of the
 // ancestor that stored it (without a table of origins, in row b).  So beams are reordered
 // by their tables, and no key moves.
+//
+// Bound by latency and by HBM at few rows: 4 beams over 517 keys 7 us and the join 3.5; 64
+// requests of up to 700 own keys over 4096 38 us for 107 MB, of which about 10 are the two
+// launches' chains of latencies; own keys alone stream at 4.2-5.6 TB/s.  By prompt
+// attention's matrix products and exponentials at many: 12 prompts over 4096 0.7 PFLOP/s.
 #include <algorithm>
 #include <new>
-#ifndef TM_NT
-#define TM_NT 2
-#endif
-#ifndef TM_OWNFIRST
-#define TM_OWNFIRST 0
-#endif
 
 #include "attn_tile.h"
 #include "prompt_parts.h"
@@ -39,6 +43,7 @@ struct BranchParams : PromptParams {   // k, v: the layer's [rows, capacity, kvh
   const int4* units;                   // (branch, tile, first token, tokens), or NULL:
   int count, unit_tiles;               // `count` tokens of every branch
   int rows, capacity;
+  int whole_units;                     // that take all keys in one part
   int span;                            // keys of a range
   int parts;                           // leaves partials even where one part has all own keys
 };
@@ -117,7 +122,8 @@ struct BranchFeed {
           V ? new_v + (int64_t)key * p.new_v_stride : new_k + (int64_t)key * p.new_k_stride;
       const int chunk = (lane & (S::kChunks - 1)) ^ (V ? S::swz_v(j) : S::swz_k(j));
       __builtin_amdgcn_global_load_lds((glb_void*)((key < len ? held : fresh_) + chunk * 8),
-                                       (lds_void*)(tile + (wave() * kLoads + i) * 1024), 16, 0, AUX);
+                                       (lds_void*)(tile + (wave() * kLoads + i) * 1024), 16, 0,
+                                       AUX);
     }
   }
   __device__ __forceinline__ void load_k(const BranchParams& p, uint8_t* tile) {
@@ -132,12 +138,13 @@ struct BranchFeed {
   __device__ __forceinline__ void load_v(const BranchParams& p, uint8_t* tile) {
     load_any<true>(p, v_first, v_left, v_row, tile);
   }
-  // What a branch holds alone is read once; NT_FIGURES
+  // What a branch holds alone is read once, and goes past the caches: 256 branches of 350 keys
+  // 81 us, else 86; 16 of up to 4000 48, 53.  (What beams share is read by several.)
   template <bool V>
   __device__ __forceinline__ void load_any(const BranchParams& p, int first_, int left_, int row_,
                                            uint8_t* tile) const {
     if (p.origin == nullptr)
-      load<V, TM_NT>(p, first_, left_, row_, tile);
+      load<V, 2>(p, first_, left_, row_, tile);
     else
       load<V, 0>(p, first_, left_, row_, tile);
   }
@@ -158,7 +165,11 @@ __device__ __forceinline__ Work work_of(const BranchParams& p, int kvhead, int a
                                         int base = 0) {
   Work w;
   w.kvhead = kvhead;
-  const int chunk = at % p.chunks, unit = at / p.chunks;
+  // the first units take all keys, the others' are split
+  const bool split = at >= p.whole_units;
+  const int rest = at - p.whole_units, chunks = split ? p.chunks : 1;
+  const int chunk = split ? rest % p.chunks : 0;
+  const int unit = split ? p.whole_units + rest / p.chunks : at;
   Item& it = w.it;
   if (p.units != nullptr) {
     const int4 u = p.units[unit];
@@ -174,13 +185,13 @@ __device__ __forceinline__ Work work_of(const BranchParams& p, int kvhead, int a
   }
   w.len = min(max(__builtin_amdgcn_readfirstlane(p.lengths[it.k0]), 0), p.capacity);
   it.k_len = base + w.len + it.q_len;
-  const int per = (it.k_len + p.chunks - 1) / p.chunks;
-  const int span = max((per + STAGE - 1) / STAGE * STAGE, p.span);
+  const int per = (it.k_len + chunks - 1) / chunks;
+  const int span = max((per + STAGE - 1) / STAGE * STAGE, split ? p.span : 0);
   const int last_token = min(it.q_len - 1, (it.tile * tile_rows + tile_rows - 1) / p.group);
   it.begin = (int)min((int64_t)chunk * span, (int64_t)it.k_len);
   const int end = min(it.begin + span, it.k_len);
   it.end = min(end, base + w.len + last_token + 1);
-  it.slot = p.parts ? unit * p.chunks + chunk : -1;
+  it.slot = p.parts && split ? rest : -1;
   w.hi = it.tile == 0 ? end - base : 0;
   w.lo = max(it.begin - base, w.len);
   return w;
@@ -413,15 +424,15 @@ __device__ __forceinline__ void wave_body(const BranchParams& p, const Work& w, 
 
 // Shared keys and the branches' own, where no branch adds more than 32 rows, in one launch:
 // the shared ones' workgroups first, tiles of 32 rows (where that is all) or of 128; then
-// four parts of the branches' own a workgroup.  The products over the shared keys run
-// beside the reading of the others.
+// the branches' own, a workgroup or (WAVES) a wave a part.  The products over the shared keys
+// run beside the reading of the others.
 enum Shared { kNone, kLeanTile, kShortTile };
-template <int DT, int HD, int SHARED>
+template <int DT, int HD, int SHARED, bool WAVES>
 __global__ void __launch_bounds__(kThreads, 2) tm_branch_kernel(PromptParams s, BranchParams p,
                                                                int shared_blocks, int own_parts) {
   __shared__ __attribute__((aligned(1024))) LeanShared<HD> lds;
   static_assert(sizeof(lds.tiles) == 4 * Shape<HD>::kTile, "two stages of 64 keys");
-  const int block = TM_OWNFIRST ? ((int)blockIdx.x + shared_blocks) % (int)gridDim.x : (int)blockIdx.x;
+  const int block = blockIdx.x;
   if (SHARED != kNone && block < shared_blocks) {
     // (KV heads innermost: with 8 of them a head's workgroups, which share its keys, run
     // on one XCD)
@@ -431,6 +442,13 @@ __global__ void __launch_bounds__(kThreads, 2) tm_branch_kernel(PromptParams s, 
     else
       short_body<DT, HD, Feed<HD, true, 4>>(s, item_of(s, at, 128), kvhead, lds.tiles[0],
                                             lds.tiles[1], lds.tiles[2], lds.tiles[3]);
+    return;
+  }
+  if constexpr (!WAVES) {
+    const int at = block - shared_blocks;
+    const Work w = work_of<kLean>(p, at % p.kvh, at / p.kvh, 32);
+    store_new<HD, kThreads>(p, w, threadIdx.x);
+    lean_body<DT, HD, BranchFeed<HD, 1, kLean>>(p, w.it, w.kvhead, lds);
     return;
   }
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -535,14 +553,19 @@ __global__ void __launch_bounds__(kThreads, 2) tm_branch_chain_short_kernel(Chai
   short_body<DT, HD, ChainFeed<HD, 4>>(p, w.it, w.kvhead, tiles[0], tiles[1], tiles[2], tiles[3]);
 }
 
-// Branches whose call has ended hold `count` more keys, or counts[b].
-__global__ void __launch_bounds__(kThreads) tm_branch_advance_kernel(int32_t* lengths,
-                                                                     const int32_t* counts,
-                                                                     int count, int rows,
-                                                                     int capacity) {
-  const int b = (int)(blockIdx.x * kThreads + threadIdx.x);
-  if (b < rows)
-    lengths[b] = min(max(lengths[b], 0) + max(counts != nullptr ? counts[b] : count, 0), capacity);
+// Branches whose call has ended hold `count` more keys, or counts[b], which lie in their own
+// rows.  A workgroup a branch.
+__global__ void __launch_bounds__(64) tm_branch_advance_kernel(int32_t* lengths,
+                                                               const int32_t* counts, int count,
+                                                               int capacity, int32_t* origin,
+                                                               int64_t origin_stride) {
+  const int b = blockIdx.x;
+  const int len = min(max(__builtin_amdgcn_readfirstlane(lengths[b]), 0), capacity);
+  const int n = counts != nullptr ? __builtin_amdgcn_readfirstlane(counts[b]) : count;
+  const int end = (int)min((int64_t)len + max(n, 0), (int64_t)capacity);
+  if (origin != nullptr)
+    for (int t = len + (int)threadIdx.x; t < end; t += 64) origin[b * origin_stride + t] = b;
+  if (threadIdx.x == 0) lengths[b] = end;
 }
 
 // Parts of one kind: `chunks` of every tile, as `few` lays rows down or as whole tiles.
@@ -556,6 +579,7 @@ struct BranchJoin {
   Parts shared, own;
   const int4* tokens;  // (branch, place in it, its first unit), or NULL:
   int count, unit_tiles;
+  int whole_units;     // the first ones, without parts
   int T, Hq, kvh, group;
   uint16_t* out;
   int64_t out_stride;
@@ -606,6 +630,8 @@ __global__ void __launch_bounds__(kThreads) tm_branch_join_kernel(BranchJoin p) 
     place = t % p.count;
     unit0 = t / p.count * p.unit_tiles;
   }
+  unit0 -= p.whole_units;
+  if (unit0 + (place * p.group + g) / p.own.tile_rows < 0) return;  // it has its output
   // part c: the shared ones first
   const RowParts r0 = parts_of<HD>(p.shared, p.kvh, kvhead, 0, t * p.group + g, e);
   const RowParts r1 = parts_of<HD>(p.own, p.kvh, kvhead, unit0, place * p.group + g, e);
@@ -672,15 +698,20 @@ __global__ void __launch_bounds__(kThreads) tm_branch_join_kernel(BranchJoin p) 
 
 // ------------------------------------------------------------------- host --
 
-#ifndef TM_C1
-#define TM_C1 128
-#endif
-#ifndef TM_C2
-#define TM_C2 128
-#endif
-#ifndef TM_W2
-#define TM_W2 3072
-#endif
+// How the work is split, measured at 32 heads over 8 of 128 in bf16, in us of a pass (graph
+// replays on changing inputs), one token a branch unless said:
+//   shared keys in as many workgroups as kSharedBlocks: 64 requests over 4096 with 64, 128
+//   and 256 of them 38, 40, 44; 48 chains of five tokens over 2003 29, 22, 23; 256 requests
+//   over 4096 114, 105, 119;
+//   own keys by workgroups (LEAN) or waves: 8 branches of up to 400 keys 14.3, 15.9; 16 16.6,
+//   15.9; 32 21.8, 18.7; 64 of up to 700 42, 40; 128 of up to 60 27, 21;
+//   at most kOwnWaves parts by waves: 64 of up to 700 with 2048, 3072 and 4096 44, 40, 44; 256
+//   of them 102, 103, 112; 16 of up to 4000 52, 47, 50.
+constexpr int64_t kSharedBlocks = 128;
+constexpr int64_t kOwnWaves = 3072;
+constexpr int64_t kLeanUnits = 64;     // (branch, KV head) pairs up to which a part is a workgroup
+constexpr int64_t kWaveKeys = 64;      // of a wave's part, or more
+constexpr int64_t kLongKeys = 8192;    // beyond them a branch leaves too many parts by waves
 constexpr int64_t kMaxStride = 1 << 24;
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -691,14 +722,18 @@ int check_heads(int64_t Hq, int64_t kvh, int64_t hd) {
 }
 
 // Rows of a tile of a branch: 32 where no branch has more, else 128.
-int64_t own_tile_rows(int64_t max_count, int64_t group) { return max_count * group <= 32 ? 32 : 128; }
+int64_t own_tile_rows(int64_t max_count, int64_t group) {
+  return max_count * group <= 32 ? 32 : 128;
+}
 
 struct BranchPlan {
   PrefixPlan prefix;               // the shared keys
   Shared shared;
   bool few;                        // one launch for both kinds of keys
+  bool waves;                      // a wave a part of own keys
   bool chain, pair;                // both as one sequence; with eight waves
   int64_t units, chunks, span;     // of the branches' own keys
+  int64_t whole_units;             // the first, which take them in one part
   int64_t own_rows;                // rows of one of their partials
   int64_t prefix_slots, own_slots; // (of one KV head)
   int64_t prefix_floats, floats;   // of the workspace
@@ -717,7 +752,6 @@ int plan_branches(int64_t T, int64_t units, int64_t max_count, int64_t S, int64_
   o->few = rows == 32;
   o->units = units;
   if (S > 0 && o->few) {
-    // ranges of shared keys: FIGURES
     const int64_t all = T * group;
     o->shared = all <= 32 ? kLeanTile : kShortTile;
     PrefixPlan& f = o->prefix;
@@ -726,34 +760,43 @@ int plan_branches(int64_t T, int64_t units, int64_t max_count, int64_t S, int64_
     f.tiles = ceil_div(all, f.tile_rows);
     f.part_rows = o->shared == kLeanTile ? all : 128;
     const int64_t step = o->shared == kLeanTile ? 4 * kLean : kKeys;
-    const int64_t want = std::max<int64_t>(1, TM_C1 / std::max<int64_t>(f.tiles * kvh, 1));
+    const int64_t want = std::max<int64_t>(1, kSharedBlocks / std::max<int64_t>(f.tiles * kvh, 1));
     const int64_t chunks = std::max<int64_t>(
         1, std::min(std::min<int64_t>(want, kMaxParts),
                     ceil_div(S, o->shared == kLeanTile ? 4 * kLean : 4 * kKeys)));
     f.chunk_len = std::max(step, ceil_div(ceil_div(S, chunks), step) * step);
     f.chunks = ceil_div(S, f.chunk_len);
   }
-  // Tiles of 128 rows that the branches fill by themselves have nothing to share.  CHAIN_FIGURES
+  // Tiles of 128 rows that the branches fill by themselves, three quarters of them at least,
+  // have nothing to share: 12 prompts of 1-333 tokens over 4096 206 us so, 257 with the shared
+  // keys and the own ones apart, joined.
   const int64_t base = ceil_div(S, kKeys) * kKeys;
-  o->chain = !o->few && 4 * T * group >= 3 * units * 128 && base + longest + max_count < INT32_MAX / 2;
+  o->chain = !o->few && 4 * T * group >= 3 * units * 128;
   if (S > 0 && !o->few && !o->chain) {
     const int rc = tm_prefix_plan(T, S, Hq, kvh, &o->prefix);
     if (rc) return rc;
   }
   const int64_t keys = longest + max_count + (o->chain ? base : 0);
   o->pair = o->chain && keys >= 8 * kKeys;
-  const int64_t slots = o->few ? TM_W2 : o->pair ? kCUs : 2 * kCUs;
-  const int64_t want = std::min<int64_t>(slots / std::max<int64_t>(units * kvh, 1), kMaxParts);
-  const int64_t least = o->few ? TM_C2 : o->pair ? 8 * kKeys : 4 * kKeys;
+  o->waves = o->few && units * kvh > kLeanUnits && keys <= kLongKeys;
+  const int64_t slots = o->waves ? kOwnWaves : o->pair ? kCUs : 2 * kCUs;
+  // Chained, as many as fill the chip's slots some whole times stay whole, and those left are
+  // split: of 600 tiles on 256 slots the last 88 (206 us, whole 234).
+  o->whole_units = o->chain ? units * kvh / slots * slots / kvh : 0;
+  const int64_t want = std::min<int64_t>(
+      slots / std::max<int64_t>((units - o->whole_units) * kvh, 1), kMaxParts);
+  const int64_t least = o->waves ? kWaveKeys : o->pair ? 8 * kKeys : 4 * kKeys;
   const int64_t stage = o->few ? kLean : o->pair ? 2 * kKeys : kKeys;
   o->chunks = std::max<int64_t>(1, std::min(want, ceil_div(keys, least)));
+  if (o->chain && o->chunks == 1) o->whole_units = units;
   o->span = ceil_div(ceil_div(keys, o->chunks), stage) * stage;
   o->own_rows = o->few ? std::min<int64_t>(32, max_count * group) : rows;
   o->prefix_slots = S > 0 && !o->chain ? o->prefix.tiles * o->prefix.chunks : 0;
   const bool joined = o->prefix_slots > 0 || o->chunks > 1;
-  o->own_slots = joined ? units * o->chunks : 0;
+  const int64_t split = units - o->whole_units;
+  o->own_slots = joined ? split * o->chunks : 0;
   if (o->own_slots > INT32_MAX ||
-      (o->prefix_slots + units * o->chunks) * kvh > UINT32_MAX / 512 ||
+      (o->prefix_slots + o->whole_units + split * o->chunks) * kvh > UINT32_MAX / 512 ||
       T * Hq > UINT32_MAX / 64)
     return TM_ERR_SHAPE;
   o->prefix_floats = kvh * (hd + 2) * o->prefix_slots * o->prefix.part_rows;
@@ -764,11 +807,26 @@ int plan_branches(int64_t T, int64_t units, int64_t max_count, int64_t S, int64_
 
 bool vec_ok(const void* p, int64_t stride) { return (uintptr_t)p % 16 == 0 && stride % 8 == 0; }
 
+template <int DT, int HD, bool WAVES>
+void launch_few(const PromptParams& s, const BranchParams& p, const BranchPlan& o, int64_t shared,
+                int64_t own, int64_t parts, hipStream_t st) {
+  const dim3 grid((unsigned)(shared + own)), block(kThreads);
+  if (o.shared == kNone)
+    hipLaunchKernelGGL((tm_branch_kernel<DT, HD, kNone, WAVES>), grid, block, 0, st, s, p,
+                       (int)shared, (int)parts);
+  else if (o.shared == kLeanTile)
+    hipLaunchKernelGGL((tm_branch_kernel<DT, HD, kLeanTile, WAVES>), grid, block, 0, st, s, p,
+                       (int)shared, (int)parts);
+  else
+    hipLaunchKernelGGL((tm_branch_kernel<DT, HD, kShortTile, WAVES>), grid, block, 0, st, s, p,
+                       (int)shared, (int)parts);
+}
 template <int DT, int HD>
 void launch_own(const PromptParams& s, const BranchParams& p, const BranchPlan& o,
                 hipStream_t st) {
-  const int64_t parts = o.units * o.chunks, shared = o.prefix_slots * p.kvh;
-  const int64_t own = o.few ? ceil_div(parts * p.kvh, 4) : parts * p.kvh;
+  const int64_t parts = o.whole_units + (o.units - o.whole_units) * o.chunks;
+  const int64_t shared = o.prefix_slots * p.kvh;
+  const int64_t own = o.waves ? ceil_div(parts * p.kvh, 4) : parts * p.kvh;
   const dim3 block(kThreads);
   if (o.chain) {
     ChainParams c;
@@ -784,15 +842,10 @@ void launch_own(const PromptParams& s, const BranchParams& p, const BranchPlan& 
                          c);
   } else if (!o.few)
     hipLaunchKernelGGL((tm_branch_short_kernel<DT, HD>), dim3((unsigned)own), block, 0, st, p);
-  else if (o.shared == kNone)
-    hipLaunchKernelGGL((tm_branch_kernel<DT, HD, kNone>), dim3((unsigned)own), block, 0, st, s, p,
-                       0, (int)parts);
-  else if (o.shared == kLeanTile)
-    hipLaunchKernelGGL((tm_branch_kernel<DT, HD, kLeanTile>), dim3((unsigned)(own + shared)),
-                       block, 0, st, s, p, (int)shared, (int)parts);
+  else if (o.waves)
+    launch_few<DT, HD, true>(s, p, o, shared, own, parts, st);
   else
-    hipLaunchKernelGGL((tm_branch_kernel<DT, HD, kShortTile>), dim3((unsigned)(own + shared)),
-                       block, 0, st, s, p, (int)shared, (int)parts);
+    launch_few<DT, HD, false>(s, p, o, shared, own, parts, st);
 }
 template <int DT, int HD>
 void launch_join(const BranchJoin& j, hipStream_t st) {
@@ -935,7 +988,7 @@ extern "C" int tm_branch_attention(
     s.k_len = (int)seq_len;
     while ((int64_t(1) << s.page_shift) < page_size) ++s.page_shift;
     s.cache_pages = (int)cache_pages;
-    // keys of a stage that a wave takes from one page: 16 (of prompt attention's tallest tiles 8)
+    // (keys of a stage that a wave takes from one page)
     s.wide = page_size >= 16 ? 1 : 0;
     const int64_t part_rows = o.prefix_slots * kvh * o.prefix.part_rows;
     s.part = at;
@@ -972,6 +1025,7 @@ extern "C" int tm_branch_attention(
   p.rows = (int)rows;
   p.capacity = (int)capacity;
   p.chunks = (int)o.chunks;
+  p.whole_units = (int)o.whole_units;
   p.span = (int)o.span;
   p.parts = o.own_slots > 0;
   p.part_rows = (int)o.own_rows;
@@ -981,6 +1035,7 @@ extern "C" int tm_branch_attention(
   j.tokens = (const int4*)tokens;
   j.count = (int)max_count;
   j.unit_tiles = (int)unit_tiles;
+  j.whole_units = (int)o.whole_units;
   j.T = (int)T;
   j.Hq = (int)Hq;
   j.kvh = (int)kvh;
@@ -989,7 +1044,7 @@ extern "C" int tm_branch_attention(
   j.out_stride = out_stride;
 #define TM_BRANCH(DT, HD)                             \
   do {                                                \
-    launch_own<DT, HD>(s, p, o, st);                    \
+    launch_own<DT, HD>(s, p, o, st);                  \
     if (p.parts) launch_join<DT, HD>(j, st);          \
   } while (0)
   if (dtype == TM_DTYPE_F16) {
@@ -1009,15 +1064,18 @@ extern "C" int tm_branch_attention(
 }
 
 extern "C" int tm_branch_advance(int32_t* lengths, const int32_t* counts, int64_t count,
-                                 int64_t rows, int64_t capacity, void* stream) {
-  if (rows < 0 || rows > INT32_MAX - kThreads || capacity < 0 || capacity > TM_MAX_PROMPT_KEYS ||
-      count < 0 || count > TM_MAX_PROMPT_KEYS)
+                                 int64_t rows, int64_t capacity, int32_t* origin,
+                                 int64_t origin_stride, void* stream) {
+  if (rows < 0 || rows > UINT32_MAX / 64 || capacity < 0 || capacity > TM_MAX_PROMPT_KEYS ||
+      count < 0 || count > TM_MAX_PROMPT_KEYS ||
+      (origin != nullptr && rows > 1 && origin_stride < capacity))
     return TM_ERR_SHAPE;
   if (rows == 0) return TM_OK;
-  if ((uintptr_t)lengths % 4 || (uintptr_t)counts % 4) return TM_ERR_ALIGN;
-  hipLaunchKernelGGL(tm_branch_advance_kernel, dim3((unsigned)ceil_div(rows, kThreads)),
-                     dim3(kThreads), 0, (hipStream_t)stream, lengths, counts, (int)count,
-                     (int)rows, (int)capacity);
+  if ((uintptr_t)lengths % 4 || (uintptr_t)counts % 4 || (uintptr_t)origin % 4)
+    return TM_ERR_ALIGN;
+  hipLaunchKernelGGL(tm_branch_advance_kernel, dim3((unsigned)rows), dim3(64), 0,
+                     (hipStream_t)stream, lengths, counts, (int)count, (int)capacity, origin,
+                     origin_stride);
   TM_HIP_CHECK_LAUNCH();
   return TM_OK;
 }

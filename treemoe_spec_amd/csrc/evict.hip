@@ -84,7 +84,15 @@ __global__ void __launch_bounds__(kThreads, 2) tm_mass_stats_kernel(MassParams p
   __shared__ __attribute__((aligned(1024))) uint8_t s_k0[S::kTile];
   __shared__ __attribute__((aligned(1024))) uint8_t s_k1[S::kTile];
   const int kvhead = (int)blockIdx.x % p.kvh, at_item = (int)blockIdx.x / p.kvh;
-  const Item it = item_of(p, at_item, 128);
+  Item it = item_of(p, at_item, 128);
+  {
+    // The tiles with the most keys first, then from the fewest up: of workgroups that are
+    // given out in turn a CU gets some of each.
+    const int t = at_item / p.chunks, first = (p.tiles + 1) / 2;
+    it.tile = t < first ? p.tiles - 1 - t : t - first;
+    const int last_token = min(it.q_len - 1, (it.tile * 128 + 127) / p.group);
+    it.end = min(it.begin + p.chunk_len, it.k_len - it.q_len + last_token + 1);
+  }
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int n = it.end > it.begin ? (it.end - it.begin + kKeys - 1) / kKeys : 0;
   Rows<HD> r;
@@ -208,20 +216,33 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 ? 4 : 2) tm_mass_sum_ke
   // the key's first row, and that of the workgroup's last key
   const int seen = max(min(key, p.k_len - 1) - past, 0) * p.group;
   const int all = max(min(first + 32 * WAVES, p.k_len) - 1 - past, 0) * p.group;
-  const int stage0 = max(first - past, 0) * p.group / kKeys;
+  const int stage0 = max(min(first, p.k_len - 1) - past, 0) * p.group / kKeys;
   const int per = (whole / kKeys - stage0 + p.splits - 1) / p.splits;
   const int begin = stage0 + split * per, end = min(begin + per, whole / kKeys);
-  // row `in` of a stage, of the loads of this wave
+  // The rows of a stage that this wave loads.  Where a stage is whole tokens the next stage
+  // lies a fixed step behind: a division for each row costs as much as its exponentials.
+  const bool even = kKeys % p.group == 0;
+  const int64_t stage_step = (int64_t)(kKeys / p.group) * p.q_stride;
+  int64_t lane_off[kLoads];
+  auto offset_of = [&](int row, int in) TM_INLINE {
+    const int token = row / p.group;
+    return (int64_t)token * p.q_stride +
+           (int64_t)(kvhead * p.group + row - token * p.group) * HD +
+           (((lane & (S::kChunks - 1)) ^ S::swz_k(in)) * 8);
+  };
+  auto row_in = [&](int i) TM_INLINE {
+    return (wave * kLoads + i) * S::kKeysPerLoad + lane / S::kChunks;
+  };
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) lane_off[i] = offset_of(row_in(i), row_in(i));
   auto load = [&](int stage, uint8_t* tile) TM_INLINE {
+    const bool whole_stage = even && (stage + 1) * kKeys <= rows;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int in = (wave * kLoads + i) * S::kKeysPerLoad + lane / S::kChunks;
-      const int row = min(stage * kKeys + in, rows - 1);
-      const int token = row / p.group;
-      const uint16_t* const qr = p.q + (int64_t)token * p.q_stride +
-                                 (int64_t)(kvhead * p.group + row - token * p.group) * HD +
-                                 (((lane & (S::kChunks - 1)) ^ S::swz_k(in)) * 8);
-      __builtin_amdgcn_global_load_lds((glb_void*)qr,
+      const int64_t off = whole_stage
+                              ? lane_off[i] + stage * stage_step
+                              : offset_of(min(stage * kKeys + row_in(i), rows - 1), row_in(i));
+      __builtin_amdgcn_global_load_lds((glb_void*)(p.q + off),
                                        (lds_void*)(tile + (wave * kLoads + i) * 1024), 16, 0, 0);
     }
   };
@@ -718,9 +739,8 @@ int plan_mass(int64_t T, int64_t S, int64_t Hq, int64_t kvh, int64_t hd, MassPla
   // the sums' rows in parts of eight stages or more, two workgroups a slot of the chip
   o->key_tiles = ceil_div(S, o->own ? 128 : 256);
   const int64_t stages = ceil_div(o->rows, kKeys);
-  o->splits = o->own ? 1
-                     : std::max<int64_t>(1, std::min(4 * kCUs / std::max<int64_t>(o->key_tiles * kvh, 1),
-                                                     stages / 8));
+  const int64_t splits = 4 * kCUs / std::max<int64_t>(o->key_tiles * kvh, 1);
+  o->splits = o->own ? 1 : std::max<int64_t>(1, std::min(splits, stages / 8));
   o->stats = o->own || o->chunks > 1 ? 2 * o->chunks * kvh * o->rows : 0;
   o->consts = o->own ? 0 : kvh * stages * kKeys;
   o->parts = o->splits > 1 ? o->splits * kvh * S : 0;

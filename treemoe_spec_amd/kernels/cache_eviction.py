@@ -38,7 +38,8 @@ def attention_mass(q: torch.Tensor, kv, layer: int, mass: torch.Tensor | None = 
     tokens that see it and the query heads of its KV head, added to ``mass`` [kv_heads, >=
     seq_len] where given.  A row whose scores are all -inf gives nothing.  ``out``
     [kv_heads, >= seq_len] takes the first seq_len columns of the result; it may be
-    ``mass``, or shares no memory with it."""
+    ``mass``, or shares no memory with it.  A replay of a captured call repeats the length of
+    the capture."""
     dt, t, hq, hd, qs, _ = _check_q(q, None)
     kc, vc = kv.k, kv.v
     index = q.get_device()
@@ -74,8 +75,8 @@ def attention_mass(q: torch.Tensor, kv, layer: int, mass: torch.Tensor | None = 
     nbytes = _capi.workspace_bytes("mass_workspace", t, n, hq, kvh, hd)
     ws = out.new_empty(nbytes // 4) if nbytes else None
     _capi.launch("tm_attention_mass", index, q.data_ptr(), qs, t,
-                 kc.data_ptr() + kc.element_size() * cst[0] * (layer % layers), cst[1], cst[2], page,
-                 pages, table.data_ptr(), len(kv.block_table), n, hq, kvh, hd, scale, dt,
+                 kc.data_ptr() + kc.element_size() * cst[0] * (layer % layers), cst[1], cst[2],
+                 page, pages, table.data_ptr(), len(kv.block_table), n, hq, kvh, hd, scale, dt,
                  ptr(mass), 0 if mass is None else mass.stride(0), out.data_ptr(), out.stride(0),
                  ptr(ws), nbytes)
     return out
@@ -98,7 +99,7 @@ def evict(kv, mass: torch.Tensor, keep: int, *, positions: torch.Tensor | None =
     ``seq_len``).  ``next_position`` is also the position to rotate the next token by: tokens
     go on in slot ``kv.seq_len``, so rotate with ``rotary_embed`` and store with ``kv.append``.
     Every attention over the whole cache goes on as before, since it does not depend on
-    the order of the slots."""
+    the order of the slots.  A replay of a captured call repeats the lengths of the capture."""
     kc, vc = kv.k, kv.v
     index = kc.get_device()
     if not _capi.ready(index, kc, vc, mass, positions):

@@ -10,6 +10,7 @@ at offset ``q % page_size`` (reference ``slot_of``, :57-58).
 
 from __future__ import annotations
 
+import operator
 from dataclasses import dataclass
 
 import torch
@@ -296,7 +297,9 @@ class BranchCache:
         up to it."""
         from treemoe_spec_amd import _capi
 
-        uniform = isinstance(counts, int)
+        uniform = not hasattr(counts, "counts")
+        if uniform:
+            counts = operator.index(counts)
         added = [counts] * self.rows if uniform else counts.counts
         if len(added) != self.rows or (uniform and counts < 0):
             raise ValueError(f"counts must be a number or a plan for {self.rows} branches")
@@ -304,13 +307,16 @@ class BranchCache:
         if max(now) > self.capacity:
             raise ValueError(f"a branch would hold {max(now)} keys, over the capacity of "
                              f"{self.capacity}")
-        dev = self.lengths.device
-        _capi.require("BranchCache.advance", dev, lengths=self.lengths)
+        index = self.lengths.get_device()
         table = None if uniform else counts.device_counts
-        _capi.launch("tm_branch_advance", dev.index, self.lengths.data_ptr(), _capi.ptr(table),
-                     counts if uniform else 0, self.rows, self.capacity)
+        if not _capi.ready(index, self.lengths, self.origin, table):
+            _capi.require("BranchCache.advance", self.lengths.device, lengths=self.lengths,
+                          origin=self.origin, plan=table)
+        _capi.launch("tm_branch_advance", index, self.lengths.data_ptr(), _capi.ptr(table),
+                     counts if uniform else 0, self.rows, self.capacity, _capi.ptr(self.origin),
+                     self.capacity)
         if not uniform:
-            _capi.used_by(dev.index, counts.made_on, table)
+            _capi.used_by(index, counts.made_on, table)
         self.host_lengths, self.longest = now, max(now)
 
     def read_lengths(self) -> None:
@@ -327,10 +333,6 @@ class BranchCache:
             raise ValueError("lengths must be 0 .. the branches' present ones, one for each")
         if self.origin is not None:
             self._check_groups(lengths)
-            own = torch.arange(self.rows, dtype=torch.int32)[:, None].to(self.origin.device)
-            at = torch.arange(self.capacity).to(self.origin.device)
-            new = torch.tensor(lengths).to(self.origin.device)
-            self.origin.copy_(torch.where(at[None, :] < new[:, None], self.origin, own))
         self.lengths.copy_(torch.tensor(lengths, dtype=torch.int32))
         self.host_lengths, self.longest = lengths, max(lengths)
 
@@ -346,7 +348,7 @@ class BranchCache:
     def reorder(self, parents: torch.Tensor) -> None:
         """Beam i of group g goes on from what beam ``parents[g, i]`` holds (int32
         [groups, beams], as ``beam_select`` gives them; one outside the group
-        leaves the beam as it is).  Moves entries of ``origin``, all layers at once."""
+        leaves the beam as it is).  Moves entries of ``origin``, for all layers at once."""
         from treemoe_spec_amd.kernels.beam_search import reorder_rows
 
         if self.origin is None:
@@ -354,4 +356,4 @@ class BranchCache:
         if tuple(parents.shape) != (self.rows // self.beams, self.beams):
             raise ValueError(f"parents must be [{self.rows // self.beams}, {self.beams}]")
         self._check_groups(self.host_lengths)
-        reorder_rows(self.origin, parents, out=self.origin, columns=self.longest)
+        reorder_rows(self.origin, parents, out=self.origin)
