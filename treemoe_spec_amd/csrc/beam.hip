@@ -29,9 +29,9 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 // Logits of a lane, 256 times as many of a workgroup, which leaves one list.  A wave's
 // ranks, merges and barriers cost the same whatever it holds: many where the chip is full
-// anyway.  Selection in us with 16, 32 and 64 (graph replays, with the reorder): 256 rows of
-// 131072 bf16 80, 68, 67; 1024 of 32000 fp32 65, 60, 57; 256 of 32000 bf16, which 64 would
-// leave half the CUs without, 37, 35, 38.
+// anyway.  Selection in us with 16, 32 and 64 (graph replays, with the reorder; before the join
+// counted ranks by all its lanes): 256 rows of 131072 bf16 80, 68, 67; 1024 of 32000 fp32 65,
+// 60, 57; 256 of 32000 bf16, which 64 would leave half the CUs without, 37, 35, 38.
 constexpr int kFewPer = 16, kManyPer = 64;
 constexpr int kMaxNum = TM_MAX_BEAMS;
 constexpr int kJoin = 512;               // threads of a group's workgroup, a list each
@@ -329,9 +329,24 @@ __device__ __forceinline__ Cand cand_of(double score, int beam, uint32_t logit, 
                                    (((1u << kTokenBits) - 1) - token)};
 }
 
+// Neighbouring lanes that count for one of n entries: as many as the workgroup has.
+__device__ __forceinline__ int lanes_of(int n) {
+  int P = 64;
+  while (P > 1 && P * n > kJoin) P /= 2;
+  return P;
+}
+// How many of n candidates are above c, which P lanes have.
+__device__ __forceinline__ int rank_of(const Cand* all, int n, const Cand& c, int P) {
+  int rank = 0;
+#pragma unroll 4
+  for (int j = (int)threadIdx.x & (P - 1); j < n; j += P) rank += above(all[j], c) ? 1 : 0;
+  for (int d = 1; d < P; d <<= 1) rank += __shfl_xor(rank, d);
+  return rank;
+}
+
 struct JoinShared {
   Cand pool[kMaxNum * (kMaxNum + 1) / 2 + kMaxNum];
-  Cand heads[kJoin / 64][kMaxNum];  // of each wave, sorted
+  Cand heads[kJoin];
   Cand best[kMaxNum];               // so far, sorted
   double base[TM_MAX_BEAMS];        // score - log of the sum, -inf for a beam without candidates
   double powers[64];
@@ -349,7 +364,6 @@ __global__ void __launch_bounds__(kJoin) tm_beam_join_kernel(BeamParams p) {
   const int64_t row0 = (int64_t)group * K;
   const int lists = K * p.segs;
   const uint64_t* const from = p.lists + row0 * p.segs * num;
-  const auto higher = [](const Cand& a, const Cand& b) { return above(a, b); };
   // (of a finished beam nothing is there, and what is read is not used)
   uint64_t head_key = tid < lists ? from[(int64_t)tid * num] : 0;
 
@@ -362,22 +376,33 @@ __global__ void __launch_bounds__(kJoin) tm_beam_join_kernel(BeamParams p) {
     const bool over = p.finished != nullptr && p.finished[row0 + b];
     float top = -INFINITY;
     double sum = 0.0;
+    // (what a finished beam's rows left there is not used)
+    float t = -INFINITY;
+    double u = 0.0;
+    if (lane < p.segs) {
+      t = p.tops[at + lane];
+      u = p.sums[at + lane];
+    }
+    const double score = p.scores[row0 + b];
     if (!over) {
-      for (int i = lane; i < p.segs; i += 64) top = fmaxf(top, p.tops[at + i]);
+      top = t;
+      for (int i = lane + 64; i < p.segs; i += 64) top = fmaxf(top, p.tops[at + i]);
 #pragma unroll
       for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
       for (int i = lane; i < p.segs; i += 64) {
-        const float t = p.tops[at + i];
+        if (i > lane) {
+          t = p.tops[at + i];
+          u = p.sums[at + i];
+        }
         if (t == top)
-          sum += p.sums[at + i];
+          sum += u;
         else if (t > -INFINITY && top < INFINITY)
-          sum += p.sums[at + i] * exp_of((double)t - (double)top, s.powers);
+          sum += u * exp_of((double)t - (double)top, s.powers);
       }
 #pragma unroll
       for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
     }
     if (lane == 0) {
-      const double score = p.scores[row0 + b];
       s.top[b] = top;
       s.base[b] = top > -INFINITY && score > -INFINITY ? score - log(sum) : -INFINITY;
     }
@@ -402,40 +427,26 @@ __global__ void __launch_bounds__(kJoin) tm_beam_join_kernel(BeamParams p) {
                : cand_of(score, beam, (uint32_t)(key >> 32), ~(uint32_t)key);
   };
   for (int first = 0; first < lists; first += kJoin) {
-    const int now = min(lists - first, kJoin), waves = (now + 63) / 64;
+    const int now = min(lists - first, kJoin);
     if (tid < num) s.list[tid] = -1;
     if (tid == 0) {
       s.least = {0, 1};  // fewer heads than num: nothing lies below
       s.count = 0;
     }
     __syncthreads();  // the sums, and the best so far
-    // the heads in order: within the waves, then over them
-    Cand head = {0, 0};
-    int rank = num;
-    if (wave < waves) {
-      const int list = first + tid;
-      if (list < lists)
-        head = cand(list / p.segs, first == 0 ? head_key : from[(int64_t)list * num]);
-      rank = 0;
-      const int n = min(now - wave * 64, 64);
-      for (int l = 0; l < n; ++l) {
-        const Cand x = {lane_of(head.hi, l), lane_of(head.lo, l)};
-        rank += above(x, head) || (x.hi == 0 && head.hi == 0 && l < lane) ? 1 : 0;
+    // the heads' order, by lanes_of(now) lanes a head
+    if (tid < now)
+      s.heads[tid] = cand((first + tid) / p.segs,
+                          first == 0 ? head_key : from[(int64_t)(first + tid) * num]);
+    __syncthreads();
+    {
+      const int P = lanes_of(now), h = tid / P;
+      const Cand head = h < now ? s.heads[h] : Cand{0, 0};
+      const int rank = rank_of(s.heads, now, head, P);
+      if ((tid & (P - 1)) == 0 && head.hi != 0 && rank < num) {
+        s.list[rank] = first + h;
+        if (rank == num - 1) s.least = head;
       }
-      if (rank < num) s.heads[wave][rank] = head;
-      if (lane >= n && lane < num) s.heads[wave][lane] = {0, 0};
-    }
-    if (waves > 1) {
-      __syncthreads();
-      if (rank < num && head.hi != 0)
-        for (int w = 0; w < waves; ++w) {
-          const Cand* const one[1] = {s.heads[w]};
-          if (w != wave) rank += above_in<1>(one, num, head, higher);
-        }
-    }
-    if (rank < num && head.hi != 0) {
-      s.list[rank] = first + tid;
-      if (rank == num - 1) s.least = head;
     }
     __syncthreads();
     // what can come out, in any order
@@ -455,11 +466,12 @@ __global__ void __launch_bounds__(kJoin) tm_beam_join_kernel(BeamParams p) {
     __syncthreads();
     const int count = s.count;
     if (tid < num && tid >= count) s.best[tid] = {0, 0};
-    for (int e = tid; e < count; e += kJoin) {
-      const Cand c = s.pool[e];
-      int r = 0;
-      for (int j = 0; j < count; ++j) r += above(s.pool[j], c) ? 1 : 0;
-      if (r < num) s.best[r] = c;
+    const int P = lanes_of(count);
+    for (int e0 = 0; e0 < count; e0 += kJoin / P) {
+      const int e = e0 + tid / P;
+      const Cand c = e < count ? s.pool[e] : Cand{0, 0};
+      const int r = rank_of(s.pool, count, c, P);
+      if ((tid & (P - 1)) == 0 && e < count && r < num) s.best[r] = c;
     }
     __syncthreads();
   }

@@ -705,10 +705,10 @@ __global__ void __launch_bounds__(kThreads) tm_branch_join_kernel(BranchJoin p) 
 //   over 4096 114, 105, 119;
 //   own keys by workgroups (LEAN) or waves: 8 branches of up to 400 keys 14.3, 15.9; 16 16.6,
 //   15.9; 32 21.8, 18.7; 64 of up to 700 42, 40; 128 of up to 60 27, 21;
-//   at most kOwnWaves parts by waves: 64 of up to 700 with 2048, 3072 and 4096 44, 40, 44; 256
+//   at most kOwnWaves parts by waves: 64 of up to 700 with 8, 12 and 16 a CU 44, 40, 44; 256
 //   of them 102, 103, 112; 16 of up to 4000 52, 47, 50.
 constexpr int64_t kSharedBlocks = 128;
-constexpr int64_t kOwnWaves = 3072;
+constexpr int64_t kOwnWaves = 12 * kCUs;
 constexpr int64_t kLeanUnits = 64;     // (branch, KV head) pairs up to which a part is a workgroup
 constexpr int64_t kWaveKeys = 64;      // of a wave's part, or more
 constexpr int64_t kLongKeys = 8192;    // beyond them a branch leaves too many parts by waves

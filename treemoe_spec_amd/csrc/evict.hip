@@ -708,8 +708,11 @@ __global__ void __launch_bounds__(kThreads) tm_evict_move_kernel(EvictParams p) 
 
 constexpr int64_t kMaxStride = 1 << 24;
 constexpr int64_t kHeld = 16 * kSelect;  // keys of a head that its workgroup holds
-// The selecting workgroups move the keys where they fill the chip, or have few to move.
-constexpr int64_t kFusedHeads = 128, kFusedMoves = 128;
+// Moves up to which the selecting workgroup makes them itself: a launch more against a CU a head
+// that moves alone.  Measured, in us, by the workgroup and by a launch: 16 heads of 256
+// moves 16.8, 18.0, of 512 19.9, 18.5; of 1000 moves 32 heads 16.7, 15.0, 64 17.6, 17.2, 128
+// 24.7, 27.7, 256 39.5, 51; 128 heads of 4000 88, 75.
+int64_t fused_moves(int64_t heads) { return std::max<int64_t>(256, 8 * heads); }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct MassPlan {
@@ -729,9 +732,12 @@ int plan_mass(int64_t T, int64_t S, int64_t Hq, int64_t kvh, int64_t hd, MassPla
   o->few = o->rows <= 32;
   o->own = o->rows <= kOwnRows;
   o->tiles = ceil_div(o->rows, o->few ? 32 : 128);
-  // ranges of keys as many as fill the chip, of four stages or more
+  // ranges of keys as many as fill the chip, of four stages or more.  Many tiles leave it
+  // uneven with one workgroup a CU: 800 rows over 7200 keys in us with 1, 2 and 3 a CU 56, 48,
+  // 50; 4000 over 4000 110, 90, 89; but 256 over 7464, whose sums join the ranges themselves,
+  // 23.3 with 1, 24.2 with 2.
   const int64_t units = std::max<int64_t>(o->tiles * kvh, 1);
-  const int64_t want = std::max<int64_t>(1, kCUs / units);
+  const int64_t want = std::max<int64_t>(1, (units < 32 ? kCUs : 2 * kCUs) / units);
   const int64_t chunks = std::max<int64_t>(1, std::min(want, ceil_div(S, 4 * kKeys)));
   const int64_t step = o->few ? 4 * kKeys : kKeys;
   o->chunk_len = std::max(step, ceil_div(ceil_div(S, chunks), step) * step);
@@ -953,7 +959,7 @@ extern "C" int tm_evict(void* k_cache, void* v_cache, int64_t elem_bytes, int64_
   p.holes = p.counts + o.heads;
   p.movers = p.holes + o.heads * o.moves;
   const hipStream_t st = (hipStream_t)stream;
-  p.fused = seq_len <= kHeld && (o.heads >= kFusedHeads || o.moves <= kFusedMoves);
+  p.fused = seq_len <= kHeld && o.moves <= fused_moves(o.heads);
   const dim3 grid((unsigned)o.heads), block(kSelect);
   if (seq_len <= 2048)
     hipLaunchKernelGGL((tm_evict_held_kernel<4, 512>), grid, dim3(512), 0, st, p);
