@@ -152,6 +152,19 @@ def test_branches_that_fill_tiles(counts, prefix, page, hq, kvh, hd, dtype):
     _run(s, counts)
 
 
+@pytest.mark.parametrize("counts,prefix,hq,kvh,hd,dtype", [
+    ([33] * 24, 1700, 16, 16, 64, F16),
+    ([9] * 30, 3900, 16, 4, 128, BF),
+    ([9, 0, 8, 1, 12, 10] * 7, 3333, 16, 4, 64, BF),
+])
+def test_branches_that_leave_tiles_empty(counts, prefix, hq, kvh, hd, dtype):
+    """Many rows short of whole tiles behind many shared keys: those once for all branches."""
+    _say(f"branches: {len(counts)} short of tiles over {prefix} heads={hq}/{kvh} hd={hd} {dtype}")
+    s = Setup(prefix, [(i * 29) % 200 for i in range(len(counts))], hq, kvh, hd, dtype, 64,
+              seed=prefix, layers=2, spare=40)
+    _run(s, counts)
+
+
 @pytest.mark.parametrize("beams,groups", [(2, 3), (4, 1), (5, 2), (8, 9)])
 @pytest.mark.parametrize("count", [1, 3, 20, 32])
 @pytest.mark.parametrize("hd", [64, 128])

@@ -12,10 +12,10 @@
 //   are taken once for all branches, whose (token, head of the group) pairs are one long list
 //   of rows: tiles of 32 where that is all, else prompt attention's tiles of 128, without a
 //   causal border.  A branch's own keys are taken by a wave or a workgroup a range.
-//   Many rows a branch (prompts behind a shared one).  Where the branches fill tiles of 128
-//   rows, shared and own keys are one sequence for a tile, and nothing is joined but the tiles
-//   of a last partial round.  Otherwise (drafts of 9 tokens, say) the shared keys go through
-//   prompt attention's kernels for all branches, the own ones through tiles of 128 rows.
+//   Many rows a branch (prompts behind a shared one), tiles of 128 rows.  Shared and own keys
+//   are one sequence for a tile, and nothing is joined but the tiles of a last partial round.
+//   But where many branches are far from filling their tiles (drafts of 9 tokens, say) and the
+//   shared keys are many, those go through prompt attention's kernels for all branches.
 //
 // Position t of branch b lies in row origin[b][t] of the branch cache, the row of the
 // ancestor that stored it (without a table of origins, in row b).  So beams are reordered
@@ -24,7 +24,7 @@
 // Bound by latency and by HBM at few rows: 4 beams over 517 keys 7 us and the join 3.5; 64
 // requests of up to 700 own keys over 4096 38 us for 107 MB, of which about 10 are the two
 // launches' chains of latencies; own keys alone stream at 4.2-5.6 TB/s.  By prompt
-// attention's matrix products and exponentials at many: 12 prompts over 4096 0.7 PFLOP/s.
+// attention's matrix products and exponentials at many: 12 prompts over 4096 0.8 PFLOP/s.
 #include <algorithm>
 #include <new>
 
@@ -157,6 +157,23 @@ struct Work {
   int len;     // keys that the branch held
   int lo, hi;  // the new keys of the range, which are stored with it
 };
+// The branch, tile and tokens of a unit.
+__device__ __forceinline__ Item unit_of(const BranchParams& p, int unit) {
+  Item it = {};
+  if (p.units != nullptr) {
+    const int4 u = p.units[unit];
+    it.k0 = __builtin_amdgcn_readfirstlane(u.x);
+    it.tile = __builtin_amdgcn_readfirstlane(u.y);
+    it.q0 = __builtin_amdgcn_readfirstlane(u.z);
+    it.q_len = __builtin_amdgcn_readfirstlane(u.w);
+  } else {
+    it.k0 = unit / p.unit_tiles;
+    it.tile = unit - it.k0 * p.unit_tiles;
+    it.q0 = it.k0 * p.count;
+    it.q_len = p.count;
+  }
+  return it;
+}
 // Part `at` of all.  Ranges are whole stages, and go by the branch's own length, so that
 // they hold all its keys even where it is longer than the host took it for.  Before the
 // branch's keys lie `base` others.
@@ -171,18 +188,7 @@ __device__ __forceinline__ Work work_of(const BranchParams& p, int kvhead, int a
   const int chunk = split ? rest % p.chunks : 0;
   const int unit = split ? p.whole_units + rest / p.chunks : at;
   Item& it = w.it;
-  if (p.units != nullptr) {
-    const int4 u = p.units[unit];
-    it.k0 = __builtin_amdgcn_readfirstlane(u.x);
-    it.tile = __builtin_amdgcn_readfirstlane(u.y);
-    it.q0 = __builtin_amdgcn_readfirstlane(u.z);
-    it.q_len = __builtin_amdgcn_readfirstlane(u.w);
-  } else {
-    it.k0 = unit / p.unit_tiles;
-    it.tile = unit - it.k0 * p.unit_tiles;
-    it.q0 = it.k0 * p.count;
-    it.q_len = p.count;
-  }
+  it = unit_of(p, unit);
   w.len = min(max(__builtin_amdgcn_readfirstlane(p.lengths[it.k0]), 0), p.capacity);
   it.k_len = base + w.len + it.q_len;
   const int per = (it.k_len + chunks - 1) / chunks;
@@ -568,7 +574,8 @@ __global__ void __launch_bounds__(64) tm_branch_advance_kernel(int32_t* lengths,
   if (threadIdx.x == 0) lengths[b] = end;
 }
 
-// Parts of one kind: `chunks` of every tile, as `few` lays rows down or as whole tiles.
+// Parts of one kind: `chunks` of every tile, a row's elements together or, `tiled`, 32 rows as
+// end_rows lays them.
 struct Parts {
   const float* part;
   const float* stats;
@@ -579,14 +586,13 @@ struct BranchJoin {
   Parts shared, own;
   const int4* tokens;  // (branch, place in it, its first unit), or NULL:
   int count, unit_tiles;
-  int whole_units;     // the first ones, without parts
   int T, Hq, kvh, group;
   uint16_t* out;
   int64_t out_stride;
 };
 constexpr int kMaxParts = 512;  // of each kind
 
-// Where a row's parts lie: chunk c's statistics at (first + c * step) * 2, its output at
+// Where a row's parts lie: chunk c's statistics at stats + c * step * 2, its output at
 // o + c * step * HD.
 struct RowParts {
   const float *stats, *o;
@@ -608,9 +614,61 @@ __device__ __forceinline__ RowParts parts_of(const Parts& s, int kvh, int kvhead
   return r;
 }
 
-// A wave joins the parts of one row: the maximum and the sum over the parts, a lane per
-// part, then the weighted outputs in their order, four elements a lane and the lanes' groups a
-// part each.  The first kAhead parts of a group are asked for before anything is known.
+// Joins 32 rows' 32 columns of a branch's tile, a wave each, shared parts first and each in
+// order: lane l has row l % 32 and the columns that the partials' layout gives it.  (A wave a
+// row, as below, takes 16 bytes of each of a part's lines: 8 branches of 100 tokens, split in
+// two, 47 us in all, so 32.)
+template <int DT, int HD>
+__global__ void __launch_bounds__(kThreads) tm_branch_join_tiles_kernel(BranchParams p,
+                                                                        Parts shared, Parts own,
+                                                                        int waves) {
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  int id = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6);
+  if (id >= waves) return;
+  const int ht = id % (HD / 32);
+  id /= HD / 32;
+  const int first = id % 4 * 32 + (lane & 31);
+  id /= 4;
+  const int kvhead = id % p.kvh, at = id / p.kvh, unit = p.whole_units + at;
+  const Item it = unit_of(p, unit);
+  const int row = it.tile * 128 + first;
+  if (row >= it.q_len * p.group) return;
+  const int e = 32 * ht + 4 * half;
+  RowParts r[2] = {{nullptr, nullptr, 0}, parts_of<HD>(own, p.kvh, kvhead, at, first, e)};
+  if (shared.chunks > 0)
+    r[0] = parts_of<HD>(shared, p.kvh, kvhead, 0, it.q0 * p.group + row, e);
+  const int count[2] = {shared.chunks, own.chunks};
+  float m = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll 4
+    for (int c = 0; c < count[k]; ++c) m = fmaxf(m, r[k].stats[c * r[k].step * 2]);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float sum = 0.0f;
+  f32x4_t o[4] = {};
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll 2
+    for (int c = 0; c < count[k]; ++c) {
+      const float2 st = *reinterpret_cast<const float2*>(r[k].stats + c * r[k].step * 2);
+      const float a = __builtin_amdgcn_exp2f(st.x - ref);
+      sum = fmaf(st.y, a, sum);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(r[k].o + c * r[k].step * HD + 256 * x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[x][i] = fmaf(v[i], a, o[x][i]);
+      }
+    }
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    store_row<DT>(p, it.q0, row, kvhead, HD, e + 8 * x, o[x], sum);
+}
+
+// Of few rows a branch: a wave joins the parts of one row: the maximum and the sum over the
+// parts, a lane per part, then the weighted outputs in their order, four elements a lane and
+// the lanes' groups a part each.  The first kAhead parts of a group are asked for before
+// anything is known.
 template <int DT, int HD>
 __global__ void __launch_bounds__(kThreads) tm_branch_join_kernel(BranchJoin p) {
   __shared__ float s_a[4][2 * kMaxParts];
@@ -630,8 +688,6 @@ __global__ void __launch_bounds__(kThreads) tm_branch_join_kernel(BranchJoin p) 
     place = t % p.count;
     unit0 = t / p.count * p.unit_tiles;
   }
-  unit0 -= p.whole_units;
-  if (unit0 + (place * p.group + g) / p.own.tile_rows < 0) return;  // it has its output
   // part c: the shared ones first
   const RowParts r0 = parts_of<HD>(p.shared, p.kvh, kvhead, 0, t * p.group + g, e);
   const RowParts r1 = parts_of<HD>(p.own, p.kvh, kvhead, unit0, place * p.group + g, e);
@@ -643,10 +699,11 @@ __global__ void __launch_bounds__(kThreads) tm_branch_join_kernel(BranchJoin p) 
     return *reinterpret_cast<const float2*>(c < n0 ? r0.stats + c * r0.step * 2
                                                    : r1.stats + (c - n0) * r1.step * 2);
   };
-  f32x4_t first[kAhead];
+  f32x4_t first[kAhead] = {};
 #pragma unroll
   for (int i = 0; i < kAhead; ++i)
-    first[i] = *reinterpret_cast<const f32x4_t*>(out_of(min(group + i * kGroups, n - 1)));
+    if (i * kGroups < n)
+      first[i] = *reinterpret_cast<const f32x4_t*>(out_of(min(group + i * kGroups, n - 1)));
   float m = -INFINITY, sum = 0.0f;
   if (n <= 64) {
     const float2 st = lane < n ? stat_of(lane) : float2{-INFINITY, 0.0f};
@@ -706,12 +763,15 @@ __global__ void __launch_bounds__(kThreads) tm_branch_join_kernel(BranchJoin p) 
 //   own keys by workgroups (LEAN) or waves: 8 branches of up to 400 keys 14.3, 15.9; 16 16.6,
 //   15.9; 32 21.8, 18.7; 64 of up to 700 42, 40; 128 of up to 60 27, 21;
 //   at most kOwnWaves parts by waves: 64 of up to 700 with 8, 12 and 16 a CU 44, 40, 44; 256
-//   of them 102, 103, 112; 16 of up to 4000 52, 47, 50.
+//   of them 102, 103, 112; 16 of up to 4000 52, 47, 50;
+//   by workgroups, of which each has more keys to itself, where a branch may hold more than
+//   kLongKeys: 64 branches of 3000-6000 keys 234, by waves 248; 12 of 7000-14000 101, 110; 16 of
+//   2000-4000 by workgroups 51, by waves 48.
 constexpr int64_t kSharedBlocks = 128;
 constexpr int64_t kOwnWaves = 12 * kCUs;
 constexpr int64_t kLeanUnits = 64;     // (branch, KV head) pairs up to which a part is a workgroup
 constexpr int64_t kWaveKeys = 64;      // of a wave's part, or more
-constexpr int64_t kLongKeys = 8192;    // beyond them a branch leaves too many parts by waves
+constexpr int64_t kLongKeys = 4096;
 constexpr int64_t kMaxStride = 1 << 24;
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -767,25 +827,30 @@ int plan_branches(int64_t T, int64_t units, int64_t max_count, int64_t S, int64_
     f.chunk_len = std::max(step, ceil_div(ceil_div(S, chunks), step) * step);
     f.chunks = ceil_div(S, f.chunk_len);
   }
-  // Tiles of 128 rows that the branches fill by themselves, three quarters of them at least,
-  // have nothing to share: 12 prompts of 1-333 tokens over 4096 206 us so, 257 with the shared
-  // keys and the own ones apart, joined.
-  const int64_t base = ceil_div(S, kKeys) * kKeys;
-  o->chain = !o->few && 4 * T * group >= 3 * units * 128;
+  // Shared and own keys as one sequence, or apart and joined.  As one, the rows that a
+  // branch's tiles are short of go against the shared keys, too; apart, two launches more and
+  // every row's parts are stored and read.  Measured, in us, as one and apart: 32 branches of 9
+  // tokens (36 rows of 128) behind 500 keys 28, 42, 1000 36, 44, 2000 53, 50; of 16 tokens
+  // behind 4000 88, 72, of 20 90, 96; 128 of 9 behind 1000 102, 105, 2000 161, 133; 8 of 16
+  // behind 4000 37, 42; 12 prompts of 1-333 tokens over 4096 177, 262.
+  const int64_t base = ceil_div(S, kKeys) * kKeys, all_rows = T * group;
+  o->chain = !o->few && (units * 128 - all_rows) * S <= all_rows * 1600 + (1 << 25) / kvh;
   if (S > 0 && !o->few && !o->chain) {
     const int rc = tm_prefix_plan(T, S, Hq, kvh, &o->prefix);
     if (rc) return rc;
   }
   const int64_t keys = longest + max_count + (o->chain ? base : 0);
-  o->pair = o->chain && keys >= 8 * kKeys;
+  // Eight waves a tile where the tiles leave CUs idle: 8 branches of 100 tokens over 400 keys
+  // 26 us, 39 with four and the keys split, joined; but 8 of 250, 512 tiles, over 400 52, 41.
+  o->pair = o->chain && units * kvh <= kCUs && keys >= 4 * kKeys;
   o->waves = o->few && units * kvh > kLeanUnits && keys <= kLongKeys;
   const int64_t slots = o->waves ? kOwnWaves : o->pair ? kCUs : 2 * kCUs;
-  // Chained, as many as fill the chip's slots some whole times stay whole, and those left are
-  // split: of 600 tiles on 256 slots the last 88 (206 us, whole 234).
+  // As one, as many tiles as fill the chip's slots some whole times stay whole, and those left are
+  // split: of 600 tiles on 512 slots the last 88 (12 prompts over 4096 179 us, all whole 234).
   o->whole_units = o->chain ? units * kvh / slots * slots / kvh : 0;
   const int64_t want = std::min<int64_t>(
       slots / std::max<int64_t>((units - o->whole_units) * kvh, 1), kMaxParts);
-  const int64_t least = o->waves ? kWaveKeys : o->pair ? 8 * kKeys : 4 * kKeys;
+  const int64_t least = o->waves ? kWaveKeys : 4 * kKeys;
   const int64_t stage = o->few ? kLean : o->pair ? 2 * kKeys : kKeys;
   o->chunks = std::max<int64_t>(1, std::min(want, ceil_div(keys, least)));
   if (o->chain && o->chunks == 1) o->whole_units = units;
@@ -848,9 +913,15 @@ void launch_own(const PromptParams& s, const BranchParams& p, const BranchPlan& 
     launch_few<DT, HD, false>(s, p, o, shared, own, parts, st);
 }
 template <int DT, int HD>
-void launch_join(const BranchJoin& j, hipStream_t st) {
-  hipLaunchKernelGGL((tm_branch_join_kernel<DT, HD>),
-                     dim3((unsigned)ceil_div((int64_t)j.T * j.Hq, 4)), dim3(kThreads), 0, st, j);
+void launch_join(const BranchParams& p, const BranchJoin& j, const BranchPlan& o, hipStream_t st) {
+  if (o.few) {
+    hipLaunchKernelGGL((tm_branch_join_kernel<DT, HD>),
+                       dim3((unsigned)ceil_div((int64_t)j.T * j.Hq, 4)), dim3(kThreads), 0, st, j);
+  } else {
+    const int64_t waves = (o.units - o.whole_units) * p.kvh * 4 * (HD / 32);
+    hipLaunchKernelGGL((tm_branch_join_tiles_kernel<DT, HD>), dim3((unsigned)ceil_div(waves, 4)),
+                       dim3(kThreads), 0, st, p, j.shared, j.own, (int)waves);
+  }
 }
 
 }  // namespace
@@ -1035,7 +1106,6 @@ extern "C" int tm_branch_attention(
   j.tokens = (const int4*)tokens;
   j.count = (int)max_count;
   j.unit_tiles = (int)unit_tiles;
-  j.whole_units = (int)o.whole_units;
   j.T = (int)T;
   j.Hq = (int)Hq;
   j.kvh = (int)kvh;
@@ -1045,7 +1115,7 @@ extern "C" int tm_branch_attention(
 #define TM_BRANCH(DT, HD)                             \
   do {                                                \
     launch_own<DT, HD>(s, p, o, st);                  \
-    if (p.parts) launch_join<DT, HD>(j, st);          \
+    if (p.parts) launch_join<DT, HD>(p, j, o, st);    \
   } while (0)
   if (dtype == TM_DTYPE_F16) {
     if (hd == 128)
