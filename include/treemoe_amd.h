@@ -694,7 +694,7 @@ int tm_mass_workspace(int64_t T, int64_t seq_len, int64_t Hq, int64_t kvh, int64
  * are all -infinity gives nothing.  In fp32.  The attention itself is the reference's
  * (treemoe/model/mixtral.py:208-250), which keeps no such sums.  Cache and q as in
  * tm_prompt_attention_cached; before and mass fp32 [kvh, >= seq_len], row strides in
- * elements, mass the same memory as before or apart from it.  The workspace (8-byte
+ * elements, mass the same memory as before or apart from it.  The workspace (16-byte
  * aligned) is this call's until it has ended on the stream.
  */
 int tm_attention_mass(const void* q, int64_t q_stride, int64_t T, const void* k_cache,

@@ -381,7 +381,7 @@ def test_workspaces_and_other_statuses():
     assert reorder(width=1 << 39, xs=1 << 39, outs=1 << 39) == 1001    # more than a grid
 
     assert lib.tm_mass_workspace(1, 7777, 32, 8, 128, ctypes.byref(n)) == 0
-    assert n.value == 31 * 8 * 4 * 8
+    assert n.value == 31 * 8 * 4 * 8 + 8 * 4 * 7808 * 4      # statistics, and the scores
     assert lib.tm_mass_workspace(5, 4, 32, 8, 128, ctypes.byref(n)) == 1001
     assert lib.tm_mass_workspace(1, 4, 32, 8, 128, None) == 1003
 

@@ -5,18 +5,23 @@
 // of the group) pairs,
 //   mass[j] += sum over the rows that see key j of exp(s_rj - m_r) / l_r,
 // with s = scale q . k, m_r the largest of a row's scores and l_r the sum of its
-// exponentials.  First m and l of every row, over ranges of keys; then, 32 keys a wave, the
-// scores again and their sums over the rows.  K is read twice, from L2 the
-// second time where a head's keys fit it (a head's workgroups share an XCD); the
-// scores of many rows would be far more to store than to compute twice.  All in fp32; the
-// order of the sums is fixed.
+// exponentials.  First m and l of every row, over ranges of keys.  Up to 32 rows (the tokens
+// of a decoding step) leave their scores, too, and a second launch sums them over the rows.  Of
+// more rows the scores would be more to store and read than to compute twice: a wave takes 32
+// keys into registers, and the rows come by.  All in fp32; the order of the sums is fixed.
+//
+// Bound by latencies at few rows: one token over 7777 keys 10.8 us of two launches, 16 MB of K.
+// By the matrix products and exponentials together at many: 4096 tokens over themselves
+// 173 us, twice 69 GFLOP and 0.27 G exponentials each time, 0.8 PFLOP/s.
 //
 // Eviction.  Of each layer's KV heads, `keep` of S keys stay: the first `sinks` and the last
 // `recent` positions, and the heaviest others.  Kept keys in slots from `keep` on move into
 // the holes below, the i-th into the i-th; all others stay where they are, so a cache that
 // is cut every few tokens moves few keys.  Attention does not go by the order of the
-// slots; the positions go along.  One workgroup a head selects (a radix search over the
-// ordered bits of the weights), a second launch moves.
+// slots; the positions go along.  One workgroup a head selects, by a radix search over the
+// ordered bits of the weights, and moves the keys, or leaves many moves of few heads to a
+// second launch.  Selection is a chain of barriers (32 layers' heads of 1088 slots 11 us, with
+// 64 moves each); 1024 moves a head, 245 MB, take the time of a copy: 68 us.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -29,6 +34,9 @@ struct MassParams : PromptParams {
   float2* row_stats;      // (m in base 2, l) [chunks][kvh][rows]
   float* row_consts;      // -(m + log2 l) [kvh][rows in whole stages], or NULL: the sums'
                           // workgroups take row_stats
+  float* scores;          // [kvh][rows][score_stride]: few rows' scores, unscaled, -inf where a
+                          // row does not see the key
+  int64_t score_stride;
   float* parts;           // [splits][kvh][keys], or NULL: the mass itself
   int splits;             // of a tile's rows
   const float* before;    // [kvh, before_stride], or NULL
@@ -127,7 +135,7 @@ __global__ void __launch_bounds__(kThreads, 2) tm_mass_stats_kernel(MassParams p
   }
 }
 
-// Up to 32 rows: the waves take the stages in turn.
+// Up to 32 rows: the waves take the stages in turn, and keep the scores.
 template <int DT, int HD>
 __global__ void __launch_bounds__(kThreads, 2) tm_mass_stats_few_kernel(MassParams p) {
   typedef Shape<HD> S;
@@ -151,6 +159,18 @@ __global__ void __launch_bounds__(kThreads, 2) tm_mass_stats_few_kernel(MassPara
     products<DT, HD, false, true>(s_k[wave], s_k[wave], r);
     if (s + 4 < n) feed.load_k(p, s_k[wave]);
     take_stats<HD>(p.scale_log2, kb, kb + kKeys - 1 > at.full, r);
+    if (at.ok) {
+      float* const to = p.scores +
+                        ((int64_t)kvhead * it.q_len * p.group + at.row) * p.score_stride + kb +
+                        4 * (lane >> 5);
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<f32x4_t*>(to + 32 * kt + 8 * j) =
+              f32x4_t{r.sc[kt][4 * j], r.sc[kt][4 * j + 1], r.sc[kt][4 * j + 2],
+                      r.sc[kt][4 * j + 3]};
+    }
   }
   const float l = r.l + __shfl_xor(r.l, 32);
   if (lane < 32) {
@@ -320,6 +340,40 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 ? 4 : 2) tm_mass_sum_ke
     if (p.before != nullptr) v += p.before[kvhead * p.before_stride + key];
     p.mass[kvhead * p.mass_stride + key] = v;
   }
+}
+
+// Sums over few rows from the scores that were kept, a thread a key.  Scored again by
+// tm_mass_sum_kernel, in us: 4 rows over 7777 keys 15.8, so 10.8; over 30001 34, 19; 32 rows over
+// 7008 15.3, 13.3.
+__global__ void __launch_bounds__(kThreads) tm_mass_kept_kernel(MassParams p) {
+  __shared__ float s_const[32];
+  const int tid = threadIdx.x, rows = p.q_len * p.group;
+  const int kvhead = (int)blockIdx.x % p.kvh;
+  const int key = (int)blockIdx.x / p.kvh * kThreads + tid, at = min(key, p.k_len - 1);
+  constexpr int kAhead = 4;
+  const float* const from = p.scores + (int64_t)kvhead * rows * p.score_stride + at;
+  float first[kAhead];
+#pragma unroll
+  for (int r = 0; r < kAhead; ++r) first[r] = r < rows ? from[r * p.score_stride] : 0.0f;
+  const float before =
+      p.before != nullptr ? p.before[kvhead * p.before_stride + at] : 0.0f;
+  int P = 64;  // lanes a row
+  while (P * rows > kThreads) P /= 2;
+  if (tid / P < rows) {
+    const float c = joined(p.row_stats + (int64_t)kvhead * rows + tid / P, (int64_t)p.kvh * rows,
+                           p.chunks, P);
+    if ((tid & (P - 1)) == 0) s_const[tid / P] = c;
+  }
+  __syncthreads();
+  float sum = 0.0f;
+#pragma unroll
+  for (int r = 0; r < kAhead; ++r)
+    if (r < rows)
+      sum += __builtin_amdgcn_exp2f(fmaf(first[r], p.scale_log2, s_const[r]));
+#pragma unroll 4
+  for (int r = kAhead; r < rows; ++r)
+    sum += __builtin_amdgcn_exp2f(fmaf(from[r * p.score_stride], p.scale_log2, s_const[r]));
+  if (key < p.k_len) p.mass[kvhead * p.mass_stride + key] = before + sum;
 }
 
 // The splits' sums, in their order.
@@ -719,7 +773,8 @@ struct MassPlan {
   bool few, own;
   int64_t rows, tiles, chunks, chunk_len;
   int64_t key_tiles, splits;               // of the sums
-  int64_t stats, consts, parts, bytes;     // floats, floats, floats; of the workspace
+  int64_t stats, consts, parts, scores;    // floats of the workspace
+  int64_t bytes;                           // of all of it
 };
 
 int plan_mass(int64_t T, int64_t S, int64_t Hq, int64_t kvh, int64_t hd, MassPlan* o) {
@@ -750,7 +805,9 @@ int plan_mass(int64_t T, int64_t S, int64_t Hq, int64_t kvh, int64_t hd, MassPla
   o->stats = o->own || o->chunks > 1 ? 2 * o->chunks * kvh * o->rows : 0;
   o->consts = o->own ? 0 : kvh * stages * kKeys;
   o->parts = o->splits > 1 ? o->splits * kvh * S : 0;
-  o->bytes = 4 * (o->stats + o->consts + o->parts);
+  o->stats = ceil_div(o->stats, 4) * 4;    // (16-byte stores behind them)
+  o->scores = o->few ? kvh * o->rows * ceil_div(S, kKeys) * kKeys : 0;
+  o->bytes = 4 * (o->stats + o->consts + o->parts + o->scores);
   if (o->tiles * o->chunks * kvh > UINT32_MAX / kThreads ||
       o->key_tiles * o->splits * kvh > UINT32_MAX / 512 || kvh * stages * kKeys > UINT32_MAX)
     return TM_ERR_SHAPE;
@@ -767,6 +824,11 @@ void launch_mass(const MassParams& p, const MassPlan& o, hipStream_t st) {
       hipLaunchKernelGGL((tm_mass_stats_few_kernel<DT, HD>), items, block, 0, st, p);
     else
       hipLaunchKernelGGL((tm_mass_stats_kernel<DT, HD>), items, block, 0, st, p);
+  }
+  if (o.few) {
+    hipLaunchKernelGGL(tm_mass_kept_kernel,
+                       dim3((unsigned)(ceil_div(p.k_len, kThreads) * p.kvh)), block, 0, st, p);
+    return;
   }
   if (o.own) {
     hipLaunchKernelGGL((tm_mass_sum_kernel<DT, HD, 4, true>), sums, block, 0, st, p);
@@ -842,7 +904,7 @@ extern "C" int tm_attention_mass(const void* q, int64_t q_stride, int64_t T, con
     return TM_ERR_SHAPE;
   if ((uintptr_t)q % 16 || (T > 1 && q_stride % 8) || (uintptr_t)k_cache % 16 ||
       stride_slot % 8 || stride_page % 8 || (uintptr_t)block_table % 4 || (uintptr_t)before % 4 ||
-      (uintptr_t)mass % 4 || (uintptr_t)workspace % 8)
+      (uintptr_t)mass % 4 || (uintptr_t)workspace % 16)
     return TM_ERR_ALIGN;
   MassParams p = {};
   p.q = (const uint16_t*)q;
@@ -867,6 +929,8 @@ extern "C" int tm_attention_mass(const void* q, int64_t q_stride, int64_t T, con
   p.row_stats = (float2*)at;
   p.row_consts = o.own ? nullptr : at + o.stats;
   p.parts = o.splits > 1 ? at + o.stats + o.consts : nullptr;
+  p.scores = at + o.stats;  // (few only: nothing else lies there then)
+  p.score_stride = ceil_div(seq_len, kKeys) * kKeys;
   p.splits = (int)o.splits;
   p.before = before;
   p.before_stride = before_stride;
