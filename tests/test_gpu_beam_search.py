@@ -95,6 +95,21 @@ def test_large_vocabularies(v, beams, num):
     _check(*_inputs(1, beams, v, BF, v), num)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("groups,beams,v", [(64, 8, 300), (33, 8, 8193), (130, 4, 4096)])
+@pytest.mark.parametrize("num", [1, 16, 17, 64])
+def test_many_rows(groups, beams, v, num, dtype):
+    """Rows that fill the chip; few lists for many to come out; logits of few values, and in
+    order, so that a few threads have all of the largest."""
+    _say(f"beam_select {groups}x{beams} num {num} of {v} {dtype}")
+    logits, scores = _inputs(groups, beams, v, dtype, num)
+    logits[1::5] = (logits[1::5] / 4).round()
+    logits[2::5] = logits[2::5].sort(descending=True).values
+    logits[3::5] = logits[3::5].sort().values
+    logits[4, 7:] = -INF
+    _check(logits, scores, num)
+
+
 @pytest.mark.parametrize("num", [1, 8, 64])
 def test_flat_and_tied_rows(num):
     """All logits equal, or of few values: the lower beam and the lower token first."""

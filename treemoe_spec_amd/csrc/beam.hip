@@ -12,13 +12,17 @@
 // beam the order is that of the logits, so a row is cut to its best `num` before any
 // score is known.
 //
-// A wave takes 1024 logits of a row: its sum, and its best `num` as sorted keys (ordered
-// bits of the logit, inverted token), all distinct.  At least `num` logits reach the
-// num-th largest of the 64 lanes' largest, and only the `num` lanes that reach it hold
-// such, 16 at most each: the list never overflows.  Four waves' lists become one.  Then one
-// workgroup a group joins the sums and ranks the lists' heads.  Entry i of the list whose
-// head is the r-th has r + i above it: what is left when that is `num` or more, and what
-// lies below the num-th head, cannot come out; the rest is ranked by counting.
+// A workgroup takes 4096 or 8192 logits of a row: their sum, and their best `num` as sorted
+// keys (ordered bits of the logit, inverted token), all distinct.  At least `num` logits reach
+// the num-th largest of the 256 threads' largest, and only the `num` threads that reach it hold
+// such: the list never overflows.  Then one workgroup a group joins the sums and ranks the
+// lists' heads.  Entry i of the list whose head is the r-th has r + i above it: what is left
+// when that is `num` or more, and what lies below the num-th head, cannot come out; the rest
+// is ranked by counting.
+//
+// Bound by instructions at many logits, the 64-bit exponentials 10 of 40 us (256 rows of 131072
+// in 37 us and the join 7, 67 MB), and by chains of barriers and latencies at few: 4 rows of
+// 32000 7.5 and 5 us.
 #include <cmath>
 
 #include "tm_vec.h"
@@ -27,12 +31,12 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-// Logits of a lane, 256 times as many of a workgroup, which leaves one list.  A wave's
-// ranks, merges and barriers cost the same whatever it holds: many where the chip is full
-// anyway.  Selection in us with 16, 32 and 64 (graph replays, with the reorder; before the join
-// counted ranks by all its lanes): 256 rows of 131072 bf16 80, 68, 67; 1024 of 32000 fp32 65,
-// 60, 57; 256 of 32000 bf16, which 64 would leave half the CUs without, 37, 35, 38.
-constexpr int kFewPer = 16, kManyPer = 64;
+// Logits of a lane, 256 times as many of a workgroup, which leaves one list.  What a list costs
+// (bound, barriers, ranks, the join) is the same whatever it stands for: many where the chip
+// is full anyway.  Selection in us with 16, 32 and 64 (graph replays, with the reorder): 256
+// rows of 131072 bf16 59, 52, 51; 64 rows 32, 28, 27; 1024 of 32000 fp32 56, 54, 54; 256 of
+// 32000 bf16 27, 28, 32; 4 of 32000 fp32 15, 17, 20.
+constexpr int kFewPer = 16, kManyPer = 32;
 constexpr int kMaxNum = TM_MAX_BEAMS;
 constexpr int kJoin = 512;               // threads of a group's workgroup, a list each
 
@@ -151,156 +155,147 @@ __device__ __forceinline__ double exp_of(double d, const double* powers) {
                               ((int64_t)(k >> 6) << 52));
 }
 
-// How many of the lanes' first `n` keys are larger than this lane's.
-__device__ __forceinline__ int rank_in_wave(uint64_t key, int n) {
-  int rank = 0;
-  for (int l = 0; l < n; ++l) rank += lane_of(key, l) > key ? 1 : 0;
-  return rank;
-}
-
-// The num-th largest of the lanes' keys, or a bound that just num of them reach: by
-// bisection of the logits' ordered bits, which ends as soon as a count is num; where
-// logits are equal, by the keys' ranks.
-__device__ __forceinline__ uint64_t least_of(uint64_t key, float top, int num) {
-  const uint32_t own = (uint32_t)(key >> 32);
-  // reached by num or more (all lanes reach -inf); above it: by fewer
-  uint32_t lo = 0x007fffffu, hi = order_bits(top);
+// The largest value from lo to hi that num or more reach, all reaching lo, or one that just
+// num reach.  `reach`: how many reach a value.
+template <class REACH>
+__device__ __forceinline__ uint32_t last_reached(uint32_t lo, uint32_t hi, int num, REACH&& reach) {
   while (lo < hi) {
     const uint32_t mid = lo + (hi - lo + 1) / 2;
-    const int count = __popcll(__ballot(own >= mid));
-    if (count == num) return (uint64_t)mid << 32;
+    const int count = reach(mid);
+    if (count == num) return mid;
     if (count > num)
       lo = mid;
     else
       hi = mid - 1;
   }
-  const uint64_t at = __ballot(rank_in_wave(key, 64) == num - 1);
-  return lane_of(key, __ffsll((unsigned long long)at) - 1);
+  return lo;
 }
 
-// How many of each of N sorted lists' entries, `num` with zeros behind the last, are above
-// x: N searches side by side.
-template <int N, typename T, class ABOVE>
-__device__ __forceinline__ int above_in(const T* const (&lists)[N], int num, const T& x,
-                                        ABOVE&& above) {
-  int at[N] = {};
-  int step = 1;
-  while (2 * step <= num) step *= 2;
-  for (; step > 0; step /= 2) {
+// A bound that just num of the threads' keys reach, by one wave: of the logits' ordered bits, and
+// where the logits there are equal of the tokens first .. last, inverted.
+__device__ __forceinline__ uint64_t least_of(const uint64_t (&keys)[kThreads], float top, int num,
+                                             int first, int last) {
+  uint32_t logit[kWaves], token[kWaves];
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (at[i] + step <= num && above(lists[i][at[i] + step - 1], x)) at[i] += step;
+  for (int i = 0; i < kWaves; ++i) {
+    const uint64_t k = keys[64 * i + (threadIdx.x & 63)];
+    logit[i] = (uint32_t)(k >> 32);
+    token[i] = (uint32_t)k;
   }
-  int sum = 0;
+  auto reach = [&](uint32_t v) {
+    int count = 0;
 #pragma unroll
-  for (int i = 0; i < N; ++i) sum += at[i];
-  return sum;
+    for (int i = 0; i < kWaves; ++i) count += __popcll(__ballot(logit[i] >= v));
+    return count;
+  };
+  const uint32_t lowest = 0x007fffffu;  // -inf: all reach it
+  const uint32_t v = last_reached(lowest, order_bits(top), num, reach);
+  if (reach(v) == num) return (uint64_t)v << 32;
+  const int need = num - reach(v + 1);
+  const uint32_t t =
+      last_reached(~(uint32_t)last, ~(uint32_t)first, need, [&](uint32_t u) {
+        int count = 0;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i)
+          count += __popcll(__ballot(logit[i] == v && token[i] >= u));
+        return count;
+      });
+  return ((uint64_t)v << 32) | t;
 }
 
 template <int DT, int kPer>
 __global__ void __launch_bounds__(kThreads) tm_beam_rows_kernel(BeamParams p) {
-  extern __shared__ uint64_t s_lists[];  // [kWaves][num * kPer]
-  __shared__ uint64_t s_best[kWaves][kMaxNum];
+  extern __shared__ uint64_t s_list[];  // [num * kPer]
+  __shared__ uint64_t s_key[kThreads];
+  __shared__ uint64_t s_least;
   __shared__ double s_sum[kWaves];
   __shared__ float s_top[kWaves];
-  __shared__ int s_found[kWaves];
+  __shared__ int s_count;
   __shared__ double s_powers[64];
   const int tid = threadIdx.x, lane = tid & 63, num = p.num;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t unit = blockIdx.x;
   const int row = (int)(unit / p.segs), seg = (int)(unit - (int64_t)row * p.segs);
   if (p.finished != nullptr && p.finished[row]) return;
-  const int base = (seg * kWaves + wave) * 64 * kPer;
-  uint64_t* const list = s_lists + wave * num * kPer;
+  const int first = seg * kThreads * kPer, base = first + wave * 64 * kPer;
+  uint64_t* const out = p.lists + unit * num;
   float x[kPer];
   fetch<DT, kPer>(p, row, base, x);
   if (tid < 64) s_powers[tid] = kPowers[tid];
+  if (tid == 0) s_count = 0;
   float top = x[0];
 #pragma unroll
   for (int e = 1; e < kPer; ++e) top = fmaxf(top, x[e]);
   int at = 0;  // of the lane's largest, the lowest index
 #pragma unroll
   for (int e = kPer - 1; e >= 0; --e) at = x[e] == top ? index_of<DT>(e) : at;
-  const uint64_t best = key_of(top, base + at);
+  s_key[tid] = key_of(top, base + at);
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  if (lane == 0) s_top[wave] = top;
   __syncthreads();
-  int n = 0;
-  double sum = 0.0;
-  if (top > -INFINITY) {  // (else no candidate, and no weight)
-    double part[2] = {0.0, 0.0};
-    if (top < INFINITY) {
 #pragma unroll
-      for (int e = 0; e < kPer; ++e)
-        part[e & 1] += exp_of((double)x[e] - (double)top, s_powers);
-    } else {  // infinite ones weigh 1, and all finite ones nothing
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) part[e & 1] += x[e] == top ? 1.0 : 0.0;
-    }
-    sum = part[0] + part[1];
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-    // the num-th largest of the lanes' largest, and what reaches it
-    const uint64_t least = least_of(best, top, num);
-    const float least_logit = float_of((uint32_t)(least >> 32));
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      if (!__any(x[e] >= least_logit)) continue;
-      const uint64_t k = key_of(x[e], base + index_of<DT>(e));
-      const bool in = k >= least && x[e] > -INFINITY;
-      const uint64_t who = __ballot(in);
-      if (in) list[n + lanes_before(who)] = k;
-      n += __popcll(who);
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (n <= 64) {
-      const uint64_t k = lane < n ? list[lane] : 0;
-      const int rank = rank_in_wave(k, n);
-      if (lane < n && rank < num) s_best[wave][rank] = k;
-    } else {
-      for (int i = lane; i < n; i += 64) {
-        const uint64_t k = list[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += list[j] > k ? 1 : 0;
-        if (rank < num) s_best[wave][rank] = k;
-      }
-    }
-  }
-  n = min(n, num);
-  if (lane >= n && lane < num) s_best[wave][lane] = 0;
-  if (lane == 0) {
-    s_sum[wave] = sum;
-    s_top[wave] = top;
-    s_found[wave] = n;
-  }
-  __syncthreads();
-  // the waves' lists and sums as one
-  if (tid < kWaves) {
-    float most = s_top[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) most = fmaxf(most, s_top[w]);
-    const float own = s_top[tid];
-    double all = own == most        ? s_sum[tid]
-                 : most == INFINITY ? 0.0
-                                    : s_sum[tid] * exp_of((double)own - (double)most, s_powers);
-#pragma unroll
-    for (int d = 1; d < kWaves; d <<= 1) all += __shfl_xor(all, d);
+  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, s_top[w]);
+  if (top == -INFINITY) {  // no candidate, and no weight
+    if (tid < num) out[tid] = 0;
     if (tid == 0) {
-      p.sums[unit] = all;
-      p.tops[unit] = most;
+      p.sums[unit] = 0.0;
+      p.tops[unit] = top;
     }
+    return;
   }
-  uint64_t* const out = p.lists + unit * num;
-  if (lane < n) {
-    const uint64_t k = s_best[wave][lane];
-    const uint64_t* const lists[kWaves] = {s_best[0], s_best[1], s_best[2], s_best[3]};
-    const int rank = above_in<kWaves>(lists, num, k, [](uint64_t a, uint64_t b) { return a > b; });
-    if (rank < num) out[rank] = k;
+  // one wave finds what reaches the num-th largest of the threads' largest, while the others
+  // have begun with the sum
+  if (wave == 0) {
+    const uint64_t least = least_of(s_key, top, num, first, first + kThreads * kPer - 1);
+    if (lane == 0) s_least = least;
   }
-  int found = 0;
+  double part[2] = {0.0, 0.0};
+  if (top < INFINITY) {
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) found += s_found[w];
-  if (tid >= found && tid < num) out[tid] = 0;
+    for (int e = 0; e < kPer; ++e)
+      part[e & 1] += exp_of((double)x[e] - (double)top, s_powers);
+  } else {  // infinite ones weigh 1, and all finite ones nothing
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) part[e & 1] += x[e] == top ? 1.0 : 0.0;
+  }
+  double sum = part[0] + part[1];
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+  if (lane == 0) s_sum[wave] = sum;
+  __syncthreads();
+  const uint64_t least = s_least;
+  const float least_logit = float_of((uint32_t)(least >> 32));
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    if (!__any(x[e] >= least_logit)) continue;
+    const uint64_t k = key_of(x[e], base + index_of<DT>(e));
+    const bool in = k >= least && x[e] > -INFINITY;
+    const uint64_t who = __ballot(in);
+    int to = 0;
+    if (lane == 0) to = atomicAdd(&s_count, __popcll(who));
+    to = __builtin_amdgcn_readfirstlane(to);
+    if (in) s_list[to + lanes_before(who)] = k;
+  }
+  __syncthreads();
+  // in order, by neighbouring lanes a key: as many as the workgroup has
+  const int n = s_count;
+  int P = 64;
+  while (P > 1 && P * n > kThreads) P /= 2;
+  for (int e0 = 0; e0 < n; e0 += kThreads / P) {
+    const int e = e0 + tid / P;
+    const uint64_t k = e < n ? s_list[e] : 0;
+    int rank = 0;
+#pragma unroll 4
+    for (int j = tid & (P - 1); j < n; j += P) rank += s_list[j] > k ? 1 : 0;
+    for (int d = 1; d < P; d <<= 1) rank += __shfl_xor(rank, d);
+    if ((tid & (P - 1)) == 0 && e < n && rank < num) out[rank] = k;
+  }
+  if (tid >= n && tid < num) out[tid] = 0;
+  if (tid == 0) {
+    p.sums[unit] = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+    p.tops[unit] = top;
+  }
 }
 
 // A candidate: ordered bits of its score, then the beam (inverted), the logit's ordered
@@ -344,20 +339,29 @@ __device__ __forceinline__ int rank_of(const Cand* all, int n, const Cand& c, in
   return rank;
 }
 
+constexpr int kSteps = 128;     // lists up to which further entries bound what can come out
+constexpr int kLevels = 6;      // entries 0, 1, 3, 7, 15, 31 of a list
+
+template <bool STEPS>
 struct JoinShared {
   Cand pool[kMaxNum * (kMaxNum + 1) / 2 + kMaxNum];
   Cand heads[kJoin];
+  Cand steps[STEPS ? kLevels - 1 : 1][STEPS ? kSteps : 1];
   Cand best[kMaxNum];               // so far, sorted
   double base[TM_MAX_BEAMS];        // score - log of the sum, -inf for a beam without candidates
   double powers[64];
   float top[TM_MAX_BEAMS];
-  Cand least;                       // the num-th of the heads
+  Cand least[kLevels];              // the num-th of the heads, and so on
   int list[kMaxNum];                // the lists in their heads' order
   int count;                        // of the pool
 };
 
+// STEPS: few lists for many to come out.  Their heads bound little, entry i of num / (i + 1)
+// lists as well bounds more: 32 of 32 lists 69 us, so 35; but up to 16 are ranked sooner than
+// bounded (8 of 16 lists 17, so 20).
+template <bool STEPS>
 __global__ void __launch_bounds__(kJoin) tm_beam_join_kernel(BeamParams p) {
-  __shared__ JoinShared s;
+  __shared__ JoinShared<STEPS> s;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group = blockIdx.x, K = p.beams, num = p.num;
@@ -366,6 +370,14 @@ __global__ void __launch_bounds__(kJoin) tm_beam_join_kernel(BeamParams p) {
   const uint64_t* const from = p.lists + row0 * p.segs * num;
   // (of a finished beam nothing is there, and what is read is not used)
   uint64_t head_key = tid < lists ? from[(int64_t)tid * num] : 0;
+  int levels = 1;
+  uint64_t step_key[kLevels - 1];
+  if constexpr (STEPS) {
+    while (levels < kLevels && (1 << levels) <= num) ++levels;
+#pragma unroll
+    for (int l = 1; l < kLevels; ++l)
+      step_key[l - 1] = l < levels && tid < lists ? from[(int64_t)tid * num + (1 << l) - 1] : 0;
+  }
 
   if (tid < 64) s.powers[tid] = kPowers[tid];
   if (tid < num) s.best[tid] = {0, 0};
@@ -429,15 +441,19 @@ __global__ void __launch_bounds__(kJoin) tm_beam_join_kernel(BeamParams p) {
   for (int first = 0; first < lists; first += kJoin) {
     const int now = min(lists - first, kJoin);
     if (tid < num) s.list[tid] = -1;
-    if (tid == 0) {
-      s.least = {0, 1};  // fewer heads than num: nothing lies below
-      s.count = 0;
-    }
+    if (tid < kLevels) s.least[tid] = {0, 1};  // fewer heads than num: nothing lies below
+    if (tid == 0) s.count = 0;
     __syncthreads();  // the sums, and the best so far
     // the heads' order, by lanes_of(now) lanes a head
-    if (tid < now)
-      s.heads[tid] = cand((first + tid) / p.segs,
-                          first == 0 ? head_key : from[(int64_t)(first + tid) * num]);
+    if (tid < now) {
+      const int beam = (first + tid) / p.segs;
+      s.heads[tid] = cand(beam, first == 0 ? head_key : from[(int64_t)(first + tid) * num]);
+      if constexpr (STEPS) {
+#pragma unroll
+        for (int l = 1; l < kLevels; ++l)
+          if (l < levels) s.steps[l - 1][tid] = cand(beam, step_key[l - 1]);
+      }
+    }
     __syncthreads();
     {
       const int P = lanes_of(now), h = tid / P;
@@ -445,12 +461,22 @@ __global__ void __launch_bounds__(kJoin) tm_beam_join_kernel(BeamParams p) {
       const int rank = rank_of(s.heads, now, head, P);
       if ((tid & (P - 1)) == 0 && head.hi != 0 && rank < num) {
         s.list[rank] = first + h;
-        if (rank == num - 1) s.least = head;
+        if (rank == num - 1) s.least[0] = head;
       }
+      if constexpr (STEPS)
+        for (int l = 1; l < levels; ++l) {
+          const Cand c = h < now ? s.steps[l - 1][h] : Cand{0, 0};
+          const int at = rank_of(s.steps[l - 1], now, c, P);
+          if ((tid & (P - 1)) == 0 && c.hi != 0 && at == (num + (1 << l) - 1) / (1 << l) - 1)
+            s.least[l] = c;
+        }
     }
     __syncthreads();
     // what can come out, in any order
-    const Cand least = s.least;
+    Cand least = s.least[0];
+    if constexpr (STEPS)
+      for (int l = 1; l < levels; ++l)
+        if (above(s.least[l], least)) least = s.least[l];
     for (int e = tid; e < num * num + num; e += kJoin) {
       const int r = e / num, i = e - r * num;
       Cand c = {0, 0};
@@ -554,10 +580,9 @@ __global__ void __launch_bounds__(kThreads) tm_reorder_within_kernel(ReorderPara
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Logits of a lane, by the workgroups that many of them would leave; a lane's largest are
-// kept apart in LDS, `num` lanes' at most.
-int per_of(int64_t rows, int64_t V, int64_t num) {
-  return num <= 24 && rows * ceil_div(V, kThreads * kManyPer) >= 2 * 256 ? kManyPer : kFewPer;
+// Logits of a lane, by the workgroups that many of them would leave.
+int per_of(int64_t rows, int64_t V) {
+  return rows * ceil_div(V, kThreads * kManyPer) >= 2 * 256 ? kManyPer : kFewPer;
 }
 
 int check_beams(int64_t G, int64_t K, int64_t V, int64_t num) {
@@ -571,7 +596,7 @@ int check_beams(int64_t G, int64_t K, int64_t V, int64_t num) {
 template <int DT>
 void launch_rows(const BeamParams& p, int per, hipStream_t st) {
   const dim3 grid((unsigned)(p.rows * p.segs)), block(kThreads);
-  const size_t lds = (size_t)kWaves * p.num * per * sizeof(uint64_t);
+  const size_t lds = (size_t)p.num * per * sizeof(uint64_t);
   if (per == kManyPer)
     hipLaunchKernelGGL((tm_beam_rows_kernel<DT, kManyPer>), grid, block, lds, st, p);
   else
@@ -606,7 +631,7 @@ extern "C" int tm_beam_workspace(int64_t G, int64_t K, int64_t V, int64_t num, i
   const int rc = check_beams(G, K, V, num);
   if (rc) return rc;
   if (bytes == nullptr) return TM_ERR_ARG;
-  *bytes = G * K * ceil_div(V, kThreads * per_of(G * K, V, num)) * (8 * num + 8 + 4);
+  *bytes = G * K * ceil_div(V, kThreads * per_of(G * K, V)) * (8 * num + 8 + 4);
   return TM_OK;
 }
 
@@ -635,7 +660,7 @@ extern "C" int tm_beam_select(const void* logits, int dtype, int64_t G, int64_t 
   p.rows = (int)(G * K);
   p.beams = (int)K;
   p.vocab = (int)V;
-  const int per = per_of(G * K, V, num);
+  const int per = per_of(G * K, V);
   p.segs = (int)ceil_div(V, kThreads * per);
   p.num = (int)num;
   const int64_t units = (int64_t)p.rows * p.segs;
@@ -653,7 +678,11 @@ extern "C" int tm_beam_select(const void* logits, int dtype, int64_t G, int64_t 
     launch_rows<TM_DTYPE_F16>(p, per, st);
   else
     launch_rows<TM_DTYPE_BF16>(p, per, st);
-  hipLaunchKernelGGL(tm_beam_join_kernel, dim3((unsigned)G), dim3(kJoin), 0, st, p);
+  const int64_t lists = K * p.segs;
+  if (num > 16 && lists <= kSteps && lists < 4 * num)
+    hipLaunchKernelGGL(tm_beam_join_kernel<true>, dim3((unsigned)G), dim3(kJoin), 0, st, p);
+  else
+    hipLaunchKernelGGL(tm_beam_join_kernel<false>, dim3((unsigned)G), dim3(kJoin), 0, st, p);
   TM_HIP_CHECK_LAUNCH();
   return TM_OK;
 }
