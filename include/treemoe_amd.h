@@ -8,6 +8,9 @@
  *   op4  fused_verify_commit                treemoe/kernels/op4_commit.py:170-272
  *   tree attention (verification forward)   treemoe/model/mixtral.py:208-250
  *
+ * Around them: norm, rotary positions, attention of prompts, sampling; and attention of many
+ * branches of one sequence, beam search's selection, attention mass and cache eviction.
+ *
  * Conventions (all entry points):
  *   - plain device pointers and sizes; no torch types, no allocation inside;
  *   - every call is asynchronous on `stream` (a hipStream_t, may be NULL for the

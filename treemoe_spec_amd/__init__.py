@@ -10,7 +10,10 @@ Module layout mirrors the reference package:
   treemoe_spec_amd.kernels.rotary            RotaryPlan, rotary_embed, rotary_append
   treemoe_spec_amd.kernels.prompt_attention  PromptPlan, prompt_attention, prompt_attention_cached
   treemoe_spec_amd.kernels.sample_tokens     sample_tokens
-  treemoe_spec_amd.kv_cache               PagedKVCache (page size configurable)
+  treemoe_spec_amd.kernels.branch_attention  BranchPlan, branch_attention
+  treemoe_spec_amd.kernels.beam_search       beam_select, reorder_rows
+  treemoe_spec_amd.kernels.cache_eviction    attention_mass, evict
+  treemoe_spec_amd.kv_cache               PagedKVCache (page size configurable), BranchCache
 The GPU work lives in libtreemoe_amd.so (C ABI: include/treemoe_amd.h).
 """
 

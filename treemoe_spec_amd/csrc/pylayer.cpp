@@ -1,8 +1,8 @@
 // _tmlayer: CPython calls of the entry points that a forward makes once or more per
-// layer (norm, rotary positions, attention of prompts and branches) and per step
-// (sampling).  Each
-// function takes the entry point's arguments in order, addresses as integers, and
-// returns its status; conversions follow the C parameter types.  ctypes spends
+// layer (norm, rotary positions, attention of prompts and branches, attention mass) and per
+// step (sampling, beams, eviction).  Each function takes the entry point's arguments in order,
+// addresses as integers, and returns its status, a size query its status and the bytes;
+// conversions follow the C parameter types.  ctypes spends
 // ~3.5 us on a call of twenty arguments, this ~0.5 us.  The interpreter lock is
 // released during the call, whose launch waits when the stream's queue is full.
 #define PY_SSIZE_T_CLEAN
