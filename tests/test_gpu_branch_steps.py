@@ -8,6 +8,7 @@ call's bits on one stream."""
 
 from __future__ import annotations
 
+import functools
 import threading
 
 import pytest
@@ -25,6 +26,13 @@ LAYERS, HQ, KVH, HD, VOCAB = 2, 8, 2, 64, 700
 
 def _say(msg):
     print(msg, flush=True)
+
+
+@functools.cache
+def _streams():
+    """Four at once: streams go over the card's four hardware queues in turn, one of which is the
+    default stream's, so tests that come later get theirs as if these were not there."""
+    return [torch.cuda.Stream() for _ in range(4)]
 
 
 class Search:
@@ -100,8 +108,9 @@ class Search:
 
     def state(self):
         self.br.read_lengths()
-        return [x.clone() for x in (self.br.k, self.br.v, self.br.lengths, self.br.origin, self.held,
-                                    self.scores, self.tokens, self.position, self.logits)]
+        return [x.clone() for x in (self.br.k, self.br.v, self.br.lengths, self.br.origin,
+                                    self.held, self.scores, self.tokens, self.position,
+                                    self.logits)]
 
 
 def test_search_behind_a_cut_cache():
@@ -142,7 +151,7 @@ def test_captured_step():
     _say("captured search step")
     eager, replayed = Search(seed=3), Search(seed=3)
     other = Search(seed=4)
-    stream = torch.cuda.Stream()
+    stream = _streams()[0]
     with torch.cuda.stream(stream):
         for s in (eager, replayed):
             s.step()
@@ -241,7 +250,7 @@ def test_two_streams_and_two_threads():
             s.step()
         want.append(s.state())
     pair = [Search(seed=seed) for seed in (6, 7)]
-    streams = [torch.cuda.Stream() for _ in pair]
+    streams = _streams()[:2]
     torch.cuda.synchronize()
     for _ in range(5):
         for s, stream in zip(pair, streams):
