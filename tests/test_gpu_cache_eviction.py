@@ -86,6 +86,15 @@ def test_mass_long(t, n, dtype, hd):
     _mass(t, n, 8, 2, hd, dtype, 16, t, add=True)
 
 
+@pytest.mark.parametrize("t,n,hq,kvh,hd,dtype", [(300, 2100, 64, 16, 128, BF),
+                                                 (350, 2050, 48, 16, 64, F16),
+                                                 (3000, 3000, 16, 16, 64, BF)])
+def test_mass_many_heads(t, n, hq, kvh, hd, dtype):
+    """Tiles of keys that fill the chip."""
+    _say(f"mass t={t} n={n} heads={hq}/{kvh} hd={hd} {dtype}")
+    _mass(t, n, hq, kvh, hd, dtype, 64, t, add=True)
+
+
 def test_mass_scale_strides_and_out():
     from treemoe_spec_amd.kernels.cache_eviction import attention_mass
 

@@ -773,7 +773,7 @@ int64_t fused_moves(int64_t heads) { return std::max<int64_t>(256, 8 * heads); }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct MassPlan {
-  bool few, own;
+  bool few, own, wide;
   int64_t rows, tiles, chunks, chunk_len;
   int64_t key_tiles, splits;               // of the sums
   int64_t stats, consts, parts, scores;    // floats of the workspace
@@ -800,12 +800,16 @@ int plan_mass(int64_t T, int64_t S, int64_t Hq, int64_t kvh, int64_t hd, MassPla
   const int64_t step = o->few ? 4 * kKeys : kKeys;
   o->chunk_len = std::max(step, ceil_div(ceil_div(S, chunks), step) * step);
   o->chunks = std::max<int64_t>(1, ceil_div(S, o->chunk_len));
-  // the sums' rows in parts of eight stages or more, four workgroups a CU: 16384 rows over 4096
-  // keys 177 us in all, with two 189, with eight 176
-  o->key_tiles = ceil_div(S, o->own ? 128 : 256);
+  // The sums' keys by eight waves where those tiles give half the CUs one, else by four (which
+  // read the rows twice as often): 4096 tokens over themselves 172 us in all, by four 176; 2048
+  // 67, 62; 512 27, 21.  Their rows in parts of eight or four stages or more, four workgroups a
+  // CU: 4096 tokens with two a CU 189, with eight 176 where four gave 177.
+  o->wide = !o->own && ceil_div(S, 256) * kvh >= kCUs / 2;
+  o->key_tiles = ceil_div(S, o->wide ? 256 : 128);
   const int64_t stages = ceil_div(o->rows, kKeys);
   const int64_t splits = 4 * kCUs / std::max<int64_t>(o->key_tiles * kvh, 1);
-  o->splits = o->own ? 1 : std::max<int64_t>(1, std::min(splits, stages / 8));
+  o->splits =
+      o->own ? 1 : std::max<int64_t>(1, std::min(splits, stages / (o->wide ? 8 : 4)));
   o->stats = o->own || o->chunks > 1 ? 2 * o->chunks * kvh * o->rows : 0;
   o->consts = o->own ? 0 : kvh * stages * kKeys;
   o->parts = o->splits > 1 ? o->splits * kvh * S : 0;
@@ -842,7 +846,10 @@ void launch_mass(const MassParams& p, const MassPlan& o, hipStream_t st) {
   if (o.chunks > 1)
     hipLaunchKernelGGL(tm_mass_rows_kernel, dim3((unsigned)ceil_div(p.kvh * whole, kThreads)),
                        block, 0, st, p, (int)o.rows, (int)whole);
-  hipLaunchKernelGGL((tm_mass_sum_kernel<DT, HD, 8, false>), sums, dim3(512), 0, st, p);
+  if (o.wide)
+    hipLaunchKernelGGL((tm_mass_sum_kernel<DT, HD, 8, false>), sums, dim3(512), 0, st, p);
+  else
+    hipLaunchKernelGGL((tm_mass_sum_kernel<DT, HD, 4, false>), sums, block, 0, st, p);
   if (o.splits > 1)
     hipLaunchKernelGGL(tm_mass_join_kernel,
                        dim3((unsigned)ceil_div(p.k_len, kThreads), (unsigned)p.kvh), block, 0, st,
