@@ -215,9 +215,9 @@ __global__ void __launch_bounds__(kThreads) tm_mass_rows_kernel(MassParams p, in
 }
 
 // Rows whose constants a workgroup of the sums makes by itself, instead of a launch before
-// it, in us: 800 rows over 7200 keys 58, 59; 1024 over 7256 54, 57; 1000 over 3250 38, 37; 2000
-// over 3500 70, 60; 2048 over 512 43, 27.
-constexpr int kOwnRows = 1024;
+// it, in us: 256 rows over 7464 keys 23.3, 26.2; 500 over 7125 34, 35; 800 over 7200 49, 49; 1000
+// over 3250 37, 34; 2000 over 3500 59, 51; 2048 over 512 43, 21.
+constexpr int kOwnRows = 512;
 
 // Sums over the rows: a wave has 32 keys, one a column, and 64 rows at a time come by in LDS,
 // for all waves.  A lane's products with a stage belong to its key, so they are summed in
