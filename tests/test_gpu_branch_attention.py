@@ -165,6 +165,18 @@ def test_branches_that_leave_tiles_empty(counts, prefix, hq, kvh, hd, dtype):
     _run(s, counts)
 
 
+@pytest.mark.parametrize("counts,prefix,hq,kvh,hd,dtype", [
+    ([230] * 8 + [225, 0, 1], 600, 32, 8, 64, F16),
+    ([240] * 22, 150, 12, 3, 128, BF),
+])
+def test_tiles_of_more_than_a_round(counts, prefix, hq, kvh, hd, dtype):
+    """The first tiles whole, those of the last round in ranges, joined."""
+    _say(f"branches: {len(counts)} of {counts[0]} over {prefix} heads={hq}/{kvh} hd={hd} {dtype}")
+    s = Setup(prefix, [(i * 53) % 170 for i in range(len(counts))], hq, kvh, hd, dtype, 16,
+              seed=prefix, layers=2, capacity=420)
+    _run(s, counts)
+
+
 @pytest.mark.parametrize("beams,groups", [(2, 3), (4, 1), (5, 2), (8, 9)])
 @pytest.mark.parametrize("count", [1, 3, 20, 32])
 @pytest.mark.parametrize("hd", [64, 128])
