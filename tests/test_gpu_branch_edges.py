@@ -1,0 +1,44 @@
+"""Branch attention and attention mass at the edges of their value ranges and head shapes.
+Tolerances: test_gpu_prompt_attention and test_gpu_cache_eviction."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests import test_gpu_cache_eviction as t_evict
+from tests import test_gpu_prompt_attention as t_attn
+
+pytestmark = pytest.mark.gpu
+
+BF = torch.bfloat16
+INF, NAN = float("inf"), float("nan")
+U = 2.0 ** -24
+
+
+def _say(msg):
+    print(msg, flush=True)
+
+
+@pytest.mark.parametrize("bad", [NAN, INF])
+@pytest.mark.parametrize("t,past", [(2, 0), (2, 300), (8, 1), (10, 70), (16, 500), (17, 500)])
+def test_mass_of_a_row_that_is_not_a_number(t, past, bad):
+    """Of few rows and of more: it reaches the keys that it sees, of its KV head, and no others."""
+    from treemoe_spec_amd.kernels.cache_eviction import attention_mass
+
+    _say(f"mass with a query of {bad}, {t} tokens behind {past}")
+    n, at = t + past, t // 2
+    q, k, v = t_attn._qkv(t, n, 4, 2, 64, BF, t + past)
+    k[:, 1, 7] = k[:, 1, 7].abs() + 0.5        # (an infinite query scores +infinity there)
+    kv = t_attn._cache(n, 2, 64, BF, 16, t)
+    kv.append(0, k.cuda(), v.cuda(), 0)
+    q[at, 3, 7] = bad
+    got = attention_mass(q.cuda(), kv, 0).cpu().double()
+    assert bool(got[1, :past + at + 1].isnan().all())
+    q[at, 3] = 0.0                             # (what it gives lies before the keys compared)
+    want = t_evict._want(q, k, 64 ** -0.5)
+    ds = 130 * U * 64 ** -0.5 * float(q.abs().max()) * float(k.abs().max()) * 64
+    bound = (2 * ds + 736 * U) * want + 2.0 ** -90
+    off = (got - want).abs()
+    assert bool((off[0] <= bound[0]).all())
+    assert bool((off[1, past + at + 1:] <= bound[1, past + at + 1:]).all())

@@ -345,8 +345,9 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 ? 4 : 2) tm_mass_sum_ke
   }
 }
 
-// Sums over few rows from the scores that were kept, a thread a key.  Scored again by
-// tm_mass_sum_kernel, in us: 4 rows over 7777 keys 15.8, so 10.8; over 30001 34, 19; 32 rows over
+// Sums over few rows from the scores that were kept, a thread a key.  Rows that do not see the key
+// give 0 by their index, not by their score of -inf: a constant that is NaN would reach it.
+// Scored again by tm_mass_sum_kernel, in us: 4 rows over 7777 keys 15.8, so 10.8; over 30001 34, 19; 32 rows over
 // 7008 15.3, 13.3.
 __global__ void __launch_bounds__(kThreads) tm_mass_kept_kernel(MassParams p) {
   __shared__ float s_const[32];
@@ -360,6 +361,7 @@ __global__ void __launch_bounds__(kThreads) tm_mass_kept_kernel(MassParams p) {
   for (int r = 0; r < kAhead; ++r) first[r] = r < rows ? from[r * p.score_stride] : 0.0f;
   const float before =
       p.before != nullptr ? p.before[kvhead * p.before_stride + at] : 0.0f;
+  const int seen = max(at - (p.k_len - p.q_len), 0) * p.group;  // the key's first row
   int P = 64;  // lanes a row
   while (P * rows > kThreads) P /= 2;
   if (tid / P < rows) {
@@ -371,11 +373,16 @@ __global__ void __launch_bounds__(kThreads) tm_mass_kept_kernel(MassParams p) {
   float sum = 0.0f;
 #pragma unroll
   for (int r = 0; r < kAhead; ++r)
-    if (r < rows)
-      sum += __builtin_amdgcn_exp2f(fmaf(first[r], p.scale_log2, s_const[r]));
+    if (r < rows) {
+      const float e = __builtin_amdgcn_exp2f(fmaf(first[r], p.scale_log2, s_const[r]));
+      sum += r >= seen ? e : 0.0f;
+    }
 #pragma unroll 4
-  for (int r = kAhead; r < rows; ++r)
-    sum += __builtin_amdgcn_exp2f(fmaf(from[r * p.score_stride], p.scale_log2, s_const[r]));
+  for (int r = kAhead; r < rows; ++r) {
+    const float e =
+        __builtin_amdgcn_exp2f(fmaf(from[r * p.score_stride], p.scale_log2, s_const[r]));
+    sum += r >= seen ? e : 0.0f;
+  }
   if (key < p.k_len) p.mass[kvhead * p.mass_stride + key] = before + sum;
 }
 
