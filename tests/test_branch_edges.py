@@ -1,0 +1,24 @@
+"""CPU: calls of the branch, beam and eviction operators at the edges of what they take."""
+
+from __future__ import annotations
+
+import pytest
+
+from treemoe_spec_amd import _capi
+from treemoe_spec_amd.kernels import branch_attention as ba
+from tests.test_branch_args import _branch_args
+
+
+@pytest.mark.parametrize("heads", [128, 144, 256, 1024])
+def test_plan_of_more_heads_than_a_tile_has_rows(heads):
+    """A token of a plan may take several tiles.  (The address of k, checked behind the sizes,
+    ends the call before a launch.)"""
+    plan = ba.BranchPlan([1, 2, 0], num_heads=heads, num_kv_heads=1, device="cpu")
+    assert plan.num_units == -(-heads // 128) + -(-2 * heads // 128)
+    args = dict(q_stride=64 * heads, out_stride=64 * heads, k=8, T=3, rows=3, units=16, tokens=16,
+                num_units=plan.num_units, max_count=2, Hq=heads, kvh=1)
+    lib = _capi.lib()
+    assert lib.tm_branch_attention(*_branch_args(**args)) == 1002
+    most = 3 * -(-heads // 128)
+    assert lib.tm_branch_attention(*_branch_args(**args | dict(num_units=most))) == 1002
+    assert lib.tm_branch_attention(*_branch_args(**args | dict(num_units=most + 1))) == 1001

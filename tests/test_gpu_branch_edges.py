@@ -6,12 +6,13 @@ from __future__ import annotations
 import pytest
 import torch
 
+from tests import test_gpu_branch_attention as t_branch
 from tests import test_gpu_cache_eviction as t_evict
 from tests import test_gpu_prompt_attention as t_attn
 
 pytestmark = pytest.mark.gpu
 
-BF = torch.bfloat16
+BF, F16 = torch.bfloat16, torch.float16
 INF, NAN = float("inf"), float("nan")
 U = 2.0 ** -24
 
@@ -42,3 +43,18 @@ def test_mass_of_a_row_that_is_not_a_number(t, past, bad):
     off = (got - want).abs()
     assert bool((off[0] <= bound[0]).all())
     assert bool((off[1, past + at + 1:] <= bound[1, past + at + 1:]).all())
+
+
+@pytest.mark.parametrize("hq,hd,dtype", [(144, 64, BF), (256, 128, F16)])
+@pytest.mark.parametrize("counts,prefix", [([1, 1], 0), ([2, 0, 1], 70), ([1, 3, 1, 0], 1000),
+                                           ([2, 2], 300)])
+def test_more_heads_than_a_tile_has_rows(counts, prefix, hq, hd, dtype):
+    """A token's heads fill several tiles, with a plan and without."""
+    from treemoe_spec_amd.kernels.branch_attention import BranchPlan
+
+    _say(f"branches: {hq} heads over one, {counts} behind {prefix}")
+    s = t_branch.Setup(prefix, [(7 * i + 3) % 90 for i in range(len(counts))], hq, 1, hd, dtype,
+                       seed=22)
+    t_branch._run(s, counts, plan=BranchPlan(counts, num_heads=hq, num_kv_heads=1))
+    if len(set(counts)) == 1:
+        t_branch._run(s, counts, layer=0)

@@ -1006,13 +1006,15 @@ extern "C" int tm_branch_attention(
     return TM_ERR_SHAPE;
   if (T == 0) return TM_OK;
   if ((units == nullptr) != (tokens == nullptr)) return TM_ERR_ARG;
+  if (max_count < 1 || max_count > T || T > INT32_MAX) return TM_ERR_SHAPE;
+  const int64_t tile = own_tile_rows(max_count, group);
   int64_t unit_tiles = 1;
   if (units == nullptr) {
-    if (max_count < 1 || rows < 1 || T != rows * max_count) return TM_ERR_SHAPE;
-    unit_tiles = ceil_div(max_count * group, own_tile_rows(max_count, group));
+    if (rows < 1 || T != rows * max_count) return TM_ERR_SHAPE;
+    unit_tiles = ceil_div(max_count * group, tile);
     if (num_units != rows * unit_tiles) return TM_ERR_SHAPE;
-  } else if (num_units < 1 || num_units > T) {
-    return TM_ERR_SHAPE;
+  } else if (num_units < 1 || num_units > T * ceil_div(group, tile)) {
+    return TM_ERR_SHAPE;  // (n tokens of a branch have at most n times a token's tiles)
   }
   BranchPlan o;
   rc = plan_branches(T, num_units, max_count, seq_len, longest, Hq, kvh, hd, &o);
