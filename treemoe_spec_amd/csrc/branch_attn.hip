@@ -356,6 +356,10 @@ __device__ __forceinline__ void lean_body(const typename FEED::Params& p, const 
   }
 }
 
+// The sum of a part without keys, which has no output: added it changes nothing, and by its
+// sign the join tells it from the sum of keys without weight.
+constexpr float kNoOutput = -0.0f;
+
 // A branch's own keys, up to 32 rows against one range by one wave: no barrier, and no
 // join within the workgroup.  What such a part costs most is its chain of latencies (the
 // length, the first keys, the last stores), so all of a step's are to run at once.
@@ -367,12 +371,12 @@ __device__ __forceinline__ void wave_body(const BranchParams& p, const Work& w, 
   const int n = it.end > it.begin ? (it.end - it.begin + kLean - 1) / kLean : 0;
   const int rows = min(it.q_len * p.group, 32);
   uint8_t* const vt = kt + kLean * Shape<HD>::kRow;
-  if (n == 0) {  // (what the join does not read is not written)
+  if (n == 0) {  // no output is written, and the sum says so
     if (lane < rows && it.slot >= 0) {
       float* const st =
           p.stats + (((int64_t)it.slot * p.kvh + w.kvhead) * p.part_rows + lane) * 2;
       st[0] = -INFINITY;
-      st[1] = 0.0f;
+      st[1] = kNoOutput;
     }
     return;
   }
@@ -699,6 +703,10 @@ __global__ void __launch_bounds__(kThreads) tm_branch_join_kernel(BranchJoin p) 
     return *reinterpret_cast<const float2*>(c < n0 ? r0.stats + c * r0.step * 2
                                                    : r1.stats + (c - n0) * r1.step * 2);
   };
+  // the part's factor; -1 of one that has no output
+  auto factor_of = [&](const float2& st, float a) {
+    return __float_as_uint(st.y) == __float_as_uint(kNoOutput) ? -1.0f : a;
+  };
   f32x4_t first[kAhead] = {};
 #pragma unroll
   for (int i = 0; i < kAhead; ++i)
@@ -712,7 +720,7 @@ __global__ void __launch_bounds__(kThreads) tm_branch_join_kernel(BranchJoin p) 
     for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
     const float a = __builtin_amdgcn_exp2f(st.x - (m == -INFINITY ? 0.0f : m));
     sum = st.y * a;
-    s_a[wave][lane] = a;
+    s_a[wave][lane] = factor_of(st, a);
   } else {
     for (int c = lane; c < n; c += 64) m = fmaxf(m, stat_of(c).x);
 #pragma unroll
@@ -722,7 +730,7 @@ __global__ void __launch_bounds__(kThreads) tm_branch_join_kernel(BranchJoin p) 
       const float2 st = stat_of(c);
       const float a = __builtin_amdgcn_exp2f(st.x - ref);
       sum = fmaf(st.y, a, sum);
-      s_a[wave][c] = a;
+      s_a[wave][c] = factor_of(st, a);
     }
   }
 #pragma unroll
@@ -731,9 +739,9 @@ __global__ void __launch_bounds__(kThreads) tm_branch_join_kernel(BranchJoin p) 
   f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
   auto add = [&](int c, const f32x4_t& x) {
     const float a = s_a[wave][c];
-    // (a part without keys has no output)
+    // (a factor of 0 makes NaN of an infinity, as any product of the sum does)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = a == 0.0f ? o[i] : fmaf(x[i], a, o[i]);
+    for (int i = 0; i < 4; ++i) o[i] = a < 0.0f ? o[i] : fmaf(x[i], a, o[i]);
   };
 #pragma unroll
   for (int i = 0; i < kAhead; ++i)
