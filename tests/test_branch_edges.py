@@ -3,10 +3,12 @@
 from __future__ import annotations
 
 import pytest
+import torch
 
 from treemoe_spec_amd import _capi
+from treemoe_spec_amd.kernels import beam_search as bs
 from treemoe_spec_amd.kernels import branch_attention as ba
-from tests.test_branch_args import _branch_args
+from tests.test_branch_args import _branch_args, calls  # noqa: F401  (a fixture)
 
 
 @pytest.mark.parametrize("heads", [128, 144, 256, 1024])
@@ -22,3 +24,17 @@ def test_plan_of_more_heads_than_a_tile_has_rows(heads):
     most = 3 * -(-heads // 128)
     assert lib.tm_branch_attention(*_branch_args(**args | dict(num_units=most))) == 1002
     assert lib.tm_branch_attention(*_branch_args(**args | dict(num_units=most + 1))) == 1001
+
+
+def test_reorder_of_views_that_torch_has_not_computed(calls):  # noqa: F811
+    """Bytes are moved, so a conjugation or negation put off by torch is refused, not lost."""
+    x = torch.zeros(6, 4, dtype=torch.complex64)
+    parents = torch.zeros(2, 3, dtype=torch.int32)
+    for bad in (x.conj(), torch._neg_view(torch.zeros(6, 4))):
+        with pytest.raises(ValueError, match="materialised"):
+            bs.reorder_rows(bad, parents)
+        with pytest.raises(ValueError, match="materialised"):
+            bs.reorder_rows(torch.zeros(6, 4, dtype=bad.dtype), parents, out=bad)
+    assert not calls
+    bs.reorder_rows(x, parents)
+    assert calls[0][0] == "tm_reorder_rows"

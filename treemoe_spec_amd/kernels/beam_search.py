@@ -111,6 +111,9 @@ def reorder_rows(x: torch.Tensor, parents: torch.Tensor, *, out: torch.Tensor | 
         if n > 1 and (x.stride(d) != width or out.stride(d) != width):
             raise ValueError("each row of x and out must be contiguous")
         width *= n
+    # (bytes move: a conjugation or negation that torch has put off would be lost)
+    if x.is_conj() or x.is_neg() or out.is_conj() or out.is_neg():
+        raise ValueError("x and out must be materialised: no pending conjugation or negation")
     if rows == 0 or width == 0:
         return out
     xs, outs = (x.stride(0), out.stride(0)) if rows > 1 else (width, width)
