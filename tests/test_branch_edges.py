@@ -8,7 +8,8 @@ import torch
 from treemoe_spec_amd import _capi
 from treemoe_spec_amd.kernels import beam_search as bs
 from treemoe_spec_amd.kernels import branch_attention as ba
-from tests.test_branch_args import _branch_args, calls  # noqa: F401  (a fixture)
+from treemoe_spec_amd.kv_cache import BranchCache
+from tests.test_branch_args import CFG, _branch_args, calls  # noqa: F401  (a fixture)
 
 
 @pytest.mark.parametrize("heads", [128, 144, 256, 1024])
@@ -38,3 +39,14 @@ def test_reorder_of_views_that_torch_has_not_computed(calls):  # noqa: F811
     assert not calls
     bs.reorder_rows(x, parents)
     assert calls[0][0] == "tm_reorder_rows"
+
+
+def test_lengths_are_whole_numbers(calls):  # noqa: F811
+    br = BranchCache(CFG, 2, 10, device="cpu")
+    br.advance(5)
+    for bad in ([1.9, 2], [2, "3"], torch.tensor([1.0, 2.0])):
+        with pytest.raises(TypeError):
+            br.set_lengths(bad)
+    assert br.host_lengths == [5, 5]
+    br.set_lengths(torch.tensor([3, 0]))
+    assert br.host_lengths == [3, 0] and br.longest == 3 and br.lengths.tolist() == [3, 0]

@@ -327,7 +327,7 @@ class BranchCache:
     def set_lengths(self, lengths) -> None:
         """Cuts branches back to ``lengths`` keys (0 for a new request; a chain whose
         last tokens were rejected).  The beams of a group are cut alike."""
-        lengths = [int(n) for n in lengths]
+        lengths = [operator.index(n) for n in lengths]
         if len(lengths) != self.rows or any(not 0 <= n <= m for n, m in
                                             zip(lengths, self.host_lengths)):
             raise ValueError("lengths must be 0 .. the branches' present ones, one for each")
