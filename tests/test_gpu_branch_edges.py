@@ -108,3 +108,67 @@ def test_more_heads_than_a_tile_has_rows(counts, prefix, hq, hd, dtype):
     t_branch._run(s, counts, plan=BranchPlan(counts, num_heads=hq, num_kv_heads=1))
     if len(set(counts)) == 1:
         t_branch._run(s, counts, layer=0)
+
+
+@pytest.mark.parametrize("hq", [144, 1024])
+@pytest.mark.parametrize("t,past", [(1, 0), (2, 65), (5, 700)])
+def test_mass_of_more_heads_than_a_tile_has_rows(t, past, hq):
+    _say(f"mass of {hq} heads over one, {t} tokens behind {past}")
+    t_evict._mass(t, t + past, hq, 1, 64, BF, 16, t, add=past > 0)
+
+
+def test_mass_of_rows_beyond_a_few_stages():
+    """The bound of the sum over a key's rows, all positive, from the rows: an accumulator takes 8
+    of each 64, each addition half a step of what is there; then 3 joins of accumulators and
+    lanes, up to 8 parts of the rows, and `before`.  The other shares are
+    test_gpu_cache_eviction's: 600 u for the sum over the keys has, a lane and stage of 64 keys
+    one addition, one product and a factor of two roundings where the maximum grew, 4 * 128, and
+    11 within a stage, 35 ranges joined."""
+    from treemoe_spec_amd.kernels.cache_eviction import attention_mass
+
+    t, hq, kvh, hd = 4096, 16, 8, 64
+    _say(f"mass of {t} tokens over themselves")
+    q, k, v = t_attn._qkv(t, t, hq, kvh, hd, BF, 31, 2.0)
+    kv = t_attn._cache(t, kvh, hd, BF, 64, 31)
+    kv.append(1, k.cuda(), v.cuda(), 0)
+    got = attention_mass(q.cuda(), kv, 1).double().cpu()
+    want = t_evict._want(q, k, hd ** -0.5)
+    ds = 130 * U * hd ** -0.5 * float(q.abs().max()) * float(k.abs().max()) * hd
+    terms = 8 * (t * hq // kvh // 64) + 3 + 8 + 1
+    off = (got - want).abs()
+    assert bool((off <= (2 * ds + (8 + 64 + 600 + terms) * U) * want + 2.0 ** -90).all())
+
+
+@pytest.mark.parametrize("hd,page", [(16, 16), (64, 1), (80, 64), (128, 16)])
+@pytest.mark.parametrize("n,keep", [(100, 60), (1100, 1030), (2500, 300)])
+def test_evict_of_one_byte_elements(n, keep, hd, page):
+    _say(f"evict {n} -> {keep} of one byte, hd={hd}")
+    g = torch.Generator().manual_seed(n + hd)
+    kv = t_evict._cache_of(2, n, 3, hd, torch.int8, page, g)
+    for x in (kv.k, kv.v):
+        x.copy_(torch.randint(-128, 128, x.shape, generator=g, dtype=torch.int8))
+    mass = torch.exp(2 * torch.randn(2, 3, n, generator=g))
+    t_evict._check_evict(kv, mass, keep, recent=16, sinks=4)
+
+
+def test_evict_of_float8():
+    """The bytes of 8-bit floats move as they are, NaN among them."""
+    from treemoe_spec_amd.kernels.cache_eviction import evict
+    from treemoe_spec_amd.kv_cache import MixtralConfig, PagedKVCache
+
+    _say("evict float8")
+    g = torch.Generator().manual_seed(32)
+    kv = PagedKVCache(MixtralConfig(num_layers=2, num_kv_heads=2, head_dim=64), 10,
+                      dtype=torch.float8_e4m3fn, page_size=16, tree_size=1)
+    same = PagedKVCache(kv.config, 10, dtype=torch.int8, page_size=16, tree_size=1)
+    for x, y in ((kv.k, same.k), (kv.v, same.v)):
+        y.copy_(torch.randint(-128, 128, y.shape, generator=g, dtype=torch.int8))
+        x.view(torch.int8).copy_(y)
+    mass = torch.rand(2, 2, 130, generator=g).cuda()
+    got = []
+    for c in (kv, same):
+        c._ensure_capacity(130)
+        c.seq_len = 130
+        got.append(evict(c, mass, 70, recent=8))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    assert torch.equal(kv.k.view(torch.int8), same.k) and torch.equal(kv.v.view(torch.int8), same.v)
