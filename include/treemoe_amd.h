@@ -607,10 +607,11 @@ int tm_branch_workspace(int64_t T, int64_t units, int64_t max_count, int64_t seq
 
 /*
  * Attention of T tokens of many branches of one sequence (requests behind a shared
- * prompt, beams, drafted chains), one launch per part of the keys: the shared ones
- * are taken once for all branches.  The reference continues one sequence at a time
- * (treemoe/model/mixtral.py:208-250); for one branch this is its append, gather and
- * causal `F.scaled_dot_product_attention`.
+ * prompt, beams, drafted chains).  Where branches have few rows, or leave most of their
+ * tiles empty behind many shared keys, those are read once for all branches; else each tile
+ * of a branch takes shared and own keys as one sequence.  The reference continues one
+ * sequence at a time (treemoe/model/mixtral.py:208-250); for one branch this is its append,
+ * gather and causal `F.scaled_dot_product_attention`.
  *
  * q, out [T, Hq, hd] and k, v [T, kvh, hd], bf16 or fp16, hd 64 or 128, heads
  * contiguous, token strides in elements, 16-byte aligned: branch after branch, with
@@ -657,8 +658,9 @@ int tm_beam_workspace(int64_t G, int64_t K, int64_t V, int64_t num, int64_t* byt
  *   scores[b] + l_b[v] - log sum_u exp l_b[u]     (l_b: row g K + b of logits)
  * and, for a beam b with finished[b], of (scores[b], pad_token) alone.  Larger
  * scores first; of equal ones the lower beam, then the larger logit, then the lower
- * token.  Scores are formed in 64 bits and written in fp32.  The reference decodes one
- * continuation (greedy or sampled) and has no counterpart.
+ * token.  Scores are formed in 64 bits, from exponentials good to 2e-13 of their values, and
+ * written in fp32.  The reference decodes one continuation (greedy or sampled) and has no
+ * counterpart.
  *
  * logits [G K, V] of dtype, row stride in elements; scores fp32 [G, K]; finished [G, K]
  * bytes, or NULL.  NaN logits count as -infinity; of a row with infinite logits those

@@ -7,10 +7,10 @@
 // order: larger score first, of equal ones the lower beam, then the larger logit, then
 // the lower token.
 //
-// Arithmetic.  Scores are formed in 64 bits, the sum of the exponentials too, so that beams
-// are not exchanged by rounding; each is rounded to fp32 once, when it is written.  Within a
-// beam the order is that of the logits, so a row is cut to its best `num` before any
-// score is known.
+// Arithmetic.  Scores are formed in 64 bits, the sum of the exponentials too (each off by 2e-13
+// at most), so that beams are not exchanged by the rounding of 32; each score is rounded to fp32
+// once, when it is written.  Within a beam the order is that of the logits, so a row is cut to
+// its best `num` before any score is known.
 //
 // A workgroup takes 4096 or 8192 logits of a row: their sum, and their best `num` as sorted
 // keys (ordered bits of the logit, inverted token), all distinct.  At least `num` logits reach
@@ -76,7 +76,9 @@ __device__ __forceinline__ int lanes_before(uint64_t ballot) {
                                         __builtin_amdgcn_mbcnt_lo((uint32_t)ballot, 0));
 }
 
-// The logits base + index_of(e) of a lane; what lies past the end, and NaN, as -inf.
+// The logits base + index_of(e) of a lane; what lies past the end, and NaN, as -inf.  Rows that do
+// not start on 16 bytes come an element at a time: 256 rows of 131072 in bf16 75 us, aligned
+// 52; of 50257 44, 35; 4 of 50257 17, 15.
 template <int DT>
 __device__ __forceinline__ int index_of(int e) {
   constexpr int kVec = DT == TM_DTYPE_F32 ? 4 : 8;
@@ -137,7 +139,8 @@ __constant__ const double kPowers[64] = {
 
 // e^d for d <= 0, in 64 bits: with t = 64 d log2(e) and k the integer nearest to it,
 // 2^(k / 64) e^x, x = d - k ln 2 / 64, |x| <= ln 2 / 128: 2^(j / 64) from a table, e^x from
-// its Taylor polynomial of degree 4 (truncation below 4e-14).  Below -700 it is e^-700.
+// its Taylor polynomial of degree 4 (truncation below 4e-14; the rounding of t, largest at -700,
+// brings it to 2e-13).  Below -700 it is e^-700.
 // A library exponential, with its wider range and half an ulp, takes three times as long.
 __device__ __forceinline__ double exp_of(double d, const double* powers) {
   constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to integers
@@ -542,7 +545,8 @@ __global__ void __launch_bounds__(kThreads) tm_reorder_kernel(ReorderParams p, i
 
 // Rows within x: a workgroup takes `cols` pieces of a group's rows, those that are parents of
 // others into LDS, and from there to where they go.  A beam that goes on from itself, or
-// whose parent is no beam of the group, stays.
+// whose parent is no beam of the group, stays.  32 groups of 8 rows of 32 KB 7.5 us (into rows
+// apart 4.6), one group of 4 of 4 KB 3.5 (2.6).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) tm_reorder_within_kernel(ReorderParams p, int cols) {
   __shared__ __attribute__((aligned(16))) T rows[kReorderPieces];

@@ -21,10 +21,11 @@
 // ancestor that stored it (without a table of origins, in row b).  So beams are reordered
 // by their tables, and no key moves.
 //
-// Bound by latency and by HBM at few rows: 4 beams over 517 keys 7 us and the join 3.5; 64
+// Bound by latency and by HBM at few rows: 4 beams over 517 keys 7 us and the join 4; 64
 // requests of up to 700 own keys over 4096 38 us for 107 MB, of which about 10 are the two
-// launches' chains of latencies; own keys alone stream at 4.2-5.6 TB/s.  By prompt
-// attention's matrix products and exponentials at many: 12 prompts over 4096 0.8 PFLOP/s.
+// launches' chains of latencies; own keys alone stream at 3.1 TB/s there, at
+// 4.3-5.3 where they are more (256 branches of 350, 64 of 3000-6000).  By prompt attention's
+// matrix products and exponentials at many: 12 prompts over 4096 0.77-0.82 PFLOP/s.
 #include <algorithm>
 #include <new>
 
@@ -835,7 +836,8 @@ int plan_branches(int64_t T, int64_t units, int64_t max_count, int64_t S, int64_
     f.chunk_len = std::max(step, ceil_div(ceil_div(S, chunks), step) * step);
     f.chunks = ceil_div(S, f.chunk_len);
   }
-  // Shared and own keys as one sequence, or apart and joined.  As one, the rows that a
+  // Shared and own keys as one sequence, or apart and joined (the same heads measured; others take
+  // the same rule).  As one, the rows that a
   // branch's tiles are short of go against the shared keys, too; apart, two launches more and
   // every row's parts are stored and read.  Measured, in us, as one and apart: 32 branches of 9
   // tokens (36 rows of 128) behind 500 keys 28, 42, 1000 36, 44, 2000 53, 50; of 16 tokens

@@ -12,7 +12,8 @@
 //
 // Bound by latencies at few rows: one token over 7777 keys 10.8 us of two launches, 16 MB of K.
 // By the matrix products and exponentials together at many: 4096 tokens over themselves
-// 173 us, twice 69 GFLOP and 0.27 G exponentials each time, 0.8 PFLOP/s.
+// 168-181 us, twice 69 GFLOP and 0.27 G exponentials each time, 0.76-0.82 PFLOP/s; the vector
+// unit is busy in 64-70 % of the CUs' busy cycles, the matrix pipe in 44-46 %.
 //
 // Eviction.  Of each layer's KV heads, `keep` of S keys stay: the first `sinks` and the last
 // `recent` positions, and the heaviest others.  Kept keys in slots from `keep` on move into
@@ -347,8 +348,8 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 ? 4 : 2) tm_mass_sum_ke
 
 // Sums over few rows from the scores that were kept, a thread a key.  Rows that do not see the key
 // give 0 by their index, not by their score of -inf: a constant that is NaN would reach it.
-// Scored again by tm_mass_sum_kernel, in us: 4 rows over 7777 keys 15.8, so 10.8; over 30001 34, 19; 32 rows over
-// 7008 15.3, 13.3.
+// Scored again by tm_mass_sum_kernel, in us: 4 rows over 7777 keys 15.8, so 10.8; over 30001 34,
+// 19; 32 rows over 7008 15.3, 13.3.
 __global__ void __launch_bounds__(kThreads) tm_mass_kept_kernel(MassParams p) {
   __shared__ float s_const[32];
   const int tid = threadIdx.x, rows = p.q_len * p.group;
@@ -657,7 +658,8 @@ __global__ void __launch_bounds__(THREADS) tm_evict_held_kernel(EvictParams p) {
 }
 
 // Selection of any number of keys, read again for each pass: the threshold from histograms
-// of 11, 11 and 10 bits.
+// of 11, 11 and 10 bits.  With the moves, half kept: 32 heads of 16385 slots 79 us (of 16384, held
+// in registers, 53), of 32768 154; 8 of 131072 408, one CU a head.
 __global__ void __launch_bounds__(kSelect) tm_evict_select_kernel(EvictParams p) {
   __shared__ uint32_t s_bins[kBins];
   __shared__ int s_waves[kSelect / 64];

@@ -24,11 +24,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, num: int | None =
     ``logits`` [G * K, V] (float32, bfloat16 or float16, rows at any stride), the rows of
     a group's K beams one after the other; ``scores`` [G, K] float32, the beams' summed
     log-probabilities.  A beam's candidates are every token with ``scores + log
-    softmax(logits)``, formed in 64 bits; one that has ``finished`` [G, K] (bool) has a
-    single candidate, ``pad_token`` with its score unchanged.  Returns (scores float32,
-    parents int32, tokens int64), each [G, num], the larger score first, of equal ones the
-    lower beam, then the larger logit, then the lower token; parents are beams within the
-    group.
+    softmax(logits)``, formed in 64 bits (exponentials good to 2e-13); one that has
+    ``finished`` [G, K] (bool) has a single candidate, ``pad_token`` with its score
+    unchanged.  Returns (scores float32, parents int32, tokens int64), each [G, num], the
+    larger score first, of equal ones the lower beam, then the larger logit, then the lower
+    token; parents are beams within the group.
 
     NaN logits count as -inf; a score of -inf or NaN, or a row with no logit above -inf,
     gives no candidates; where fewer than ``num`` are left, the rest are -inf, -1 and -1.

@@ -3,8 +3,8 @@ drafted chains.
 
 The reference continues one sequence at a time (treemoe/model/mixtral.py:208-250).  Here
 the tokens of all branches go through a layer together: ``branch_attention`` reads the
-shared sequence's pages once for all of them, each branch's own keys from a
-``BranchCache``, and stores the new keys and values there.  The context comes back as
+shared sequence's pages (once for all branches, where each adds few tokens), each branch's
+own keys from a ``BranchCache``, and stores the new keys and values there.  The context comes back as
 [T, Hq * hd], the layout ``o_proj`` takes.
 """
 

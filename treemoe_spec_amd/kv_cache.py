@@ -293,8 +293,8 @@ class BranchCache:
     def advance(self, counts=1) -> None:
         """After the last layer of a step in which every branch has added ``counts``
         tokens (a number, or the step's ``BranchPlan``): they now hold them.  A replay of
-        a captured call advances ``lengths`` alone; ``read_lengths`` brings the host's
-        up to it."""
+        a captured call advances ``lengths`` alone, and not past the capacity;
+        ``read_lengths`` brings the host's up to it."""
         from treemoe_spec_amd import _capi
 
         uniform = not hasattr(counts, "counts")
@@ -326,7 +326,8 @@ class BranchCache:
 
     def set_lengths(self, lengths) -> None:
         """Cuts branches back to ``lengths`` keys (0 for a new request; a chain whose
-        last tokens were rejected).  The beams of a group are cut alike."""
+        last tokens were rejected).  The beams of a group are cut alike.  The lengths are
+        copied from the host, and the call waits for that copy."""
         lengths = [operator.index(n) for n in lengths]
         if len(lengths) != self.rows or any(not 0 <= n <= m for n, m in
                                             zip(lengths, self.host_lengths)):
